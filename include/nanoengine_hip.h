@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define NE_ABI_VERSION 10
+#define NE_ABI_VERSION 11
 
 /* status codes */
 #define NE_OK 0
@@ -423,6 +423,55 @@ int ne_advance_and_propose(const int32_t* history, int64_t history_stride, const
                            uint64_t* steps, int32_t* num_guesses, int32_t k, int32_t num_seqs,
                            int32_t max_ngram, int32_t min_ngram, int32_t max_drafts, int32_t* drafts,
                            int32_t* num_drafts, void* stream);
+
+/*
+ * Copies of KV blocks within a pool (no counterpart in the reference, whose blocks are
+ * never copied): for every buffer b and pair i, block dst[i] takes block src[i]'s bytes.
+ * buffers, block_bytes, src and dst are HOST arrays, read before the call returns (a
+ * captured graph keeps the pairs it was recorded with).
+ *   buffers      [num_buffers] device pointers: keys, values and scales of every layer
+ *   block_bytes  [num_buffers] bytes of one block (block_size slots); at most 2^30
+ *   src, dst     [num_pairs] block numbers in [0, num_blocks)
+ * No block may be a destination twice, nor the destination of one pair and the source of
+ * another: the copies of a call are unordered.  A pair of a block with itself copies
+ * nothing.
+ */
+int ne_kv_copy_blocks(void* const* buffers, const int64_t* block_bytes, int32_t num_buffers,
+                      int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t num_pairs,
+                      void* stream);
+
+/*
+ * Sampling from given uniforms under temperature, top-k, top-p and min-p (the sampling of
+ * ne/engine/sampling.py:21-42 with two more filters and explicit randomness).  Per row, in
+ * the order of logits (descending) then index (ascending), with weights
+ * w_j = exp((x_j - max x) / T): the first n = min(n_k, n_p, n_m) tokens are kept,
+ *   n_k = top_k (all tokens when 0 or less),
+ *   n_p = the fewest whose weight reaches top_p times the weight of the first n_k (all
+ *         when top_p is 1 or more),
+ *   n_m = the tokens with w_j >= min_p (all when min_p is 0 or less),
+ * at least one; the token is the first whose running weight exceeds u times the kept
+ * weight (u below 0 or NaN: the first; u of 1 or more: the last kept).  Temperature 0 (or
+ * less, or NaN) takes the first token.  NaN and -inf logits are never drawn, tokens at
+ * +inf share the row, and a row of no token gives -1.
+ *   logits    [rows, vocab] bf16, fp16 or fp32 (dtype), row stride ld; vocab <= 2^20
+ *   uniforms  [rows] fp32
+ *   temperatures, top_ks, top_ps, min_ps: [rows] device arrays, or null: the scalar
+ *             beside each for every row (its temperature finite and >= 0)
+ *   tokens    [rows] int32 out
+ *   probs     null, or [rows, vocab] fp32 out, row stride ld_probs: w_j / kept weight
+ *             for the kept tokens, 0 for the others (rows that ne_accept takes as
+ *             fp32 draft_rows)
+ *   workspace ne_sample_workspace_size() bytes, 16-byte aligned; written and consumed
+ *             within the call
+ * Weights are 64-bit integers summed exactly, so results do not depend on the order of
+ * any sum (sample.hip).
+ */
+size_t ne_sample_workspace_size(int32_t rows, int32_t vocab, int32_t dtype);
+int ne_sample(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t vocab,
+              const float* uniforms, const float* temperatures, float temperature,
+              const int32_t* top_ks, int32_t top_k, const float* top_ps, float top_p,
+              const float* min_ps, float min_p, int32_t* tokens, float* probs, int64_t ld_probs,
+              void* workspace, size_t workspace_bytes, void* stream);
 
 /* Plain device copy of `bytes` bytes (16-byte aligned); used to calibrate the
  * hardware byte counters against a kernel of known traffic. */

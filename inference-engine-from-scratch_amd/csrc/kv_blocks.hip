@@ -1,0 +1,159 @@
+// Copying KV blocks within a pool: block dst[i] of every buffer (keys, values and scales
+// of every layer) takes block src[i]'s bytes, in one launch for all layers.
+//
+// What bounds it: memory (each byte read once and written once); a fork's few blocks are
+// bound by the launch and one round trip of memory.  The buffers' addresses and the block
+// pairs travel by value in the kernel's arguments: block numbers live in host lists, and
+// uploading a list of seven pairs would cost more than copying them.  A work-group copies
+// about 32 KB of one buffer (one 16-token block of 8 bf16 heads): its 256 threads issue
+// eight 16-byte loads each before the first store, so a copy of few blocks is one round
+// trip, and a buffer of small blocks (scales, 256 bytes a block) takes many pairs per
+// work-group instead of many work-groups of one wave.
+#include <stdlib.h>
+
+#include "ne_common.hpp"
+
+namespace ne {
+
+namespace {
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 8;
+constexpr int kCopyBytes = kCopyThreads * kCopyUnroll * 16;  // per work-group
+constexpr int kCopyBuffers = 128;                            // per launch
+constexpr int kCopyPairs = 224;
+
+// At most 4 KB of kernel arguments.
+struct CopyParams {
+  char* buffer[kCopyBuffers];
+  uint32_t block_bytes[kCopyBuffers];
+  uint32_t first[kCopyBuffers];  // first work-group of each buffer
+  int32_t src[kCopyPairs];
+  int32_t dst[kCopyPairs];
+  int32_t num_buffers;
+  int32_t num_pairs;
+};
+static_assert(sizeof(CopyParams) <= 4096, "kernel arguments");
+
+// Work-groups of one buffer: consecutive pairs, whole blocks of at least kCopyBytes where
+// blocks are small.
+__host__ __device__ inline uint32_t pairs_per_group(uint32_t block_bytes) {
+  return block_bytes >= kCopyBytes ? 1 : kCopyBytes / block_bytes;
+}
+
+__global__ __launch_bounds__(kCopyThreads) void kv_copy_blocks_kernel(CopyParams p) {
+  // the buffer whose work-groups hold this one
+  int lo = 0, hi = p.num_buffers - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (p.first[mid] <= blockIdx.x)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  char* const buffer = p.buffer[lo];
+  const uint32_t bytes = p.block_bytes[lo];
+  const uint32_t per = pairs_per_group(bytes);
+  const uint32_t pair0 = (blockIdx.x - p.first[lo]) * per;
+  const uint32_t pairs = min(per, p.num_pairs - pair0);
+  if (bytes % 16 == 0 && (uintptr_t)buffer % 16 == 0) {
+    const uint32_t vecs = bytes / 16;
+    const uint32_t total = pairs * vecs;
+    for (uint32_t base = 0; base < total; base += kCopyThreads * kCopyUnroll) {
+      u32x4 x[kCopyUnroll];
+      uint64_t to[kCopyUnroll];
+#pragma unroll
+      for (int j = 0; j < kCopyUnroll; ++j) {
+        const uint32_t v = min(base + j * kCopyThreads + threadIdx.x, total - 1);
+        const uint32_t i = per == 1 ? 0 : v / vecs;
+        const uint64_t at = (uint64_t)(v - i * vecs) * 16;
+        to[j] = (uint64_t)p.dst[pair0 + i] * bytes + at;
+        x[j] = *(const u32x4*)(buffer + (uint64_t)p.src[pair0 + i] * bytes + at);
+      }
+#pragma unroll
+      for (int j = 0; j < kCopyUnroll; ++j)
+        if (base + j * kCopyThreads + threadIdx.x < total) *(u32x4*)(buffer + to[j]) = x[j];
+    }
+  } else {  // blocks off the 16-byte grid: byte by byte
+    const uint32_t total = pairs * bytes;
+    for (uint32_t v = threadIdx.x; v < total; v += kCopyThreads) {
+      const uint32_t i = v / bytes;
+      buffer[(uint64_t)p.dst[pair0 + i] * bytes + v - i * bytes] = buffer[(uint64_t)p.src[pair0 + i] * bytes + v - i * bytes];
+    }
+  }
+}
+
+// Checks the pairs: in range, no destination twice, and no destination that is another
+// pair's source (all reads and writes of a call are unordered).
+int check_pairs(const int32_t* src, const int32_t* dst, int32_t n, int32_t num_blocks) {
+  for (int i = 0; i < n; ++i)
+    NE_CHECK_ARG(src[i] >= 0 && src[i] < num_blocks && dst[i] >= 0 && dst[i] < num_blocks,
+                 "copy %d: block %d -> %d of %d blocks", i, src[i], dst[i], num_blocks);
+  const size_t words = ((size_t)num_blocks + 63) / 64;
+  uint64_t* seen = (uint64_t*)calloc(2 * words, sizeof(uint64_t));
+  NE_CHECK_ARG(seen, "no host memory to check %d blocks", num_blocks);
+  uint64_t* read = seen + words;
+  int bad = -1, why = 0;
+  for (int i = 0; i < n; ++i)
+    if (src[i] != dst[i]) read[src[i] / 64] |= 1ull << (src[i] % 64);
+  for (int i = 0; i < n && bad < 0; ++i) {
+    const uint64_t bit = 1ull << (dst[i] % 64);
+    if (seen[dst[i] / 64] & bit) {
+      bad = i;
+      why = 1;
+    } else if (src[i] != dst[i] && (read[dst[i] / 64] & bit)) {
+      bad = i;
+      why = 2;
+    }
+    seen[dst[i] / 64] |= bit;
+  }
+  free(seen);
+  NE_CHECK_ARG(why != 1, "copy %d: block %d is a destination twice", bad, dst[bad]);
+  NE_CHECK_ARG(why != 2, "copy %d: destination %d is another copy's source", bad, dst[bad]);
+  return NE_OK;
+}
+
+}  // namespace
+
+}  // namespace ne
+
+extern "C" int ne_kv_copy_blocks(void* const* buffers, const int64_t* block_bytes, int32_t num_buffers,
+                                 int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t num_pairs,
+                                 void* stream) {
+  using namespace ne;
+  NE_CHECK_ARG(num_buffers >= 0 && num_pairs >= 0 && num_blocks >= 0, "bad sizes: %d buffers, %d pairs, %d blocks",
+               num_buffers, num_pairs, num_blocks);
+  if (num_buffers == 0 || num_pairs == 0) return NE_OK;
+  NE_CHECK_ARG(buffers && block_bytes && src && dst, "null pointer argument");
+  for (int b = 0; b < num_buffers; ++b) {
+    NE_CHECK_ARG(buffers[b], "null pointer argument (buffer %d)", b);
+    NE_CHECK_ARG(block_bytes[b] > 0 && block_bytes[b] <= (1 << 30), "buffer %d: bad block of %lld bytes", b,
+                 (long long)block_bytes[b]);
+  }
+  int rc = check_pairs(src, dst, num_pairs, num_blocks);
+  if (rc != NE_OK) return rc;
+  CopyParams p;
+  for (int i0 = 0; i0 < num_pairs;) {
+    p.num_pairs = 0;
+    for (; i0 < num_pairs && p.num_pairs < kCopyPairs; ++i0) {
+      if (src[i0] == dst[i0]) continue;  // nothing to move
+      p.src[p.num_pairs] = src[i0];
+      p.dst[p.num_pairs++] = dst[i0];
+    }
+    if (p.num_pairs == 0) continue;
+    for (int b0 = 0; b0 < num_buffers; b0 += kCopyBuffers) {
+      p.num_buffers = num_buffers - b0 < kCopyBuffers ? num_buffers - b0 : kCopyBuffers;
+      uint32_t groups = 0;
+      for (int b = 0; b < p.num_buffers; ++b) {
+        p.buffer[b] = (char*)buffers[b0 + b];
+        p.block_bytes[b] = (uint32_t)block_bytes[b0 + b];
+        p.first[b] = groups;
+        groups += ceil_div(p.num_pairs, pairs_per_group(p.block_bytes[b]));
+      }
+      hipLaunchKernelGGL(kv_copy_blocks_kernel, dim3(groups), dim3(kCopyThreads), 0, (hipStream_t)stream, p);
+      rc = check_launch("kv_copy_blocks");
+      if (rc != NE_OK) return rc;
+    }
+  }
+  return NE_OK;
+}

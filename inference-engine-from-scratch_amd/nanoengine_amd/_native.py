@@ -14,7 +14,7 @@ from pathlib import Path
 
 LIBRARY_NAME = "libnanoengine_hip.so"
 LIBRARY_PATH = Path(__file__).resolve().parent / LIBRARY_NAME
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 # status codes (nanoengine_hip.h)
 NE_OK = 0
@@ -136,6 +136,17 @@ SIGNATURES: dict[str, tuple] = {
         [_vp, _i64, _vp, _vp, _vp, _vp, _u64p, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp],
     ),
     "ne_copy_bytes": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
+    "ne_kv_copy_blocks": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp]),
+    "ne_sample_workspace_size": (_sz, [_i32, _i32, _i32]),
+    "ne_sample": (
+        ctypes.c_int,
+        [
+            _vp, _i32, _i64, _i32, _i32, _vp,  # logits, dtype, ld, rows, vocab, uniforms
+            _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32,  # temperature, top-k, top-p, min-p: per row, or one for all
+            _vp, _vp, _i64,  # tokens, probs, their ld
+            _vp, _sz, _vp,  # workspace, bytes, stream
+        ],
+    ),
 }
 SIGNATURES["ne_paged_verify_attention_planned"] = SIGNATURES["ne_paged_verify_attention"]
 # the allocation-free variant: (workspace, bytes) replaced by the caller's error-flag word

@@ -134,6 +134,59 @@ def kv_write(
     )
 
 
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """``_native.call`` with ``device`` current: a launch goes to the current device, whichever
+    device its stream belongs to."""
+    if torch.cuda.current_device() == device.index:
+        _native.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _native.call(name, *args)
+
+
+# ------------------------------------------------------------------- block copies
+def copy_kv_blocks(buffers: list[torch.Tensor], block_size: int, src: list[int], dst: list[int]) -> None:
+    """Copy block ``src[i]`` to block ``dst[i]`` in every buffer: caches and scales
+    ``[num_slots (+ 1), ...]`` whose slots ``b * block_size ..`` are block ``b``, as a
+    :class:`~nanoengine_amd.memory.KVCachePool` holds them, all layers in one launch.
+
+    ``src`` and ``dst`` are host lists.  The copies are unordered, so no block may be a
+    destination twice or the destination of one copy and the source of another.  Under graph
+    capture the graph keeps the blocks of this call."""
+    _check(block_size >= 1, "block_size must be at least 1")
+    _check(len(src) == len(dst), f"{len(src)} sources for {len(dst)} destinations")
+    if not buffers:
+        raise ValueError("no buffers to copy in")
+    device = _require_gpu(*buffers)
+    slots = {t.shape[0] for t in buffers if t.dim() > 0}
+    _check(len(slots) == 1 and all(t.dim() > 0 and t.is_contiguous() for t in buffers),
+           "buffers must be contiguous and hold the same slots")
+    num_slots = slots.pop()
+    _check(num_slots > 0, "buffers hold no slots")
+    n = len(buffers)
+    block_bytes = [t.numel() // num_slots * t.element_size() * block_size for t in buffers]
+    _copy_blocks(device, _pointers(buffers), (ctypes.c_int64 * n)(*block_bytes), n, num_slots // block_size, src, dst)
+
+
+def _pointers(buffers: list[torch.Tensor]):
+    return (ctypes.c_void_p * len(buffers))(*[t.data_ptr() for t in buffers])
+
+
+def _block_list(blocks: list[int]):
+    try:
+        return (ctypes.c_int32 * len(blocks))(*blocks)
+    except TypeError as error:
+        raise TypeError("blocks must be a list of ints") from error
+
+
+def _copy_blocks(device: torch.device, pointers, block_bytes, num_buffers: int, num_blocks: int, src: list[int],
+                 dst: list[int]) -> None:
+    if len(src) and (max(max(src), max(dst)) >= num_blocks or min(min(src), min(dst)) < 0):
+        raise ValueError(f"blocks outside [0, {num_blocks})")
+    _call_on(device, "ne_kv_copy_blocks", pointers, block_bytes, num_buffers, num_blocks, _block_list(src),
+             _block_list(dst), len(src), _stream(device))
+
+
 # --------------------------------------------------------------------------- A6
 @dataclass
 class AttentionWorkspace:
@@ -790,6 +843,85 @@ def accept(
         _stream(device),
     )
     return out_tokens, num_out
+
+
+# ---------------------------------------------------------------------- sampling
+def _row_parameter(value, rows: int, dtype: torch.dtype, name: str, device: torch.device):
+    """(device pointer or None, scalar) of a sampling parameter: one value, or one per row."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    _check(value.dtype == dtype and value.dim() == 1 and value.shape[0] == rows and value.is_contiguous(),
+           f"{name} must be one value or contiguous {dtype} [{rows}]")
+    if value.device != device:
+        raise RuntimeError(f"{name} is on {value.device}, the logits on {device}")
+    return value.data_ptr(), 0
+
+
+def sample(
+    logits: torch.Tensor,
+    uniforms: torch.Tensor,
+    temperature: float | torch.Tensor = 1.0,
+    top_k: int | torch.Tensor = 0,
+    top_p: float | torch.Tensor = 1.0,
+    min_p: float | torch.Tensor = 0.0,
+    out: torch.Tensor | None = None,
+    probs: bool | torch.Tensor = False,
+    workspace: torch.Tensor | None = None,
+):
+    """A token per row of ``logits [rows, vocab]`` (bf16, fp16 or fp32) from ``uniforms [rows]``
+    fp32 in [0, 1): int32 ``[rows]``, and with ``probs`` (True, or an fp32 tensor to write) the
+    filtered distribution ``[rows, vocab]`` too, as :func:`accept` takes it for ``draft_probs``.
+
+    Tokens are ordered by logit, equal ones by index.  Kept are the first ``top_k`` (0: all), of
+    those the fewest that reach ``top_p`` of their weight, of those the ones at least ``min_p``
+    times as likely as the first; the token is the first whose running weight exceeds the
+    uniform's share of the kept weight.  ``temperature`` 0 takes the argmax.  Each parameter is
+    one value or a tensor ``[rows]`` (fp32; ``top_k`` int32).  NaN and -inf logits are never
+    drawn; a row without any other gives -1."""
+    device = _require_gpu(logits, uniforms)
+    _check(logits.dim() == 2 and logits.stride(1) == 1 or logits.dim() == 2 and logits.shape[1] == 1,
+           "logits must be [rows, vocab] with contiguous rows")
+    _check(logits.dtype in (torch.bfloat16, torch.float16, torch.float32), "logits must be bf16, fp16 or fp32")
+    rows, vocab = logits.shape
+    _check(uniforms.dtype == torch.float32 and uniforms.dim() == 1 and uniforms.shape[0] == rows
+           and uniforms.is_contiguous(), f"uniforms must be contiguous fp32 [{rows}]")
+    t_ptr, t = _row_parameter(temperature, rows, torch.float32, "temperature", device)
+    k_ptr, k = _row_parameter(top_k, rows, torch.int32, "top_k", device)
+    p_ptr, p = _row_parameter(top_p, rows, torch.float32, "top_p", device)
+    m_ptr, m = _row_parameter(min_p, rows, torch.float32, "min_p", device)
+    if t_ptr is None:
+        _check(0.0 <= t < math.inf, f"temperature must be finite and >= 0, got {t}")
+    _check(p == p and m == m, "top_p and min_p must not be NaN")
+    k = max(0, min(int(k), vocab))
+    if out is None:
+        out = torch.empty((rows,), dtype=torch.int32, device=device)
+    _check(out.dtype == torch.int32 and tuple(out.shape) == (rows,) and out.is_contiguous() and out.device == device,
+           f"out must be contiguous int32 [{rows}] on {device}")
+    table = None
+    if isinstance(probs, torch.Tensor):
+        table = probs
+        _check(table.dtype == torch.float32 and tuple(table.shape) == (rows, vocab) and table.device == device
+               and (table.stride(1) == 1 or vocab == 1), f"probs must be fp32 [{rows}, {vocab}] on {device}")
+    elif probs:
+        table = torch.empty((rows, vocab), dtype=torch.float32, device=device)
+    if rows > 0:
+        code = dtype_code(logits.dtype)
+        nbytes = _native.load().ne_sample_workspace_size(rows, vocab, code)
+        _check(nbytes > 0, f"unsupported sampling shape: {rows} rows of {vocab}")
+        if workspace is None:
+            workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+        _check(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == device,
+               f"workspace must be contiguous uint8 on {device}")
+        _call_on(device, "ne_sample", logits.data_ptr(), code, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                 uniforms.data_ptr(), t_ptr, t, k_ptr, k, p_ptr, p, m_ptr, m, out.data_ptr(),
+                 None if table is None else table.data_ptr(), 0 if table is None or rows < 2 else table.stride(0),
+                 workspace.data_ptr(), workspace.numel(), _stream(device))
+    return out if table is None else (out, table)
+
+
+def sample_workspace_bytes(rows: int, vocab: int, dtype: torch.dtype) -> int:
+    """Bytes of workspace that :func:`sample` needs for these logits (by itself it allocates them)."""
+    return _native.load().ne_sample_workspace_size(rows, vocab, dtype_code(dtype))
 
 
 def prepare_verify_step(

@@ -18,6 +18,8 @@ from collections import OrderedDict, deque
 import numpy as np
 import torch
 
+from nanoengine_amd import kernels
+
 BYTES_PER_MEGABYTE = 1024 * 1024
 
 
@@ -53,6 +55,21 @@ class KVCachePool:
         if is_int8_cache:
             self.key_scales = [torch.zeros(scale_shape, device=device, dtype=dtype) for _ in range(num_layers)]
             self.value_scales = [torch.zeros(scale_shape, device=device, dtype=dtype) for _ in range(num_layers)]
+
+    @property
+    def num_blocks(self) -> int:
+        return self.num_slots // self.block_size
+
+    @property
+    def buffers(self) -> list[torch.Tensor]:
+        """Every layer's keys, values and scales."""
+        scales = (self.key_scales or []) + (self.value_scales or [])
+        return self.key_caches + self.value_caches + scales
+
+    def copy_blocks(self, src: list[int], dst: list[int]) -> None:
+        """Copy block ``src[i]`` to block ``dst[i]`` in every layer (one launch on the current
+        stream; :func:`nanoengine_amd.kernels.copy_kv_blocks`)."""
+        kernels.copy_kv_blocks(self.buffers, self.block_size, src, dst)
 
     def key_scale_2d(self, layer: int) -> torch.Tensor | None:
         return None if self.key_scales is None else self.key_scales[layer].view(self.num_slots + 1, -1)
@@ -185,6 +202,29 @@ class PagedSlotAllocator:
     def free(self, sequence) -> None:
         for block in self._tables.pop(_request_id(sequence), []):
             self._blocks.free(block)
+
+    def fork(self, parent, child, num_tokens: int) -> tuple[list[int], list[int]]:
+        """Give ``child`` (a new request) the first ``num_tokens`` cached tokens of ``parent``:
+        a table of its own whose contents the caller copies before either sequence writes again
+        (``KVCachePool.copy_blocks(*fork)``).  Without reference counts every block is copied.
+        Returns (source blocks, destination blocks)."""
+        pid, cid = _request_id(parent), _request_id(child)
+        table = self._fork_source(pid, cid, num_tokens)
+        if len(table) > self._blocks.num_free_blocks:
+            raise OutOfKVMemoryError(f"no blocks to fork {num_tokens} tokens of {pid}")
+        self._tables[cid] = [self._blocks.allocate() for _ in table]
+        return table, list(self._tables[cid])
+
+    def _fork_source(self, pid: str, cid: str, num_tokens: int) -> list[int]:
+        """The parent's blocks that hold its first ``num_tokens`` tokens."""
+        if pid not in self._tables:
+            raise ValueError(f"{pid} holds no blocks")
+        if cid in self._tables:
+            raise ValueError(f"{cid} already holds blocks")
+        needed = -(-num_tokens // self.block_size)
+        if num_tokens < 0 or needed > len(self._tables[pid]):
+            raise ValueError(f"{pid} holds no {num_tokens} tokens")
+        return self._tables[pid][:needed]
 
     def on_tokens_cached(self, sequence) -> None:
         """Called after a step wrote more of a sequence into the cache (no-op without a prefix cache)."""
@@ -321,6 +361,8 @@ class PrefixCachingSlotAllocator(PagedSlotAllocator):
         # hash of the last registered block's key per request: verified tokens never
         # change, so registration extends the chain instead of rehashing a long history
         self._chain: dict[str, int] = {}
+        # full blocks a request shares with a fork: no longer its own to write
+        self._num_forked: dict[str, int] = {}
         self._hit_tokens = 0
 
     @property
@@ -389,12 +431,37 @@ class PrefixCachingSlotAllocator(PagedSlotAllocator):
         self._chain[rid] = hash(keys[-1])
 
     def first_writable_position(self, sequence) -> int:
-        return self._num_registered.get(_request_id(sequence), 0) * self.block_size
+        rid = _request_id(sequence)
+        return max(self._num_registered.get(rid, 0), self._num_forked.get(rid, 0)) * self.block_size
+
+    def fork(self, parent, child, num_tokens: int) -> tuple[list[int], list[int]]:
+        """As the paged allocator's, but the full blocks are shared: only a last, partly
+        filled block is copied.  Neither sequence may write below the shared blocks' end
+        afterwards (``first_writable_position`` of both)."""
+        pid, cid = _request_id(parent), _request_id(child)
+        table = self._fork_source(pid, cid, num_tokens)
+        full = num_tokens // self.block_size
+        src = table[full:]
+        if len(src) > self._blocks.num_free_blocks:
+            raise OutOfKVMemoryError(f"no blocks to fork {num_tokens} tokens of {pid}")
+        for block in table[:full]:
+            self._blocks.share(block)
+        dst = [self._blocks.allocate() for _ in src]
+        self._tables[cid] = table[:full] + dst
+        for rid in (pid, cid):
+            self._num_forked[rid] = max(self._num_forked.get(rid, 0), full)
+        # the child goes on registering where the parent's registered blocks end, if it shares
+        # them all; otherwise its chain starts over (a block that is registered keeps its entry)
+        if self._num_registered.get(pid, 0) <= full:
+            self._num_registered[cid] = self._num_registered.get(pid, 0)
+            self._chain[cid] = self._chain.get(pid, ROOT_PARENT_HASH)
+        return src, dst
 
     def free(self, sequence) -> None:
         super().free(sequence)
         self._num_registered.pop(_request_id(sequence), None)
         self._chain.pop(_request_id(sequence), None)
+        self._num_forked.pop(_request_id(sequence), None)
 
 
 def slots_for_budget(num_layers: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype,
