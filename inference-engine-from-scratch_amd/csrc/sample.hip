@@ -52,7 +52,7 @@ constexpr int kBinsPerLog2 = 16;
 constexpr int kScanThreads = 512;
 constexpr int kScanWaves = kScanThreads / kWave;
 constexpr int kScanSegs = 2;          // segments per wave and iteration
-constexpr int kPickThreads = 512;
+constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / kWave;
 constexpr int kList = 4096;           // tokens that pick sorts in LDS
 constexpr int kShortTopK = 1024;      // up to here the scan counts tokens and leaves their weights to pick
@@ -191,44 +191,49 @@ __device__ __forceinline__ RowParams row_params(const SampleParams& p, int row) 
 }
 
 // ---- weights ----
-// 2^(j / 16), j = 0..15.  y in sixteenths is split into its floor f (a bin) and r in [0, 1):
+// y in sixteenths is split into its floor f (a bin) and a remainder r in [0, 1):
 // 2^(y - Y) = 2^((f - 16 Y) / 16) * 2^(r / 16); floor and remainder are exact, so a
-// token's bin is the same under every base.
+// token's bin is the same under every base.  Table: 2^(j / 16 + 1 / 32), j = 0..15.
 __constant__ const double kRoots[16] = {
-    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721, 1.241857812073484,
-    1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079408,
-    1.6104903319492543, 1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+    1.0218971486541166, 1.0671404006768237, 1.1143867425958924, 1.1637248587775775, 1.215247359980469,
+    1.2690509571917332, 1.3252366431597413, 1.383909881963832, 1.4451808069770467, 1.5091644275934228,
+    1.5759808451078865, 1.645755478153965, 1.718619298122478, 1.7947090750031072, 1.8741676341103,
+    1.9571441241754002};
 
-// The token's bin below base (0 = largest y) and its remainder; base > y, up to the rounding of
-// values past 2^53 (a temperature next to 0), which the lower bound catches.
-__device__ __forceinline__ int bin_of(double y16, double base, double& rem) {
+// The token's bin below base16 = 16 Y (0 = largest y) and its remainder; base16 > 16 y, up to the
+// rounding of values past 2^53 (a temperature next to 0), which the lower bound catches.
+__device__ __forceinline__ int bin_of(double y16, double base16, double& rem) {
   const double f = floor(y16);
   rem = y16 - f;
   // past kBins - 1: too small to weigh
-  return (int)fmin(fmax(kBinsPerLog2 * base - f, 1.0), (double)(1 << 20)) - 1;
+  return max((int)fmin(base16 - f, (double)(1 << 20)), 1) - 1;
 }
-// 2^(y - Y) for a token of bin b and remainder rem.  2^(rem / 16) by its series around 1 / 32:
-// |ln 2 (rem / 16 - 1 / 32)| < 0.0217, whose seventh power over 7! is 4.5e-16.
-__device__ __forceinline__ double weight_of(int b, double rem, const double* roots) {
+// 2^(y - Y + s) for a token of bin b and remainder rem, above 2^-1000.  2^(rem / 16 - 1 / 32) by its
+// series in t = rem - 1/2, coefficients (ln 2 / 16)^k / k!: |t ln 2 / 16| < 0.0217, whose seventh
+// power over 7! is 4.5e-16.  The exponent is added to the bits.
+__device__ __forceinline__ double weight_of(int b, double rem, int s, const double* roots) {
+  constexpr double L = 0.6931471805599453 / kBinsPerLog2;
   const int q = b + 1;
-  const double z = (rem - 0.5) * (0.6931471805599453 / kBinsPerLog2);
-  double e = 1.0 / 720;
-  e = fma(e, z, 1.0 / 120);
-  e = fma(e, z, 1.0 / 24);
-  e = fma(e, z, 1.0 / 6);
-  e = fma(e, z, 0.5);
-  e = fma(e, z, 1.0);
-  e = fma(e, z, 1.0);
-  return ldexp(e * (1.0218971486541166 /* 2^(1/32) */ * roots[-q & 15]), -((q + 15) >> 4));
+  const double t = rem - 0.5;
+  double e = L * L * L * L * L * L / 720;
+  e = fma(e, t, L * L * L * L * L / 120);
+  e = fma(e, t, L * L * L * L / 24);
+  e = fma(e, t, L * L * L / 6);
+  e = fma(e, t, L * L / 2);
+  e = fma(e, t, L);
+  e = fma(e, t, 1.0);
+  const u64 bits = __builtin_bit_cast(u64, e * roots[-q & 15]);
+  const uint32_t high = (uint32_t)(bits >> 32) + ((uint32_t)(s - ((q + 15) >> 4)) << 20);
+  return __builtin_bit_cast(double, ((u64)high << 32) | (uint32_t)bits);
 }
-// rint(w * 2^S) below 2^52, S <= 51: adding 2^52 leaves the integer in the low mantissa bits
-__device__ __forceinline__ u64 weight_int(double w, int s) {
-  return __builtin_bit_cast(u64, ldexp(w, s) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+// rint of a weight below 2^52: adding 2^52 leaves the integer in the low mantissa bits
+__device__ __forceinline__ u64 weight_int(double w) {
+  return __builtin_bit_cast(u64, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
 }
-__device__ __forceinline__ u64 weight_of_key(uint32_t key, const RowParams& r, double base, int s, const double* roots) {
+__device__ __forceinline__ u64 weight_of_key(uint32_t key, const RowParams& r, double base16, int s, const double* roots) {
   double rem;
-  const int b = bin_of(finite(logit_of(key)) * r.scale, base, rem);
-  return b < kBins ? weight_int(weight_of(b, rem, roots), s) : 0;
+  const int b = bin_of(finite(logit_of(key)) * r.scale, base16, rem);
+  return b < kBins ? weight_int(weight_of(b, rem, s, roots)) : 0;
 }
 
 __device__ __forceinline__ u64 wave_max_u64(u64 v) {
@@ -252,7 +257,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
   __shared__ uint32_t s_count[kBins];
   __shared__ u64 s_weight[kBins];
   __shared__ double s_roots[16];
-  __shared__ uint32_t s_max[2][kScanWaves];
+  __shared__ float s_max[2][kScanWaves];
   __shared__ u64 s_best[kScanWaves];
   __shared__ uint32_t s_tokens;
   const int tid = threadIdx.x;
@@ -272,7 +277,8 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
     s_count[tid + b * kScanThreads] = 0;
     s_weight[tid + b * kScanThreads] = 0;
   }
-  uint32_t best_key = 0, best_index = 0, tokens = 0;
+  float best_logit = -INFINITY;
+  uint32_t best_index = 0, tokens = 0;
   double base = 0;
   bool any = false;  // base is set
   constexpr int kStep = kScanWaves * kScanSegs;
@@ -290,37 +296,36 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
   int turn = 0;
   for (int s0 = seg0; s0 < seg1; s0 += kStep, turn ^= 1) {
     float val[kScanSegs][E];
-    uint32_t most = 0;
+    float most = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kScanSegs; ++j) {
       const int seg = s0 + wave * kScanSegs + j;
       const int v = seg * kWave + lane;
 #pragma unroll
       for (int e = 0; e < E; ++e) val[j][e] = NAN;
-      uint32_t here = 0;
       if (seg < seg1) {
+        float here = -INFINITY;
         if (v < x.vecs) x.values(v, raw[j], whole[j], val[j]);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const uint32_t k = key_of(val[j][e]);
-          if (k > best_key) {  // a lane's tokens come in order of index
-            best_key = k;
+          if (val[j][e] > best_logit) {  // a lane's tokens come in order of index
+            best_logit = val[j][e];
             best_index = v * E + e - x.skew;
           }
-          here = max(here, k);
+          here = fmaxf(here, val[j][e]);  // (not NaN)
         }
-        here = wave_max_u32(here);
-        if (lane == 0) p.seg_max[(int64_t)row * p.segs + seg] = here;
+        here = wave_max(here);
+        if (lane == 0) p.seg_max[(int64_t)row * p.segs + seg] = key_of(here);
+        most = fmaxf(most, here);
       }
-      most = max(most, here);
     }
     if (s0 + kStep < seg1) load(s0 + kStep);
     if (lane == 0) s_max[turn][wave] = most;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kScanWaves; ++w) most = max(most, s_max[turn][w]);
-    if (r.greedy || most == 0) continue;
-    const double top = floor(finite(logit_of(most)) * r.scale / kBinsPerLog2) + 1.0;
+    for (int w = 0; w < kScanWaves; ++w) most = fmaxf(most, s_max[turn][w]);
+    if (r.greedy || !(most > -INFINITY)) continue;
+    const double top = floor(finite(most) * r.scale / kBinsPerLog2) + 1.0;
     if (!any) {
       base = top;
       any = true;
@@ -343,23 +348,28 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
       __syncthreads();
       base = top;
     }
+    const double base16 = kBinsPerLog2 * base;
 #pragma unroll
     for (int j = 0; j < kScanSegs; ++j) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (key_of(val[j][e]) == 0) continue;
-        ++tokens;
+        const bool is = val[j][e] > -INFINITY;
+        tokens += is;
         double rem;
-        const int b = bin_of(finite(val[j][e]) * r.scale, base, rem);
-        if (b >= kBins - 1) continue;  // the last bin is what the others leave
-        atomicAdd(&s_count[b], 1u);
-        if (r.weigh) atomicAdd(&s_weight[b], weight_int(weight_of(b, rem, s_roots), p.weight_exp));
+        const int b = bin_of(finite(val[j][e]) * r.scale, base16, rem);
+        if (is && b < kBins - 1) {  // the last bin is what the others leave
+          atomicAdd(&s_count[b], 1u);
+          if (r.weigh) atomicAdd(&s_weight[b], weight_int(weight_of(b, rem, p.weight_exp, s_roots)));
+        }
       }
     }
   }
+  const uint32_t best_key = key_of(best_logit);
   const u64 best = wave_max_u64(best_key ? order_word(best_key, best_index) : 0);
   if (lane == 0) s_best[wave] = best;
-  if (tokens) atomicAdd(&s_tokens, tokens);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) tokens += __shfl_xor((int)tokens, o);
+  if (lane == 0 && tokens) atomicAdd(&s_tokens, tokens);
   __syncthreads();
   const int64_t at = (int64_t)row * p.chunks + chunk;
   if (tid == 0) {
@@ -390,274 +400,15 @@ struct PickShared {
       u64 sum[kList];  // weight of entries 0 .. i
     } list;
     struct {
-      uint32_t count[kSub];
+      uint32_t count[kSub];  // tokens in buckets 0 .. c
       u64 weight[kSub];
     } sub;
+    int down[2 * kNumCu];  // each chunk's base below the row's
   };
   double roots[16];
   u64 part[2 * kPickWaves];
   u64 red[4];
   uint32_t n;
-};
-
-// A border in the row's order: the token at it, and the tokens and weight up to it, itself included.
-struct Border {
-  u64 word;
-  u64 tokens;
-  u64 weight;
-};
-
-template <int DT>
-struct Pick {
-  const SampleParams& p;
-  const RowParams& r;
-  const Row<DT> x;
-  const uint32_t* seg_max;
-  PickShared& s;
-  double base;
-  int tid, wave, lane;
-
-  __device__ Pick(const SampleParams& p_, const RowParams& r_, int row, PickShared& s_)
-      : p(p_), r(r_), x(p_, row), seg_max(p_.seg_max + (int64_t)row * p_.segs), s(s_), base(0) {
-    tid = threadIdx.x;
-    wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    lane = tid % kWave;
-  }
-
-  // fn(key, index) for every token of the row with key >= least, in no order; segments
-  // without one are not read.
-  template <typename F>
-  __device__ __forceinline__ void each(uint32_t least, F fn) const {
-    constexpr int E = kVec<DT>;
-    constexpr int kAhead = 4;
-    const int segs = (x.vecs + kWave - 1) / kWave;
-    for (int s0 = wave * kAhead; s0 < segs; s0 += kPickWaves * kAhead) {
-      u32x4 raw[kAhead];
-      bool whole[kAhead], want[kAhead];
-      uint32_t most[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) most[j] = s0 + j < segs ? seg_max[s0 + j] : 0;
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        want[j] = most[j] != 0 && most[j] >= least;
-        whole[j] = false;
-        if (want[j]) raw[j] = x.raw((s0 + j) * kWave + lane, whole[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int v = (s0 + j) * kWave + lane;
-        if (!want[j] || v >= x.vecs) continue;
-        float val[E];
-        x.values(v, raw[j], whole[j], val);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t k = key_of(val[e]);
-          if (k != 0 && k >= least) fn(k, (uint32_t)(v * E + e - x.skew));
-        }
-      }
-    }
-  }
-
-  __device__ __forceinline__ int bin(uint32_t key) const {
-    double rem;
-    return min(bin_of(finite(logit_of(key)) * r.scale, base, rem), kBins - 1);
-  }
-  __device__ __forceinline__ u64 weight(uint32_t key) const { return weight_of_key(key, r, base, p.weight_exp, s.roots); }
-
-  // Inclusive sums over the threads, in thread order, of two values at once.
-  __device__ void block_scan(u64& a, u64& b) {
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const u64 y = __shfl_up(a, o), z = __shfl_up(b, o);
-      if (lane >= o) {
-        a += y;
-        b += z;
-      }
-    }
-    __syncthreads();
-    if (lane == kWave - 1) {
-      s.part[wave] = a;
-      s.part[kPickWaves + wave] = b;
-    }
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-      a += s.part[w];
-      b += s.part[kPickWaves + w];
-    }
-  }
-
-  // First bin (of `bins` inclusive sums) whose sum reaches target; the last if none does.
-  template <typename T>
-  __device__ static int first_reaching(const T* sums, int bins, u64 target) {
-    int lo = 0, hi = bins - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if ((u64)sums[mid] >= target)
-        hi = mid;
-      else
-        lo = mid + 1;
-    }
-    return lo;
-  }
-
-  // Tokens with key in [klo, khi] and bin in [blo, bhi], in order of the row, with running weights.
-  // The caller knows that at most kList qualify.
-  __device__ int gather(uint32_t klo, uint32_t khi, int blo, int bhi, uint32_t ilo = 0, uint32_t ihi = 0xFFFFFFFFu) {
-    __syncthreads();
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    each(klo, [&](uint32_t k, uint32_t i) {
-      if (k > khi || i < ilo || i > ihi) return;
-      const int b = bin(k);
-      if (b < blo || b > bhi) return;
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < kList) s.list.word[at] = order_word(k, i);
-    });
-    __syncthreads();
-    const int n = min((int)s.n, kList);
-    int size = kWave;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += kPickThreads) s.list.word[i] = 0;
-    __syncthreads();
-    // bitonic, largest first
-    for (int k = 2; k <= size; k <<= 1) {
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        for (int t = tid; t < size / 2; t += kPickThreads) {
-          const int a = 2 * t - (t & (j - 1));
-          const u64 u = s.list.word[a], v = s.list.word[a + j];
-          if (((a & k) == 0) ? u < v : u > v) {
-            s.list.word[a] = v;
-            s.list.word[a + j] = u;
-          }
-        }
-        __syncthreads();
-      }
-    }
-    // running weights: each thread a run of consecutive entries
-    const int per = (n + kPickThreads - 1) / kPickThreads;
-    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
-    u64 mine = 0, none = 0;
-    for (int i = i0; i < i1; ++i) {
-      mine += weight(word_key(s.list.word[i]));
-      s.list.sum[i] = mine;
-    }
-    u64 incl = mine;
-    block_scan(incl, none);
-    for (int i = i0; i < i1; ++i) s.list.sum[i] += incl - mine;
-    __syncthreads();
-    return n;
-  }
-
-  // The border in bin b at which the running count (by_count) or weight first reaches
-  // target; before: what lies in front of the bin.
-  __device__ Border border(int b, bool by_count, u64 target) {
-    u64 count0 = b > 0 ? s.count[b - 1] : 0, weight0 = b > 0 ? s.weight[b - 1] : 0;
-    u64 n = s.count[b] - count0;
-    uint32_t klo = 1, khi = 0xFFFFFFFFu;
-    bool first = true;
-    while (n > (u64)kList) {  // too many to sort: narrow by key
-      if (first) {  // the bin's own smallest and largest key
-        u64 lo = 0xFFFFFFFFu, hi = 0;
-        each(1, [&](uint32_t k, uint32_t) {
-          if (bin(k) != b) return;
-          lo = k < lo ? k : lo;
-          hi = k > hi ? k : hi;
-        });
-        lo = 0xFFFFFFFFu - wave_max_u64(0xFFFFFFFFu - lo);
-        hi = wave_max_u64(hi);
-        __syncthreads();
-        if (lane == 0) {
-          s.part[wave] = lo;
-          s.part[kPickWaves + wave] = hi;
-        }
-        __syncthreads();
-        for (int w = 0; w < kPickWaves; ++w) {
-          lo = s.part[w] < lo ? s.part[w] : lo;
-          hi = s.part[kPickWaves + w] > hi ? s.part[kPickWaves + w] : hi;
-        }
-        klo = (uint32_t)lo;
-        khi = (uint32_t)hi;
-        first = false;
-      }
-      if (klo >= khi) break;
-      int shift = 0;
-      while (((khi - klo) >> shift) >= kSub) ++shift;
-      narrow([&](uint32_t k, uint32_t) { return k >= klo && k <= khi && bin(k) == b ? (int)((khi - k) >> shift) : -1; }, klo);
-      // (the histogram's sums may differ from these tokens' in the last place: a weight past them is their end)
-      const u64 most = s.sub.weight[kSub - 1], want = target - weight0;
-      const int c = by_count ? first_reaching(s.sub.count, kSub, target - count0)
-                             : first_reaching(s.sub.weight, kSub, want < most ? want : most);
-      const u64 had = c > 0 ? s.sub.count[c - 1] : 0;
-      n = s.sub.count[c] - had;
-      count0 += had;
-      weight0 += c > 0 ? s.sub.weight[c - 1] : 0;
-      const uint32_t top = khi - ((uint32_t)c << shift);
-      klo = max(klo, top - ((1u << shift) - 1u));
-      khi = top;
-      __syncthreads();
-    }
-    uint32_t ilo = 0, ihi = 0xFFFFFFFFu;
-    if (n > (u64)kList) {  // one logit: find the token by its index
-      const u64 w = weight(klo);
-      u64 rank = by_count ? target - count0 - 1 : (w ? (target - weight0 + w - 1) / w - 1 : 0);
-      if (rank >= n) rank = n - 1;
-      int shift = 0;
-      while (((uint32_t)(p.vocab - 1) >> shift) >= kSub) ++shift;
-      narrow([&](uint32_t k, uint32_t i) { return k == klo ? (int)(i >> shift) : -1; }, klo);
-      const int c = first_reaching(s.sub.count, kSub, rank + 1);
-      const u64 had = c > 0 ? s.sub.count[c - 1] : 0;
-      count0 += had;
-      weight0 += had * w;
-      ilo = (uint32_t)c << shift;
-      ihi = ilo + (1u << shift) - 1u;
-      if (!by_count) target = weight0 + (rank - had + 1) * w;  // the token of that rank, whatever w
-      else
-        target = count0 + (rank - had) + 1;
-      __syncthreads();
-    }
-    const int m = gather(klo, khi, b, b, ilo, ihi);
-    const u64 want = by_count ? target - count0 : target - weight0;
-    int i = by_count ? (int)(want < (u64)m ? want : (u64)m) - 1 : first_reaching(s.list.sum, m, want);
-    i = max(i, 0);
-    const Border out = {s.list.word[i], count0 + i + 1, weight0 + s.list.sum[i]};
-    __syncthreads();
-    return out;
-  }
-
-  // Inclusive counts and weights of the tokens by bucket (which(key, index), -1: none).
-  template <typename F>
-  __device__ void narrow(F which, uint32_t least) {
-    __syncthreads();
-    for (int i = tid; i < kSub; i += kPickThreads) {
-      s.sub.count[i] = 0;
-      s.sub.weight[i] = 0;
-    }
-    __syncthreads();
-    each(least, [&](uint32_t k, uint32_t i) {
-      const int c = which(k, i);
-      if (c < 0) return;
-      atomicAdd(&s.sub.count[c], 1u);
-      atomicAdd(&s.sub.weight[c], weight(k));
-    });
-    __syncthreads();
-    constexpr int per = kSub / kPickThreads;
-    u64 a = 0, b = 0;
-    for (int i = 0; i < per; ++i) {
-      a += s.sub.count[tid * per + i];
-      b += s.sub.weight[tid * per + i];
-    }
-    u64 sa = a, sb = b;
-    block_scan(sa, sb);
-    sa -= a;
-    sb -= b;
-    for (int i = 0; i < per; ++i) {
-      sa += s.sub.count[tid * per + i];
-      sb += s.sub.weight[tid * per + i];
-      s.sub.count[tid * per + i] = (uint32_t)sa;
-      s.sub.weight[tid * per + i] = sb;
-    }
-    __syncthreads();
-  }
 };
 
 // f * sum rounded down, or up; exact (equal weights make borders that a rounded product would
@@ -690,24 +441,91 @@ __device__ __forceinline__ u64 reach_at(float top_p, u64 sum) {
   return i > 1 ? i : 1;
 }
 
+// The work-group's state is the same in every lane: kept in scalar registers.
+__device__ __forceinline__ uint32_t uni(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ u64 uni(u64 v) { return ((u64)uni((uint32_t)(v >> 32)) << 32) | uni((uint32_t)v); }
+__device__ __forceinline__ double uni(double v) { return __builtin_bit_cast(double, uni(__builtin_bit_cast(u64, v))); }
+
+// First of n inclusive sums that reaches target; the last if none does.
+template <typename T>
+__device__ __forceinline__ int first_reaching(const T* sums, int n, u64 target) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if ((u64)sums[mid] >= target)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return uni(lo);
+}
+
+// Sums of two values over the threads up to each, in thread order.
+__device__ __forceinline__ void block_scan(PickShared& s, u64& a, u64& b) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const u64 y = __shfl_up(a, o), z = __shfl_up(b, o);
+    if (lane >= o) {
+      a += y;
+      b += z;
+    }
+  }
+  __syncthreads();
+  if (lane == kWave - 1) {
+    s.part[wave] = a;
+    s.part[kPickWaves + wave] = b;
+  }
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) {
+    a += s.part[w];
+    b += s.part[kPickWaves + w];
+  }
+}
+
+// What a pass over the row does with the tokens of bins blo..bhi, keys klo..khi and indexes ilo..ihi.
+enum Act {
+  kGather,    // the sorted list, with running weights (the caller knows that it fits)
+  kKeyRange,  // red[0..1]: smallest and largest key
+  kByKey,     // buckets of (khi - key) >> shift
+  kByIndex,   // buckets of index >> shift
+  kWeigh,     // the bins' weights
+  kAbove,     // red[0..2]: tokens, weight and smallest order word of those with y >= y_min
+};
+// What the pass is for: all tokens that can be kept, or a border.
+enum Step { kAll, kTopK, kTopP, kMinP, kBeforeMinP, kDraw, kDone };
+
 template <int DT>
 __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams p) {
+  constexpr int E = kVec<DT>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   PickShared& s = *(PickShared*)smem;
   const int row = blockIdx.x;
   const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lane = tid % kWave;
   const RowParams r = row_params(p, row);
-  Pick<DT> k(p, r, row, s);
+  const Row<DT> x(p, row);
+  const int segs = (x.vecs + kWave - 1) / kWave;
+  const uint32_t* seg_max = p.seg_max + (int64_t)row * p.segs;
   const ChunkHead* heads = p.heads + (int64_t)row * p.chunks;
-  u64 best = 0;
+  u64 best = 0, tokens = 0;
   double base = -INFINITY;
-  u64 tokens = 0;
-  for (int c = 0; c < p.chunks; ++c) {
+  for (int c = lane; c < p.chunks; c += kWave) {
     const ChunkHead h = heads[c];
     best = h.best > best ? h.best : best;
     if (h.tokens) base = fmax(base, h.base);
     tokens += h.tokens;
   }
+  best = uni(wave_max_u64(best));
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    base = fmax(base, __shfl_xor(base, o));
+    tokens += __shfl_xor(tokens, o);
+  }
+  base = uni(base);
+  tokens = uni(tokens);
   RowResult out;
   out.last = best;
   out.base = base;
@@ -720,173 +538,412 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
     }
     return;
   }
-  k.base = base;
+  const double base16 = kBinsPerLog2 * base;
   if (tid < 16) s.roots[tid] = kRoots[tid];
   // ---- the row's histogram, as sums from the first bin on ----
-  constexpr int per = kBins / kPickThreads;
-  u64 count[per], weight[per], ca = 0, wa = 0;
-#pragma unroll
-  for (int i = 0; i < per; ++i) count[i] = weight[i] = 0;
-  for (int c = 0; c < p.chunks; ++c) {
-    if (heads[c].tokens == 0) continue;
-    const int down = (int)fmin(base - heads[c].base, 64.0);
-    const int64_t at = ((int64_t)row * p.chunks + c) * kBins;
-#pragma unroll
-    for (int i = 0; i < per; ++i) {
-      const int from = tid * per + i - kBinsPerLog2 * down;
-      if (from < 0) continue;
-      count[i] += p.counts[at + from];
-      if (r.weigh) weight[i] += down < 64 ? p.weights[at + from] >> down : 0;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < per; ++i) {
-    ca += count[i];
-    wa += weight[i];
-  }
+  for (int c = tid; c < p.chunks; c += kPickThreads)  // (at most 2 kNumCu of them)
+    s.down[c] = heads[c].tokens ? (int)fmin(base - heads[c].base, 64.0) : 64;
+  __syncthreads();
+  static_assert(kBins == kPickThreads, "a bin per thread");
   {
-    u64 cs = ca, ws = wa;
-    k.block_scan(cs, ws);
-    cs -= ca;
-    ws -= wa;
-#pragma unroll
-    for (int i = 0; i < per; ++i) {
-      cs += count[i];
-      ws += weight[i];
-      s.count[tid * per + i] = tid * per + i == kBins - 1 ? (uint32_t)tokens : (uint32_t)cs;
-      s.weight[tid * per + i] = ws;
+    u64 count = 0, weight = 0;
+    const uint32_t* counts = p.counts + (int64_t)row * p.chunks * kBins;
+    const u64* weights = p.weights + (int64_t)row * p.chunks * kBins;
+#pragma unroll 4
+    for (int c = 0; c < p.chunks; ++c) {
+      const int down = s.down[c];
+      const int from = max(tid - kBinsPerLog2 * down, 0);
+      const bool has = tid >= kBinsPerLog2 * down && down < 64;
+      const uint32_t n = counts[(int64_t)c * kBins + from];
+      const u64 w = r.weigh ? weights[(int64_t)c * kBins + from] : 0;
+      count += has ? n : 0;
+      weight += has ? w >> down : 0;
     }
+    block_scan(s, count, weight);
+    s.count[tid] = tid == kBins - 1 ? (uint32_t)tokens : (uint32_t)count;
+    s.weight[tid] = weight;
   }
   __syncthreads();
   const u64 top_k = r.top_k && (u64)r.top_k < tokens ? r.top_k : tokens;
   const float u = p.uniforms[row];
-  const bool cut_p = r.top_p < 1.f;
-  const double y_best = finite(logit_of(word_key(best))) * r.scale;
-  const double y_min = y_best + kBinsPerLog2 * r.log2_min_p;  // min-p's border in sixteenths of log2
+  const bool cut_p = r.top_p < 1.f, cut_m = r.log2_min_p != -INFINITY;
+  // min-p's border in sixteenths of log2, and its bin
+  const double y_min = uni(finite(logit_of(word_key(best))) * r.scale + kBinsPerLog2 * r.log2_min_p);
   double rem;
-  const int bin_m = r.log2_min_p == -INFINITY ? kBins - 1 : min(bin_of(y_min, base, rem), kBins - 1);
-  // ---- the last bin with a kept token, from above ----
-  const int bin_k = k.first_reaching(s.count, kBins, top_k);
-  int last = bin_k;
+  const int bin_m = uni(cut_m ? min(bin_of(y_min, base16, rem), kBins - 1) : kBins - 1);
+  const int bin_k = first_reaching(s.count, kBins, top_k);
   bool weighed = r.weigh;
-  if (!weighed && s.count[bin_k] > kList) {
-    // a short top-k among many nearly equal logits: the row's weights after all
-    weighed = true;
-    u64 w[per] = {};
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kPickThreads) s.weight[i] = 0;
-    __syncthreads();
-    k.each(1, [&](uint32_t key, uint32_t) {
-      const int b = k.bin(key);
-      if (b < kBins - 1) atomicAdd(&s.weight[b], k.weight(key));
-    });
-    __syncthreads();
-    u64 a = 0, none = 0;
-    for (int i = 0; i < per; ++i) a += w[i] = s.weight[tid * per + i];
-    u64 sum = a;
-    k.block_scan(sum, none);
-    sum -= a;
-    for (int i = 0; i < per; ++i) s.weight[tid * per + i] = sum += w[i];
-    __syncthreads();
-  }
+
+  // ---- passes over the row, each for one step ----
+  Step step = kAll;
+  Act act = kGather;
+  int blo = 0, bhi = bin_k, shift = 0;  // the pass's tokens
+  uint32_t klo = 1, khi = 0xFFFFFFFFu, ilo = 0, ihi = 0xFFFFFFFFu;
+  bool by_count = false;  // the border: where the running count, or weight, first reaches target
+  u64 target = 0, count0 = 0, weight0 = 0, left = 0;  // what lies before the pass's tokens, and how many they are
+  u64 end_word = 1, end_weight = 0;  // the last kept token (1: every token), and the kept weight
+  u64 border_word = 0, border_weight = 0;
+  u64 reach = ~0ull;  // top-p's share of the first top_k's weight
+
+  auto start_border = [&](Step what, bool count, u64 to) {
+    step = what;
+    by_count = count;
+    target = to;
+    blo = bhi = count ? first_reaching(s.count, kBins, to) : first_reaching(s.weight, kBins, to);
+    count0 = uni(bhi > 0 ? (u64)s.count[bhi - 1] : 0);
+    weight0 = uni(bhi > 0 ? s.weight[bhi - 1] : 0);
+    left = uni((u64)s.count[bhi]) - count0;
+    klo = 1;
+    khi = ihi = 0xFFFFFFFFu;
+    ilo = 0;
+    act = left > (u64)kList ? kKeyRange : kGather;
+  };
+  auto start_all = [&]() {
+    step = kAll;
+    act = kGather;
+    blo = 0;
+    klo = 1;
+    khi = ihi = 0xFFFFFFFFu;
+    ilo = 0;
+    bhi = min(bin_k, bin_m);
+    if (cut_p) bhi = min(bhi, first_reaching(s.weight, kBins, reach != ~0ull ? reach : reach_at(r.top_p, uni(s.weight[bin_k]))));
+  };
+  // the border of top_k is known (or there is none): top-p's, min-p's, or the draw
+  auto after_top_k = [&]() {
+    if (cut_p) {
+      reach = reach_at(r.top_p, end_weight);
+      start_border(kTopP, false, reach);
+    } else {
+      step = kTopP;
+    }
+  };
+  auto start_draw = [&]() { start_border(kDraw, false, draw_at(u, end_weight) + 1); };
+  auto after_top_p = [&]() {
+    if (cut_m && uni(bin_m > 0 ? s.weight[bin_m - 1] : 0) < end_weight) {
+      step = kMinP;
+      act = kAbove;
+      blo = bhi = bin_m;
+      klo = 1;
+      khi = ihi = 0xFFFFFFFFu;
+      ilo = 0;
+    } else {
+      start_draw();
+    }
+  };
+  auto first_wide = [&]() {  // a wide nucleus: each border in its own bin
+    end_weight = uni(s.weight[kBins - 1]);
+    if (top_k < tokens) {
+      start_border(kTopK, true, top_k);
+    } else {
+      after_top_k();
+      if (!cut_p) after_top_p();
+    }
+  };
+  auto first = [&]() {
+    start_all();
+    if (uni(s.count[bhi]) > (uint32_t)kList) first_wide();
+  };
   if (weighed) {
-    last = min(last, bin_m);
-    if (cut_p) last = min(last, k.first_reaching(s.weight, kBins, reach_at(r.top_p, s.weight[bin_k])));
+    first();
+  } else if (uni(s.count[bin_k]) > (uint32_t)kList) {  // a short top-k among many nearly equal logits
+    act = kWeigh;
+    bhi = kBins - 2;
   }
-  if (s.count[last] <= kList) {
-    // ---- every token that can be kept, in one sorted list ----
-    const int n = k.gather(1, 0xFFFFFFFFu, 0, last);
-    // top-p's border is a share of the weight of the first top_k: of the list's, or, where the list
-    // ends before them, of the histogram's
-    u64 of = 0;
-    const int nk = (int)(top_k < (u64)n ? top_k : (u64)n);
-    if ((u64)nk == top_k) {
-      of = s.list.sum[nk - 1];
-    } else if (cut_p) {
-      of = top_k == tokens ? s.weight[kBins - 1] : s.weight[bin_k];
-      if (top_k != tokens) {
-        const Border e = k.border(bin_k, true, top_k);
-        of = e.weight;
-        k.gather(1, 0xFFFFFFFFu, 0, last);
+
+  while (true) {
+    // ---- clear ----
+    __syncthreads();
+    if (act == kGather) {
+      if (tid == 0) s.n = 0;
+    } else if (act == kByKey || act == kByIndex) {
+      for (int i = tid; i < kSub; i += kPickThreads) {
+        s.sub.count[i] = 0;
+        s.sub.weight[i] = 0;
+      }
+    } else if (act == kWeigh) {
+      s.weight[tid] = 0;
+    }
+    __syncthreads();
+    // ---- the row's segments whose largest key reaches the pass's tokens, four at a time ----
+    u64 acc0 = act == kKeyRange ? 0xFFFFFFFFu : 0, acc1 = 0, acc2 = ~0ull;
+    for (int s0 = 0; s0 < segs; s0 += kPickThreads) {
+      const int mine = s0 + lane * kPickWaves + wave;
+      const uint32_t top = mine < segs ? seg_max[mine] : 0;
+      u64 want = __ballot(top != 0 && top >= klo && min(bin_of(finite(logit_of(top)) * r.scale, base16, rem), kBins - 1) <= bhi);
+      while (want) {
+        constexpr int kAhead = 4;
+        u32x4 raw[kAhead];
+        bool whole[kAhead];
+        int v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          v[j] = x.vecs;
+          whole[j] = false;
+          if (want) {
+            v[j] = (s0 + (int)__builtin_ctzll(want) * kPickWaves + wave) * kWave + lane;
+            want &= want - 1;
+            raw[j] = x.raw(v[j], whole[j]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          if (v[j] >= x.vecs) continue;
+          float val[E];
+          x.values(v[j], raw[j], whole[j], val);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const uint32_t k = key_of(val[e]);
+            const uint32_t i = (uint32_t)(v[j] * E + e - x.skew);
+            if (k < klo || k > khi || i < ilo || i > ihi) continue;
+            const double y16 = finite(val[e]) * r.scale;
+            const int b = bin_of(y16, base16, rem);
+            if (min(b, kBins - 1) < blo || min(b, kBins - 1) > bhi) continue;
+            if (act == kGather) {
+              const uint32_t at = atomicAdd(&s.n, 1u);
+              if (at < (uint32_t)kList) s.list.word[at] = order_word(k, i);
+              continue;
+            }
+            const u64 w = b < kBins ? weight_int(weight_of(b, rem, p.weight_exp, s.roots)) : 0;
+            if (act == kKeyRange) {
+              acc0 = k < acc0 ? k : acc0;
+              acc1 = k > acc1 ? k : acc1;
+            } else if (act == kWeigh) {
+              atomicAdd(&s.weight[b], w);
+            } else if (act == kAbove) {
+              if (y16 >= y_min) {
+                const u64 o = order_word(k, i);
+                ++acc0;
+                acc1 += w;
+                acc2 = o < acc2 ? o : acc2;
+              }
+            } else {
+              const uint32_t c = act == kByKey ? (khi - k) >> shift : i >> shift;
+              atomicAdd(&s.sub.count[c], 1u);
+              atomicAdd(&s.sub.weight[c], w);
+            }
+          }
+        }
       }
     }
-    const u64 reach = cut_p ? reach_at(r.top_p, of) : ~0ull;
-    u64 kept_p = 0, kept_m = 0;
-    for (int i = tid; i < nk; i += kPickThreads) {
-      const uint32_t key = word_key(s.list.word[i]);
-      kept_p += i == 0 || s.list.sum[i - 1] < reach;
-      kept_m += finite(logit_of(key)) * r.scale >= y_min;
-    }
-    k.block_scan(kept_p, kept_m);
-    if (tid == kPickThreads - 1) {
-      s.red[0] = kept_p;
-      s.red[1] = kept_m;
-    }
     __syncthreads();
-    int kept = (int)min(s.red[0], s.red[1]);
-    kept = max(1, min(kept, nk));
-    const u64 sum = s.list.sum[kept - 1];
-    const int at = k.first_reaching(s.list.sum, kept, draw_at(u, sum) + 1);
-    if (tid == 0) {
-      p.tokens[row] = (int32_t)word_index(s.list.word[at]);
-      out.last = s.list.word[kept - 1];
-      out.sum = ldexp((double)sum, -p.weight_exp);
-      p.results[row] = out;
+    // ---- what the pass found ----
+    if (act == kWeigh) {
+      u64 w = s.weight[tid], none = 0;
+      block_scan(s, w, none);
+      s.weight[tid] = w;
+      __syncthreads();
+      weighed = true;
+      first();
+      continue;
     }
-    return;
-  }
-  // ---- a wide nucleus: each border in its own bin ----
-  Border end;
-  end.word = 1;  // every token
-  end.weight = s.weight[kBins - 1];
-  if (top_k < tokens) end = k.border(bin_k, true, top_k);
-  if (cut_p) {
-    const u64 reach = reach_at(r.top_p, end.weight);
-    const int b = k.first_reaching(s.weight, kBins, reach);
-    const Border e = k.border(b, false, reach);
-    if (e.word > end.word) end = e;
-  }
-  if (r.log2_min_p != -INFINITY && (bin_m > 0 ? s.weight[bin_m - 1] : 0) < end.weight) {
-    // tokens of bin_m on the kept side of min-p's border, and the smallest of their order words
-    u64 n = 0, w = 0, lo = ~0ull;
-    k.each(1, [&](uint32_t key, uint32_t i) {
-      if (k.bin(key) != bin_m || !(finite(logit_of(key)) * r.scale >= y_min)) return;
-      ++n;
-      w += k.weight(key);
-      const u64 o = order_word(key, i);
-      lo = o < lo ? o : lo;
-    });
-    lo = ~wave_max_u64(~lo);
-    k.block_scan(n, w);
-    if (tid == kPickThreads - 1) {
-      s.red[0] = n;
-      s.red[1] = w;
-    }
-    __syncthreads();
-    if (k.lane == 0) s.part[k.wave] = lo;
-    __syncthreads();
-    for (int i = 0; i < kPickWaves; ++i) lo = s.part[i] < lo ? s.part[i] : lo;
-    const u64 sum = (bin_m > 0 ? s.weight[bin_m - 1] : 0) + s.red[1];
-    __syncthreads();
-    if (s.red[0] == 0) {
-      // the border lies above every token of its bin: the last kept token is the last one before the bin
-      if (bin_m > 0 && s.count[bin_m - 1] > 0) {
-        const u64 before = s.count[bin_m - 1];
-        const Border e = k.border(k.first_reaching(s.count, kBins, before), true, before);
-        if (e.word > end.word) end = e;
+    if (act == kKeyRange || act == kAbove) {
+      if (act == kKeyRange) {
+        acc0 = ~wave_max_u64(~acc0);
+        acc1 = wave_max_u64(acc1);
+      } else {
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+          acc0 += __shfl_xor(acc0, o);
+          acc1 += __shfl_xor(acc1, o);
+        }
+        acc2 = ~wave_max_u64(~acc2);
       }
-    } else if (lo > end.word) {
-      end.word = lo;
-      end.weight = sum;
+      u64* all = s.list.sum;  // [3][waves], the list is not in use
+      if (lane == 0) {
+        all[wave] = acc0;
+        all[kPickWaves + wave] = acc1;
+        all[2 * kPickWaves + wave] = acc2;
+      }
+      __syncthreads();
+      for (int w = 0; w < kPickWaves; ++w) {
+        if (w == wave) continue;
+        const u64 a = all[w], b = all[kPickWaves + w], c = all[2 * kPickWaves + w];
+        if (act == kKeyRange) {
+          acc0 = a < acc0 ? a : acc0;
+          acc1 = b > acc1 ? b : acc1;
+        } else {
+          acc0 += a;
+          acc1 += b;
+          acc2 = c < acc2 ? c : acc2;
+        }
+      }
+    }
+    if (act == kAbove) {
+      const u64 before = uni(bin_m > 0 ? (u64)s.count[bin_m - 1] : 0);
+      acc0 = uni(acc0);
+      acc1 = uni(acc1);
+      acc2 = uni(acc2);
+      if (acc0 > 0) {
+        if (acc2 > end_word) {
+          end_word = acc2;
+          end_weight = uni(bin_m > 0 ? s.weight[bin_m - 1] : 0) + acc1;
+        }
+        start_draw();
+      } else if (before > 0) {  // no token of its bin: the last kept one is the last before the bin
+        start_border(kBeforeMinP, true, before);
+      } else {
+        start_draw();
+      }
+      continue;
+    }
+    if (act == kKeyRange) {
+      klo = uni((uint32_t)acc0);
+      khi = uni((uint32_t)acc1);
+    } else if (act == kByKey || act == kByIndex) {
+      static_assert(kSub == 2 * kPickThreads, "two buckets per thread");
+      const u64 a = s.sub.count[2 * tid], b = s.sub.weight[2 * tid];
+      u64 sa = a + s.sub.count[2 * tid + 1], sb = b + s.sub.weight[2 * tid + 1];
+      const u64 ta = sa, tb = sb;
+      block_scan(s, sa, sb);
+      s.sub.count[2 * tid] = (uint32_t)(sa - ta + a);
+      s.sub.weight[2 * tid] = sb - tb + b;
+      s.sub.count[2 * tid + 1] = (uint32_t)sa;
+      s.sub.weight[2 * tid + 1] = sb;
+      __syncthreads();
+      const u64 most = uni(s.sub.weight[kSub - 1]);
+      // (the histogram's sums may differ from these tokens' in the last place: a weight past them is their end)
+      const int c = by_count || act == kByIndex ? first_reaching(s.sub.count, kSub, target - count0)
+                                                : first_reaching(s.sub.weight, kSub, min(target - weight0, most));
+      const u64 had = uni(c > 0 ? (u64)s.sub.count[c - 1] : 0);
+      left = uni((u64)s.sub.count[c]) - had;
+      count0 += had;
+      weight0 += uni(c > 0 ? s.sub.weight[c - 1] : 0);
+      if (act == kByKey) {
+        const uint32_t top = khi - ((uint32_t)c << shift);
+        klo = max(klo, top - ((1u << shift) - 1u));
+        khi = top;
+      } else {
+        ilo = (uint32_t)c << shift;
+        ihi = ilo + (1u << shift) - 1u;
+      }
+    }
+    if (act != kGather) {  // narrower, until the tokens fit the list
+      if (left <= (u64)kList) {
+        act = kGather;
+      } else if (klo < khi) {
+        act = kByKey;
+        shift = 0;
+        while (((khi - klo) >> shift) >= (uint32_t)kSub) ++shift;
+      } else {  // one logit: from here on a rank decides, and the index finds it
+        if (!by_count) {
+          const u64 w = uni(weight_of_key(klo, r, base16, p.weight_exp, s.roots));
+          u64 rank = w ? (target - weight0 + w - 1) / w : 1;
+          rank = min(max(rank, (u64)1), left);
+          by_count = true;
+          target = count0 + rank;
+        }
+        act = kByIndex;
+        shift = 0;
+        while (((uint32_t)(p.vocab - 1) >> shift) >= (uint32_t)kSub) ++shift;
+      }
+      continue;
+    }
+    // ---- sort the list, largest first ----
+    const int n = uni(min((int)s.n, kList));
+    if (n <= 256) {  // each token counts those before it
+      const u64 mine = tid < n ? s.list.word[tid] : 0;
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += s.list.word[i] > mine;
+      __syncthreads();
+      if (tid < n) s.list.word[rank] = mine;
+      __syncthreads();
+    } else {
+      int size = 512;
+      while (size < n) size <<= 1;
+      for (int i = n + tid; i < size; i += kPickThreads) s.list.word[i] = 0;
+      __syncthreads();
+      for (int k = 2; k <= size; k <<= 1) {  // bitonic
+        for (int j = k >> 1; j > 0; j >>= 1) {
+          for (int t = tid; t < size / 2; t += kPickThreads) {
+            const int a = 2 * t - (t & (j - 1));
+            const u64 c = s.list.word[a], d = s.list.word[a + j];
+            if (((a & k) == 0) ? c < d : c > d) {
+              s.list.word[a] = d;
+              s.list.word[a + j] = c;
+            }
+          }
+          __syncthreads();
+        }
+      }
+    }
+    {  // running weights: each thread a run of consecutive entries
+      const int per = (n + kPickThreads - 1) / kPickThreads;
+      const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+      u64 mine = 0, none = 0;
+      for (int i = i0; i < i1; ++i) {
+        mine += weight_of_key(word_key(s.list.word[i]), r, base16, p.weight_exp, s.roots);
+        s.list.sum[i] = mine;
+      }
+      u64 incl = mine;
+      block_scan(s, incl, none);
+      for (int i = i0; i < i1; ++i) s.list.sum[i] += incl - mine;
+      __syncthreads();
+    }
+    if (step == kAll) {
+      // every token that can be kept is in the list; top-p's share is of the first top_k's weight: the
+      // list's, or, where the list ends before them, the histogram's
+      const int nk = (int)min(top_k, (u64)n);
+      if (cut_p && reach == ~0ull) {
+        if ((u64)nk == top_k) {
+          reach = reach_at(r.top_p, uni(s.list.sum[nk - 1]));
+        } else if (top_k == tokens) {
+          reach = reach_at(r.top_p, uni(s.weight[kBins - 1]));
+        } else {
+          start_border(kTopK, true, top_k);
+          end_weight = ~0ull;  // and back here, with reach
+          continue;
+        }
+      }
+      u64 kept_p = 0, kept_m = 0;
+      for (int i = tid; i < nk; i += kPickThreads) {
+        kept_p += i == 0 || s.list.sum[i - 1] < reach;
+        kept_m += finite(logit_of(word_key(s.list.word[i]))) * r.scale >= y_min;
+      }
+      block_scan(s, kept_p, kept_m);
+      if (tid == kPickThreads - 1) {
+        s.red[0] = kept_p;
+        s.red[1] = kept_m;
+      }
+      __syncthreads();
+      const int kept = uni(max(1, min((int)min(s.red[0], s.red[1]), nk)));
+      const u64 sum = uni(s.list.sum[kept - 1]);
+      const int at = first_reaching(s.list.sum, kept, draw_at(u, sum) + 1);
+      end_word = uni(s.list.word[kept - 1]);
+      end_weight = sum;
+      border_word = uni(s.list.word[at]);
+      break;
+    }
+    // ---- a border ----
+    {
+      const int i = by_count ? (int)min(target - count0, (u64)n) - 1 : first_reaching(s.list.sum, n, target - weight0);
+      border_word = uni(s.list.word[max(i, 0)]);
+      border_weight = weight0 + uni(s.list.sum[max(i, 0)]);
+    }
+    if (step == kTopK && end_weight == ~0ull) {
+      reach = reach_at(r.top_p, border_weight);
+      end_weight = 0;
+      start_all();
+      continue;
+    }
+    if (step == kDraw) break;
+    if (border_word > end_word) {
+      end_word = border_word;
+      end_weight = border_weight;
+    }
+    if (step == kTopK) {
+      after_top_k();
+      if (!cut_p) after_top_p();
+    } else if (step == kTopP) {
+      after_top_p();
+    } else {
+      start_draw();
     }
   }
-  const u64 t = draw_at(u, end.weight) + 1;
-  const Border d = k.border(k.first_reaching(s.weight, kBins, t), false, t);
   if (tid == 0) {
     // sums of a bin's tokens and of the histogram may differ in the last place
-    p.tokens[row] = (int32_t)word_index(d.word > end.word ? d.word : (end.word > 1 ? end.word : d.word));
-    out.last = end.word;
-    out.sum = ldexp((double)end.weight, -p.weight_exp);
+    p.tokens[row] = (int32_t)word_index(border_word > end_word || end_word == 1 ? border_word : end_word);
+    out.last = end_word;
+    out.sum = ldexp((double)end_weight, -p.weight_exp);
     p.results[row] = out;
   }
 }
@@ -894,6 +951,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
 // ---- probs ----
 constexpr int kProbsThreads = 256;
 constexpr int kProbsPer = 2;  // vectors per thread
+constexpr int kFarBins = 16 * 160;  // below 2^-160 a probability is 0 in fp32
 
 template <int DT>
 __global__ __launch_bounds__(kProbsThreads) void sample_probs_kernel(SampleParams p, int groups) {
@@ -905,7 +963,7 @@ __global__ __launch_bounds__(kProbsThreads) void sample_probs_kernel(SampleParam
   __syncthreads();
   const Row<DT> x(p, row);
   const RowResult r = p.results[row];
-  const double inv = 1.0 / r.sum;
+  const double inv = 1.0 / r.sum, base16 = kBinsPerLog2 * r.base;
   float* to = p.probs + (int64_t)row * p.ld_probs;
   u32x4 raw[kProbsPer];
   bool whole[kProbsPer];
@@ -930,8 +988,8 @@ __global__ __launch_bounds__(kProbsThreads) void sample_probs_kernel(SampleParam
         out[e] = 1.f;
       } else {
         double rem;
-        const int b = bin_of(finite(val[e]) * r.scale, r.base, rem);
-        out[e] = (float)(weight_of(b, rem, s_roots) * inv);
+        const int b = bin_of(finite(val[e]) * r.scale, base16, rem);
+        out[e] = b < kFarBins ? (float)(weight_of(b, rem, 0, s_roots) * inv) : 0.f;
       }
     }
     if (whole[j] && ((uintptr_t)(to + t0) & 15) == 0) {
