@@ -425,6 +425,56 @@ int ne_advance_and_propose(const int32_t* history, int64_t history_stride, const
                            int32_t* num_drafts, void* stream);
 
 /*
+ * Attention of a batch whose sequences share prefixes (no counterpart in the reference, which
+ * attends sequence by sequence): the same function of the same paged pool as
+ * ne_paged_verify_attention, with the keys of a prefix that several sequences hold in the
+ * same blocks read once for all of them.
+ *   group_seqs   [num_seqs] every sequence's index, group after group, in any order
+ *   group_start  [num_groups + 1] first entry of each group in group_seqs; 0 first,
+ *                num_seqs last.  A sequence that shares nothing is a group of one
+ *   prefix_len   [num_groups] tokens whose blocks the group's block tables have in common
+ *                (rounded down to 16; a group whose members hold fewer tokens before their
+ *                queries, or with one active member, shares what it can)
+ * Sequences with q_len or ctx_len 0 are idle and may sit in any group.  The other arguments are
+ * ne_paged_verify_attention's; num_rows is the number of query tokens in q and out,
+ * num_blocks the pool's blocks, and max_q_len, max_ctx_len, max_prefix_len bound the lengths.
+ * A row that sees no key is 0.  Rows of no sequence are left as they are.  int8 pools need
+ * |q| < 65504.
+ *
+ * ne_shared_prefix_plan writes the work plan of a step into the workspace, from the step's
+ * lengths and groups on the device; ne_shared_prefix_attention computes one layer with it, as
+ * often as there are layers, while lengths, groups and block tables stay as they were.
+ * Both take the same sizes, and a workspace of ne_shared_prefix_workspace_size() bytes
+ * (16-byte aligned), which one stream at a time may use.  Its first word is the error word
+ * of the last plan and the calls on it: 1 a context beyond max_ctx_len (keys past it are
+ * dropped), 2 a sequence of more than max_q_len queries or with rows outside q (not computed),
+ * 4 a group list that is out of order or names a sequence twice or outside the batch (such
+ * entries are not computed), 8 a block table entry outside the pool (block 0 is read).
+ * head_dim 128, block_size a multiple of 16, at most 1,024 sequences, any number of query
+ * heads per KV head; bf16 pools, or int8 pools with bf16 or fp16 scales.
+ */
+size_t ne_shared_prefix_workspace_size(int32_t num_seqs, int32_t num_groups, int32_t num_q_heads,
+                                       int32_t num_kv_heads, int32_t max_q_len,
+                                       int32_t max_ctx_len, int32_t max_prefix_len);
+int ne_shared_prefix_plan(const int32_t* ctx_len, const int32_t* q_start, const int32_t* q_len,
+                          int32_t num_rows, const int32_t* group_seqs, const int32_t* group_start,
+                          const int32_t* prefix_len, int32_t num_seqs, int32_t num_groups,
+                          int32_t num_q_heads, int32_t num_kv_heads, int32_t max_q_len,
+                          int32_t max_ctx_len, int32_t max_prefix_len, int32_t block_table_stride,
+                          int32_t block_size, int32_t num_blocks, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int ne_shared_prefix_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                               const void* k_cache, const void* v_cache, const void* k_scale,
+                               const void* v_scale, int32_t kv_dtype, int32_t scale_dtype,
+                               const int32_t* block_tables, int32_t block_table_stride,
+                               int32_t block_size, int32_t num_blocks, int32_t num_seqs,
+                               int32_t num_groups, int32_t num_q_heads, int32_t num_kv_heads,
+                               int32_t head_dim, int32_t max_q_len, int32_t max_ctx_len,
+                               int32_t max_prefix_len, float softmax_scale, void* out,
+                               int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
  * Copies of KV blocks within a pool (no counterpart in the reference, whose blocks are
  * never copied): for every buffer b and pair i, block dst[i] takes block src[i]'s bytes.
  * buffers, block_bytes, src and dst are HOST arrays, read before the call returns (a

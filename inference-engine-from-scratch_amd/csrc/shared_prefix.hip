@@ -1,0 +1,1233 @@
+// Attention of a batch whose sequences share prefixes: the keys of a shared prefix are
+// read once for all its sequences' queries, the rest per sequence.
+//
+// Mathematics.  A query row's keys are cut into parts; part a gives its largest score m_a
+// (or a reference below which nothing is lost), l_a = sum 2^(s - m_a) and
+// O_a = sum 2^(s - m_a) v, and the row is sum_a 2^(m_a - M) O_a / sum_a 2^(m_a - M) l_a.
+// Which rows compute a part together does not matter, so a prefix's parts serve every
+// row of its group (a matrix product of all their queries with the shared keys) and the
+// rest of each sequence has parts of its own.
+//
+// Three kernels.
+//   plan   one work-group, once per step for all layers: the groups' common lengths from
+//          the sequences' present ones (a member may be idle, a group may shrink to one),
+//          the tokens of each group in order, and the work items.
+//   parts  an item is one of
+//            a tile of 64, 128 or 256 rows of a group (tokens x heads of one KV head) over a
+//            range of the prefix, or of one sequence with more than 32 rows per KV head over
+//            a range of its own keys: 128 keys at a time staged in LDS as MFMA operands,
+//            eight waves of 32 rows (qt_* in attention_tile.hpp), key groups where rows are
+//            few;
+//            a light item: a range of the own keys of one sequence with at most 32 rows per
+//            KV head: one wave per KV head, K and V straight from memory to registers, the
+//            rows as the second operand of S^T = K Q^T, whose result is the second operand of
+//            O^T = V^T P^T.
+//          Items are cut so that the longest is about the batch's work over the chip.
+//   merge  16 threads per row.
+// What bounds it: reading the keys once (long prefixes and contexts), else the chain of
+// round trips of the three kernels; the partial sums (520 bytes a row and part) stay in the
+// memory-side cache.
+//
+// int8 pools: codes become fp16 exactly, the key scale multiplies the score, the value
+// scale the probability.  Probabilities enter the second product with 16 bits (11 significant
+// ones for int8 pools, 8 for bf16 pools, as the values themselves have): each is off by at
+// most half a step, and those errors average over the keys.  Value scales are taken relative
+// to a power of two that follows the largest met so far, so that small scales keep their bits in fp16.
+// A key that a row does not see never reaches it, whatever its value holds: where values of
+// partly hidden keys are not finite, they are added key by key.
+#include <string.h>
+
+#include <type_traits>
+
+#include "attention_tile.hpp"
+
+namespace ne {
+
+namespace {
+
+constexpr int kSpThreads = kQtThreads;
+constexpr int kSpWaves = kQtWaves;
+constexpr int kSpMaxSeqs = 1024;
+constexpr int kLightRows = 32;       // rows per KV head of a light item
+constexpr int kLightMinTiles = 8;    // least 16-key tiles per wave of a split sequence
+constexpr int kSpItemInts = 8;
+constexpr int kSpSeqInts = 12;
+constexpr float kSpLazy = 256.f;     // probabilities' sum per lane and step before the reference moves
+
+// What bits of the error word mean.
+enum : uint32_t { kErrContext = 1, kErrRows = 2, kErrGroups = 4, kErrBlock = 8 };
+
+struct SpParams {
+  const uint16_t* q;
+  int64_t q_tok_stride, q_head_stride;
+  const void* k_cache;
+  const void* v_cache;
+  const void* k_scale;
+  const void* v_scale;
+  const int32_t* block_tables;
+  int32_t bt_stride, block_size, num_blocks;
+  const int32_t* ctx_len;
+  const int32_t* q_start;
+  const int32_t* q_len;
+  const int32_t* group_seqs;
+  const int32_t* group_start;
+  const int32_t* prefix_len;
+  int32_t num_seqs, num_groups, num_rows;  // num_rows: query tokens of q and out
+  int32_t num_kv_heads, group;             // group: query heads per KV head
+  int32_t max_q, max_ctx;
+  float qk_scale;  // softmax_scale * log2(e)
+  uint16_t* out;
+  int64_t o_tok_stride, o_head_stride;
+  // workspace
+  uint32_t* head;      // [0] error word, [1] tile items, [2] light items
+  int32_t* tokens;     // row of q of every group's tokens, group after group
+  int32_t* tiles;      // [max_tiles][kSpItemInts]
+  int32_t* lights;     // [max_lights][kSpItemInts]
+  int32_t* seqs;       // [num_seqs][kSpSeqInts]
+  float* part_o;       // [parts' rows][128]
+  float* part_ml;      // [parts' rows][2]
+  int32_t max_tiles, max_lights;
+  int32_t light_heads, light_keys;  // a light work-group's KV heads, and its waves per KV head
+  int32_t head_blocks;              // work-groups per light item
+  int64_t part_rows;
+};
+
+__host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
+// Row tiles of 256 or fewer rows: 64, 128 or 256.
+__host__ __device__ inline int tile_rows_of(int rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+
+// ---- plan ----
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+
+// Exclusive sum over the threads, and the total.
+__device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* s_part, int64_t& total) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int64_t incl = v;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int64_t y = __shfl_up(incl, o);
+    if (lane >= o) incl += y;
+  }
+  __syncthreads();
+  if (lane == kWave - 1) s_part[wave] = incl;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    const int64_t x = s_part[w];
+    before += w < wave ? x : 0;
+    total += x;
+  }
+  return before + incl - v;
+}
+// Largest i in [0, n) with first[i] <= x (first[0] <= x).
+__device__ __forceinline__ int last_from(const int* first, int n, int x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (first[mid] <= x)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void shared_prefix_plan_kernel(SpParams p, int max_prefix) {
+  __shared__ int64_t s_part[kPlanWaves];
+  __shared__ int s_start[kSpMaxSeqs + 1];   // groups' first entries
+  __shared__ int s_least[kSpMaxSeqs];       // per group: fewest keys before a member's queries
+  __shared__ int s_leader[kSpMaxSeqs];      // first active entry
+  __shared__ int s_members[kSpMaxSeqs];
+  __shared__ int s_prefix[kSpMaxSeqs];      // keys shared (0: none)
+  __shared__ int s_token0[kSpMaxSeqs + 1];  // per entry: its first token
+  __shared__ int s_parts[kSpMaxSeqs];       // per group
+  __shared__ int s_item0[kSpMaxSeqs];       // per group: its first tile item
+  __shared__ int64_t s_row0[kSpMaxSeqs];    // per group: its first partial row
+  __shared__ int s_owner[kSpMaxSeqs];       // per sequence: its first entry
+  __shared__ int s_row[kSpMaxSeqs];         // per entry: its first row of q
+  const int e = threadIdx.x;
+  const int n = p.num_seqs, G = p.num_groups;
+  if (e < G) {
+    s_start[e] = p.group_start[e];
+    s_least[e] = 0x7FFFFFFF;
+    s_leader[e] = 0x7FFFFFFF;
+    s_members[e] = 0;
+  }
+  if (e == 0) {
+    s_start[G] = p.group_start[G];
+    p.head[0] = 0;
+  }
+  if (e < n) {
+    s_owner[e] = 0x7FFFFFFF;
+    p.seqs[(int64_t)e * kSpSeqInts] = 0;  // a sequence that no entry names has no rows
+  }
+  __syncthreads();
+  uint32_t error = 0;
+  // ---- entry e of the groups' list ----
+  int seq = -1, ctx = 0, ql = 0, qs = 0;
+  if (e < n) {
+    seq = p.group_seqs[e];
+    if (seq < 0 || seq >= n) {
+      error |= kErrGroups;
+      seq = -1;
+    } else {
+      ctx = p.ctx_len[seq];
+      ql = p.q_len[seq];
+      qs = p.q_start[seq];
+      if (ql > p.max_q || (ql > 0 && (qs < 0 || qs > p.num_rows - ql))) {
+        error |= kErrRows;
+        ql = 0;
+      }
+      if (ctx > p.max_ctx) error |= kErrContext;
+      if (ctx <= 0) ql = 0;
+      ql = max(ql, 0);
+    }
+  }
+  __syncthreads();
+  if (seq >= 0) atomicMin(&s_owner[seq], e);
+  __syncthreads();
+  if (seq >= 0 && s_owner[seq] != e) {  // named twice: the first entry counts
+    error |= kErrGroups;
+    seq = -1;
+    ql = 0;
+  }
+  if (e == 0 && (s_start[0] != 0 || s_start[G] != n)) error |= kErrGroups;
+  if (e < G && s_start[e] > s_start[e + 1]) error |= kErrGroups;
+  // the sequence's group: a list that does not start at 0, or ends early, leaves singles
+  int g = -1;
+  if (e < n && G > 0 && s_start[0] <= e && e < s_start[G]) {
+    g = last_from(s_start, G, e);
+    if (s_start[g] > e || e >= s_start[g + 1]) g = -1;  // not in order
+  }
+  if (e < n && g < 0) error |= kErrGroups;
+  if (ql > 0 && g >= 0) {
+    atomicMin(&s_least[g], max(ctx - ql, 0));
+    atomicMin(&s_leader[g], e);
+    atomicAdd(&s_members[g], 1);
+  }
+  int64_t tokens;
+  const int t0 = (int)plan_scan(ql, s_part, tokens);
+  if (e < n) {
+    s_token0[e] = t0;
+    s_row[e] = qs;
+  }
+  if (e == 0) s_token0[n] = (int)tokens;
+  __syncthreads();
+  // ---- group e ----
+  int rows = 0, stages = 0, tile_count = 0, prefix = 0;
+  if (e < G && s_members[e] > 1) {
+    prefix = min(min(p.prefix_len[e], s_least[e]), min(max_prefix, p.max_ctx));
+    prefix = max(min(prefix, p.bt_stride * p.block_size), 0) & ~(kTileKeys - 1);
+    if (prefix > 0) {
+      rows = (s_token0[min(max(s_start[e + 1], 0), n)] - s_token0[min(max(s_start[e], 0), n)]) * p.group;
+      tile_count = cdiv(rows, tile_rows_of(rows));
+      stages = cdiv(prefix, kQtKeys);
+    }
+  }
+  int64_t work, items, part_rows;
+  plan_scan((int64_t)tile_count * stages * p.num_kv_heads, s_part, work);
+  const int share = (int)max((work + kNumCu - 1) / kNumCu, (int64_t)1);
+  const int parts = stages > 0 ? max(stages / share, 1) : 0;
+  const int item0 = (int)plan_scan((int64_t)tile_count * parts, s_part, items);
+  const int64_t row0 = plan_scan((int64_t)rows * parts * p.num_kv_heads, s_part, part_rows);
+  if (e < G) {
+    s_prefix[e] = prefix;
+    s_parts[e] = parts;
+    s_item0[e] = item0;
+    s_row0[e] = row0;
+  }
+  __syncthreads();
+  // ---- entry e: its own keys ----
+  const int from = g >= 0 ? s_prefix[g] : 0;
+  const int kend = min(min(ctx, p.max_ctx), p.bt_stride * p.block_size);
+  const int own = ql > 0 ? max(kend - from, 0) : 0;
+  const int rows_s = ql * p.group;
+  const bool light = rows_s <= kLightRows;
+  const int tiles16 = light ? cdiv(own, kTileKeys) : 0;
+  const int heavy_tiles = light || own == 0 ? 0 : cdiv(rows_s, tile_rows_of(rows_s));
+  const int heavy_stages = light ? 0 : cdiv(own, kQtKeys);
+  int64_t light_work, heavy_work;
+  plan_scan((int64_t)tiles16 * p.head_blocks, s_part, light_work);
+  plan_scan((int64_t)heavy_tiles * heavy_stages * p.num_kv_heads, s_part, heavy_work);
+  const int64_t light_share = (light_work + kNumCu * p.light_keys - 1) / (kNumCu * p.light_keys);
+  const int lshare = (int)max(light_share, (int64_t)kLightMinTiles);
+  const int hshare = (int)max((heavy_work + kNumCu - 1) / kNumCu, (int64_t)2);
+  const int parts_s = light ? (tiles16 > 0 ? max(tiles16 / lshare, 1) : 0) : (heavy_stages > 0 ? max(heavy_stages / hshare, 1) : 0);
+  const int light_items = light ? cdiv(parts_s, p.light_keys) : 0;
+  int64_t lights, heavies, part_rows_s;
+  const int light0 = (int)plan_scan(light_items, s_part, lights);
+  const int heavy0 = (int)plan_scan((int64_t)heavy_tiles * parts_s, s_part, heavies);
+  const int64_t srow0 = part_rows + plan_scan((int64_t)rows_s * parts_s * p.num_kv_heads, s_part, part_rows_s);
+  // (the workspace's bounds hold for any lengths and groups in order; a list out of order may exceed them)
+  const bool fits = items + heavies <= p.max_tiles && lights <= p.max_lights && part_rows + part_rows_s <= p.part_rows;
+  if (!fits) error |= kErrGroups;
+  if (e < n && seq >= 0) {
+    int32_t* d = p.seqs + (int64_t)seq * kSpSeqInts;
+    d[0] = fits ? ql : 0;
+    d[1] = qs;
+    d[2] = g >= 0 && from > 0 ? s_parts[g] : 0;  // parts of the prefix
+    d[3] = parts_s;                              // parts of its own keys
+    const int64_t pr = g >= 0 ? s_row0[g] + (int64_t)(t0 - s_token0[min(max(s_start[g], 0), n)]) * p.group : 0;
+    d[4] = (int32_t)(pr & 0xFFFFFFFF);
+    d[5] = (int32_t)(pr >> 32);
+    d[6] = g >= 0 ? (s_token0[min(max(s_start[g + 1], 0), n)] - s_token0[min(max(s_start[g], 0), n)]) * p.group : 0;
+    d[7] = (int32_t)(srow0 & 0xFFFFFFFF);
+    d[8] = (int32_t)(srow0 >> 32);
+    d[9] = rows_s;
+    d[10] = ctx;
+    d[11] = from;
+  }
+  if (e == 0) {
+    p.head[1] = fits ? (uint32_t)(items + heavies) : 0;
+    p.head[2] = fits ? (uint32_t)lights : 0;
+  }
+  if (error) atomicOr(p.head, error);
+  __syncthreads();
+  if (!fits) return;
+  // ---- the groups' tokens, and the items ----
+  for (int i = e; i < (int)tokens; i += kPlanThreads) {
+    const int k = last_from(s_token0, n, i);  // (of entries with the same first token, the last holds it)
+    p.tokens[i] = s_row[k] + i - s_token0[k];
+  }
+  for (int i = e; i < (int)items; i += kPlanThreads) {
+    const int k = last_from(s_item0, G, i);
+    const int first = s_start[k];
+    const int rows_g = (s_token0[min(max(s_start[k + 1], 0), n)] - s_token0[min(max(first, 0), n)]) * p.group;
+    const int tr = tile_rows_of(rows_g), count = cdiv(rows_g, tr);
+    const int tile = (i - s_item0[k]) % count, part = (i - s_item0[k]) / count;
+    const int st = cdiv(s_prefix[k], kQtKeys);
+    const int64_t row = s_row0[k] + (int64_t)part * p.num_kv_heads * rows_g;
+    int32_t* d = p.tiles + (int64_t)i * kSpItemInts;
+    d[0] = -1 - p.group_seqs[s_leader[k]];  // the sequence whose table is read; negative: a group's item
+    d[1] = s_token0[first];
+    d[2] = rows_g;
+    d[3] = tile * tr;
+    d[4] = (int)((int64_t)st * part / s_parts[k]) * kQtKeys;
+    d[5] = min((int)((int64_t)st * (part + 1) / s_parts[k]) * kQtKeys, s_prefix[k]);
+    d[6] = (int32_t)(row & 0xFFFFFFFF);
+    d[7] = (int32_t)(row >> 32);
+  }
+  // entry e's own items (few each)
+  if (seq >= 0 && parts_s > 0) {
+    for (int i = 0; i < heavy_tiles * parts_s; ++i) {
+      const int tr = tile_rows_of(rows_s);
+      const int tile = i % heavy_tiles, part = i / heavy_tiles;
+      const int64_t row = srow0 + (int64_t)part * p.num_kv_heads * rows_s;
+      int32_t* d = p.tiles + ((int64_t)items + heavy0 + i) * kSpItemInts;
+      d[0] = seq;
+      d[1] = t0;
+      d[2] = rows_s;
+      d[3] = tile * tr;
+      d[4] = from + (int)((int64_t)heavy_stages * part / parts_s) * kQtKeys;
+      d[5] = min(from + (int)((int64_t)heavy_stages * (part + 1) / parts_s) * kQtKeys, kend);
+      d[6] = (int32_t)(row & 0xFFFFFFFF);
+      d[7] = (int32_t)(row >> 32);
+    }
+    for (int i = 0; i < light_items; ++i) {
+      int32_t* d = p.lights + ((int64_t)light0 + i) * kSpItemInts;
+      d[0] = seq;
+      d[1] = i * p.light_keys;  // first part
+      d[2] = parts_s;
+      d[3] = from;
+      d[4] = kend;
+      d[5] = tiles16;
+      d[6] = (int32_t)(srow0 & 0xFFFFFFFF);
+      d[7] = (int32_t)(srow0 >> 32);
+    }
+  }
+}
+
+// ---- a row's state ----
+template <bool INT8>
+struct SpState {
+  QFrag<INT8> q[kQtMT];
+  float m[kQtMT], l[kQtMT];
+  floatx4 o[kQtMT][8];
+};
+
+template <bool INT8>
+__device__ __forceinline__ floatx4 sp_mfma(u32x4 a, const std::conditional_t<INT8, f16x8, bf16x8>& b, floatx4 c) {
+  if constexpr (INT8)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b, c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), b, c, 0, 0, 0);
+}
+
+// 16 bytes of a query row as a B operand (bf16 -> fp16 is exact for |q| in [2^-14, 65504), and
+// rounds smaller ones to 2^-25).
+template <bool INT8>
+__device__ __forceinline__ auto sp_q_operand(u32x4 raw) {
+  if constexpr (INT8) {
+    u32x4 h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      h[i] = pack_f16x2(bf16_to_f32((uint16_t)(raw[i] & 0xFFFFu)), bf16_to_f32((uint16_t)(raw[i] >> 16)));
+    return __builtin_bit_cast(f16x8, h);
+  } else {
+    return __builtin_bit_cast(bf16x8, raw);
+  }
+}
+
+// Probabilities of a 32-key step for MT row tiles: s[mt][t][i] is the score of key 16 t + 4 g + i.
+// kf / vf: the keys' score factors and value factors (int8).  hidden(mt, e): key of slot e = 4 t + i
+// is not seen.  Returns the second product's operands in pb, the probabilities in pr.
+template <bool INT8, int MT, typename Hidden>
+__device__ __forceinline__ void sp_softmax(const floatx4 (&s)[MT][2], const floatx4 (&kf)[2], const floatx4 (&vf)[2],
+                                           float qk_scale, bool masked, Hidden hidden, SpState<INT8>& st,
+                                           float (&pr)[MT][8], u32x4 (&pb)[MT]) {
+  auto factor = [&](int e) { return INT8 ? kf[e >> 2][e & 3] : qk_scale; };
+  float psum[MT];
+  auto probs = [&]() {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        pr[mt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][e >> 2][e & 3], factor(e), -st.m[mt]));
+    if (masked) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pr[mt][e] = hidden(mt, e) ? 0.f : pr[mt][e];
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      psum[mt] = pr[mt][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) psum[mt] += pr[mt][e];
+    }
+  };
+  probs();
+  bool grow = false;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) grow |= psum[mt] > kSpLazy;
+  if (__ballot(grow)) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float mx = kNegBig;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, masked && hidden(mt, e) ? kNegBig : s[mt][e >> 2][e & 3] * factor(e));
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float m_new = fmaxf(st.m[mt], mx);
+      const float alpha = __builtin_amdgcn_exp2f(st.m[mt] - m_new);
+      st.l[mt] *= alpha;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) st.o[mt][j] *= alpha;
+      st.m[mt] = m_new;
+    }
+    probs();
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    st.l[mt] += psum[mt];
+    const float(&x)[8] = pr[mt];
+    if constexpr (INT8) {
+      // (a hidden key's value scale may be anything)
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = x[e] * vf[e >> 2][e & 3];
+        if (masked) y[e] = hidden(mt, e) ? 0.f : y[e];
+      }
+      pb[mt] = u32x4{pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7])};
+    } else {
+      pb[mt] = u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    }
+  }
+}
+
+__device__ __forceinline__ bool bf16x2_wild(uint32_t x) {  // either half infinite or NaN
+  return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
+}
+
+// Exponent of a positive finite scale, as an integer power of two above it.
+__device__ __forceinline__ int scale_exp(float x) { return (int)((__builtin_bit_cast(uint32_t, x) >> 23) & 0xFF) - 126; }
+// 2^e by its bits, e in [-126, 127].
+__device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+
+// A slot's block, or block 0 (and a flag) where the table names none of the pool's.
+__device__ __forceinline__ int sp_slot(const SpParams& p, const int32_t* bt, int key) {
+  int block = bt[key / p.block_size];
+  if (block < 0 || block >= p.num_blocks) {
+    atomicOr(p.head, kErrBlock);
+    block = 0;
+  }
+  return block * p.block_size + key % p.block_size;
+}
+
+// ---- tiles ----
+constexpr int kSpExpOff = kQtSlotOff + 2 * 8 * 4;  // int [2 buffers][2 waves]: the stage's largest value-scale exponents
+constexpr int kSpWildOff = kSpExpOff + 2 * 2 * 4;  // int [2 buffers][8 waves]: values that are not finite
+constexpr int kSpLds = kSpWildOff + 2 * 8 * 4;
+
+template <bool INT8, int SDT>
+__device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int head, char* smem) {
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lane = tid % kWave;
+  const ConstI32* d = (const ConstI32*)(p.tiles + (int64_t)item * kSpItemInts);
+  const int who = d[0], tok0 = d[1], rows_total = d[2], row0 = d[3], kstart = d[4], kend = d[5];
+  const int64_t part_row = ((int64_t)d[7] << 32) | (uint32_t)d[6];
+  const bool of_group = who < 0;
+  const int seq = of_group ? -1 - who : who;
+  const int kg_count = 256 / tile_rows_of(rows_total);
+  const int row_groups = kSpWaves / kg_count;
+  // keys that row R sees: all of a prefix, those up to its query's position of a sequence's own
+  int first_seen = kend;
+  if (!of_group) {
+    const ConstI32* sd = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
+    first_seen = sd[10] - sd[0] + 1;  // of query 0
+  }
+  const int r = lane & 15;
+  const int g = lane >> 4;
+  const int kg = wave / row_groups;
+  const int wrow0 = row0 + (wave % row_groups) * kQtWaveRows;
+  int* s_slot = (int*)(smem + kQtSlotOff);
+  int* s_exp = (int*)(smem + kSpExpOff);
+  int* s_wild = (int*)(smem + kSpWildOff);
+  const int32_t* bt = p.block_tables + (int64_t)seq * p.bt_stride;
+  auto tile_slot = [&](int tile16) {
+    return sp_slot(p, bt, min(kstart + kTileKeys * tile16, (kend - 1) & ~(kTileKeys - 1)));
+  };
+  int slot0 = 0;
+  if (tid < 16) slot0 = tile_slot(tid);
+  SpState<INT8> st;
+  int kend_row[kQtMT], kend_wave = 0, kfull_wave = kend;
+#pragma unroll
+  for (int mt = 0; mt < kQtMT; ++mt) {
+    const int row = wrow0 + kRows * mt + r;
+    const bool valid = row < rows_total;
+    const int t = valid ? row / p.group : 0;
+    const int token = p.tokens[tok0 + t];  // a row past the last reads the first token; it is never stored
+    kend_row[mt] = valid ? min(kend, of_group ? kend : first_seen + t) : 0;
+    const uint16_t* src = p.q + (int64_t)token * p.q_tok_stride +
+                          (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride + 8 * g;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) st.q[mt].q[c] = sp_q_operand<INT8>(*(const u32x4*)(src + 32 * c));
+    st.m[mt] = kNegBig;
+    st.l[mt] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.o[mt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (wrow0 < rows_total) {
+    const int last = (min(wrow0 + kQtWaveRows, rows_total) - 1) / p.group;
+    kend_wave = of_group ? kend : min(kend, first_seen + last);
+    kfull_wave = of_group ? kend : min(kend, first_seen + wrow0 / p.group);
+  }
+  if (tid < 16) s_slot[tid] = slot0;
+  __syncthreads();
+  QtRegs<INT8> R;
+  int vexp = -126;  // value scales are taken relative to 2^vexp
+  auto stage_store = [&](int buf, int kb) {
+    qt_store_kv<INT8>(smem, buf, tid, R);
+    if constexpr (INT8) {
+      if (tid < 2 * kQtKeys) {
+        float* sc = (float*)(smem + kQtScaleOff) + buf * 2 * kQtKeys;
+        sc[tid] = tid < kQtKeys ? R.sc * p.qk_scale : R.sc;
+        if (tid >= kQtKeys) {
+          const bool finite = fabsf(R.sc) < INFINITY;
+          int x = finite ? scale_exp(R.sc) : -126;
+#pragma unroll
+          for (int o = 32; o >= 1; o >>= 1) x = max(x, __shfl_xor(x, o));
+          if (lane == 0) s_exp[buf * 2 + wave - kQtKeys / kWave] = x;
+        }
+      }
+    } else {
+      bool wild = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wild |= bf16x2_wild(R.v[e][0]) || bf16x2_wild(R.v[e][1]);
+      const bool any = __ballot(wild) != 0;
+      if (lane == 0) s_wild[buf * kSpWaves + wave] = any;
+    }
+  };
+  const int n_stages = (kend - kstart + kQtKeys - 1) / kQtKeys;
+  qt_load<INT8, SDT>(p, s_slot, kstart, kend, head, tid, R);
+  stage_store(0, kstart);
+  __syncthreads();
+  for (int t = 0; t < n_stages; ++t) {
+    const int buf = t & 1;
+    const int kb0 = kstart + t * kQtKeys;
+    const bool more = t + 1 < n_stages;
+    int next_slot = 0;
+    if (more) {
+      qt_load<INT8, SDT>(p, s_slot + 8 * (buf ^ 1), kb0 + kQtKeys, kend, head, tid, R);
+      if (tid < 8) next_slot = tile_slot(8 * (t + 2) + tid);
+    }
+    __asm__ __volatile__("" ::: "memory");  // the loads go out before the products
+    float vscale = 1.f;
+    bool wild = false;
+    if constexpr (INT8) {
+      const int x = __builtin_amdgcn_readfirstlane(max(s_exp[buf * 2], s_exp[buf * 2 + 1]));
+      if (x > vexp) {
+        const float down = pow2(vexp - x);  // (2^-126 or less: what was added so far had scales that small)
+#pragma unroll
+        for (int mt = 0; mt < kQtMT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) st.o[mt][j] *= down;
+        vexp = x;
+      }
+      vscale = pow2(-vexp);
+    } else {
+      int any = 0;
+#pragma unroll
+      for (int w = 0; w < kSpWaves; ++w) any |= s_wild[buf * kSpWaves + w];
+      wild = __builtin_amdgcn_readfirstlane(any) != 0;
+    }
+#pragma unroll 1
+    for (int u = kg; u < 4; u += kg_count) {
+      const int kb = kb0 + 32 * u;
+      if (kb >= kend_wave) break;
+      const bool masked = kb + 32 > kfull_wave;
+      const char* ks = smem + buf * kQtStage;
+      const char* vs = ks + kQtTileBytes;
+      floatx4 s[kQtMT][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int mt = 0; mt < kQtMT; ++mt) s[mt][h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const u32x4 a = *(const u32x4*)(ks + (32 * u + 16 * h + r) * 256 + qt_k_pos(r, 4 * c + g) * 16);
+#pragma unroll
+          for (int mt = 0; mt < kQtMT; ++mt) s[mt][h] = sp_mfma<INT8>(a, st.q[mt].q[c], s[mt][h]);
+        }
+      }
+      floatx4 kf[2], vf[2];
+      if constexpr (INT8) {
+        const float* sc = (const float*)(smem + kQtScaleOff) + buf * 2 * kQtKeys + 32 * u + 4 * g;
+        kf[0] = *(const floatx4*)sc;
+        kf[1] = *(const floatx4*)(sc + 16);
+        vf[0] = *(const floatx4*)(sc + kQtKeys) * vscale;
+        vf[1] = *(const floatx4*)(sc + kQtKeys + 16) * vscale;
+      }
+      float pr[kQtMT][8];
+      u32x4 pb[kQtMT];
+      sp_softmax<INT8, kQtMT>(
+          s, kf, vf, p.qk_scale, masked,
+          [&](int mt, int e) { return kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend_row[mt]; }, st, pr, pb);
+      if (!INT8 && wild && masked) {  // key by key
+#pragma unroll
+        for (int mt = 0; mt < kQtMT; ++mt) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            for (int gg = 0; gg < 4; ++gg) {
+              const float x = __shfl(pr[mt][e], r + 16 * gg);
+              const int key = 16 * (e >> 2) + 4 * gg + (e & 3);
+              if (kb + key >= kend_row[mt]) continue;
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int dim = 16 * j + 4 * g + i;
+                  const uint16_t* v = (const uint16_t*)(vs + dim * 256 + qt_v_pos(dim & 15, 4 * u + gg) * 16);
+                  st.o[mt][j][i] += x * bf16_to_f32(v[e]);
+                }
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const u32x4 a = *(const u32x4*)(vs + r * 256 + qt_v_pos(r, 4 * u + g) * 16 + j * 16 * 256);
+#pragma unroll
+          for (int mt = 0; mt < kQtMT; ++mt) {
+            if constexpr (INT8)
+              st.o[mt][j] = sp_mfma<true>(a, __builtin_bit_cast(f16x8, pb[mt]), st.o[mt][j]);
+            else
+              st.o[mt][j] = sp_mfma<false>(a, __builtin_bit_cast(bf16x8, pb[mt]), st.o[mt][j]);
+          }
+        }
+      }
+    }
+    if (more) {
+      stage_store(buf ^ 1, kb0 + kQtKeys);
+      if (tid < 8) s_slot[8 * buf + tid] = next_slot;
+    }
+    __syncthreads();
+  }
+  // ---- merge the key groups through LDS ----
+#pragma unroll
+  for (int mt = 0; mt < kQtMT; ++mt) {
+    st.l[mt] += __shfl_xor(st.l[mt], 16);
+    st.l[mt] += __shfl_xor(st.l[mt], 32);
+  }
+  if (kg_count > 1) {
+    floatx4* s_part = (floatx4*)smem;
+    auto part_at = [&](int q, int mt, int j) -> floatx4& {
+      return s_part[((((q - 1) * row_groups + wave % row_groups) * kQtMT + mt) * 9 + j) * kWave + lane];
+    };
+    // (KG - 1) * row groups is 6 for 64 rows, 4 for 128
+    static_assert(6 * kQtMT * 9 * kWave * 16 <= kQtScaleOff, "partials fit the stages");
+    if (kg > 0) {
+#pragma unroll
+      for (int mt = 0; mt < kQtMT; ++mt) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part_at(kg, mt, j) = st.o[mt][j];
+        part_at(kg, mt, 8) = floatx4{st.m[mt], st.l[mt], 0.f, 0.f};
+      }
+    }
+    __syncthreads();
+    if (kg > 0) return;
+    for (int q = 1; q < kg_count; ++q) {
+#pragma unroll
+      for (int mt = 0; mt < kQtMT; ++mt) {
+        const floatx4 ml = part_at(q, mt, 8);
+        const float mm = fmaxf(st.m[mt], ml[0]);
+        const float a0 = __builtin_amdgcn_exp2f(st.m[mt] - mm);
+        const float a1 = __builtin_amdgcn_exp2f(ml[0] - mm);
+        st.l[mt] = a0 * st.l[mt] + a1 * ml[1];
+        st.m[mt] = mm;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) st.o[mt][j] = a0 * st.o[mt][j] + a1 * part_at(q, mt, j);
+      }
+    }
+  }
+  const float back = INT8 ? pow2(vexp) : 1.f;
+#pragma unroll
+  for (int mt = 0; mt < kQtMT; ++mt) {
+    const int row = wrow0 + kRows * mt + r;
+    if (row >= rows_total) continue;
+    const int64_t to = part_row + (int64_t)head * rows_total + row;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) *(floatx4*)(p.part_o + to * kHeadDim + 16 * j + 4 * g) = st.o[mt][j] * back;
+    if (g == 0) *(float2*)(p.part_ml + to * 2) = float2{st.m[mt], st.l[mt]};
+  }
+}
+
+// ---- light items ----
+// A wave's registers of a 32-key step on its way from memory.
+template <bool INT8>
+struct LightRegs;
+template <>
+struct LightRegs<true> {
+  u32x4 k[2][2];  // [tile][half]: bytes 64 half + 16 g .. of key r
+  u32x2 v[8];     // [slot e]: bytes 8 r .. of key 16 (e / 4) + 4 g + e % 4
+  float sc;       // lanes 0..31: key scale of key lane; 32..63: value scale of key lane - 32
+};
+template <>
+struct LightRegs<false> {
+  u32x4 k[2][4];  // [tile][chunk]: dims 32 chunk + 8 g .. of key r
+  u32x4 v[8];     // [slot e]: dims 8 r .. of the key
+};
+
+template <bool INT8, int SDT>
+__device__ __forceinline__ void light_load(const SpParams& p, int slot_a, int slot_b, int head, int lane, LightRegs<INT8>& R) {
+  constexpr int kEsz = INT8 ? 1 : 2;
+  const int64_t slot_bytes = (int64_t)p.num_kv_heads * kHeadDim * kEsz;
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int64_t at = (t ? slot_b : slot_a) * slot_bytes + (int64_t)head * kHeadDim * kEsz;
+    const char* kc = (const char*)p.k_cache + at + r * slot_bytes + 16 * g;
+    const char* vc = (const char*)p.v_cache + at + 4 * g * slot_bytes + 8 * kEsz * r;
+#pragma unroll
+    for (int c = 0; c < (INT8 ? 2 : 4); ++c) R.k[t][c] = *(const u32x4*)(kc + 64 * c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (INT8)
+        R.v[4 * t + i] = *(const u32x2*)(vc + i * slot_bytes);
+      else
+        R.v[4 * t + i] = *(const u32x4*)(vc + i * slot_bytes);
+    }
+  }
+  if constexpr (INT8) {
+    const int64_t slot = ((lane & 16) ? slot_b : slot_a) + (lane & 15);
+    R.sc = load_scale<SDT>(lane < 32 ? p.k_scale : p.v_scale, slot * p.num_kv_heads + head);
+  }
+}
+
+template <bool INT8, int SDT, int MT>
+__device__ __forceinline__ void sp_light(const SpParams& p, int seq, int head, int kstart, int kend, int64_t part_row, char* smem) {
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lane = tid % kWave;
+  const int r = lane & 15, g = lane >> 4;
+  const ConstI32* sd = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
+  const int ql = sd[0], qs = sd[1], rows_total = sd[9], ctx = sd[10];
+  const int first_seen = ctx - ql + 1;
+  const int32_t* bt = p.block_tables + (int64_t)seq * p.bt_stride;
+  SpState<INT8> st;
+  int kend_row[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = kRows * mt + r;
+    const bool valid = row < rows_total;
+    const int t = valid ? row / p.group : 0;
+    kend_row[mt] = valid ? min(kend, first_seen + t) : 0;
+    const uint16_t* src = p.q + (int64_t)(qs + t) * p.q_tok_stride +
+                          (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      // int8 keys come as bytes 64 h + 16 g + 8 c' of chunk 2 h + c': the same dims of the query
+      const int at = INT8 ? 64 * (c >> 1) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
+      st.q[mt].q[c] = sp_q_operand<INT8>(*(const u32x4*)(src + at));
+    }
+    st.m[mt] = kNegBig;
+    st.l[mt] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.o[mt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int n_tiles = (kend - kstart + kTileKeys - 1) / kTileKeys;
+  const int n_steps = (n_tiles + 1) / 2;
+  const int kfull = min(kend, first_seen);
+  // slots of 64 tiles at a time, one per lane
+  int slots = 0;
+  auto fetch_slots = [&](int tile0) { slots = sp_slot(p, bt, kstart + kTileKeys * min(tile0 + lane, n_tiles - 1)); };
+  auto slot_of = [&](int tile) { return __builtin_amdgcn_readlane(slots, min(tile, n_tiles - 1) & 63); };
+  fetch_slots(0);
+  LightRegs<INT8> R, N;
+  light_load<INT8, SDT>(p, slot_of(0), slot_of(1), head, lane, R);
+  int vexp = -126;
+  float* s_sc = (float*)smem + wave * kWave;
+  for (int it = 0; it < n_steps; ++it) {
+    if (it + 1 < n_steps) {
+      if (((2 * it + 2) & 63) == 0) fetch_slots(2 * it + 2);
+      light_load<INT8, SDT>(p, slot_of(2 * it + 2), slot_of(2 * it + 3), head, lane, N);
+    }
+    __asm__ __volatile__("" ::: "memory");
+    const int kb = kstart + 32 * it;
+    const bool masked = kb + 32 > kfull;
+    floatx4 s[MT][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) s[mt][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        u32x4 a;
+        if constexpr (INT8)
+          a = i8x8_f16x8(R.k[t][c >> 1][2 * (c & 1)], R.k[t][c >> 1][2 * (c & 1) + 1]);
+        else
+          a = R.k[t][c];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][t] = sp_mfma<INT8>(a, st.q[mt].q[c], s[mt][t]);
+      }
+    }
+    floatx4 kf[2], vf[2];
+    if constexpr (INT8) {
+      const int key = kb + (lane & 31);
+      const float x = key < kend ? R.sc : 0.f;  // a slot past the end may hold anything
+      int ex = lane >= 32 && fabsf(x) < INFINITY ? scale_exp(x) : -126;
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) ex = max(ex, __shfl_xor(ex, o));
+      ex = __builtin_amdgcn_readfirstlane(ex);
+      if (ex > vexp) {
+        const float down = pow2(vexp - ex);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) st.o[mt][j] *= down;
+        vexp = ex;
+      }
+      s_sc[lane] = x * (lane < 32 ? p.qk_scale : pow2(-vexp));
+      __builtin_amdgcn_wave_barrier();
+      kf[0] = *(const floatx4*)(s_sc + 4 * g);
+      kf[1] = *(const floatx4*)(s_sc + 16 + 4 * g);
+      vf[0] = *(const floatx4*)(s_sc + 32 + 4 * g);
+      vf[1] = *(const floatx4*)(s_sc + 48 + 4 * g);
+      __builtin_amdgcn_wave_barrier();
+    }
+    float pr[MT][8];
+    u32x4 pb[MT];
+    sp_softmax<INT8, MT>(
+        s, kf, vf, p.qk_scale, masked,
+        [&](int mt, int e) { return kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend_row[mt]; }, (SpState<INT8>&)st, pr, pb);
+    bool wild = false;
+    if constexpr (!INT8) {
+      if (masked) {
+        // values past the end may be stale bits; a value that a row does not see must not reach it
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend) R.v[e] = u32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) wild |= bf16x2_wild(R.v[e][w]);
+        }
+        wild = __ballot(wild) != 0;
+      }
+    }
+    if (!INT8 && wild) {  // key by key, from memory
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          for (int gg = 0; gg < 4; ++gg) {
+            const float x = __shfl(pr[mt][e], r + 16 * gg);
+            const int key = kb + 16 * (e >> 2) + 4 * gg + (e & 3);
+            if (key >= kend_row[mt]) continue;
+            const int64_t slot = (int64_t)sp_slot(p, bt, key);
+            const uint16_t* v = (const uint16_t*)p.v_cache + (slot * p.num_kv_heads + head) * kHeadDim + 32 * g;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) st.o[mt][j][i] += x * bf16_to_f32(v[8 * i + j]);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        u32x4 a;
+        if constexpr (INT8) {
+          uint32_t x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = R.v[e][j >> 2];
+          a = (j & 3) == 0   ? i8_cols_f16x8<0>(x)
+              : (j & 3) == 1 ? i8_cols_f16x8<1>(x)
+              : (j & 3) == 2 ? i8_cols_f16x8<2>(x)
+                             : i8_cols_f16x8<3>(x);
+        } else {
+          const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+          a = u32x4{__builtin_amdgcn_perm(R.v[1][j >> 1], R.v[0][j >> 1], sel), __builtin_amdgcn_perm(R.v[3][j >> 1], R.v[2][j >> 1], sel),
+                    __builtin_amdgcn_perm(R.v[5][j >> 1], R.v[4][j >> 1], sel), __builtin_amdgcn_perm(R.v[7][j >> 1], R.v[6][j >> 1], sel)};
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          if constexpr (INT8)
+            st.o[mt][j] = sp_mfma<true>(a, __builtin_bit_cast(f16x8, pb[mt]), st.o[mt][j]);
+          else
+            st.o[mt][j] = sp_mfma<false>(a, __builtin_bit_cast(bf16x8, pb[mt]), st.o[mt][j]);
+        }
+      }
+    }
+    R = N;
+  }
+  const float back = INT8 ? pow2(vexp) : 1.f;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = kRows * mt + r;
+    float l = st.l[mt];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (row >= rows_total) continue;
+    const int64_t to = part_row + (int64_t)head * rows_total + row;
+    float* po = p.part_o + to * kHeadDim + 32 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *(floatx4*)(po + 8 * i) = floatx4{st.o[mt][0][i], st.o[mt][1][i], st.o[mt][2][i], st.o[mt][3][i]} * back;
+      *(floatx4*)(po + 8 * i + 4) = floatx4{st.o[mt][4][i], st.o[mt][5][i], st.o[mt][6][i], st.o[mt][7][i]} * back;
+    }
+    if (g == 0) *(float2*)(p.part_ml + to * 2) = float2{st.m[mt], l};
+  }
+}
+
+template <bool INT8, int SDT>
+__global__ __launch_bounds__(kSpThreads) void shared_prefix_parts_kernel(SpParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const ConstI32* head = (const ConstI32*)p.head;
+  const int tile_groups = p.max_tiles * p.num_kv_heads;
+  if ((int)blockIdx.x < tile_groups) {
+    const int item = blockIdx.x / p.num_kv_heads;
+    if (item < head[1]) sp_tile_item<INT8, SDT>(p, item, blockIdx.x % p.num_kv_heads, smem);
+    return;
+  }
+  const int b = blockIdx.x - tile_groups;
+  const int item = b / p.head_blocks;
+  if (item >= head[2]) return;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const ConstI32* d = (const ConstI32*)(p.lights + (int64_t)item * kSpItemInts);
+  const int seq = d[0], part = d[1] + wave / p.light_heads, parts = d[2], from = d[3], kend = d[4], tiles = d[5];
+  const int kv = (b % p.head_blocks) * p.light_heads + wave % p.light_heads;
+  if (wave >= p.light_heads * p.light_keys || part >= parts || kv >= p.num_kv_heads) return;  // (no barrier follows)
+  const int k0 = from + (int)((int64_t)tiles * part / parts) * kTileKeys;
+  const int k1 = min(from + (int)((int64_t)tiles * (part + 1) / parts) * kTileKeys, kend);
+  const ConstI32* sd = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
+  const int64_t row = (((int64_t)d[7] << 32) | (uint32_t)d[6]) + (int64_t)part * p.num_kv_heads * sd[9];
+  if (sd[9] <= kRows)
+    sp_light<INT8, SDT, 1>(p, seq, kv, k0, k1, row, smem);
+  else
+    sp_light<INT8, SDT, 2>(p, seq, kv, k0, k1, row, smem);
+}
+
+// ---- merge ----
+constexpr int kMergeThreads = 256;
+constexpr int kMergeRows = kMergeThreads / 16;
+constexpr int kMergeAhead = 8;
+
+__global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpParams p, int blocks_per_seq) {
+  const int seq = blockIdx.x / blocks_per_seq;
+  const ConstI32* d = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
+  const int heads = p.num_kv_heads * p.group;
+  const int x = (blockIdx.x % blocks_per_seq) * kMergeRows + (threadIdx.x >> 4);  // query, then head
+  if (x >= d[0] * heads) return;
+  const int i = x / heads, head = x % heads;
+  const int kv = head / p.group, in = i * p.group + head % p.group;
+  const int np = d[2], n = np + d[3];
+  const int64_t prefix0 = (((int64_t)d[5] << 32) | (uint32_t)d[4]) + (int64_t)kv * d[6] + in;
+  const int64_t own0 = (((int64_t)d[8] << 32) | (uint32_t)d[7]) + (int64_t)kv * d[9] + in;
+  const int64_t prefix_step = (int64_t)p.num_kv_heads * d[6], own_step = (int64_t)p.num_kv_heads * d[9];
+  const int cd = (threadIdx.x & 15) * 8;
+  float M = kNegBig, L = 0.f;
+  float acc[8] = {};
+  for (int s0 = 0; s0 < n; s0 += kMergeAhead) {
+    float2 ml[kMergeAhead];
+    floatx4 a[kMergeAhead], b[kMergeAhead];
+#pragma unroll
+    for (int j = 0; j < kMergeAhead; ++j) {
+      const int s = min(s0 + j, n - 1);
+      const int64_t row = s < np ? prefix0 + s * prefix_step : own0 + (s - np) * own_step;
+      ml[j] = *(const float2*)(p.part_ml + row * 2);
+      a[j] = *(const floatx4*)(p.part_o + row * kHeadDim + cd);
+      b[j] = *(const floatx4*)(p.part_o + row * kHeadDim + cd + 4);
+    }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < kMergeAhead; ++j) top = fmaxf(top, s0 + j < n ? ml[j].x : kNegBig);
+    const float down = __builtin_amdgcn_exp2f(M - top);
+    L *= down;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[c] *= down;
+    M = top;
+#pragma unroll
+    for (int j = 0; j < kMergeAhead; ++j) {
+      if (s0 + j >= n) continue;
+      const float w = __builtin_amdgcn_exp2f(ml[j].x - M);
+      L += w * ml[j].y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        acc[c] += w * a[j][c];
+        acc[c + 4] += w * b[j][c];
+      }
+    }
+  }
+  // a row that sees no key is zero
+  const bool none = L == 0.f;
+  const float inv = none ? 0.f : 1.f / L;
+  uint16_t* to = p.out + (int64_t)(d[1] + i) * p.o_tok_stride + (int64_t)head * p.o_head_stride + cd;
+  *(u32x4*)to = none ? u32x4{0, 0, 0, 0}
+                     : u32x4{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
+                             pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv)};
+}
+
+// ---- host ----
+struct SpLayout {
+  int max_tiles, max_lights, light_heads, light_keys, head_blocks;
+  int64_t part_rows;
+  size_t tokens, tiles, lights, seqs, part_o, part_ml, total;
+};
+
+// Bounds that hold for any lengths within the call's (comments give the plan's counts).
+SpLayout sp_layout(int num_seqs, int num_groups, int num_q_heads, int num_kv_heads, int max_q, int max_ctx, int max_prefix) {
+  SpLayout l;
+  const int group = num_q_heads / num_kv_heads;
+  const int64_t tokens = (int64_t)num_seqs * max_q;
+  const int64_t rows = tokens * group;
+  if (max_prefix > max_ctx) max_prefix = max_ctx;
+  l.light_heads = num_kv_heads < kSpWaves ? num_kv_heads : kSpWaves;
+  l.light_keys = kSpWaves / l.light_heads;
+  l.head_blocks = cdiv(num_kv_heads, l.light_heads);
+  // prefix tiles: at most rows / 256 + one per group; a tile of n stages has at most n / share parts and
+  // at least one, share >= work / kNumCu, so parts past the first number kNumCu / kv heads at most
+  const int64_t groups = max_prefix >= kTileKeys ? (num_groups < num_seqs / 2 ? num_groups : num_seqs / 2) : 0;
+  const int64_t stages = cdiv(max_prefix, kQtKeys);
+  const int64_t more = kNumCu / num_kv_heads + 1;
+  int64_t tiles = 0, part_rows = 0;
+  if (groups > 0) {
+    const int64_t t = rows / 256 + groups;
+    const int64_t extra = t * (stages - 1) < more ? t * (stages - 1) : more;
+    tiles += t + extra;
+    // a part's rows: a tile's 256, but no more than every row in every part
+    const int64_t by_tile = rows + extra * 256, by_rows = rows * stages;
+    part_rows += (by_tile < by_rows ? by_tile : by_rows) * num_kv_heads;
+  }
+  // a sequence's own keys, in tiles or light items
+  int64_t most = 0;
+  if ((int64_t)max_q * group > kLightRows) {
+    const int64_t t = rows / 256 + num_seqs;
+    const int64_t own_stages = cdiv(max_ctx, kQtKeys);
+    const int64_t extra = t * (own_stages - 1) < more ? t * (own_stages - 1) : more;
+    tiles += t + extra;
+    const int64_t by_tile = rows + extra * 256, by_rows = rows * own_stages;
+    most = (by_tile < by_rows ? by_tile : by_rows) * num_kv_heads;
+  }
+  // light items: parts past a sequence's first number kNumCu * light_keys / head_blocks at most
+  const int64_t splits = cdiv(max_ctx, kTileKeys) / kLightMinTiles;  // of one sequence
+  const int64_t by_seq = num_seqs * (splits > 1 ? splits - 1 : 0);
+  const int64_t by_chip = (int64_t)kNumCu * l.light_keys / l.head_blocks + 1;
+  const int64_t more_parts = by_seq < by_chip ? by_seq : by_chip;
+  l.max_lights = num_seqs + cdiv((int)more_parts, l.light_keys);
+  const int64_t light_rows = max_q * group < kLightRows ? max_q * group : kLightRows;
+  const int64_t light_part_rows = (num_seqs + more_parts) * light_rows * num_kv_heads;
+  // (a batch may mix both kinds of sequences)
+  l.part_rows = part_rows + most + light_part_rows;
+  l.max_tiles = (int)tiles;
+  size_t at = 256;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  l.tokens = take((size_t)(tokens + 1) * 4);
+  l.tiles = take((size_t)tiles * kSpItemInts * 4);
+  l.lights = take((size_t)l.max_lights * kSpItemInts * 4);
+  l.seqs = take((size_t)num_seqs * kSpSeqInts * 4);
+  l.part_ml = take((size_t)l.part_rows * 8);
+  l.part_o = take((size_t)l.part_rows * kHeadDim * 4);
+  l.total = at;
+  return l;
+}
+
+bool sp_shape_ok(int num_seqs, int num_groups, int num_q_heads, int num_kv_heads, int max_q, int max_ctx) {
+  return num_seqs >= 1 && num_seqs <= kSpMaxSeqs && num_groups >= 0 && num_groups <= num_seqs && num_kv_heads >= 1 &&
+         num_kv_heads <= 256 && num_q_heads >= num_kv_heads && num_q_heads % num_kv_heads == 0 && num_q_heads <= 4096 &&
+         max_q >= 1 && max_ctx >= 1 && max_ctx <= (1 << 30) && (int64_t)num_seqs * max_q * num_q_heads < (1ll << 30);
+}
+
+int sp_check(const char* what, int num_seqs, int num_groups, int num_q_heads, int num_kv_heads, int max_q, int max_ctx, int max_prefix,
+             int block_size, int num_blocks, int bt_stride, const void* ws, size_t bytes, SpLayout& l) {
+  NE_CHECK_ARG(num_seqs >= 0 && num_groups >= 0 && num_groups <= num_seqs, "%s: bad sizes: %d sequences, %d groups", what, num_seqs, num_groups);
+  NE_CHECK_SUPPORTED(num_seqs <= kSpMaxSeqs, "%s: %d sequences exceed %d", what, num_seqs, kSpMaxSeqs);
+  NE_CHECK_ARG(sp_shape_ok(num_seqs, num_groups, num_q_heads, num_kv_heads, max_q, max_ctx),
+               "%s: bad shape: %d / %d heads, %d queries, %d keys", what, num_q_heads, num_kv_heads, max_q, max_ctx);
+  NE_CHECK_ARG(max_prefix >= 0, "%s: bad prefix bound %d", what, max_prefix);
+  NE_CHECK_SUPPORTED(block_size >= kTileKeys && block_size % kTileKeys == 0, "%s: block_size %d is not a multiple of 16", what, block_size);
+  NE_CHECK_ARG(num_blocks >= 1 && (int64_t)num_blocks * block_size < (1ll << 31), "%s: bad pool of %d blocks", what, num_blocks);
+  NE_CHECK_ARG(bt_stride >= 0, "%s: bad block table stride %d", what, bt_stride);
+  NE_CHECK_ARG(ws, "%s: null workspace", what);
+  NE_CHECK_ARG((uintptr_t)ws % 16 == 0, "%s: workspace must be 16-byte aligned", what);
+  l = sp_layout(num_seqs, num_groups, num_q_heads, num_kv_heads, max_q, max_ctx, max_prefix);
+  if (bytes < l.total) {
+    set_error("%s: workspace of %zu bytes, %zu needed", what, bytes, l.total);
+    return NE_EWORKSPACE;
+  }
+  return NE_OK;
+}
+
+void sp_bind(SpParams& p, const SpLayout& l, char* ws) {
+  p.head = (uint32_t*)ws;
+  p.tokens = (int32_t*)(ws + l.tokens);
+  p.tiles = (int32_t*)(ws + l.tiles);
+  p.lights = (int32_t*)(ws + l.lights);
+  p.seqs = (int32_t*)(ws + l.seqs);
+  p.part_o = (float*)(ws + l.part_o);
+  p.part_ml = (float*)(ws + l.part_ml);
+  p.max_tiles = l.max_tiles;
+  p.max_lights = l.max_lights;
+  p.light_heads = l.light_heads;
+  p.light_keys = l.light_keys;
+  p.head_blocks = l.head_blocks;
+  p.part_rows = l.part_rows;
+}
+
+template <bool INT8, int SDT>
+int sp_launch(const SpParams& p, hipStream_t s) {
+  static const hipError_t attr = hipFuncSetAttribute((const void*)shared_prefix_parts_kernel<INT8, SDT>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kSpLds);
+  if (attr != hipSuccess) {
+    set_error("shared_prefix_parts: cannot reserve %d bytes of LDS: %s", kSpLds, hipGetErrorString(attr));
+    return NE_ELAUNCH;
+  }
+  const int grid = p.max_tiles * p.num_kv_heads + p.max_lights * p.head_blocks;
+  hipLaunchKernelGGL((shared_prefix_parts_kernel<INT8, SDT>), dim3(grid), dim3(kSpThreads), kSpLds, s, p);
+  const int rc = check_launch("shared_prefix_parts");
+  if (rc != NE_OK) return rc;
+  const int per_seq = cdiv(p.max_q * p.num_kv_heads * p.group, kMergeRows);
+  hipLaunchKernelGGL(shared_prefix_merge_kernel, dim3(p.num_seqs * per_seq), dim3(kMergeThreads), 0, s, p, per_seq);
+  return check_launch("shared_prefix_merge");
+}
+
+}  // namespace
+
+}  // namespace ne
+
+extern "C" size_t ne_shared_prefix_workspace_size(int32_t num_seqs, int32_t num_groups, int32_t num_q_heads,
+                                                  int32_t num_kv_heads, int32_t max_q_len, int32_t max_ctx_len,
+                                                  int32_t max_prefix_len) {
+  if (!ne::sp_shape_ok(num_seqs, num_groups, num_q_heads, num_kv_heads, max_q_len, max_ctx_len) || max_prefix_len < 0) return 0;
+  return ne::sp_layout(num_seqs, num_groups, num_q_heads, num_kv_heads, max_q_len, max_ctx_len, max_prefix_len).total;
+}
+
+extern "C" int ne_shared_prefix_plan(const int32_t* ctx_len, const int32_t* q_start, const int32_t* q_len, int32_t num_rows,
+                                     const int32_t* group_seqs, const int32_t* group_start, const int32_t* prefix_len,
+                                     int32_t num_seqs, int32_t num_groups, int32_t num_q_heads, int32_t num_kv_heads,
+                                     int32_t max_q_len, int32_t max_ctx_len, int32_t max_prefix_len, int32_t block_table_stride,
+                                     int32_t block_size, int32_t num_blocks, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
+  using namespace ne;
+  if (num_seqs == 0) return NE_OK;
+  SpLayout l;
+  const int rc = sp_check("shared_prefix_plan", num_seqs, num_groups, num_q_heads, num_kv_heads, max_q_len, max_ctx_len,
+                          max_prefix_len, block_size, num_blocks, block_table_stride, workspace, workspace_bytes, l);
+  if (rc != NE_OK) return rc;
+  NE_CHECK_ARG(ctx_len && q_start && q_len && group_seqs && group_start && (prefix_len || num_groups == 0),
+               "null pointer argument");
+  NE_CHECK_ARG(num_rows >= 0, "bad row count %d", num_rows);
+  SpParams p;
+  memset(&p, 0, sizeof(p));
+  sp_bind(p, l, (char*)workspace);
+  p.ctx_len = ctx_len;
+  p.q_start = q_start;
+  p.q_len = q_len;
+  p.group_seqs = group_seqs;
+  p.group_start = group_start;
+  p.prefix_len = prefix_len;
+  p.num_rows = num_rows;
+  p.num_seqs = num_seqs;
+  p.num_groups = num_groups;
+  p.num_kv_heads = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads;
+  p.max_q = max_q_len;
+  // a prefix longer than its bound is read as own keys past it
+  p.max_ctx = max_ctx_len;
+  p.bt_stride = block_table_stride;
+  p.block_size = block_size;
+  hipLaunchKernelGGL(shared_prefix_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, p, max_prefix_len);
+  return check_launch("shared_prefix_plan");
+}
+
+extern "C" int ne_shared_prefix_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                                          const void* v_cache, const void* k_scale, const void* v_scale, int32_t kv_dtype,
+                                          int32_t scale_dtype, const int32_t* block_tables, int32_t block_table_stride,
+                                          int32_t block_size, int32_t num_blocks, int32_t num_seqs, int32_t num_groups,
+                                          int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_q_len,
+                                          int32_t max_ctx_len, int32_t max_prefix_len, float softmax_scale, void* out,
+                                          int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  using namespace ne;
+  if (num_seqs == 0) return NE_OK;
+  NE_CHECK_SUPPORTED(head_dim == kHeadDim, "head_dim %d: only 128 is supported", head_dim);
+  SpLayout l;
+  const int rc = sp_check("shared_prefix_attention", num_seqs, num_groups, num_q_heads, num_kv_heads, max_q_len, max_ctx_len,
+                          max_prefix_len, block_size, num_blocks, block_table_stride, workspace, workspace_bytes, l);
+  if (rc != NE_OK) return rc;
+  NE_CHECK_ARG(q && k_cache && v_cache && block_tables && out, "null pointer argument");
+  NE_CHECK_ARG(kv_dtype == NE_DTYPE_BF16 || kv_dtype == NE_DTYPE_INT8, "the cache must be bf16 or int8");
+  NE_CHECK_ARG(softmax_scale == softmax_scale, "softmax_scale is NaN");
+  const bool int8 = kv_dtype == NE_DTYPE_INT8;
+  if (int8) {
+    NE_CHECK_ARG(k_scale && v_scale, "int8 cache needs scales");
+    NE_CHECK_ARG(scale_dtype == NE_DTYPE_BF16 || scale_dtype == NE_DTYPE_FP16, "scales must be bf16 or fp16");
+  }
+  NE_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 &&
+                   (q_token_stride | q_head_stride | out_token_stride | out_head_stride) % 8 == 0,
+               "q, out and the caches must be 16-byte aligned, row and head strides multiples of 8 elements");
+  SpParams p;
+  memset(&p, 0, sizeof(p));
+  sp_bind(p, l, (char*)workspace);
+  p.q = (const uint16_t*)q;
+  p.q_tok_stride = q_token_stride;
+  p.q_head_stride = q_head_stride;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.block_tables = block_tables;
+  p.bt_stride = block_table_stride;
+  p.block_size = block_size;
+  p.num_blocks = num_blocks;
+  p.num_seqs = num_seqs;
+  p.num_groups = num_groups;
+  p.num_kv_heads = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads;
+  p.max_q = max_q_len;
+  p.max_ctx = max_ctx_len;
+  p.qk_scale = softmax_scale * kLog2e;
+  p.out = (uint16_t*)out;
+  p.o_tok_stride = out_token_stride;
+  p.o_head_stride = out_head_stride;
+  if (!int8) return sp_launch<false, NE_DTYPE_BF16>(p, (hipStream_t)stream);
+  return scale_dtype == NE_DTYPE_BF16 ? sp_launch<true, NE_DTYPE_BF16>(p, (hipStream_t)stream)
+                                      : sp_launch<true, NE_DTYPE_FP16>(p, (hipStream_t)stream);
+}

@@ -137,6 +137,29 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "ne_copy_bytes": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
     "ne_kv_copy_blocks": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp]),
+    "ne_shared_prefix_workspace_size": (_sz, [_i32] * 7),
+    "ne_shared_prefix_plan": (
+        ctypes.c_int,
+        [
+            _vp, _vp, _vp, _i32,  # ctx_len, q_start, q_len, rows
+            _vp, _vp, _vp,  # group seqs, group start, prefix len
+            _i32, _i32, _i32, _i32, _i32, _i32, _i32,  # seqs, groups, heads, kv heads, max q, max ctx, max prefix
+            _i32, _i32, _i32,  # block table stride, block size, blocks
+            _vp, _sz, _vp,  # workspace, bytes, stream
+        ],
+    ),
+    "ne_shared_prefix_attention": (
+        ctypes.c_int,
+        [
+            _vp, _i64, _i64,  # q, strides
+            _vp, _vp, _vp, _vp, _i32, _i32,  # caches, scales, dtypes
+            _vp, _i32, _i32, _i32,  # block tables, stride, block size, blocks
+            _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,  # seqs, groups, heads, kv heads, dim, max q, max ctx, max prefix
+            _f32,  # softmax scale
+            _vp, _i64, _i64,  # out, strides
+            _vp, _sz, _vp,  # workspace, bytes, stream
+        ],
+    ),
     "ne_sample_workspace_size": (_sz, [_i32, _i32, _i32]),
     "ne_sample": (
         ctypes.c_int,

@@ -482,6 +482,155 @@ def paged_kv_stream_runs(
     )
 
 
+# ----------------------------------------------------------- shared prefixes
+@dataclass(frozen=True)
+class PrefixGroups:
+    """Which sequences of a batch hold the same tokens in the same blocks from the start on:
+    device tensors that a step reads, so their contents may change between replays of a graph."""
+
+    seqs: torch.Tensor  # [b] int32: every sequence's index, group after group
+    start: torch.Tensor  # [groups + 1] int32: first entry of each group; 0 first, b last
+    prefix_len: torch.Tensor  # [groups] int32: tokens the group's tables have in common
+    max_prefix_len: int  # bound on prefix_len
+
+    @classmethod
+    def from_lists(cls, groups: list[list[int]], prefix_lens: list[int], device: torch.device) -> "PrefixGroups":
+        """From host lists: each group's sequences, and the tokens each shares."""
+        _check(len(groups) == len(prefix_lens), "one prefix length per group")
+        seqs = [s for members in groups for s in members]
+        _check(sorted(seqs) == list(range(len(seqs))), "every sequence belongs to one group")
+        start = [0]
+        for members in groups:
+            start.append(start[-1] + len(members))
+        flat = torch.tensor(seqs + start + prefix_lens, dtype=torch.int32).to(device)
+        n, g = len(seqs), len(groups)
+        return cls(flat[:n], flat[n : n + g + 1], flat[n + g + 1 :], max(prefix_lens, default=0))
+
+
+@dataclass(frozen=True)
+class SharedPrefixPlan:
+    """The work plan of one step (:func:`shared_prefix_plan`) and what it was made for."""
+
+    workspace: torch.Tensor
+    block_tables: torch.Tensor
+    block_size: int
+    num_rows: int
+    num_q_heads: int
+    num_kv_heads: int
+    max_q_len: int
+    max_ctx_len: int
+    num_blocks: int
+    groups: PrefixGroups
+
+    def error_flag(self) -> int:
+        """The error word of the plan and the calls on it (waits for them)."""
+        return int(self.workspace[:4].view(torch.int32).item())
+
+
+def shared_prefix_workspace_bytes(num_seqs: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_q_len: int,
+                                  max_ctx_len: int, max_prefix_len: int) -> int:
+    return _native.load().ne_shared_prefix_workspace_size(num_seqs, num_groups, num_q_heads, num_kv_heads, max_q_len,
+                                                          max_ctx_len, max_prefix_len)
+
+
+def shared_prefix_plan(
+    block_tables: torch.Tensor,
+    block_size: int,
+    ctx_len: torch.Tensor,
+    q_start: torch.Tensor,
+    q_len: torch.Tensor,
+    groups: PrefixGroups,
+    num_q_heads: int,
+    num_kv_heads: int,
+    max_q_len: int,
+    max_ctx_len: int,
+    num_rows: int | None = None,
+    num_blocks: int | None = None,
+    workspace: torch.Tensor | None = None,
+) -> SharedPrefixPlan:
+    """Plan a step's :func:`shared_prefix_attention` calls (one per layer) from its lengths and
+    groups on the device.  ``num_rows`` (default: the most the sequences can hold) bounds the
+    query rows, ``num_blocks`` (default: unknown) the block tables' entries.  ``workspace``
+    (default: allocated here) is a uint8 tensor of :func:`shared_prefix_workspace_bytes` that no
+    other plan uses until this one's calls are done."""
+    device = _require_gpu(block_tables, ctx_len, q_start, q_len, groups.seqs, groups.start, groups.prefix_len)
+    for name, t in (("block_tables", block_tables), ("ctx_len", ctx_len), ("q_start", q_start), ("q_len", q_len),
+                    ("group seqs", groups.seqs), ("group start", groups.start), ("prefix_len", groups.prefix_len)):
+        _int32(t, name)
+    num_seqs, num_groups = ctx_len.shape[0], groups.prefix_len.shape[0]
+    _check(block_tables.dim() == 2 and block_tables.shape[0] >= num_seqs, "block_tables must be [b, max_blocks]")
+    _check(q_start.shape[0] == num_seqs and q_len.shape[0] == num_seqs and groups.seqs.shape[0] == num_seqs
+           and groups.start.shape[0] == num_groups + 1, "lengths and groups of different batches")
+    nbytes = _native.load().ne_shared_prefix_workspace_size(num_seqs, num_groups, num_q_heads, num_kv_heads, max_q_len,
+                                                            max_ctx_len, groups.max_prefix_len)
+    _check(nbytes > 0 or num_seqs == 0, "bad attention shape")
+    if workspace is None:
+        workspace = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=device)
+    _check(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == device,
+           f"workspace must be contiguous uint8 on {device}")
+    if num_rows is None:
+        num_rows = (1 << 31) - 1
+    if num_blocks is None:
+        num_blocks = ((1 << 31) - 1) // block_size
+    plan = SharedPrefixPlan(workspace, block_tables, block_size, num_rows, num_q_heads, num_kv_heads, max_q_len, max_ctx_len,
+                            num_blocks, groups)
+    _call_on(device, "ne_shared_prefix_plan", ctx_len.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), num_rows,
+             groups.seqs.data_ptr(), groups.start.data_ptr(), groups.prefix_len.data_ptr(), num_seqs, num_groups,
+             num_q_heads, num_kv_heads, max_q_len, max_ctx_len, groups.max_prefix_len, block_tables.stride(0), block_size,
+             num_blocks, workspace.data_ptr(), workspace.numel(), _stream(device))
+    return plan
+
+
+def shared_prefix_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor | None,
+    v_scale: torch.Tensor | None,
+    plan: SharedPrefixPlan,
+    softmax_scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Paged attention of a batch whose sequences share prefixes: :func:`paged_verify_attention`'s
+    function of the same pool, a prefix's keys read once for its whole group.  ``q`` / ``out``
+    are ``[rows, q_heads, 128]`` bf16; the pool is bf16, or int8 with bf16 or fp16 scales.  The
+    block tables and lengths the plan was made from must not have changed."""
+    device = _require_gpu(q, k_cache, v_cache, k_scale, v_scale, out, plan.workspace)
+    _check(q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1,
+           "q must be [rows, heads, 128] bf16")
+    _check(q.shape[1] == plan.num_q_heads, f"the plan is for {plan.num_q_heads} query heads")
+    _check(k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.dim() == 3
+           and k_cache.shape[1] == plan.num_kv_heads and k_cache.shape[2] == HEAD_DIM,
+           f"caches must be [slots, {plan.num_kv_heads}, 128]")
+    _check(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
+    is_int8 = k_cache.dtype == torch.int8
+    scale_code = DTYPE_BF16
+    if is_int8:
+        _check(k_scale is not None and v_scale is not None, "int8 cache needs scales")
+        _check(k_scale.dtype == v_scale.dtype and k_scale.is_contiguous() and v_scale.is_contiguous()
+               and k_scale.numel() == v_scale.numel() == k_cache.shape[0] * k_cache.shape[1],
+               "scales must be contiguous, one per slot and KV head")
+        scale_code = dtype_code(k_scale.dtype)
+    else:
+        _check(k_cache.dtype == torch.bfloat16, "cache must be int8 or bf16")
+    if plan.num_rows != (1 << 31) - 1:
+        _check(q.shape[0] >= plan.num_rows, f"q has {q.shape[0]} rows, the plan {plan.num_rows}")
+    if out is None:
+        out = torch.empty_like(q)
+    _check(out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1, "out must match q")
+    if softmax_scale is None:
+        softmax_scale = 1.0 / math.sqrt(HEAD_DIM)
+    groups = plan.groups
+    _call_on(device, "ne_shared_prefix_attention", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+             v_cache.data_ptr(), k_scale.data_ptr() if is_int8 else None, v_scale.data_ptr() if is_int8 else None,
+             DTYPE_INT8 if is_int8 else DTYPE_BF16, scale_code, plan.block_tables.data_ptr(), plan.block_tables.stride(0),
+             plan.block_size, min(plan.num_blocks, k_cache.shape[0] // plan.block_size), groups.seqs.shape[0],
+             groups.prefix_len.shape[0], plan.num_q_heads, plan.num_kv_heads, HEAD_DIM, plan.max_q_len, plan.max_ctx_len,
+             groups.max_prefix_len, softmax_scale, out.data_ptr(), out.stride(0), out.stride(1), plan.workspace.data_ptr(),
+             plan.workspace.numel(), _stream(device))
+    return out
+
+
 def plan_supported(num_q_heads: int, num_kv_heads: int, max_q_len: int, num_seqs: int, kv_dtype, scale_dtype) -> bool:
     """Whether :func:`paged_attention_plan` / ``planned=True`` serve this shape."""
     cache_ok = kv_dtype == torch.bfloat16 or (kv_dtype == torch.int8 and scale_dtype in (torch.bfloat16,
