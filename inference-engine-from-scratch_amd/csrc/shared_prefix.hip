@@ -33,8 +33,9 @@
 // ones for int8 pools, 8 for bf16 pools, as the values themselves have): each is off by at
 // most half a step, and those errors average over the keys.  Value scales are taken relative
 // to a power of two that follows the largest met so far, so that small scales keep their bits in fp16.
-// A key that a row does not see never reaches it, whatever its value holds: where values of
-// partly hidden keys are not finite, they are added key by key.
+// A key that a row does not see never reaches it, whatever its value holds: values of partly
+// hidden keys that are not finite enter the products as 0, and the merge adds them to the rows
+// that see them.
 #include <string.h>
 
 #include <type_traits>
@@ -51,7 +52,7 @@ constexpr int kSpMaxSeqs = 1024;
 constexpr int kLightRows = 32;       // rows per KV head of a light item
 constexpr int kLightMinTiles = 8;    // least 16-key tiles per wave of a split sequence
 constexpr int kSpItemInts = 8;
-constexpr int kSpSeqInts = 12;
+constexpr int kSpSeqInts = 10;
 constexpr float kSpLazy = 256.f;     // probabilities' sum per lane and step before the reference moves
 
 // What bits of the error word mean.
@@ -97,30 +98,39 @@ __host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ inline int tile_rows_of(int rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
 
 // ---- plan ----
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = kPlanThreads / kWave;
+constexpr int kPlanMaxThreads = kSpMaxSeqs;
 
-// Exclusive sum over the threads, and the total.
-__device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* s_part, int64_t& total) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  int64_t incl = v;
+// Sums of K values over the threads before each, and over all, in two barriers.
+template <int K>
+__device__ __forceinline__ void plan_scan(const int (&v)[K], int (*s_part)[kPlanMaxThreads / kWave], int (&before)[K], int (&total)[K]) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+  int incl[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) incl[k] = v[k];
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) {
-    const int64_t y = __shfl_up(incl, o);
-    if (lane >= o) incl += y;
-  }
-  __syncthreads();
-  if (lane == kWave - 1) s_part[wave] = incl;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
 #pragma unroll
-  for (int w = 0; w < kPlanWaves; ++w) {
-    const int64_t x = s_part[w];
-    before += w < wave ? x : 0;
-    total += x;
+    for (int k = 0; k < K; ++k) {
+      const int y = __shfl_up(incl[k], o);
+      incl[k] += lane >= o ? y : 0;
+    }
   }
-  return before + incl - v;
+  __syncthreads();
+  if (lane == kWave - 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) s_part[k][wave] = incl[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    before[k] = incl[k] - v[k];
+    total[k] = 0;
+    for (int w = 0; w < waves; ++w) {
+      const int x = s_part[k][w];
+      before[k] += w < wave ? x : 0;
+      total[k] += x;
+    }
+  }
 }
 // Largest i in [0, n) with first[i] <= x (first[0] <= x).
 __device__ __forceinline__ int last_from(const int* first, int n, int x) {
@@ -134,22 +144,28 @@ __device__ __forceinline__ int last_from(const int* first, int n, int x) {
   }
   return lo;
 }
+__device__ __forceinline__ int ceil_share(int64_t work, int workers) { return (int)((work + workers - 1) / workers); }
 
-__global__ __launch_bounds__(kPlanThreads) void shared_prefix_plan_kernel(SpParams p, int max_prefix) {
-  __shared__ int64_t s_part[kPlanWaves];
+// One work-group of a thread per sequence; thread e serves entry e of the groups' list, group e and
+// sequence e.  (Counts fit 32 bits: the host bounds the workspace's rows.)
+__global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpParams p, int max_prefix) {
+  __shared__ int s_part[5][kPlanMaxThreads / kWave];
   __shared__ int s_start[kSpMaxSeqs + 1];   // groups' first entries
   __shared__ int s_least[kSpMaxSeqs];       // per group: fewest keys before a member's queries
   __shared__ int s_leader[kSpMaxSeqs];      // first active entry
   __shared__ int s_members[kSpMaxSeqs];
   __shared__ int s_prefix[kSpMaxSeqs];      // keys shared (0: none)
   __shared__ int s_token0[kSpMaxSeqs + 1];  // per entry: its first token
+  __shared__ int s_row[kSpMaxSeqs];         // per entry: its first row of q
+  __shared__ int s_owner[kSpMaxSeqs];       // per sequence: its first entry
   __shared__ int s_parts[kSpMaxSeqs];       // per group
   __shared__ int s_item0[kSpMaxSeqs];       // per group: its first tile item
-  __shared__ int64_t s_row0[kSpMaxSeqs];    // per group: its first partial row
-  __shared__ int s_owner[kSpMaxSeqs];       // per sequence: its first entry
-  __shared__ int s_row[kSpMaxSeqs];         // per entry: its first row of q
-  const int e = threadIdx.x;
+  __shared__ int s_row0[kSpMaxSeqs];        // per group: its first partial row
+  const int e = threadIdx.x, threads = blockDim.x;
   const int n = p.num_seqs, G = p.num_groups;
+  uint32_t error = 0;
+  int seq = e < n ? p.group_seqs[e] : -1;
+  const int stated = e < G ? p.prefix_len[e] : 0;
   if (e < G) {
     s_start[e] = p.group_start[e];
     s_least[e] = 0x7FFFFFFF;
@@ -164,12 +180,9 @@ __global__ __launch_bounds__(kPlanThreads) void shared_prefix_plan_kernel(SpPara
     s_owner[e] = 0x7FFFFFFF;
     p.seqs[(int64_t)e * kSpSeqInts] = 0;  // a sequence that no entry names has no rows
   }
-  __syncthreads();
-  uint32_t error = 0;
   // ---- entry e of the groups' list ----
-  int seq = -1, ctx = 0, ql = 0, qs = 0;
+  int ctx = 0, ql = 0, qs = 0;
   if (e < n) {
-    seq = p.group_seqs[e];
     if (seq < 0 || seq >= n) {
       error |= kErrGroups;
       seq = -1;
@@ -208,134 +221,126 @@ __global__ __launch_bounds__(kPlanThreads) void shared_prefix_plan_kernel(SpPara
     atomicMin(&s_leader[g], e);
     atomicAdd(&s_members[g], 1);
   }
-  int64_t tokens;
-  const int t0 = (int)plan_scan(ql, s_part, tokens);
+  int t0[1], tokens[1];
+  plan_scan<1>({ql}, s_part, t0, tokens);
   if (e < n) {
-    s_token0[e] = t0;
+    s_token0[e] = t0[0];
     s_row[e] = qs;
   }
-  if (e == 0) s_token0[n] = (int)tokens;
+  if (e == 0) s_token0[n] = tokens[0];
   __syncthreads();
+  auto first_token = [&](int entry) { return s_token0[min(max(entry, 0), n)]; };
   // ---- group e ----
+  const int table_keys = (int)min((int64_t)p.bt_stride * p.block_size, (int64_t)0x7FFFFFFF);
   int rows = 0, stages = 0, tile_count = 0, prefix = 0;
   if (e < G && s_members[e] > 1) {
-    prefix = min(min(p.prefix_len[e], s_least[e]), min(max_prefix, p.max_ctx));
-    prefix = max(min(prefix, p.bt_stride * p.block_size), 0) & ~(kTileKeys - 1);
+    prefix = min(min(stated, s_least[e]), min(max_prefix, p.max_ctx));
+    prefix = max(min(prefix, table_keys), 0) & ~(kTileKeys - 1);
     if (prefix > 0) {
-      rows = (s_token0[min(max(s_start[e + 1], 0), n)] - s_token0[min(max(s_start[e], 0), n)]) * p.group;
+      rows = (first_token(s_start[e + 1]) - first_token(s_start[e])) * p.group;
       tile_count = cdiv(rows, tile_rows_of(rows));
       stages = cdiv(prefix, kQtKeys);
     }
   }
-  int64_t work, items, part_rows;
-  plan_scan((int64_t)tile_count * stages * p.num_kv_heads, s_part, work);
-  const int share = (int)max((work + kNumCu - 1) / kNumCu, (int64_t)1);
-  const int parts = stages > 0 ? max(stages / share, 1) : 0;
-  const int item0 = (int)plan_scan((int64_t)tile_count * parts, s_part, items);
-  const int64_t row0 = plan_scan((int64_t)rows * parts * p.num_kv_heads, s_part, part_rows);
-  if (e < G) {
-    s_prefix[e] = prefix;
-    s_parts[e] = parts;
-    s_item0[e] = item0;
-    s_row0[e] = row0;
-  }
+  if (e < G) s_prefix[e] = prefix;
   __syncthreads();
   // ---- entry e: its own keys ----
   const int from = g >= 0 ? s_prefix[g] : 0;
-  const int kend = min(min(ctx, p.max_ctx), p.bt_stride * p.block_size);
+  const int kend = min(min(ctx, p.max_ctx), table_keys);
   const int own = ql > 0 ? max(kend - from, 0) : 0;
   const int rows_s = ql * p.group;
   const bool light = rows_s <= kLightRows;
   const int tiles16 = light ? cdiv(own, kTileKeys) : 0;
   const int heavy_tiles = light || own == 0 ? 0 : cdiv(rows_s, tile_rows_of(rows_s));
   const int heavy_stages = light ? 0 : cdiv(own, kQtKeys);
-  int64_t light_work, heavy_work;
-  plan_scan((int64_t)tiles16 * p.head_blocks, s_part, light_work);
-  plan_scan((int64_t)heavy_tiles * heavy_stages * p.num_kv_heads, s_part, heavy_work);
-  const int64_t light_share = (light_work + kNumCu * p.light_keys - 1) / (kNumCu * p.light_keys);
-  const int lshare = (int)max(light_share, (int64_t)kLightMinTiles);
-  const int hshare = (int)max((heavy_work + kNumCu - 1) / kNumCu, (int64_t)2);
+  // ---- the batch's work, and each item's share of it ----
+  int skip[3], work[3];
+  plan_scan<3>({tile_count * stages, tiles16, heavy_tiles * heavy_stages}, s_part, skip, work);
+  const int share = max(ceil_share((int64_t)work[0] * p.num_kv_heads, kNumCu), 1);
+  const int lshare = max(ceil_share((int64_t)work[1] * p.head_blocks, kNumCu * p.light_keys), kLightMinTiles);
+  const int hshare = max(ceil_share((int64_t)work[2] * p.num_kv_heads, kNumCu), 2);
+  const int parts = stages > 0 ? max(stages / share, 1) : 0;
   const int parts_s = light ? (tiles16 > 0 ? max(tiles16 / lshare, 1) : 0) : (heavy_stages > 0 ? max(heavy_stages / hshare, 1) : 0);
   const int light_items = light ? cdiv(parts_s, p.light_keys) : 0;
-  int64_t lights, heavies, part_rows_s;
-  const int light0 = (int)plan_scan(light_items, s_part, lights);
-  const int heavy0 = (int)plan_scan((int64_t)heavy_tiles * parts_s, s_part, heavies);
-  const int64_t srow0 = part_rows + plan_scan((int64_t)rows_s * parts_s * p.num_kv_heads, s_part, part_rows_s);
+  // tile items of groups, their partial rows; light items, tile items and partial rows of sequences
+  int at[5], all[5];
+  plan_scan<5>({tile_count * parts, rows * parts * p.num_kv_heads, light_items, heavy_tiles * parts_s, rows_s * parts_s * p.num_kv_heads},
+               s_part, at, all);
+  if (e < G) {
+    s_parts[e] = parts;
+    s_item0[e] = at[0];
+    s_row0[e] = at[1];
+  }
+  __syncthreads();
+  const int items = all[0];
+  const int srow0 = all[1] + at[4];
   // (the workspace's bounds hold for any lengths and groups in order; a list out of order may exceed them)
-  const bool fits = items + heavies <= p.max_tiles && lights <= p.max_lights && part_rows + part_rows_s <= p.part_rows;
+  const bool fits = (int64_t)items + all[3] <= p.max_tiles && all[2] <= p.max_lights && (int64_t)all[1] + all[4] <= p.part_rows;
   if (!fits) error |= kErrGroups;
-  if (e < n && seq >= 0) {
+  if (seq >= 0) {
     int32_t* d = p.seqs + (int64_t)seq * kSpSeqInts;
+    const int group_token0 = g >= 0 ? first_token(s_start[g]) : 0;
     d[0] = fits ? ql : 0;
     d[1] = qs;
-    d[2] = g >= 0 && from > 0 ? s_parts[g] : 0;  // parts of the prefix
-    d[3] = parts_s;                              // parts of its own keys
-    const int64_t pr = g >= 0 ? s_row0[g] + (int64_t)(t0 - s_token0[min(max(s_start[g], 0), n)]) * p.group : 0;
-    d[4] = (int32_t)(pr & 0xFFFFFFFF);
-    d[5] = (int32_t)(pr >> 32);
-    d[6] = g >= 0 ? (s_token0[min(max(s_start[g + 1], 0), n)] - s_token0[min(max(s_start[g], 0), n)]) * p.group : 0;
-    d[7] = (int32_t)(srow0 & 0xFFFFFFFF);
-    d[8] = (int32_t)(srow0 >> 32);
-    d[9] = rows_s;
-    d[10] = ctx;
-    d[11] = from;
+    d[2] = from > 0 ? s_parts[g] : 0;  // parts of the prefix
+    d[3] = parts_s;                    // parts of its own keys
+    d[4] = g >= 0 ? s_row0[g] + (t0[0] - group_token0) * p.group : 0;
+    d[5] = g >= 0 ? (first_token(s_start[g + 1]) - group_token0) * p.group : 0;
+    d[6] = srow0;
+    d[7] = rows_s;
+    d[8] = ctx;
+    d[9] = 0;  // set where a partly hidden key's value is not finite
   }
   if (e == 0) {
-    p.head[1] = fits ? (uint32_t)(items + heavies) : 0;
-    p.head[2] = fits ? (uint32_t)lights : 0;
+    p.head[1] = fits ? (uint32_t)(items + all[3]) : 0;
+    p.head[2] = fits ? (uint32_t)all[2] : 0;
   }
   if (error) atomicOr(p.head, error);
-  __syncthreads();
   if (!fits) return;
   // ---- the groups' tokens, and the items ----
-  for (int i = e; i < (int)tokens; i += kPlanThreads) {
+  for (int i = e; i < tokens[0]; i += threads) {
     const int k = last_from(s_token0, n, i);  // (of entries with the same first token, the last holds it)
     p.tokens[i] = s_row[k] + i - s_token0[k];
   }
-  for (int i = e; i < (int)items; i += kPlanThreads) {
+  for (int i = e; i < items; i += threads) {
     const int k = last_from(s_item0, G, i);
     const int first = s_start[k];
-    const int rows_g = (s_token0[min(max(s_start[k + 1], 0), n)] - s_token0[min(max(first, 0), n)]) * p.group;
+    const int rows_g = (first_token(s_start[k + 1]) - first_token(first)) * p.group;
     const int tr = tile_rows_of(rows_g), count = cdiv(rows_g, tr);
     const int tile = (i - s_item0[k]) % count, part = (i - s_item0[k]) / count;
     const int st = cdiv(s_prefix[k], kQtKeys);
-    const int64_t row = s_row0[k] + (int64_t)part * p.num_kv_heads * rows_g;
     int32_t* d = p.tiles + (int64_t)i * kSpItemInts;
     d[0] = -1 - p.group_seqs[s_leader[k]];  // the sequence whose table is read; negative: a group's item
-    d[1] = s_token0[first];
+    d[1] = first_token(first);
     d[2] = rows_g;
     d[3] = tile * tr;
     d[4] = (int)((int64_t)st * part / s_parts[k]) * kQtKeys;
     d[5] = min((int)((int64_t)st * (part + 1) / s_parts[k]) * kQtKeys, s_prefix[k]);
-    d[6] = (int32_t)(row & 0xFFFFFFFF);
-    d[7] = (int32_t)(row >> 32);
+    d[6] = s_row0[k] + part * p.num_kv_heads * rows_g;
   }
   // entry e's own items (few each)
   if (seq >= 0 && parts_s > 0) {
     for (int i = 0; i < heavy_tiles * parts_s; ++i) {
-      const int tr = tile_rows_of(rows_s);
       const int tile = i % heavy_tiles, part = i / heavy_tiles;
-      const int64_t row = srow0 + (int64_t)part * p.num_kv_heads * rows_s;
-      int32_t* d = p.tiles + ((int64_t)items + heavy0 + i) * kSpItemInts;
+      int32_t* d = p.tiles + ((int64_t)items + at[3] + i) * kSpItemInts;
       d[0] = seq;
-      d[1] = t0;
+      d[1] = t0[0];
       d[2] = rows_s;
-      d[3] = tile * tr;
+      d[3] = tile * tile_rows_of(rows_s);
       d[4] = from + (int)((int64_t)heavy_stages * part / parts_s) * kQtKeys;
       d[5] = min(from + (int)((int64_t)heavy_stages * (part + 1) / parts_s) * kQtKeys, kend);
-      d[6] = (int32_t)(row & 0xFFFFFFFF);
-      d[7] = (int32_t)(row >> 32);
+      d[6] = srow0 + part * p.num_kv_heads * rows_s;
     }
     for (int i = 0; i < light_items; ++i) {
-      int32_t* d = p.lights + ((int64_t)light0 + i) * kSpItemInts;
+      int32_t* d = p.lights + ((int64_t)at[2] + i) * kSpItemInts;
       d[0] = seq;
       d[1] = i * p.light_keys;  // first part
       d[2] = parts_s;
       d[3] = from;
       d[4] = kend;
       d[5] = tiles16;
-      d[6] = (int32_t)(srow0 & 0xFFFFFFFF);
-      d[7] = (int32_t)(srow0 >> 32);
+      d[6] = srow0;
+      d[7] = rows_s;
     }
   }
 }
@@ -373,13 +378,14 @@ __device__ __forceinline__ auto sp_q_operand(u32x4 raw) {
 
 // Probabilities of a 32-key step for MT row tiles: s[mt][t][i] is the score of key 16 t + 4 g + i.
 // kf / vf: the keys' score factors and value factors (int8).  hidden(mt, e): key of slot e = 4 t + i
-// is not seen.  Returns the second product's operands in pb, the probabilities in pr.
+// is not seen.  down: what the outputs so far shrink by (1: nothing changed).  Returns the second
+// product's operands in pb.
 template <bool INT8, int MT, typename Hidden>
 __device__ __forceinline__ void sp_softmax(const floatx4 (&s)[MT][2], const floatx4 (&kf)[2], const floatx4 (&vf)[2],
-                                           float qk_scale, bool masked, Hidden hidden, SpState<INT8>& st,
-                                           float (&pr)[MT][8], u32x4 (&pb)[MT]) {
+                                           float qk_scale, bool masked, Hidden hidden, float down, SpState<INT8>& st,
+                                           u32x4 (&pb)[MT]) {
   auto factor = [&](int e) { return INT8 ? kf[e >> 2][e & 3] : qk_scale; };
-  float psum[MT];
+  float pr[MT][8], psum[MT];
   auto probs = [&]() {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -400,7 +406,7 @@ __device__ __forceinline__ void sp_softmax(const floatx4 (&s)[MT][2], const floa
     }
   };
   probs();
-  bool grow = false;
+  bool grow = INT8 && down != 1.f;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) grow |= psum[mt] > kSpLazy;
   if (__ballot(grow)) {
@@ -408,12 +414,13 @@ __device__ __forceinline__ void sp_softmax(const floatx4 (&s)[MT][2], const floa
     for (int mt = 0; mt < MT; ++mt) {
       float mx = kNegBig;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, masked && hidden(mt, e) ? kNegBig : s[mt][e >> 2][e & 3] * factor(e));
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, hidden(mt, e) ? kNegBig : s[mt][e >> 2][e & 3] * factor(e));
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float m_new = fmaxf(st.m[mt], mx);
-      const float alpha = __builtin_amdgcn_exp2f(st.m[mt] - m_new);
+      float alpha = __builtin_amdgcn_exp2f(st.m[mt] - m_new);
       st.l[mt] *= alpha;
+      if constexpr (INT8) alpha *= down;
 #pragma unroll
       for (int j = 0; j < 8; ++j) st.o[mt][j] *= alpha;
       st.m[mt] = m_new;
@@ -423,24 +430,26 @@ __device__ __forceinline__ void sp_softmax(const floatx4 (&s)[MT][2], const floa
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     st.l[mt] += psum[mt];
-    const float(&x)[8] = pr[mt];
+    float(&x)[8] = pr[mt];
     if constexpr (INT8) {
-      // (a hidden key's value scale may be anything)
-      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = x[e] * vf[e >> 2][e & 3];
-        if (masked) y[e] = hidden(mt, e) ? 0.f : y[e];
+      for (int e = 0; e < 8; ++e) x[e] *= vf[e >> 2][e & 3];
+      if (masked) {  // (a hidden key's value scale may be anything)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = hidden(mt, e) ? 0.f : x[e];
       }
-      pb[mt] = u32x4{pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7])};
+      pb[mt] = u32x4{pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7])};
     } else {
       pb[mt] = u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
     }
   }
 }
 
-__device__ __forceinline__ bool bf16x2_wild(uint32_t x) {  // either half infinite or NaN
-  return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
+// Two bf16 values with 0 in the place of those that are not finite; wild: there was one.
+__device__ __forceinline__ uint32_t bf16x2_tame(uint32_t x, bool& wild) {
+  const bool lo = (x & 0x7F80u) == 0x7F80u, hi = (x & 0x7F800000u) == 0x7F800000u;
+  wild |= lo || hi;
+  return (lo ? 0 : x & 0xFFFFu) | (hi ? 0 : x & 0xFFFF0000u);
 }
 
 // Exponent of a positive finite scale, as an integer power of two above it.
@@ -460,8 +469,7 @@ __device__ __forceinline__ int sp_slot(const SpParams& p, const int32_t* bt, int
 
 // ---- tiles ----
 constexpr int kSpExpOff = kQtSlotOff + 2 * 8 * 4;  // int [2 buffers][2 waves]: the stage's largest value-scale exponents
-constexpr int kSpWildOff = kSpExpOff + 2 * 2 * 4;  // int [2 buffers][8 waves]: values that are not finite
-constexpr int kSpLds = kSpWildOff + 2 * 8 * 4;
+constexpr int kSpLds = kSpExpOff + 2 * 2 * 4;
 
 template <bool INT8, int SDT>
 __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int head, char* smem) {
@@ -470,7 +478,7 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
   const int lane = tid % kWave;
   const ConstI32* d = (const ConstI32*)(p.tiles + (int64_t)item * kSpItemInts);
   const int who = d[0], tok0 = d[1], rows_total = d[2], row0 = d[3], kstart = d[4], kend = d[5];
-  const int64_t part_row = ((int64_t)d[7] << 32) | (uint32_t)d[6];
+  const int64_t part_row = d[6];
   const bool of_group = who < 0;
   const int seq = of_group ? -1 - who : who;
   const int kg_count = 256 / tile_rows_of(rows_total);
@@ -479,7 +487,7 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
   int first_seen = kend;
   if (!of_group) {
     const ConstI32* sd = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
-    first_seen = sd[10] - sd[0] + 1;  // of query 0
+    first_seen = sd[8] - sd[0] + 1;  // of query 0
   }
   const int r = lane & 15;
   const int g = lane >> 4;
@@ -487,7 +495,6 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
   const int wrow0 = row0 + (wave % row_groups) * kQtWaveRows;
   int* s_slot = (int*)(smem + kQtSlotOff);
   int* s_exp = (int*)(smem + kSpExpOff);
-  int* s_wild = (int*)(smem + kSpWildOff);
   const int32_t* bt = p.block_tables + (int64_t)seq * p.bt_stride;
   auto tile_slot = [&](int tile16) {
     return sp_slot(p, bt, min(kstart + kTileKeys * tile16, (kend - 1) & ~(kTileKeys - 1)));
@@ -522,25 +529,30 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
   QtRegs<INT8> R;
   int vexp = -126;  // value scales are taken relative to 2^vexp
   auto stage_store = [&](int buf, int kb) {
+    if constexpr (!INT8) {
+      if (kb + kQtKeys > first_seen) {  // keys that some row does not see
+        bool wild = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (kb + qt_octet_key(tid >> 5, e) < first_seen) continue;
+          R.v[e][0] = bf16x2_tame(R.v[e][0], wild);
+          R.v[e][1] = bf16x2_tame(R.v[e][1], wild);
+        }
+        if (wild) p.seqs[(int64_t)seq * kSpSeqInts + 9] = 1;
+      }
+    }
     qt_store_kv<INT8>(smem, buf, tid, R);
     if constexpr (INT8) {
       if (tid < 2 * kQtKeys) {
         float* sc = (float*)(smem + kQtScaleOff) + buf * 2 * kQtKeys;
         sc[tid] = tid < kQtKeys ? R.sc * p.qk_scale : R.sc;
         if (tid >= kQtKeys) {
-          const bool finite = fabsf(R.sc) < INFINITY;
-          int x = finite ? scale_exp(R.sc) : -126;
+          int x = fabsf(R.sc) < INFINITY ? scale_exp(R.sc) : -126;
 #pragma unroll
           for (int o = 32; o >= 1; o >>= 1) x = max(x, __shfl_xor(x, o));
           if (lane == 0) s_exp[buf * 2 + wave - kQtKeys / kWave] = x;
         }
       }
-    } else {
-      bool wild = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) wild |= bf16x2_wild(R.v[e][0]) || bf16x2_wild(R.v[e][1]);
-      const bool any = __ballot(wild) != 0;
-      if (lane == 0) s_wild[buf * kSpWaves + wave] = any;
     }
   };
   const int n_stages = (kend - kstart + kQtKeys - 1) / kQtKeys;
@@ -557,24 +569,14 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
       if (tid < 8) next_slot = tile_slot(8 * (t + 2) + tid);
     }
     __asm__ __volatile__("" ::: "memory");  // the loads go out before the products
-    float vscale = 1.f;
-    bool wild = false;
+    float vscale = 1.f, down = 1.f;
     if constexpr (INT8) {
-      const int x = __builtin_amdgcn_readfirstlane(max(s_exp[buf * 2], s_exp[buf * 2 + 1]));
-      if (x > vexp) {
-        const float down = pow2(vexp - x);  // (2^-126 or less: what was added so far had scales that small)
-#pragma unroll
-        for (int mt = 0; mt < kQtMT; ++mt)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) st.o[mt][j] *= down;
+      if (kb0 + 32 * kg < kend_wave) {  // (a wave without a step here keeps its own power)
+        const int x = max(__builtin_amdgcn_readfirstlane(max(s_exp[buf * 2], s_exp[buf * 2 + 1])), vexp);
+        down = pow2(vexp - x);  // (2^-126 or less: what was added so far had scales that small)
         vexp = x;
       }
       vscale = pow2(-vexp);
-    } else {
-      int any = 0;
-#pragma unroll
-      for (int w = 0; w < kSpWaves; ++w) any |= s_wild[buf * kSpWaves + w];
-      wild = __builtin_amdgcn_readfirstlane(any) != 0;
     }
 #pragma unroll 1
     for (int u = kg; u < 4; u += kg_count) {
@@ -603,42 +605,20 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
         vf[0] = *(const floatx4*)(sc + kQtKeys) * vscale;
         vf[1] = *(const floatx4*)(sc + kQtKeys + 16) * vscale;
       }
-      float pr[kQtMT][8];
       u32x4 pb[kQtMT];
       sp_softmax<INT8, kQtMT>(
           s, kf, vf, p.qk_scale, masked,
-          [&](int mt, int e) { return kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend_row[mt]; }, st, pr, pb);
-      if (!INT8 && wild && masked) {  // key by key
+          [&](int mt, int e) { return kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend_row[mt]; }, down, st, pb);
+      down = 1.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const u32x4 a = *(const u32x4*)(vs + r * 256 + qt_v_pos(r, 4 * u + g) * 16 + j * 16 * 256);
 #pragma unroll
         for (int mt = 0; mt < kQtMT; ++mt) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            for (int gg = 0; gg < 4; ++gg) {
-              const float x = __shfl(pr[mt][e], r + 16 * gg);
-              const int key = 16 * (e >> 2) + 4 * gg + (e & 3);
-              if (kb + key >= kend_row[mt]) continue;
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int dim = 16 * j + 4 * g + i;
-                  const uint16_t* v = (const uint16_t*)(vs + dim * 256 + qt_v_pos(dim & 15, 4 * u + gg) * 16);
-                  st.o[mt][j][i] += x * bf16_to_f32(v[e]);
-                }
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const u32x4 a = *(const u32x4*)(vs + r * 256 + qt_v_pos(r, 4 * u + g) * 16 + j * 16 * 256);
-#pragma unroll
-          for (int mt = 0; mt < kQtMT; ++mt) {
-            if constexpr (INT8)
-              st.o[mt][j] = sp_mfma<true>(a, __builtin_bit_cast(f16x8, pb[mt]), st.o[mt][j]);
-            else
-              st.o[mt][j] = sp_mfma<false>(a, __builtin_bit_cast(bf16x8, pb[mt]), st.o[mt][j]);
-          }
+          if constexpr (INT8)
+            st.o[mt][j] = sp_mfma<true>(a, __builtin_bit_cast(f16x8, pb[mt]), st.o[mt][j]);
+          else
+            st.o[mt][j] = sp_mfma<false>(a, __builtin_bit_cast(bf16x8, pb[mt]), st.o[mt][j]);
         }
       }
     }
@@ -653,6 +633,10 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
   for (int mt = 0; mt < kQtMT; ++mt) {
     st.l[mt] += __shfl_xor(st.l[mt], 16);
     st.l[mt] += __shfl_xor(st.l[mt], 32);
+    if constexpr (INT8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) st.o[mt][j] *= pow2(vexp);
+    }
   }
   if (kg_count > 1) {
     floatx4* s_part = (floatx4*)smem;
@@ -685,70 +669,117 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
       }
     }
   }
-  const float back = INT8 ? pow2(vexp) : 1.f;
 #pragma unroll
   for (int mt = 0; mt < kQtMT; ++mt) {
     const int row = wrow0 + kRows * mt + r;
     if (row >= rows_total) continue;
     const int64_t to = part_row + (int64_t)head * rows_total + row;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) *(floatx4*)(p.part_o + to * kHeadDim + 16 * j + 4 * g) = st.o[mt][j] * back;
+    for (int j = 0; j < 8; ++j) *(floatx4*)(p.part_o + to * kHeadDim + 16 * j + 4 * g) = st.o[mt][j];
     if (g == 0) *(float2*)(p.part_ml + to * 2) = float2{st.m[mt], st.l[mt]};
   }
 }
 
 // ---- light items ----
-// A wave's registers of a 32-key step on its way from memory.
+// A wave streams its KV head's tiles of 16 keys through a ring in LDS, copied by the memory system
+// (no registers in flight), and holds one 32-key step in registers: the ring's two slots are
+// requested again as soon as they are read.  Rows are swizzled in 16-byte chunks so that the
+// fragment reads are free of conflicts.
+template <bool INT8>
+struct Light {
+  static constexpr int kRowBytes = INT8 ? kHeadDim : 2 * kHeadDim;
+  static constexpr int kTile = kTileKeys * kRowBytes;           // K (or V) of a tile
+  static constexpr int kScale = INT8 ? 256 : 0;                 // key scales' dwords, then value scales'
+  static constexpr int kSlot = 2 * kTile + kScale;
+  static constexpr int kRing = INT8 ? 4 : 2;                    // tiles
+  static constexpr int kCopies = 2 * kTile / 1024 + (INT8 ? 1 : 0);  // copy instructions per tile
+  static constexpr int kChunks = kRowBytes / 16;                // per row
+};
+constexpr int kLightWindow = 512;  // tiles whose slots a wave lists at a time
+constexpr int kLightWaveBytes = Light<true>::kRing * Light<true>::kSlot;
+static_assert(Light<false>::kRing * Light<false>::kSlot <= kLightWaveBytes, "a wave's ring");
+constexpr int kLightSlotOff = kSpWaves * kLightWaveBytes;  // int [waves][kLightWindow]
+constexpr int kLightScaleOff = kLightSlotOff + kSpWaves * kLightWindow * 4;  // float [waves][64]
+constexpr int kLightLds = kLightScaleOff + kSpWaves * kWave * 4;
+static_assert(kLightLds <= 160 * 1024, "LDS of one CU");
+
+template <int BYTES>
+__device__ __forceinline__ void copy_to_lds(const void* src, void* lds) {
+  static_assert(BYTES == 16 || BYTES == 4, "bytes per lane");
+  if constexpr (BYTES == 16)
+    __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+  else
+    __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+}
+// s_waitcnt with only vmcnt or only lgkmcnt (0) constrained
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+__device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4)); }
+// At most the copies of the n newest tiles (0 .. 2) still in flight.
+template <int PER>
+__device__ __forceinline__ void wait_tiles(int n) {
+  if (n <= 0)
+    wait_vmcnt<0>();
+  else if (n == 1)
+    wait_vmcnt<PER>();
+  else
+    wait_vmcnt<2 * PER>();
+}
+
+// A 32-key step in registers: K chunk c of tile t holds dims 32 g + 8 c .. of key r (int8: bytes of
+// two chunks in one vector); V slot e dims 8 r .. of key 16 (e / 4) + 4 g + e % 4.
 template <bool INT8>
 struct LightRegs;
 template <>
 struct LightRegs<true> {
-  u32x4 k[2][2];  // [tile][half]: bytes 64 half + 16 g .. of key r
-  u32x2 v[8];     // [slot e]: bytes 8 r .. of key 16 (e / 4) + 4 g + e % 4
-  float sc;       // lanes 0..31: key scale of key lane; 32..63: value scale of key lane - 32
+  u32x4 k[2][2];
+  u32x2 v[8];
 };
 template <>
 struct LightRegs<false> {
-  u32x4 k[2][4];  // [tile][chunk]: dims 32 chunk + 8 g .. of key r
-  u32x4 v[8];     // [slot e]: dims 8 r .. of the key
+  u32x4 k[2][4];
+  u32x4 v[8];
 };
 
-template <bool INT8, int SDT>
-__device__ __forceinline__ void light_load(const SpParams& p, int slot_a, int slot_b, int head, int lane, LightRegs<INT8>& R) {
-  constexpr int kEsz = INT8 ? 1 : 2;
-  const int64_t slot_bytes = (int64_t)p.num_kv_heads * kHeadDim * kEsz;
-  const int r = lane & 15, g = lane >> 4;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int64_t at = (t ? slot_b : slot_a) * slot_bytes + (int64_t)head * kHeadDim * kEsz;
-    const char* kc = (const char*)p.k_cache + at + r * slot_bytes + 16 * g;
-    const char* vc = (const char*)p.v_cache + at + 4 * g * slot_bytes + 8 * kEsz * r;
-#pragma unroll
-    for (int c = 0; c < (INT8 ? 2 : 4); ++c) R.k[t][c] = *(const u32x4*)(kc + 64 * c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (INT8)
-        R.v[4 * t + i] = *(const u32x2*)(vc + i * slot_bytes);
-      else
-        R.v[4 * t + i] = *(const u32x4*)(vc + i * slot_bytes);
-    }
-  }
-  if constexpr (INT8) {
-    const int64_t slot = ((lane & 16) ? slot_b : slot_a) + (lane & 15);
-    R.sc = load_scale<SDT>(lane < 32 ? p.k_scale : p.v_scale, slot * p.num_kv_heads + head);
-  }
-}
-
 template <bool INT8, int SDT, int MT>
-__device__ __forceinline__ void sp_light(const SpParams& p, int seq, int head, int kstart, int kend, int64_t part_row, char* smem) {
+__device__ __forceinline__ void sp_light(const SpParams& p, int seq, int head, int kstart0, int kend0, int64_t part_row, char* smem) {
+  using L = Light<INT8>;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
   const int r = lane & 15, g = lane >> 4;
   const ConstI32* sd = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
-  const int ql = sd[0], qs = sd[1], rows_total = sd[9], ctx = sd[10];
+  const int ql = sd[0], qs = sd[1], rows_total = sd[7], ctx = sd[8];
   const int first_seen = ctx - ql + 1;
   const int32_t* bt = p.block_tables + (int64_t)seq * p.bt_stride;
+  char* ring = smem + wave * kLightWaveBytes;
+  int* s_slot = (int*)(smem + kLightSlotOff) + wave * kLightWindow;
+  float* s_sc = (float*)(smem + kLightScaleOff) + wave * kWave;
+  const int64_t slot_bytes = (int64_t)p.num_kv_heads * L::kRowBytes;
+  // this lane's part of a copy: key, and chunk position
+  constexpr int kPerCopy = 1024 / L::kRowBytes;  // keys per copy
+  const int copy_key = lane / L::kChunks, copy_pos = lane % L::kChunks;
+  auto copy_tile = [&](int t) {  // tile t of the window
+    const int64_t slot0 = __builtin_amdgcn_readfirstlane(s_slot[t]);
+    char* dst = ring + (t % L::kRing) * L::kSlot;
+    const char* kc = (const char*)p.k_cache + slot0 * slot_bytes + (int64_t)head * L::kRowBytes;
+    const char* vc = (const char*)p.v_cache + slot0 * slot_bytes + (int64_t)head * L::kRowBytes;
+#pragma unroll
+    for (int j = 0; j < L::kTile / 1024; ++j) {
+      const int key = j * kPerCopy + copy_key;
+      const uint32_t off = (uint32_t)key * (uint32_t)slot_bytes + 16u * (uint32_t)(copy_pos ^ (key & (L::kChunks - 1)));
+      copy_to_lds<16>(kc + off, dst + j * 1024);
+      copy_to_lds<16>(vc + off, dst + L::kTile + j * 1024);
+    }
+    if constexpr (INT8) {
+      // lanes 0..15: the dwords that hold the keys' scales, 16..31 the values' (the rest repeat them)
+      const int64_t at = (slot0 + (lane & 15)) * p.num_kv_heads + head;
+      copy_to_lds<4>((const char*)((lane & 16) ? p.v_scale : p.k_scale) + (at & ~1ll) * 2, dst + 2 * L::kTile);
+    }
+  };
   SpState<INT8> st;
   int kend_row[MT];
 #pragma unroll
@@ -756,144 +787,152 @@ __device__ __forceinline__ void sp_light(const SpParams& p, int seq, int head, i
     const int row = kRows * mt + r;
     const bool valid = row < rows_total;
     const int t = valid ? row / p.group : 0;
-    kend_row[mt] = valid ? min(kend, first_seen + t) : 0;
+    kend_row[mt] = valid ? min(kend0, first_seen + t) : 0;
     const uint16_t* src = p.q + (int64_t)(qs + t) * p.q_tok_stride +
-                          (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride;
+                          (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride + 32 * g;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      // int8 keys come as bytes 64 h + 16 g + 8 c' of chunk 2 h + c': the same dims of the query
-      const int at = INT8 ? 64 * (c >> 1) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
-      st.q[mt].q[c] = sp_q_operand<INT8>(*(const u32x4*)(src + at));
-    }
+    for (int c = 0; c < 4; ++c) st.q[mt].q[c] = sp_q_operand<INT8>(*(const u32x4*)(src + 8 * c));
     st.m[mt] = kNegBig;
     st.l[mt] = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) st.o[mt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  const int n_tiles = (kend - kstart + kTileKeys - 1) / kTileKeys;
-  const int n_steps = (n_tiles + 1) / 2;
-  const int kfull = min(kend, first_seen);
-  // slots of 64 tiles at a time, one per lane
-  int slots = 0;
-  auto fetch_slots = [&](int tile0) { slots = sp_slot(p, bt, kstart + kTileKeys * min(tile0 + lane, n_tiles - 1)); };
-  auto slot_of = [&](int tile) { return __builtin_amdgcn_readlane(slots, min(tile, n_tiles - 1) & 63); };
-  fetch_slots(0);
-  LightRegs<INT8> R, N;
-  light_load<INT8, SDT>(p, slot_of(0), slot_of(1), head, lane, R);
   int vexp = -126;
-  float* s_sc = (float*)smem + wave * kWave;
-  for (int it = 0; it < n_steps; ++it) {
-    if (it + 1 < n_steps) {
-      if (((2 * it + 2) & 63) == 0) fetch_slots(2 * it + 2);
-      light_load<INT8, SDT>(p, slot_of(2 * it + 2), slot_of(2 * it + 3), head, lane, N);
-    }
-    __asm__ __volatile__("" ::: "memory");
-    const int kb = kstart + 32 * it;
-    const bool masked = kb + 32 > kfull;
-    floatx4 s[MT][2];
+  const int kfull = min(kend0, first_seen);
+  for (int kstart = kstart0; kstart < kend0; kstart += kLightWindow * kTileKeys) {
+    const int kend = min(kend0, kstart + kLightWindow * kTileKeys);
+    const int n_tiles = (kend - kstart + kTileKeys - 1) / kTileKeys;
+    const int n_steps = (n_tiles + 1) / 2;
+    for (int t = lane; t < n_tiles; t += kWave) s_slot[t] = sp_slot(p, bt, kstart + kTileKeys * t);
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < L::kRing; ++t)
+      if (t < n_tiles) copy_tile(t);
+#pragma unroll 1
+    for (int it = 0; it < n_steps; ++it) {
+      const int kb = kstart + 32 * it;
+      const bool masked = kb + 32 > kfull;
+      wait_tiles<L::kCopies>(min(n_tiles, 2 * it + L::kRing) - (2 * it + 2));
+      LightRegs<INT8> R;
+      float sc = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) s[mt][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t) {
+        const char* sl = ring + ((2 * it + t) % L::kRing) * L::kSlot;
+        if constexpr (INT8) {
+          R.k[t][0] = *(const u32x4*)(sl + r * 128 + ((2 * g) ^ (r & 7)) * 16);
+          R.k[t][1] = *(const u32x4*)(sl + r * 128 + ((2 * g + 1) ^ (r & 7)) * 16);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        u32x4 a;
-        if constexpr (INT8)
-          a = i8x8_f16x8(R.k[t][c >> 1][2 * (c & 1)], R.k[t][c >> 1][2 * (c & 1) + 1]);
-        else
-          a = R.k[t][c];
+          for (int i = 0; i < 4; ++i) {
+            const int key = 4 * g + i;
+            R.v[4 * t + i] = *(const u32x2*)(sl + L::kTile + key * 128 + ((r >> 1) ^ (key & 7)) * 16 + (r & 1) * 8);
+          }
+        } else {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[mt][t] = sp_mfma<INT8>(a, st.q[mt].q[c], s[mt][t]);
-      }
-    }
-    floatx4 kf[2], vf[2];
-    if constexpr (INT8) {
-      const int key = kb + (lane & 31);
-      const float x = key < kend ? R.sc : 0.f;  // a slot past the end may hold anything
-      int ex = lane >= 32 && fabsf(x) < INFINITY ? scale_exp(x) : -126;
+          for (int c = 0; c < 4; ++c) R.k[t][c] = *(const u32x4*)(sl + r * 256 + ((4 * g + c) ^ r) * 16);
 #pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) ex = max(ex, __shfl_xor(ex, o));
-      ex = __builtin_amdgcn_readfirstlane(ex);
-      if (ex > vexp) {
-        const float down = pow2(vexp - ex);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) st.o[mt][j] *= down;
-        vexp = ex;
-      }
-      s_sc[lane] = x * (lane < 32 ? p.qk_scale : pow2(-vexp));
-      __builtin_amdgcn_wave_barrier();
-      kf[0] = *(const floatx4*)(s_sc + 4 * g);
-      kf[1] = *(const floatx4*)(s_sc + 16 + 4 * g);
-      vf[0] = *(const floatx4*)(s_sc + 32 + 4 * g);
-      vf[1] = *(const floatx4*)(s_sc + 48 + 4 * g);
-      __builtin_amdgcn_wave_barrier();
-    }
-    float pr[MT][8];
-    u32x4 pb[MT];
-    sp_softmax<INT8, MT>(
-        s, kf, vf, p.qk_scale, masked,
-        [&](int mt, int e) { return kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend_row[mt]; }, (SpState<INT8>&)st, pr, pb);
-    bool wild = false;
-    if constexpr (!INT8) {
-      if (masked) {
-        // values past the end may be stale bits; a value that a row does not see must not reach it
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend) R.v[e] = u32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) wild |= bf16x2_wild(R.v[e][w]);
-        }
-        wild = __ballot(wild) != 0;
-      }
-    }
-    if (!INT8 && wild) {  // key by key, from memory
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          for (int gg = 0; gg < 4; ++gg) {
-            const float x = __shfl(pr[mt][e], r + 16 * gg);
-            const int key = kb + 16 * (e >> 2) + 4 * gg + (e & 3);
-            if (key >= kend_row[mt]) continue;
-            const int64_t slot = (int64_t)sp_slot(p, bt, key);
-            const uint16_t* v = (const uint16_t*)p.v_cache + (slot * p.num_kv_heads + head) * kHeadDim + 32 * g;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) st.o[mt][j][i] += x * bf16_to_f32(v[8 * i + j]);
+          for (int i = 0; i < 4; ++i) {
+            const int key = 4 * g + i;
+            R.v[4 * t + i] = *(const u32x4*)(sl + L::kTile + key * 256 + (r ^ key) * 16);
           }
         }
       }
-    } else {
+      if constexpr (INT8) {
+        // lanes 0..31: key scale of key lane; 32..63: value scale of key lane - 32
+        const int key = lane & 31;
+        const char* sl = ring + ((2 * it + (key >> 4)) % L::kRing) * L::kSlot + 2 * L::kTile;
+        const uint32_t two = *(const uint32_t*)(sl + ((lane >> 5) * 16 + (key & 15)) * 4);
+        const int64_t at = (int64_t)(key & 15) * p.num_kv_heads + head;  // (a tile's first slot is even)
+        const uint16_t raw = (uint16_t)((at & 1) ? two >> 16 : two);
+        sc = SDT == NE_DTYPE_BF16 ? bf16_to_f32(raw) : f16_to_f32(raw);
+        sc = kb + key < kend ? sc : 0.f;  // a slot past the end may hold anything
+      }
+      wait_lgkmcnt0();  // the two slots are read: request them again
+      if (2 * it + L::kRing < n_tiles) copy_tile(2 * it + L::kRing);
+      if (2 * it + 1 + L::kRing < n_tiles) copy_tile(2 * it + 1 + L::kRing);
+      floatx4 s[MT][2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        u32x4 a;
-        if constexpr (INT8) {
-          uint32_t x[8];
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = R.v[e][j >> 2];
-          a = (j & 3) == 0   ? i8_cols_f16x8<0>(x)
-              : (j & 3) == 1 ? i8_cols_f16x8<1>(x)
-              : (j & 3) == 2 ? i8_cols_f16x8<2>(x)
-                             : i8_cols_f16x8<3>(x);
-        } else {
-          const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-          a = u32x4{__builtin_amdgcn_perm(R.v[1][j >> 1], R.v[0][j >> 1], sel), __builtin_amdgcn_perm(R.v[3][j >> 1], R.v[2][j >> 1], sel),
-                    __builtin_amdgcn_perm(R.v[5][j >> 1], R.v[4][j >> 1], sel), __builtin_amdgcn_perm(R.v[7][j >> 1], R.v[6][j >> 1], sel)};
-        }
+        for (int mt = 0; mt < MT; ++mt) s[mt][t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int c = 0; c < 4; ++c) {
+          u32x4 a;
           if constexpr (INT8)
-            st.o[mt][j] = sp_mfma<true>(a, __builtin_bit_cast(f16x8, pb[mt]), st.o[mt][j]);
+            a = i8x8_f16x8(R.k[t][c >> 1][2 * (c & 1)], R.k[t][c >> 1][2 * (c & 1) + 1]);
           else
-            st.o[mt][j] = sp_mfma<false>(a, __builtin_bit_cast(bf16x8, pb[mt]), st.o[mt][j]);
+            a = R.k[t][c];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) s[mt][t] = sp_mfma<INT8>(a, st.q[mt].q[c], s[mt][t]);
+        }
+      }
+      floatx4 kf[2], vf[2];
+      float down = 1.f;
+      if constexpr (INT8) {
+        const int ex = lane >= 32 && fabsf(sc) < INFINITY ? scale_exp(sc) : -126;
+        if (__ballot(ex > vexp)) {  // a larger value scale than so far
+          int top = ex;
+#pragma unroll
+          for (int o = 32; o >= 1; o >>= 1) top = max(top, __shfl_xor(top, o));
+          top = __builtin_amdgcn_readfirstlane(top);
+          down = pow2(vexp - top);
+          vexp = top;
+        }
+        s_sc[lane] = sc * (lane < 32 ? p.qk_scale : pow2(-vexp));
+        __builtin_amdgcn_wave_barrier();
+        kf[0] = *(const floatx4*)(s_sc + 4 * g);
+        kf[1] = *(const floatx4*)(s_sc + 16 + 4 * g);
+        vf[0] = *(const floatx4*)(s_sc + 32 + 4 * g);
+        vf[1] = *(const floatx4*)(s_sc + 48 + 4 * g);
+        __builtin_amdgcn_wave_barrier();
+      }
+      u32x4 pb[MT];
+      sp_softmax<INT8, MT>(
+          s, kf, vf, p.qk_scale, masked,
+          [&](int mt, int e) { return kb + 16 * (e >> 2) + 4 * g + (e & 3) >= kend_row[mt]; }, down, st, pb);
+      if constexpr (!INT8) {
+        if (masked) {
+          // values past the end may be stale bits; one that some row does not see must not reach that row
+          bool wild = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int key = kb + 16 * (e >> 2) + 4 * g + (e & 3);
+            if (key >= kend) R.v[e] = u32x4{0, 0, 0, 0};
+            if (key < first_seen) continue;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) R.v[e][w] = bf16x2_tame(R.v[e][w], wild);
+          }
+          if (wild) p.seqs[(int64_t)seq * kSpSeqInts + 9] = 1;
+        }
+      }
+      {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u32x4 a;
+          if constexpr (INT8) {
+            uint32_t x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = R.v[e][j >> 2];
+            a = (j & 3) == 0   ? i8_cols_f16x8<0>(x)
+                : (j & 3) == 1 ? i8_cols_f16x8<1>(x)
+                : (j & 3) == 2 ? i8_cols_f16x8<2>(x)
+                               : i8_cols_f16x8<3>(x);
+          } else {
+            const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+            a = u32x4{__builtin_amdgcn_perm(R.v[1][j >> 1], R.v[0][j >> 1], sel), __builtin_amdgcn_perm(R.v[3][j >> 1], R.v[2][j >> 1], sel),
+                      __builtin_amdgcn_perm(R.v[5][j >> 1], R.v[4][j >> 1], sel), __builtin_amdgcn_perm(R.v[7][j >> 1], R.v[6][j >> 1], sel)};
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            if constexpr (INT8)
+              st.o[mt][j] = sp_mfma<true>(a, __builtin_bit_cast(f16x8, pb[mt]), st.o[mt][j]);
+            else
+              st.o[mt][j] = sp_mfma<false>(a, __builtin_bit_cast(bf16x8, pb[mt]), st.o[mt][j]);
+          }
         }
       }
     }
-    R = N;
   }
+  wait_vmcnt<0>();  // no copy lands in LDS after the wave has left
   const float back = INT8 ? pow2(vexp) : 1.f;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -913,6 +952,8 @@ __device__ __forceinline__ void sp_light(const SpParams& p, int seq, int head, i
   }
 }
 
+constexpr int kSpAllLds = kSpLds > kLightLds ? kSpLds : kLightLds;
+
 template <bool INT8, int SDT>
 __global__ __launch_bounds__(kSpThreads) void shared_prefix_parts_kernel(SpParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -929,13 +970,13 @@ __global__ __launch_bounds__(kSpThreads) void shared_prefix_parts_kernel(SpParam
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   const ConstI32* d = (const ConstI32*)(p.lights + (int64_t)item * kSpItemInts);
   const int seq = d[0], part = d[1] + wave / p.light_heads, parts = d[2], from = d[3], kend = d[4], tiles = d[5];
+  const int rows = d[7];
   const int kv = (b % p.head_blocks) * p.light_heads + wave % p.light_heads;
   if (wave >= p.light_heads * p.light_keys || part >= parts || kv >= p.num_kv_heads) return;  // (no barrier follows)
   const int k0 = from + (int)((int64_t)tiles * part / parts) * kTileKeys;
   const int k1 = min(from + (int)((int64_t)tiles * (part + 1) / parts) * kTileKeys, kend);
-  const ConstI32* sd = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
-  const int64_t row = (((int64_t)d[7] << 32) | (uint32_t)d[6]) + (int64_t)part * p.num_kv_heads * sd[9];
-  if (sd[9] <= kRows)
+  const int64_t row = d[6] + (int64_t)part * p.num_kv_heads * rows;
+  if (rows <= kRows)
     sp_light<INT8, SDT, 1>(p, seq, kv, k0, k1, row, smem);
   else
     sp_light<INT8, SDT, 2>(p, seq, kv, k0, k1, row, smem);
@@ -955,9 +996,8 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
   const int i = x / heads, head = x % heads;
   const int kv = head / p.group, in = i * p.group + head % p.group;
   const int np = d[2], n = np + d[3];
-  const int64_t prefix0 = (((int64_t)d[5] << 32) | (uint32_t)d[4]) + (int64_t)kv * d[6] + in;
-  const int64_t own0 = (((int64_t)d[8] << 32) | (uint32_t)d[7]) + (int64_t)kv * d[9] + in;
-  const int64_t prefix_step = (int64_t)p.num_kv_heads * d[6], own_step = (int64_t)p.num_kv_heads * d[9];
+  const int64_t prefix0 = d[4] + kv * d[5] + in, own0 = d[6] + kv * d[7] + in;
+  const int64_t prefix_step = p.num_kv_heads * d[5], own_step = p.num_kv_heads * d[7];
   const int cd = (threadIdx.x & 15) * 8;
   float M = kNegBig, L = 0.f;
   float acc[8] = {};
@@ -989,6 +1029,18 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
       for (int c = 0; c < 4; ++c) {
         acc[c] += w * a[j][c];
         acc[c + 4] += w * b[j][c];
+      }
+    }
+  }
+  if (d[9]) {  // values that are not finite, of keys that only some rows see: this row's
+    const int last = min(d[8] - d[0] + i, min(d[8], p.max_ctx) - 1);  // the last key it sees
+    for (int key = max(d[8] - d[0] + 1, 0); key <= last && key / p.block_size < p.bt_stride; ++key) {
+      const int64_t slot = sp_slot(p, p.block_tables + (int64_t)seq * p.bt_stride, key);
+      const uint16_t* v = (const uint16_t*)p.v_cache + (slot * p.num_kv_heads + kv) * kHeadDim + cd;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float x = bf16_to_f32(v[c]);
+        acc[c] += fabsf(x) < INFINITY ? 0.f : x;
       }
     }
   }
@@ -1088,6 +1140,7 @@ int sp_check(const char* what, int num_seqs, int num_groups, int num_q_heads, in
   NE_CHECK_ARG(ws, "%s: null workspace", what);
   NE_CHECK_ARG((uintptr_t)ws % 16 == 0, "%s: workspace must be 16-byte aligned", what);
   l = sp_layout(num_seqs, num_groups, num_q_heads, num_kv_heads, max_q, max_ctx, max_prefix);
+  NE_CHECK_SUPPORTED(l.part_rows < (1ll << 31), "%s: %lld rows of partial sums", what, (long long)l.part_rows);
   if (bytes < l.total) {
     set_error("%s: workspace of %zu bytes, %zu needed", what, bytes, l.total);
     return NE_EWORKSPACE;
@@ -1114,13 +1167,13 @@ void sp_bind(SpParams& p, const SpLayout& l, char* ws) {
 template <bool INT8, int SDT>
 int sp_launch(const SpParams& p, hipStream_t s) {
   static const hipError_t attr = hipFuncSetAttribute((const void*)shared_prefix_parts_kernel<INT8, SDT>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kSpLds);
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kSpAllLds);
   if (attr != hipSuccess) {
-    set_error("shared_prefix_parts: cannot reserve %d bytes of LDS: %s", kSpLds, hipGetErrorString(attr));
+    set_error("shared_prefix_parts: cannot reserve %d bytes of LDS: %s", kSpAllLds, hipGetErrorString(attr));
     return NE_ELAUNCH;
   }
   const int grid = p.max_tiles * p.num_kv_heads + p.max_lights * p.head_blocks;
-  hipLaunchKernelGGL((shared_prefix_parts_kernel<INT8, SDT>), dim3(grid), dim3(kSpThreads), kSpLds, s, p);
+  hipLaunchKernelGGL((shared_prefix_parts_kernel<INT8, SDT>), dim3(grid), dim3(kSpThreads), kSpAllLds, s, p);
   const int rc = check_launch("shared_prefix_parts");
   if (rc != NE_OK) return rc;
   const int per_seq = cdiv(p.max_q * p.num_kv_heads * p.group, kMergeRows);
@@ -1173,7 +1226,8 @@ extern "C" int ne_shared_prefix_plan(const int32_t* ctx_len, const int32_t* q_st
   p.max_ctx = max_ctx_len;
   p.bt_stride = block_table_stride;
   p.block_size = block_size;
-  hipLaunchKernelGGL(shared_prefix_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, p, max_prefix_len);
+  const int threads = cdiv(num_seqs < 256 ? 256 : num_seqs, kWave) * kWave;  // one per sequence
+  hipLaunchKernelGGL(shared_prefix_plan_kernel, dim3(1), dim3(threads), 0, (hipStream_t)stream, p, max_prefix_len);
   return check_launch("shared_prefix_plan");
 }
 
@@ -1199,6 +1253,7 @@ extern "C" int ne_shared_prefix_attention(const void* q, int64_t q_token_stride,
   if (int8) {
     NE_CHECK_ARG(k_scale && v_scale, "int8 cache needs scales");
     NE_CHECK_ARG(scale_dtype == NE_DTYPE_BF16 || scale_dtype == NE_DTYPE_FP16, "scales must be bf16 or fp16");
+    NE_CHECK_ARG(((uintptr_t)k_scale | (uintptr_t)v_scale) % 4 == 0, "scales must be 4-byte aligned");
   }
   NE_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 &&
                    (q_token_stride | q_head_stride | out_token_stride | out_head_stride) % 8 == 0,
