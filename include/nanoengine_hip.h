@@ -445,8 +445,9 @@ int ne_advance_and_propose(const int32_t* history, int64_t history_stride, const
  * lengths and groups on the device; ne_shared_prefix_attention computes one layer with it, as
  * often as there are layers, while lengths, groups and block tables stay as they were.
  * Both take the same sizes, and a workspace of ne_shared_prefix_workspace_size() bytes
- * (16-byte aligned), which one stream at a time may use.  Its first word is the error word
- * of the last plan and the calls on it: 1 a context beyond max_ctx_len (keys past it are
+ * (16-byte aligned), which one stream at a time may use.  A prefix is read once for its group
+ * where that saves more than it costs; the workspace's third word is the number of work items
+ * that do.  Its first word is the error word of the last plan and the calls on it: 1 a context beyond max_ctx_len (keys past it are
  * dropped), 2 a sequence of more than max_q_len queries or with rows outside q (not computed),
  * 4 a group list that is out of order or names a sequence twice or outside the batch (such
  * entries are not computed), 8 a block table entry outside the pool (block 0 is read).

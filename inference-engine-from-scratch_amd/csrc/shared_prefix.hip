@@ -50,10 +50,41 @@ constexpr int kSpThreads = kQtThreads;
 constexpr int kSpWaves = kQtWaves;
 constexpr int kSpMaxSeqs = 1024;
 constexpr int kLightRows = 32;       // rows per KV head of a light item
-constexpr int kLightMinTiles = 8;    // least 16-key tiles per wave of a split sequence
-constexpr int kSpItemInts = 8;
+constexpr int kLightMinTiles = 4;    // least 16-key tiles per wave of a split sequence
+// The plan's costs, in the time of 16 keys of a light item that waits for nothing else (0.6 us).
+// A stage of a tile of up to 128 rows waits for its keys as much as it computes (2.9 us), one of 256 computes.
+constexpr int kStageCost = 5, kBigStageCost = 9;
+constexpr int kItemCost = 13;  // an item before its first and after its last keys: 6.5 us (light) to 10 (tile)
+// With this many tiles of 16 keys of eight heads (and as large stages of a head) per CU, 100 MB of an int8
+// pool, they come at the memory's rate.
+constexpr int kStreamTiles = 12, kStreamCost = 3;
+__host__ __device__ constexpr int stage_cost(int tile_rows) { return tile_rows <= 128 ? kStageCost : kBigStageCost; }
+// Sharing has to save this much per CU: a tile item takes longer than a light one, and its partial sums
+// go through memory.
+constexpr int kShareGain = 3;
+// Tiles of 256 rows take a tenth less per row; worth it with this much tile work per CU, as half tiles
+// spread it better.
+constexpr int kBigWork = 60;
 constexpr int kSpSeqInts = 10;
 constexpr float kSpLazy = 256.f;     // probabilities' sum per lane and step before the reference moves
+
+// A work-group's item, as the plan writes it.
+enum : int32_t { kGroupTile = 0, kOwnTile = 1, kLight = 2 };
+struct SpItem {
+  int32_t kind;
+  int32_t seq;         // whose block table is read
+  int32_t head;        // KV head (light: first of the work-group's)
+  int32_t rows_total;  // query rows per KV head of the group, or sequence
+  int32_t row0;        // tile: its first row, and the rows of a tile
+  int32_t tile_rows;
+  int32_t token;       // group tile: its first token in `tokens`; else the sequence's first row of q
+  int32_t first_seen;  // keys that query 0 sees (a later one sees one more each); group tile: all
+  int32_t k0, k1;      // keys
+  int32_t part_row;    // first partial row of KV head 0 (light: and of part 0)
+  int32_t part0, parts, tiles;  // light: its first wave's part of `parts` over `tiles` tiles from k0 on
+  int32_t pad[2];
+};
+static_assert(sizeof(SpItem) == 64, "");
 
 // What bits of the error word mean.
 enum : uint32_t { kErrContext = 1, kErrRows = 2, kErrGroups = 4, kErrBlock = 8 };
@@ -80,22 +111,23 @@ struct SpParams {
   uint16_t* out;
   int64_t o_tok_stride, o_head_stride;
   // workspace
-  uint32_t* head;      // [0] error word, [1] tile items, [2] light items
+  uint32_t* head;      // [0] error word, [1] items, [2] of them of shared prefixes
   int32_t* tokens;     // row of q of every group's tokens, group after group
-  int32_t* tiles;      // [max_tiles][kSpItemInts]
-  int32_t* lights;     // [max_lights][kSpItemInts]
+  SpItem* items;       // [max_items]: tiles, then light items
   int32_t* seqs;       // [num_seqs][kSpSeqInts]
   float* part_o;       // [parts' rows][128]
   float* part_ml;      // [parts' rows][2]
-  int32_t max_tiles, max_lights;
+  int32_t max_items;
   int32_t light_heads, light_keys;  // a light work-group's KV heads, and its waves per KV head
   int32_t head_blocks;              // work-groups per light item
   int64_t part_rows;
 };
 
 __host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
-// Row tiles of 256 or fewer rows: 64, 128 or 256.
-__host__ __device__ inline int tile_rows_of(int rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// Rows of the tiles that `rows` rows are cut into: 64, 128, or (big, if that fills them) 256.
+__host__ __device__ inline int tile_rows_of(int rows, bool big) {
+  return rows <= 64 ? 64 : !big || cdiv(rows, 256) * 256 * 8 > cdiv(rows, 128) * 128 * 9 ? 128 : 256;
+}
 
 // ---- plan ----
 constexpr int kPlanMaxThreads = kSpMaxSeqs;
@@ -158,6 +190,7 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
   __shared__ int s_token0[kSpMaxSeqs + 1];  // per entry: its first token
   __shared__ int s_row[kSpMaxSeqs];         // per entry: its first row of q
   __shared__ int s_owner[kSpMaxSeqs];       // per sequence: its first entry
+  __shared__ int s_alone[kSpMaxSeqs];       // per group: units of its prefix read by every member
   __shared__ int s_parts[kSpMaxSeqs];       // per group
   __shared__ int s_item0[kSpMaxSeqs];       // per group: its first tile item
   __shared__ int s_row0[kSpMaxSeqs];        // per group: its first partial row
@@ -232,35 +265,75 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
   auto first_token = [&](int entry) { return s_token0[min(max(entry, 0), n)]; };
   // ---- group e ----
   const int table_keys = (int)min((int64_t)p.bt_stride * p.block_size, (int64_t)0x7FFFFFFF);
-  int rows = 0, stages = 0, tile_count = 0, prefix = 0;
+  int rows = 0, stages = 0, prefix = 0;
   if (e < G && s_members[e] > 1) {
     prefix = min(min(stated, s_least[e]), min(max_prefix, p.max_ctx));
     prefix = max(min(prefix, table_keys), 0) & ~(kTileKeys - 1);
     if (prefix > 0) {
       rows = (first_token(s_start[e + 1]) - first_token(s_start[e])) * p.group;
-      tile_count = cdiv(rows, tile_rows_of(rows));
       stages = cdiv(prefix, kQtKeys);
     }
   }
+  if (e < G) {
+    s_prefix[e] = prefix;
+    s_alone[e] = 0;
+  }
+  __syncthreads();
+  // ---- what the prefixes would cost read by every member ----
+  const int rows_s = ql * p.group;
+  const bool light = rows_s <= kLightRows;
+  const int kend = min(min(ctx, p.max_ctx), table_keys);
+  if (ql > 0 && g >= 0 && s_prefix[g] > 0) {
+    const int64_t units = light ? (int64_t)(s_prefix[g] / kTileKeys) * p.head_blocks / p.light_keys
+                                : (int64_t)cdiv(rows_s, 128) * cdiv(s_prefix[g], kQtKeys) * kStageCost * p.num_kv_heads;
+    atomicAdd(&s_alone[g], (int)min(units, (int64_t)1 << 20));
+  }
+  __syncthreads();
+  const int64_t shared = (int64_t)cdiv(rows, 128) * stages * kStageCost * p.num_kv_heads;
+  const bool gains = e < G && prefix > 0 && s_alone[e] > shared;
+  int skip[3], sum[3];
+  // (capped so that the sums stay in 32 bits)
+  plan_scan<3>({gains ? (int)min(s_alone[e] - shared, (int64_t)1 << 20) : 0, gains ? min(cdiv(rows, 128) * stages, 1 << 20) : 0,
+                light ? 0 : min(cdiv(rows_s, 128) * cdiv(max(kend, 0), kQtKeys), 1 << 20)},
+               s_part, skip, sum);
+  const bool big = ((int64_t)sum[1] + sum[2]) * p.num_kv_heads * kStageCost >= (int64_t)kBigWork * kNumCu;
+  if (!gains || sum[0] < kShareGain * kNumCu) prefix = rows = stages = 0;
+  const int tile_rows = tile_rows_of(rows, big), tile_count = cdiv(rows, tile_rows);
   if (e < G) s_prefix[e] = prefix;
   __syncthreads();
   // ---- entry e: its own keys ----
   const int from = g >= 0 ? s_prefix[g] : 0;
-  const int kend = min(min(ctx, p.max_ctx), table_keys);
   const int own = ql > 0 ? max(kend - from, 0) : 0;
-  const int rows_s = ql * p.group;
-  const bool light = rows_s <= kLightRows;
+  const int tile_rows_s = tile_rows_of(rows_s, big);
   const int tiles16 = light ? cdiv(own, kTileKeys) : 0;
-  const int heavy_tiles = light || own == 0 ? 0 : cdiv(rows_s, tile_rows_of(rows_s));
+  const int heavy_tiles = light || own == 0 ? 0 : cdiv(rows_s, tile_rows_s);
   const int heavy_stages = light ? 0 : cdiv(own, kQtKeys);
-  // ---- the batch's work, and each item's share of it ----
-  int skip[3], work[3];
-  plan_scan<3>({tile_count * stages, tiles16, heavy_tiles * heavy_stages}, s_part, skip, work);
-  const int share = max(ceil_share((int64_t)work[0] * p.num_kv_heads, kNumCu), 1);
-  const int lshare = max(ceil_share((int64_t)work[1] * p.head_blocks, kNumCu * p.light_keys), kLightMinTiles);
-  const int hshare = max(ceil_share((int64_t)work[2] * p.num_kv_heads, kNumCu), 2);
-  const int parts = stages > 0 ? max(stages / share, 1) : 0;
-  const int parts_s = light ? (tiles16 > 0 ? max(tiles16 / lshare, 1) : 0) : (heavy_stages > 0 ? max(heavy_stages / hshare, 1) : 0);
+  // ---- the batch's work, and a work-group's share of it ----
+  // Each item, one work-group and one per CU at a time, gets keys worth x, so that all take about as long
+  // as the chip takes for the batch: with work W and B uncut items, W / x further ones,
+  //   kNumCu (x + F) = W + F (B + W / x), F = kItemCost.
+  // x >= W / kNumCu for any B, so there are kNumCu further items at most.
+  float x;
+  int stream;
+  {
+    const int64_t mine = ((int64_t)tile_count * stages * stage_cost(tile_rows) + (int64_t)heavy_tiles * heavy_stages * stage_cost(tile_rows_s)) * p.num_kv_heads;
+    int before[5], total[5];  // tile work (1,024 of 48 bits), light work, and uncut items
+    plan_scan<5>({(int)(mine & 0xFFFF), (int)((mine >> 16) & 0xFFFF), (int)(mine >> 32), tiles16,
+                  min((tile_count + heavy_tiles) * p.num_kv_heads + (tiles16 > 0 ? p.head_blocks : 0), 1 << 20)},
+                 s_part, before, total);
+    const float tile_work = (float)total[0] + 65536.f * (float)total[1] + 4294967296.f * (float)total[2];
+    const float light_work = (float)total[3] * (float)p.head_blocks / (float)p.light_keys;
+    stream = light_work + tile_work / (float)kStageCost >= (float)(kStreamTiles * kNumCu) ? kStreamCost : 1;
+    const float W = tile_work + light_work * (float)stream, B = (float)total[4];
+    constexpr float F = kItemCost, C = kNumCu;
+    const float b = C * F - W - F * B;
+    x = fmaxf((sqrtf(b * b + 4.f * C * F * W) - b) / (2.f * C), W / C);
+  }
+  // n / each rounded, 1 at least and n at most
+  auto parts_of = [](int n, float each) { return n > 0 ? min(max((int)((float)n / each + 0.5f), 1), n) : 0; };
+  auto stages_each = [&](int tr) { return fmaxf(x / (float)stage_cost(tr), 1.f); };
+  const int parts = parts_of(stages, stages_each(tile_rows));
+  const int parts_s = light ? parts_of(tiles16, fmaxf(x / (float)stream, (float)kLightMinTiles)) : parts_of(heavy_stages, stages_each(tile_rows_s));
   const int light_items = light ? cdiv(parts_s, p.light_keys) : 0;
   // tile items of groups, their partial rows; light items, tile items and partial rows of sequences
   int at[5], all[5];
@@ -274,15 +347,16 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
   __syncthreads();
   const int items = all[0];
   const int srow0 = all[1] + at[4];
+  const int tile_wgs = (items + all[3]) * p.num_kv_heads, light_wgs = all[2] * p.head_blocks;
   // (the workspace's bounds hold for any lengths and groups in order; a list out of order may exceed them)
-  const bool fits = (int64_t)items + all[3] <= p.max_tiles && all[2] <= p.max_lights && (int64_t)all[1] + all[4] <= p.part_rows;
+  const bool fits = tile_wgs + light_wgs <= p.max_items && (int64_t)all[1] + all[4] <= p.part_rows;
   if (!fits) error |= kErrGroups;
   if (seq >= 0) {
     int32_t* d = p.seqs + (int64_t)seq * kSpSeqInts;
     const int group_token0 = g >= 0 ? first_token(s_start[g]) : 0;
     d[0] = fits ? ql : 0;
     d[1] = qs;
-    d[2] = from > 0 ? s_parts[g] : 0;  // parts of the prefix
+    d[2] = from > 0 ? s_parts[g] : 0;  // parts of the shared prefix
     d[3] = parts_s;                    // parts of its own keys
     d[4] = g >= 0 ? s_row0[g] + (t0[0] - group_token0) * p.group : 0;
     d[5] = g >= 0 ? (first_token(s_start[g + 1]) - group_token0) * p.group : 0;
@@ -292,8 +366,8 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
     d[9] = 0;  // set where a partly hidden key's value is not finite
   }
   if (e == 0) {
-    p.head[1] = fits ? (uint32_t)(items + all[3]) : 0;
-    p.head[2] = fits ? (uint32_t)all[2] : 0;
+    p.head[1] = fits ? (uint32_t)(tile_wgs + light_wgs) : 0;
+    p.head[2] = fits ? (uint32_t)(items * p.num_kv_heads) : 0;  // of them, of shared prefixes
   }
   if (error) atomicOr(p.head, error);
   if (!fits) return;
@@ -302,45 +376,56 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
     const int k = last_from(s_token0, n, i);  // (of entries with the same first token, the last holds it)
     p.tokens[i] = s_row[k] + i - s_token0[k];
   }
-  for (int i = e; i < items; i += threads) {
+  for (int x = e; x < items * p.num_kv_heads; x += threads) {
+    const int i = x / p.num_kv_heads;
     const int k = last_from(s_item0, G, i);
     const int first = s_start[k];
     const int rows_g = (first_token(s_start[k + 1]) - first_token(first)) * p.group;
-    const int tr = tile_rows_of(rows_g), count = cdiv(rows_g, tr);
+    const int tr = tile_rows_of(rows_g, big), count = cdiv(rows_g, tr);
     const int tile = (i - s_item0[k]) % count, part = (i - s_item0[k]) / count;
     const int st = cdiv(s_prefix[k], kQtKeys);
-    int32_t* d = p.tiles + (int64_t)i * kSpItemInts;
-    d[0] = -1 - p.group_seqs[s_leader[k]];  // the sequence whose table is read; negative: a group's item
-    d[1] = first_token(first);
-    d[2] = rows_g;
-    d[3] = tile * tr;
-    d[4] = (int)((int64_t)st * part / s_parts[k]) * kQtKeys;
-    d[5] = min((int)((int64_t)st * (part + 1) / s_parts[k]) * kQtKeys, s_prefix[k]);
-    d[6] = s_row0[k] + part * p.num_kv_heads * rows_g;
+    SpItem d = {};
+    d.kind = kGroupTile;
+    d.seq = p.group_seqs[s_leader[k]];
+    d.head = x % p.num_kv_heads;
+    d.rows_total = rows_g;
+    d.row0 = tile * tr;
+    d.tile_rows = tr;
+    d.token = first_token(first);
+    d.first_seen = 0x7FFFFFFF;
+    d.k0 = (int)((int64_t)st * part / s_parts[k]) * kQtKeys;
+    d.k1 = min((int)((int64_t)st * (part + 1) / s_parts[k]) * kQtKeys, s_prefix[k]);
+    d.part_row = s_row0[k] + part * p.num_kv_heads * rows_g;
+    p.items[x] = d;
   }
   // entry e's own items (few each)
   if (seq >= 0 && parts_s > 0) {
-    for (int i = 0; i < heavy_tiles * parts_s; ++i) {
-      const int tile = i % heavy_tiles, part = i / heavy_tiles;
-      int32_t* d = p.tiles + ((int64_t)items + at[3] + i) * kSpItemInts;
-      d[0] = seq;
-      d[1] = t0[0];
-      d[2] = rows_s;
-      d[3] = tile * tile_rows_of(rows_s);
-      d[4] = from + (int)((int64_t)heavy_stages * part / parts_s) * kQtKeys;
-      d[5] = min(from + (int)((int64_t)heavy_stages * (part + 1) / parts_s) * kQtKeys, kend);
-      d[6] = srow0 + part * p.num_kv_heads * rows_s;
+    SpItem d = {};
+    d.seq = seq;
+    d.rows_total = rows_s;
+    d.token = qs;
+    d.first_seen = ctx - ql + 1;
+    for (int x = 0; x < heavy_tiles * parts_s * p.num_kv_heads; ++x) {
+      const int i = x / p.num_kv_heads, tile = i % heavy_tiles, part = i / heavy_tiles;
+      d.kind = kOwnTile;
+      d.head = x % p.num_kv_heads;
+      d.row0 = tile * tile_rows_s;
+      d.tile_rows = tile_rows_s;
+      d.k0 = from + (int)((int64_t)heavy_stages * part / parts_s) * kQtKeys;
+      d.k1 = min(from + (int)((int64_t)heavy_stages * (part + 1) / parts_s) * kQtKeys, kend);
+      d.part_row = srow0 + part * p.num_kv_heads * rows_s;
+      p.items[(items + at[3]) * p.num_kv_heads + x] = d;
     }
-    for (int i = 0; i < light_items; ++i) {
-      int32_t* d = p.lights + ((int64_t)at[2] + i) * kSpItemInts;
-      d[0] = seq;
-      d[1] = i * p.light_keys;  // first part
-      d[2] = parts_s;
-      d[3] = from;
-      d[4] = kend;
-      d[5] = tiles16;
-      d[6] = srow0;
-      d[7] = rows_s;
+    for (int x = 0; x < light_items * p.head_blocks; ++x) {
+      d.kind = kLight;
+      d.head = x % p.head_blocks * p.light_heads;
+      d.k0 = from;
+      d.k1 = kend;
+      d.part_row = srow0;
+      d.part0 = x / p.head_blocks * p.light_keys;
+      d.parts = parts_s;
+      d.tiles = tiles16;
+      p.items[tile_wgs + at[2] * p.head_blocks + x] = d;
     }
   }
 }
@@ -472,23 +557,16 @@ constexpr int kSpExpOff = kQtSlotOff + 2 * 8 * 4;  // int [2 buffers][2 waves]: 
 constexpr int kSpLds = kSpExpOff + 2 * 2 * 4;
 
 template <bool INT8, int SDT>
-__device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int head, char* smem) {
+__device__ __forceinline__ void sp_tile_item(const SpParams& p, const SpItem& d, char* smem) {
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
-  const ConstI32* d = (const ConstI32*)(p.tiles + (int64_t)item * kSpItemInts);
-  const int who = d[0], tok0 = d[1], rows_total = d[2], row0 = d[3], kstart = d[4], kend = d[5];
-  const int64_t part_row = d[6];
-  const bool of_group = who < 0;
-  const int seq = of_group ? -1 - who : who;
-  const int kg_count = 256 / tile_rows_of(rows_total);
+  const bool of_group = d.kind == kGroupTile;
+  const int head = d.head, seq = d.seq, rows_total = d.rows_total, row0 = d.row0, kstart = d.k0, kend = d.k1;
+  const int first_seen = d.first_seen;
+  const int64_t part_row = d.part_row + (int64_t)head * rows_total;
+  const int kg_count = 256 / d.tile_rows;
   const int row_groups = kSpWaves / kg_count;
-  // keys that row R sees: all of a prefix, those up to its query's position of a sequence's own
-  int first_seen = kend;
-  if (!of_group) {
-    const ConstI32* sd = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
-    first_seen = sd[8] - sd[0] + 1;  // of query 0
-  }
   const int r = lane & 15;
   const int g = lane >> 4;
   const int kg = wave / row_groups;
@@ -502,22 +580,20 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
   int slot0 = 0;
   if (tid < 16) slot0 = tile_slot(tid);
   SpState<INT8> st;
+  u32x4 raw[kQtMT][4];
   int kend_row[kQtMT], kend_wave = 0, kfull_wave = kend;
 #pragma unroll
   for (int mt = 0; mt < kQtMT; ++mt) {
     const int row = wrow0 + kRows * mt + r;
     const bool valid = row < rows_total;
     const int t = valid ? row / p.group : 0;
-    const int token = p.tokens[tok0 + t];  // a row past the last reads the first token; it is never stored
-    kend_row[mt] = valid ? min(kend, of_group ? kend : first_seen + t) : 0;
+    // (a row past the last reads the first token; it is never stored)
+    const int token = of_group ? p.tokens[d.token + t] : d.token + t;
+    kend_row[mt] = valid ? (of_group ? kend : min(kend, first_seen + t)) : 0;
     const uint16_t* src = p.q + (int64_t)token * p.q_tok_stride +
                           (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride + 8 * g;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) st.q[mt].q[c] = sp_q_operand<INT8>(*(const u32x4*)(src + 32 * c));
-    st.m[mt] = kNegBig;
-    st.l[mt] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) st.o[mt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < 4; ++c) raw[mt][c] = *(const u32x4*)(src + 32 * c);
   }
   if (wrow0 < rows_total) {
     const int last = (min(wrow0 + kQtWaveRows, rows_total) - 1) / p.group;
@@ -525,7 +601,7 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
     kfull_wave = of_group ? kend : min(kend, first_seen + wrow0 / p.group);
   }
   if (tid < 16) s_slot[tid] = slot0;
-  __syncthreads();
+  lds_barrier();  // (the query rows are still on their way)
   QtRegs<INT8> R;
   int vexp = -126;  // value scales are taken relative to 2^vexp
   auto stage_store = [&](int buf, int kb) {
@@ -557,6 +633,16 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
   };
   const int n_stages = (kend - kstart + kQtKeys - 1) / kQtKeys;
   qt_load<INT8, SDT>(p, s_slot, kstart, kend, head, tid, R);
+  __asm__ __volatile__("" ::: "memory");  // the keys are requested before the query rows are waited for
+#pragma unroll
+  for (int mt = 0; mt < kQtMT; ++mt) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) st.q[mt].q[c] = sp_q_operand<INT8>(raw[mt][c]);
+    st.m[mt] = kNegBig;
+    st.l[mt] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.o[mt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
   stage_store(0, kstart);
   __syncthreads();
   for (int t = 0; t < n_stages; ++t) {
@@ -673,7 +759,7 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, int item, int he
   for (int mt = 0; mt < kQtMT; ++mt) {
     const int row = wrow0 + kRows * mt + r;
     if (row >= rows_total) continue;
-    const int64_t to = part_row + (int64_t)head * rows_total + row;
+    const int64_t to = part_row + row;
 #pragma unroll
     for (int j = 0; j < 8; ++j) *(floatx4*)(p.part_o + to * kHeadDim + 16 * j + 4 * g) = st.o[mt][j];
     if (g == 0) *(float2*)(p.part_ml + to * 2) = float2{st.m[mt], st.l[mt]};
@@ -745,15 +831,13 @@ struct LightRegs<false> {
 };
 
 template <bool INT8, int SDT, int MT>
-__device__ __forceinline__ void sp_light(const SpParams& p, int seq, int head, int kstart0, int kend0, int64_t part_row, char* smem) {
+__device__ __forceinline__ void sp_light(const SpParams& p, const SpItem& d, int head, int kstart0, int kend0, int64_t part_row, char* smem) {
   using L = Light<INT8>;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
   const int r = lane & 15, g = lane >> 4;
-  const ConstI32* sd = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
-  const int ql = sd[0], qs = sd[1], rows_total = sd[7], ctx = sd[8];
-  const int first_seen = ctx - ql + 1;
+  const int seq = d.seq, rows_total = d.rows_total, first_seen = d.first_seen;
   const int32_t* bt = p.block_tables + (int64_t)seq * p.bt_stride;
   char* ring = smem + wave * kLightWaveBytes;
   int* s_slot = (int*)(smem + kLightSlotOff) + wave * kLightWindow;
@@ -788,7 +872,7 @@ __device__ __forceinline__ void sp_light(const SpParams& p, int seq, int head, i
     const bool valid = row < rows_total;
     const int t = valid ? row / p.group : 0;
     kend_row[mt] = valid ? min(kend0, first_seen + t) : 0;
-    const uint16_t* src = p.q + (int64_t)(qs + t) * p.q_tok_stride +
+    const uint16_t* src = p.q + (int64_t)(d.token + t) * p.q_tok_stride +
                           (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride + 32 * g;
 #pragma unroll
     for (int c = 0; c < 4; ++c) st.q[mt].q[c] = sp_q_operand<INT8>(*(const u32x4*)(src + 8 * c));
@@ -957,29 +1041,27 @@ constexpr int kSpAllLds = kSpLds > kLightLds ? kSpLds : kLightLds;
 template <bool INT8, int SDT>
 __global__ __launch_bounds__(kSpThreads) void shared_prefix_parts_kernel(SpParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const ConstI32* head = (const ConstI32*)p.head;
-  const int tile_groups = p.max_tiles * p.num_kv_heads;
-  if ((int)blockIdx.x < tile_groups) {
-    const int item = blockIdx.x / p.num_kv_heads;
-    if (item < head[1]) sp_tile_item<INT8, SDT>(p, item, blockIdx.x % p.num_kv_heads, smem);
+  // the item is requested beside the count that says whether there is one
+  SpItem d;
+  const ConstI32* src = (const ConstI32*)(p.items + blockIdx.x);
+#pragma unroll
+  for (int i = 0; i < 14; ++i) ((int32_t*)&d)[i] = src[i];
+  if ((int)blockIdx.x >= ((const ConstI32*)p.head)[1]) return;
+  if (d.kind != kLight) {
+    sp_tile_item<INT8, SDT>(p, d, smem);
     return;
   }
-  const int b = blockIdx.x - tile_groups;
-  const int item = b / p.head_blocks;
-  if (item >= head[2]) return;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
-  const ConstI32* d = (const ConstI32*)(p.lights + (int64_t)item * kSpItemInts);
-  const int seq = d[0], part = d[1] + wave / p.light_heads, parts = d[2], from = d[3], kend = d[4], tiles = d[5];
-  const int rows = d[7];
-  const int kv = (b % p.head_blocks) * p.light_heads + wave % p.light_heads;
-  if (wave >= p.light_heads * p.light_keys || part >= parts || kv >= p.num_kv_heads) return;  // (no barrier follows)
-  const int k0 = from + (int)((int64_t)tiles * part / parts) * kTileKeys;
-  const int k1 = min(from + (int)((int64_t)tiles * (part + 1) / parts) * kTileKeys, kend);
-  const int64_t row = d[6] + (int64_t)part * p.num_kv_heads * rows;
-  if (rows <= kRows)
-    sp_light<INT8, SDT, 1>(p, seq, kv, k0, k1, row, smem);
+  const int part = d.part0 + wave / p.light_heads;
+  const int head = d.head + wave % p.light_heads;
+  if (wave >= p.light_heads * p.light_keys || part >= d.parts || head >= p.num_kv_heads) return;  // (no barrier follows)
+  const int k0 = d.k0 + (int)((int64_t)d.tiles * part / d.parts) * kTileKeys;
+  const int k1 = min(d.k0 + (int)((int64_t)d.tiles * (part + 1) / d.parts) * kTileKeys, d.k1);
+  const int64_t row = d.part_row + (int64_t)part * p.num_kv_heads * d.rows_total;
+  if (d.rows_total <= kRows)
+    sp_light<INT8, SDT, 1>(p, d, head, k0, k1, row, smem);
   else
-    sp_light<INT8, SDT, 2>(p, seq, kv, k0, k1, row, smem);
+    sp_light<INT8, SDT, 2>(p, d, head, k0, k1, row, smem);
 }
 
 // ---- merge ----
@@ -1055,9 +1137,9 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
 
 // ---- host ----
 struct SpLayout {
-  int max_tiles, max_lights, light_heads, light_keys, head_blocks;
+  int max_items, light_heads, light_keys, head_blocks;
   int64_t part_rows;
-  size_t tokens, tiles, lights, seqs, part_o, part_ml, total;
+  size_t tokens, items, seqs, part_o, part_ml, total;
 };
 
 // Bounds that hold for any lengths within the call's (comments give the plan's counts).
@@ -1070,41 +1152,33 @@ SpLayout sp_layout(int num_seqs, int num_groups, int num_q_heads, int num_kv_hea
   l.light_heads = num_kv_heads < kSpWaves ? num_kv_heads : kSpWaves;
   l.light_keys = kSpWaves / l.light_heads;
   l.head_blocks = cdiv(num_kv_heads, l.light_heads);
-  // prefix tiles: at most rows / 256 + one per group; a tile of n stages has at most n / share parts and
-  // at least one, share >= work / kNumCu, so parts past the first number kNumCu / kv heads at most
+  // Items: one per (tile, KV head) and one per (sequence, head block), and those of further parts: n stages,
+  // or 16-key tiles, are cut into n / each parts, rounded, so there are less than n / each further ones;
+  // `each` is worth a kNumCu-th of all work at least, so they are kNumCu in all (a few more by rounding),
+  // and n - 1 of each n at most.
   const int64_t groups = max_prefix >= kTileKeys ? (num_groups < num_seqs / 2 ? num_groups : num_seqs / 2) : 0;
-  const int64_t stages = cdiv(max_prefix, kQtKeys);
-  const int64_t more = kNumCu / num_kv_heads + 1;
-  int64_t tiles = 0, part_rows = 0;
-  if (groups > 0) {
-    const int64_t t = rows / 256 + groups;
-    const int64_t extra = t * (stages - 1) < more ? t * (stages - 1) : more;
-    tiles += t + extra;
-    // a part's rows: a tile's 256, but no more than every row in every part
-    const int64_t by_tile = rows + extra * 256, by_rows = rows * stages;
-    part_rows += (by_tile < by_rows ? by_tile : by_rows) * num_kv_heads;
-  }
-  // a sequence's own keys, in tiles or light items
-  int64_t most = 0;
-  if ((int64_t)max_q * group > kLightRows) {
-    const int64_t t = rows / 256 + num_seqs;
-    const int64_t own_stages = cdiv(max_ctx, kQtKeys);
-    const int64_t extra = t * (own_stages - 1) < more ? t * (own_stages - 1) : more;
-    tiles += t + extra;
-    const int64_t by_tile = rows + extra * 256, by_rows = rows * own_stages;
-    most = (by_tile < by_rows ? by_tile : by_rows) * num_kv_heads;
-  }
-  // light items: parts past a sequence's first number kNumCu * light_keys / head_blocks at most
-  const int64_t splits = cdiv(max_ctx, kTileKeys) / kLightMinTiles;  // of one sequence
-  const int64_t by_seq = num_seqs * (splits > 1 ? splits - 1 : 0);
-  const int64_t by_chip = (int64_t)kNumCu * l.light_keys / l.head_blocks + 1;
-  const int64_t more_parts = by_seq < by_chip ? by_seq : by_chip;
-  l.max_lights = num_seqs + cdiv((int)more_parts, l.light_keys);
+  const bool heavy = (int64_t)max_q * group > kLightRows;
   const int64_t light_rows = max_q * group < kLightRows ? max_q * group : kLightRows;
-  const int64_t light_part_rows = (num_seqs + more_parts) * light_rows * num_kv_heads;
-  // (a batch may mix both kinds of sequences)
-  l.part_rows = part_rows + most + light_part_rows;
-  l.max_tiles = (int)tiles;
+  int64_t items = (int64_t)num_seqs * l.head_blocks, part_rows = num_seqs * light_rows * num_kv_heads, further = 0, further_rows = 0;
+  auto add_tiles = [&](int64_t tiles, int64_t stages) {
+    items += tiles * num_kv_heads;
+    part_rows += rows * num_kv_heads;
+    further += tiles * (stages - 1) * num_kv_heads;
+    further_rows += rows * (stages - 1) * num_kv_heads;
+  };
+  if (groups > 0) add_tiles(rows / 128 + groups, cdiv(max_prefix, kQtKeys));
+  if (heavy) add_tiles(rows / 128 + num_seqs, cdiv(max_ctx, kQtKeys));
+  const int64_t splits = (cdiv(max_ctx, kTileKeys) + kLightMinTiles / 2) / kLightMinTiles;  // of one sequence
+  const int64_t light_further = num_seqs * (splits > 1 ? splits - 1 : 0);  // waves' parts
+  further += light_further * l.head_blocks;
+  further_rows += light_further * light_rows * num_kv_heads;
+  const int64_t most = kNumCu + 16;
+  items += further < most ? further : most;
+  // a further part of a tile has up to 256 rows of one head; of a light item light_rows of its heads, for each of its waves' parts
+  const int64_t per = 256 > light_rows * l.light_heads * l.light_keys ? 256 : light_rows * l.light_heads * l.light_keys;
+  part_rows += further_rows < most * per ? further_rows : most * per;
+  l.part_rows = part_rows;
+  l.max_items = (int)items;
   size_t at = 256;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -1112,8 +1186,7 @@ SpLayout sp_layout(int num_seqs, int num_groups, int num_q_heads, int num_kv_hea
     return here;
   };
   l.tokens = take((size_t)(tokens + 1) * 4);
-  l.tiles = take((size_t)tiles * kSpItemInts * 4);
-  l.lights = take((size_t)l.max_lights * kSpItemInts * 4);
+  l.items = take((size_t)l.max_items * sizeof(SpItem));
   l.seqs = take((size_t)num_seqs * kSpSeqInts * 4);
   l.part_ml = take((size_t)l.part_rows * 8);
   l.part_o = take((size_t)l.part_rows * kHeadDim * 4);
@@ -1151,13 +1224,11 @@ int sp_check(const char* what, int num_seqs, int num_groups, int num_q_heads, in
 void sp_bind(SpParams& p, const SpLayout& l, char* ws) {
   p.head = (uint32_t*)ws;
   p.tokens = (int32_t*)(ws + l.tokens);
-  p.tiles = (int32_t*)(ws + l.tiles);
-  p.lights = (int32_t*)(ws + l.lights);
+  p.items = (SpItem*)(ws + l.items);
   p.seqs = (int32_t*)(ws + l.seqs);
   p.part_o = (float*)(ws + l.part_o);
   p.part_ml = (float*)(ws + l.part_ml);
-  p.max_tiles = l.max_tiles;
-  p.max_lights = l.max_lights;
+  p.max_items = l.max_items;
   p.light_heads = l.light_heads;
   p.light_keys = l.light_keys;
   p.head_blocks = l.head_blocks;
@@ -1172,8 +1243,7 @@ int sp_launch(const SpParams& p, hipStream_t s) {
     set_error("shared_prefix_parts: cannot reserve %d bytes of LDS: %s", kSpAllLds, hipGetErrorString(attr));
     return NE_ELAUNCH;
   }
-  const int grid = p.max_tiles * p.num_kv_heads + p.max_lights * p.head_blocks;
-  hipLaunchKernelGGL((shared_prefix_parts_kernel<INT8, SDT>), dim3(grid), dim3(kSpThreads), kSpAllLds, s, p);
+  hipLaunchKernelGGL((shared_prefix_parts_kernel<INT8, SDT>), dim3(p.max_items), dim3(kSpThreads), kSpAllLds, s, p);
   const int rc = check_launch("shared_prefix_parts");
   if (rc != NE_OK) return rc;
   const int per_seq = cdiv(p.max_q * p.num_kv_heads * p.group, kMergeRows);

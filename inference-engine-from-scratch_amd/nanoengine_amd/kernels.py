@@ -526,6 +526,11 @@ class SharedPrefixPlan:
         """The error word of the plan and the calls on it (waits for them)."""
         return int(self.workspace[:4].view(torch.int32).item())
 
+    def shared_items(self) -> int:
+        """Work items that read a prefix for its whole group (waits for the plan): 0 where sharing
+        would cost more than it saves, as for few sequences or short prefixes."""
+        return int(self.workspace[8:12].view(torch.int32).item())
+
 
 def shared_prefix_workspace_bytes(num_seqs: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_q_len: int,
                                   max_ctx_len: int, max_prefix_len: int) -> int:

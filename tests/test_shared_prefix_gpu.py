@@ -171,6 +171,48 @@ def test_group_sizes(kv, members):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("prefix,members,q", [(1024, 64, 1), (1040, 40, 3), (2000, 30, 1), (1500, 130, 2), (4112, 26, 5), (9000, 24, 2)])
+def test_prefixes_read_once(kv, prefix, members, q):
+    """Batches in which sharing pays: row tiles of 64, 128 and 256, stages that end inside a prefix's
+    last keys, one part and many."""
+    b = Batch([(prefix, [((7 * i) % 90, max(1, q - i % 3)) for i in range(members)])], kv=kv, seed=prefix).to_gpu()
+    plan = b.plan()
+    b.check(b.run(plan))
+    assert plan.error_flag() == 0 and plan.shared_items() > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(32, 8), (8, 8), (8, 2), (6, 1), (30, 5), (24, 12)])
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+def test_prefixes_read_once_by_other_heads(kv, heads):
+    groups = [(1600 + 16 * heads[1], [((5 * i) % 60, 1 + i % 4) for i in range(60)]), (2304, [(i, 2) for i in range(50)]), (48, [(3, 1), None])]
+    b = Batch(groups, *heads, kv=kv, seed=heads[0]).to_gpu()
+    plan = b.plan()
+    b.check(b.run(plan))
+    flag, shared = plan.error_flag(), plan.shared_items()
+    assert flag == 0
+    if heads[1] > 1:  # the keys of one head are too few for sharing to pay
+        assert shared > 0
+
+
+@pytest.mark.gpu
+def test_short_prefixes_are_read_by_each():
+    b = Batch([(64, [(9, 1), (20, 1)])]).to_gpu()
+    assert b.plan().shared_items() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+def test_prompts_on_a_prefix_read_once(kv):
+    """Members of more than 32 rows per KV head among single queries: own keys in tiles."""
+    b = Batch([(1536, [(i, 1) for i in range(50)] + [(3, 40), (0, 70), (200, 33)])], kv=kv, seed=21).to_gpu()
+    plan = b.plan()
+    b.check(b.run(plan))
+    assert plan.shared_items() > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
 @pytest.mark.parametrize("block", [16, 32, 48, 128])
 def test_block_sizes(kv, block):
     b = Batch([(5 * block, [(7, 3), (block, 1), (2 * block - 1, 1)]), (block, [(0, 2), (9, 1)])], kv=kv, block=block, seed=block)
