@@ -55,6 +55,7 @@ class EngineSettings:
     max_prefill_tokens: int = 4096
     batch_fill_timeout_ms: int = 50
     prefix_cache: bool = False
+    shared_prefix: bool = False  # read the blocks that running requests share once per step
     chunked_prefill: bool = False
     max_num_batched_tokens: int = 512
     quantization: str = "none"
@@ -97,6 +98,8 @@ class EngineSettings:
             raise ValueError(f"scheduler={self.scheduler} needs kv_cache=contiguous or paged")
         if self.prefix_cache and self.kv_cache != "paged":
             raise ValueError("prefix_cache needs kv_cache=paged (it shares blocks)")
+        if self.shared_prefix and not self.prefix_cache:
+            raise ValueError("shared_prefix needs prefix_cache (requests share blocks through it)")
         if self.chunked_prefill and self.scheduler != "continuous":
             raise ValueError("chunked_prefill needs scheduler=continuous")
         if self.kv_cache == "none" and (self.kv_cache_dtype == "int8" or self.cuda_graphs):

@@ -20,6 +20,14 @@ class SamplingParams:
     top_p: float = 1.0
     seed: int | None = None
     ignore_eos: bool = False
+    top_k: int = 0  # 0: all tokens
+    min_p: float = 0.0  # least probability, relative to the likeliest token's
+
+    @property
+    def is_filtered(self) -> bool:
+        """Whether a sampled request draws under top-k or min-p, which speculative
+        verification does not take."""
+        return self.temperature != GREEDY_TEMPERATURE and (self.top_k > 0 or self.min_p > 0.0)
 
 
 @dataclass(frozen=True)
@@ -62,6 +70,21 @@ def create_sampling_generator(seed: int | None) -> SamplingStream:
     if seed is None:
         seed = int.from_bytes(os.urandom(8), "little") & ((1 << 63) - 1)
     return SamplingStream(seed=int(seed) & ((1 << 63) - 1))
+
+
+def sampling_uniform(seed: int, step: int) -> float:
+    """The uniform in [0, 1) of one draw of a stream: word 3 of Philox4x32-10 (Salmon et al.,
+    SC'11) under key ``seed`` at counter (``step``, 15), its 24 leading bits, as the acceptance
+    kernel takes it for its draws."""
+    mask = 0xFFFFFFFF
+    c = [step & mask, step >> 32 & mask, 15, 0]
+    k = [seed & mask, seed >> 32 & mask]
+    for i in range(10):
+        if i:
+            k = [(k[0] + 0x9E3779B9) & mask, (k[1] + 0xBB67AE85) & mask]
+        a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [(b >> 32) ^ c[1] ^ k[0], b & mask, (a >> 32) ^ c[3] ^ k[1], a & mask]
+    return (c[3] >> 8) / 16777216.0
 
 
 def find_finish_reason(token_id: int, num_generated_tokens: int, params: SamplingParams,

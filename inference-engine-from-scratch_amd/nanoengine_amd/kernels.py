@@ -157,15 +157,18 @@ def copy_kv_blocks(buffers: list[torch.Tensor], block_size: int, src: list[int],
     _check(len(src) == len(dst), f"{len(src)} sources for {len(dst)} destinations")
     if not buffers:
         raise ValueError("no buffers to copy in")
-    device = _require_gpu(*buffers)
-    slots = {t.shape[0] for t in buffers if t.dim() > 0}
-    _check(len(slots) == 1 and all(t.dim() > 0 and t.is_contiguous() for t in buffers),
+    first = buffers[0]
+    if any(t.get_device() != first.get_device() for t in buffers) or not first.is_cuda:
+        _require_gpu(*buffers)  # names the tensor
+    # (one call per tensor and check: a pool has four tensors per layer)
+    shapes = [t.shape for t in buffers]
+    num_slots = shapes[0][0] if shapes[0] else 0
+    _check(all(t.is_contiguous() for t in buffers) and all(s and s[0] == num_slots for s in shapes),
            "buffers must be contiguous and hold the same slots")
-    num_slots = slots.pop()
     _check(num_slots > 0, "buffers hold no slots")
     n = len(buffers)
-    block_bytes = [t.numel() // num_slots * t.element_size() * block_size for t in buffers]
-    _copy_blocks(device, _pointers(buffers), (ctypes.c_int64 * n)(*block_bytes), n, num_slots // block_size, src, dst)
+    block_bytes = (ctypes.c_int64 * n)(*[t.nbytes // num_slots * block_size for t in buffers])
+    _copy_blocks(first.device, _pointers(buffers), block_bytes, n, num_slots // block_size, src, dst)
 
 
 def _pointers(buffers: list[torch.Tensor]):
@@ -202,6 +205,7 @@ class AttentionWorkspace:
     plan_key: tuple | None = None
     runs_key: tuple | None = None  # metadata of the last paged_kv_runs_plan (measurement)
     frozen: bool = False
+    prefix_buffer: torch.Tensor | None = None  # of shared-prefix plans
 
     def get(self, device: torch.device, nbytes: int, layout: tuple) -> torch.Tensor:
         if self.buffer is None or self.buffer.numel() < nbytes or self.buffer.device != device:
@@ -218,10 +222,19 @@ class AttentionWorkspace:
             self.plan_key = self.runs_key = None
         return self.buffer
 
+    def get_prefix(self, device: torch.device, nbytes: int) -> torch.Tensor:
+        """A buffer for :func:`shared_prefix_plan`, under the same rule."""
+        have = self.prefix_buffer
+        if have is None or have.numel() < nbytes or have.device != device:
+            if self.frozen and have is not None:
+                raise RuntimeError(f"shared-prefix workspace of {have.numel()} bytes is held by a captured HIP graph; "
+                                   f"this call needs {nbytes} bytes on {device}: size it before capture")
+            self.prefix_buffer = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
+        return self.prefix_buffer
+
     def error_flag(self) -> int:
-        if self.buffer is None:
-            return 0
-        return int(self.buffer[:4].view(torch.int32).item())
+        words = [int(b[:4].view(torch.int32).item()) for b in (self.buffer, self.prefix_buffer) if b is not None]
+        return words[0] | words[-1] if words else 0
 
 
 _default_workspaces: dict[torch.device, AttentionWorkspace] = {}
@@ -530,6 +543,21 @@ class SharedPrefixPlan:
         """Work items that read a prefix for its whole group (waits for the plan): 0 where sharing
         would cost more than it saves, as for few sequences or short prefixes."""
         return int(self.workspace[8:12].view(torch.int32).item())
+
+
+SHARED_PREFIX_MAX_SEQS = 1024  # a plan's sequences
+# Bytes of keys and values per layer that sharing has to save for shared_prefix_attention to be faster
+# than paged_verify_attention.  16 query and 8 KV heads, us with / without: 64 sequences of 5 rows on 512
+# tokens (66 MB int8) 24.5 / 13.9, on 1,024 (132 MB int8) 26.9 / 26.3, (264 MB bf16) 25.2 / 27.8, on 2,048
+# (264 MB int8) 30.7 / 36.9, on 16,384 (2.1 GB int8) 98 / 197; 16 single rows on 2,048 (126 MB bf16)
+# 15.5 / 14.1; nine prefixes of 60 sequences (180 MB int8) 54 / 34, (360 MB bf16) 56 / 52.
+SHARED_PREFIX_MIN_BYTES = 192 << 20
+
+
+def shared_prefix_pays(saved_tokens: int, num_kv_heads: int, kv_dtype: torch.dtype) -> bool:
+    """Whether a batch that need not read ``saved_tokens`` cached tokens again (a prefix's tokens
+    times its members but one, over the groups) is faster with :func:`shared_prefix_attention`."""
+    return saved_tokens * num_kv_heads * 2 * HEAD_DIM * kv_dtype.itemsize >= SHARED_PREFIX_MIN_BYTES
 
 
 def shared_prefix_workspace_bytes(num_seqs: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_q_len: int,

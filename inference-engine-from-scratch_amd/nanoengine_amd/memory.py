@@ -248,6 +248,42 @@ class PagedSlotAllocator:
         return slots.to(self._device)
 
 
+def find_shared_prefixes(tables: list) -> list[tuple[list[int], int]]:
+    """Groups of the block tables that start with the same blocks, as (indexes, common blocks):
+    of all ways to put each table into one group at most, the one that saves most reads
+    (``(members - 1) * common blocks``), so that a short prefix common to all gives way to
+    longer ones common to some."""
+    rows = [np.asarray(table, dtype=np.int64) for table in tables]
+    order = sorted(range(len(rows)), key=lambda i: rows[i].tolist())
+
+    def common(a: np.ndarray, b: np.ndarray) -> int:
+        n = min(len(a), len(b))
+        differ = np.flatnonzero(a[:n] != b[:n])
+        return int(differ[0]) if len(differ) else n
+
+    # tables in order form a tree of runs that have their first `depth` blocks in common: an
+    # entry is such a run's [depth, first table, best saving inside it, the groups that give it]
+    found: list[tuple[int, int, int]] = []
+    open_runs: list[list] = []
+    for end in range(1, len(order) + 1):
+        depth = common(rows[order[end - 1]], rows[order[end]]) if end < len(order) else 0
+        first, saving, groups = end - 1, 0, []
+        while open_runs and open_runs[-1][0] > depth:
+            run_depth, first, inside, inner = open_runs.pop()
+            saving, groups = saving + inside, inner + groups
+            whole = (end - first - 1) * run_depth
+            if whole >= saving:
+                saving, groups = whole, [(first, end, run_depth)]
+        if open_runs and open_runs[-1][0] == depth:
+            open_runs[-1][2] += saving
+            open_runs[-1][3] += groups
+        elif depth > 0:
+            open_runs.append([depth, first, saving, groups])
+        else:
+            found += groups
+    return [(sorted(order[first:end]), depth) for first, end, depth in found]
+
+
 ROOT_PARENT_HASH = 0
 
 

@@ -17,8 +17,10 @@ import torch
 
 from nanoengine_amd import kernels
 from nanoengine_amd.attention_context import AttentionContext, build_attention_mask
-from nanoengine_amd.interface import GREEDY_TEMPERATURE
+from nanoengine_amd.interface import GREEDY_TEMPERATURE, GenerationRequest, sampling_uniform
+from nanoengine_amd.memory import find_shared_prefixes
 from nanoengine_amd.qwen3 import AttentionBatch, Qwen3VerifyModel
+from nanoengine_amd.sequence_state import Sequence
 
 PADDING_TOKEN_ID = 0
 
@@ -74,9 +76,14 @@ def build_step_inputs(sequences: list, allocator, pool, device: torch.device,
 
 
 class ModelRunner:
-    """Runs the HIP forward for padded steps of a few sequences (model_runner.py:14-80)."""
+    """Runs the HIP forward for padded steps of a few sequences (model_runner.py:14-80).
 
-    def __init__(self, model: Qwen3VerifyModel, pool, allocator, device: torch.device) -> None:
+    ``shared_prefix`` lets a step read the blocks that its sequences share (a prefix cache's, or
+    those of :meth:`fork`) once for all of them, where that pays."""
+
+    def __init__(self, model: Qwen3VerifyModel, pool, allocator, device: torch.device,
+                 shared_prefix: bool = False) -> None:
+        self.shared_prefix = shared_prefix
         self._model = model
         self._pool = pool
         self.allocator = allocator
@@ -86,7 +93,35 @@ class ModelRunner:
     def vocab_size(self) -> int:
         return self._model.config.vocab_size
 
-    def _forward(self, inputs: StepInputs):
+    def _prefix_groups(self, sequences: list) -> kernels.PrefixGroups | None:
+        if len(sequences) > kernels.SHARED_PREFIX_MAX_SEQS:
+            return None
+        size = self._pool.block_size
+        found = find_shared_prefixes([self.allocator.block_table(s) for s in sequences])
+        saved = sum((len(members) - 1) * blocks * size for members, blocks in found)
+        if not kernels.shared_prefix_pays(saved, self._model.config.num_key_value_heads,
+                                          self._pool.key_caches[0].dtype):
+            return None
+        grouped = {i for members, _ in found for i in members}
+        singles = [i for i in range(len(sequences)) if i not in grouped]
+        return kernels.PrefixGroups.from_lists([members for members, _ in found] + [[i] for i in singles],
+                                               [blocks * size for _, blocks in found] + [0] * len(singles),
+                                               self._device)
+
+    def fork(self, sequence: Sequence, request: GenerationRequest) -> Sequence:
+        """A new sequence for ``request``, whose prompt starts with ``sequence``'s cached tokens:
+        it begins with their keys and values (all, or but the prompt's last token, which a step
+        has to compute), shared where the allocator shares blocks and copied otherwise."""
+        child = Sequence.from_request(request)
+        shared = min(sequence.num_cached_tokens, child.num_tokens - 1)
+        if shared < 0 or child.token_ids[:shared] != sequence.token_ids[:shared]:
+            raise ValueError(f"{child.request_id} does not start with the cached tokens of {sequence.request_id}")
+        src, dst = self.allocator.fork(sequence, child, shared)
+        self._pool.copy_blocks(src, dst)
+        child.num_cached_tokens = shared
+        return child
+
+    def _forward(self, inputs: StepInputs, sequences: list):
         """The step's real rows packed sequence after sequence, through the model; returns
         the hidden states and each sequence's first row."""
         ctx = inputs.context
@@ -106,6 +141,7 @@ class ModelRunner:
             block_tables=ctx.block_tables,
             max_q_len=max(counts),
             max_ctx_len=ctx.max_context_length,
+            prefix_groups=self._prefix_groups(sequences) if self.shared_prefix else None,
         )
         rows = sum(counts)
         if rows > self._model.max_rows:
@@ -120,20 +156,35 @@ class ModelRunner:
         """Cache the next ``token_count`` tokens of one sequence and return the logits after
         each of them, ``[token_count, vocab]`` bf16 (model_runner.py:52-62)."""
         inputs = build_step_inputs([sequence], self.allocator, self._pool, self._device, [token_count])
-        hidden, _, _ = self._forward(inputs)
+        hidden, _, _ = self._forward(inputs, [sequence])
         sequence.num_cached_tokens += token_count
         self.allocator.on_tokens_cached(sequence)
         logits, _ = self._model.compute_logits(hidden[:token_count])
         return logits
+
+    def _draw_filtered(self, logits: torch.Tensor, sequences: list, rows: list[int]) -> torch.Tensor:
+        params = [sequences[i].sampling_params for i in rows]
+        streams = [sequences[i].sampling_generator for i in rows]
+
+        def row(values, dtype=torch.float32):
+            return torch.tensor(values, dtype=dtype, device=self._device)
+
+        return kernels.sample(
+            logits[rows], row([sampling_uniform(s.seed, s.step) for s in streams]),
+            temperature=row([p.temperature for p in params]),
+            top_k=row([min(max(p.top_k, 0), self.vocab_size) for p in params], torch.int32),
+            top_p=row([p.top_p for p in params]), min_p=row([p.min_p for p in params]))
 
     @torch.inference_mode()
     def run_step(self, sequences: list, token_counts: list[int] | None = None) -> list[int]:
         """Cache the next ``token_counts`` tokens of each sequence (default: all uncached)
         and pick a token after each one's last (model_runner.py:33-50): the argmax, or for a
         sampled request a draw under the explicit-uniform contract of the acceptance kernel
-        at the request's temperature and top-p, advancing its sampling stream."""
+        at the request's temperature and top-p, advancing its sampling stream.  A request that
+        also has a top-k or min-p gets the token that ``kernels.sample`` draws, from the
+        stream's uniform of its own at each step."""
         inputs = build_step_inputs(sequences, self.allocator, self._pool, self._device, token_counts)
-        hidden, starts, counts = self._forward(inputs)
+        hidden, starts, counts = self._forward(inputs, sequences)
         last = torch.tensor([s + n - 1 for s, n in zip(starts, counts, strict=True)], device=self._device)
         logits, _ = self._model.compute_logits(hidden[last].contiguous())
         b = len(sequences)
@@ -154,6 +205,9 @@ class ModelRunner:
                 any_sampled=True,
             )
         out, _ = kernels.accept(drafts, no_drafts, row_start, self.vocab_size, logits=logits, **kwargs)
+        filtered = [i for i, p in enumerate(params) if p.is_filtered]
+        if filtered:
+            out[filtered, 0] = self._draw_filtered(logits, sequences, filtered)
         tokens = out[:, 0].tolist()
         for s, is_sampled in zip(sequences, sampled, strict=True):
             if is_sampled:

@@ -192,6 +192,8 @@ class AttentionBatch:
     block_tables: torch.Tensor  # [b, max_blocks] int32
     max_q_len: int
     max_ctx_len: int
+    # sequences that start with the same blocks: attention reads those once for each group
+    prefix_groups: kernels.PrefixGroups | None = None
 
 
 class Qwen3VerifyModel:
@@ -270,9 +272,10 @@ class Qwen3VerifyModel:
         kernels.embed_rmsnorm(tokens[:rows], w.embed, w.layers[0].input_layernorm, eps, residual=res, out=normed)
         # the attention work plan depends only on this step's metadata: made once, read by
         # every layer's attention call
-        planned = kernels.plan_supported(c.num_attention_heads, c.num_key_value_heads, batch.max_q_len,
-                                         batch.ctx_len.shape[0], pool.key_caches[0].dtype,
-                                         pool.key_scale_2d(0).dtype if pool.key_scale_2d(0) is not None else None)
+        prefix_plan = None if batch.prefix_groups is None else self._prefix_plan(rows, batch, pool, ws)
+        planned = prefix_plan is None and kernels.plan_supported(
+            c.num_attention_heads, c.num_key_value_heads, batch.max_q_len, batch.ctx_len.shape[0],
+            pool.key_caches[0].dtype, pool.key_scale_2d(0).dtype if pool.key_scale_2d(0) is not None else None)
         if planned:
             kernels.paged_attention_plan(batch.block_tables, pool.block_size, batch.ctx_len, batch.q_start,
                                          batch.q_len, c.num_attention_heads, c.num_key_value_heads,
@@ -294,12 +297,16 @@ class Qwen3VerifyModel:
                     pool.key_caches[i], pool.value_caches[i], pool.key_scale_2d(i), pool.value_scale_2d(i),
                     q_out=q,
                 )
-            kernels.paged_verify_attention(
-                q, pool.key_caches[i], pool.value_caches[i], pool.key_scale_2d(i), pool.value_scale_2d(i),
-                batch.block_tables, pool.block_size, batch.ctx_len, batch.q_start, batch.q_len,
-                batch.max_q_len, batch.max_ctx_len, self.softmax_scale, out=attn, workspace=ws,
-                planned=planned,
-            )
+            if prefix_plan is not None:
+                kernels.shared_prefix_attention(q, pool.key_caches[i], pool.value_caches[i], pool.key_scale_2d(i),
+                                                pool.value_scale_2d(i), prefix_plan, self.softmax_scale, out=attn)
+            else:
+                kernels.paged_verify_attention(
+                    q, pool.key_caches[i], pool.value_caches[i], pool.key_scale_2d(i), pool.value_scale_2d(i),
+                    batch.block_tables, pool.block_size, batch.ctx_len, batch.q_start, batch.q_len,
+                    batch.max_q_len, batch.max_ctx_len, self.softmax_scale, out=attn, workspace=ws,
+                    planned=planned,
+                )
             self._project_add_norm(attn.view(rows, -1), layer.o_int8, layer.o_scale, self.o_splits[rows],
                                    layer.post_attention_layernorm, res, delta, normed)
             kernels.w8a16_gemm(normed, layer.gate_up_int8, layer.gate_up_scale, epilogue=EPILOGUE_SWIGLU,
@@ -308,6 +315,17 @@ class Qwen3VerifyModel:
             self._project_add_norm(act, layer.down_int8, layer.down_scale, self.down_splits[rows], next_norm,
                                    res, delta, normed)
         return normed
+
+    def _prefix_plan(self, rows: int, batch: AttentionBatch, pool, ws) -> kernels.SharedPrefixPlan:
+        """The step's plan, made once and read by every layer."""
+        c = self.config
+        nbytes = kernels.shared_prefix_workspace_bytes(
+            batch.ctx_len.shape[0], batch.prefix_groups.prefix_len.shape[0], c.num_attention_heads,
+            c.num_key_value_heads, batch.max_q_len, batch.max_ctx_len, batch.prefix_groups.max_prefix_len)
+        return kernels.shared_prefix_plan(
+            batch.block_tables, pool.block_size, batch.ctx_len, batch.q_start, batch.q_len, batch.prefix_groups,
+            c.num_attention_heads, c.num_key_value_heads, batch.max_q_len, batch.max_ctx_len, num_rows=rows,
+            num_blocks=pool.num_blocks, workspace=ws.get_prefix(batch.block_tables.device, nbytes))
 
     def _project_add_norm(self, x, w_int8, w_scale, splits, norm_weight, res, delta, normed) -> None:
         """residual += bf16(x @ W^T); normed = RMSNorm(residual) (qwen3.py:145-149)."""

@@ -29,15 +29,17 @@ captured once into a HIP graph and replayed.
 
 With a prefix-caching allocator, a new sequence takes the cached blocks of its
 prompt's start and its prefill computes only the remaining rows (queries at
-positions c..p-1 over a context of p keys).
+positions c..p-1 over a context of p keys).  With ``shared_prefix`` the verify steps
+read such blocks once for all the sequences that hold them, where that pays.
 """
 
 from __future__ import annotations
 
+import itertools
 import math
 from collections import deque
 from typing import TYPE_CHECKING, NamedTuple
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 import torch
@@ -45,7 +47,7 @@ import torch
 from nanoengine_amd import host_step, kernels
 from nanoengine_amd.draft import DeviceGuesses
 from nanoengine_amd.interface import find_finish_reason
-from nanoengine_amd.memory import KVCachePool, PagedSlotAllocator
+from nanoengine_amd.memory import KVCachePool, PagedSlotAllocator, find_shared_prefixes
 from nanoengine_amd.qwen3 import AttentionBatch, Qwen3VerifyModel
 from nanoengine_amd.sequence_state import Sequence
 
@@ -114,6 +116,7 @@ class VerifyRunner:
         proposer: "DraftModelProposer | None" = None,
         graph_max_batch: int | None = None,
         graph_max_context: int | None = None,
+        shared_prefix: bool = False,
     ) -> None:
         self.model = model
         # None: n-gram drafting on the device histories; else a draft model's greedy guesses
@@ -228,6 +231,17 @@ class VerifyRunner:
         self.graph_sampled: bool | None = None
         self.batch = AttentionBatch(self.positions, self.slot_mapping, self.q_start, self.q_len,
                                     self.ctx_len, self.block_tables, self.R, self.capacity)
+        # the slots' common blocks, found anew after each slot change; the arrays keep their
+        # place (a captured step reads them), slots without a group follow one by one
+        self.shared_batch: AttentionBatch | None = None
+        if shared_prefix:
+            if max_seqs > kernels.SHARED_PREFIX_MAX_SEQS:
+                raise ValueError(f"shared_prefix takes at most {kernels.SHARED_PREFIX_MAX_SEQS} sequences")
+            groups = kernels.PrefixGroups(torch.arange(max_seqs, **i32), torch.arange(max_seqs + 1, **i32),
+                                          torch.zeros(max_seqs, **i32), self.capacity)
+            self.shared_batch = replace(self.batch, prefix_groups=groups)
+        self._sharing: bool | None = None  # None: to be found
+        self.graph_shared: bool | None = None
         # set to a list to record, per verify step, each slot's history, drafts,
         # emitted tokens and block table (used by the parity tests)
         self.trace: list | None = None
@@ -260,6 +274,7 @@ class VerifyRunner:
     def _slots_changed(self) -> None:
         self._active = None
         self._sampled = None
+        self._sharing = None
 
     def free_slots(self) -> list[int]:
         """Empty slots.  A slot whose sequence finished in a step whose results wait for
@@ -285,6 +300,33 @@ class VerifyRunner:
             self._sampled = bool((self.np_temp[self.np_active] > 0).any())
         return self._sampled
 
+    @property
+    def sharing(self) -> bool:
+        """Whether the next step reads the blocks that slots share once for each group of them."""
+        if self._sharing is None:
+            self._sharing = self.shared_batch is not None and self._find_groups()
+        return self._sharing
+
+    def _find_groups(self) -> bool:
+        """Write the active slots' groups for the device; whether they are worth it.  (Blocks
+        are shared from admission on: a slot's table only grows by blocks of its own.)"""
+        active = np.flatnonzero(self.np_active)
+        found = find_shared_prefixes([self.np_tables[i, : self.np_owned[i]] for i in active])
+        c = self.model.config
+        saved = sum((len(members) - 1) * blocks for members, blocks in found) * self.block_size
+        if not kernels.shared_prefix_pays(saved, c.num_key_value_heads, self.pool.key_caches[0].dtype):
+            return False
+        groups = [active[members].tolist() for members, _ in found]
+        grouped = set(itertools.chain(*groups))
+        groups += [[slot] for slot in range(self.max_seqs) if slot not in grouped]
+        n, empty = self.max_seqs, self.max_seqs - len(groups)
+        lens = [blocks * self.block_size for _, blocks in found]
+        arrays = self.shared_batch.prefix_groups
+        arrays.seqs.copy_(torch.tensor(list(itertools.chain(*groups)), dtype=torch.int32))
+        starts = [0, *itertools.accumulate(len(members) for members in groups)] + [n] * empty
+        arrays.start.copy_(torch.tensor(starts, dtype=torch.int32))
+        arrays.prefix_len.copy_(torch.tensor(lens + [0] * (n - len(lens)), dtype=torch.int32))
+        return True
 
     def add(self, sequences: list[Sequence]) -> list[int]:
         """Place sequences in free slots, reserve their prompts, prefill them and emit
@@ -297,6 +339,9 @@ class VerifyRunner:
             problem = request_length_error(seq.num_tokens, seq.sampling_params.max_new_tokens, self.max_model_len)
             if problem is not None:
                 raise ValueError(f"{seq.request_id}: {problem}")
+            if seq.sampling_params.is_filtered:
+                raise ValueError(f"{seq.request_id}: speculative verification samples under temperature and top_p, "
+                                 "not top_k or min_p")
         slots = free[: len(sequences)]
         results = {}
         # prefill contiguous runs of slots together
@@ -431,17 +476,18 @@ class VerifyRunner:
         )
 
     # ------------------------------------------------------------- verify step
-    def _device_step(self, sampled: bool) -> None:
+    def _device_step(self, sampled: bool, shared: bool) -> None:
         """Fixed-shape part of the verify step: pack, forward, LM head, accept.  ``sampled``:
         some slot samples, so the LM head writes every row's logits (greedy slots take
-        their argmax from them); otherwise it writes only the argmax partials."""
+        their argmax from them); otherwise it writes only the argmax partials.  ``shared``:
+        attention reads the blocks that slots have in common once."""
         kernels.prepare_verify_step(
             self.history, self.history_len, self.drafts, self.num_drafts, self.block_tables,
             self.block_size, self.pool.scratch_slot, self.tokens, self.positions, self.slot_mapping,
             self.q_start, self.q_len, self.ctx_len,
         )
         rows = self.max_seqs * self.R
-        hidden = self.model.forward(rows, self.tokens, self.batch, self.pool)
+        hidden = self.model.forward(rows, self.tokens, self.shared_batch if shared else self.batch, self.pool)
         if not sampled:
             self.model.compute_logits(hidden, logits=False, argmax=self.argmax_partials)
             logits = None
@@ -493,19 +539,19 @@ class VerifyRunner:
         torch.cuda.current_stream(self.device).synchronize()
 
     def _run_device_step(self) -> None:
-        sampled = self.any_sampled
+        sampled, shared = self.any_sampled, self.sharing
         if not self.graph_allowed():
-            self._device_step(sampled)
+            self._device_step(sampled, shared)
             return
-        if self.graph is None or self.graph_sampled != sampled:
+        if self.graph is None or self.graph_sampled != sampled or self.graph_shared != shared:
             # this step runs eagerly (which also allocates lazily created buffers and
             # workspaces); the capture below only records, so nothing runs twice
-            self._device_step(sampled)
+            self._device_step(sampled, shared)
             torch.cuda.current_stream(self.device).synchronize()
             graph = torch.cuda.CUDAGraph()
             try:
                 with torch.cuda.graph(graph):
-                    self._device_step(sampled)
+                    self._device_step(sampled, shared)
             except torch.cuda.OutOfMemoryError:
                 # as cuda_graph_runner.py:193-207: without the memory to capture, every
                 # later step runs eagerly (this one already ran)
@@ -515,7 +561,7 @@ class VerifyRunner:
                 return
             self.graph = graph
             self.model.bind_graph()
-            self.graph_sampled = sampled
+            self.graph_sampled, self.graph_shared = sampled, shared
             return
         self.graph.replay()
 

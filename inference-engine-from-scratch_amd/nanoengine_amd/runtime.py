@@ -85,7 +85,8 @@ def create_verify_engine(config: Qwen3Config, state_dict: dict[str, torch.Tensor
                           settings.ngram_max_size, settings.max_model_len, stop_token_ids,
                           use_graph=settings.cuda_graphs, proposer=proposer,
                           graph_max_batch=settings.cuda_graph_max_batch,
-                          graph_max_context=settings.cuda_graph_max_context)
+                          graph_max_context=settings.cuda_graph_max_context,
+                          shared_prefix=settings.shared_prefix)
     if settings.cuda_graphs:
         runner.capture_graph()
     return VerifyEngine(settings, model, pool, allocator, runner, EngineMetrics())
