@@ -23,7 +23,7 @@
 //            rows as the second operand of S^T = K Q^T, whose result is the second operand of
 //            O^T = V^T P^T.
 //          Items are cut so that the longest is about the batch's work over the chip.
-//   merge  16 threads per row.
+//   merge  16 threads per row, or 64.
 // What bounds it: reading the keys once (long prefixes and contexts), else the chain of
 // round trips of the three kernels; the partial sums (520 bytes a row and part) stay in the
 // memory-side cache.
@@ -55,13 +55,15 @@ constexpr int kLightMinTiles = 4;    // least 16-key tiles per wave of a split s
 // A stage of a tile of up to 128 rows waits for its keys as much as it computes (2.9 us), one of 256 computes.
 constexpr int kStageCost = 5, kBigStageCost = 9;
 constexpr int kItemCost = 13;  // an item before its first and after its last keys: 6.5 us (light) to 10 (tile)
-// With this many tiles of 16 keys of eight heads (and as large stages of a head) per CU, 100 MB of an int8
-// pool, they come at the memory's rate.
-constexpr int kStreamTiles = 12, kStreamCost = 3;
+// With this many tiles of 16 keys of eight heads (and as large stages of a head) per CU, 50 MB of an int8
+// pool, they come at the memory's rate.  64 rows on 16,384 keys (bf16) 124 us with the cost of 3, 132 with 2,
+// 161 with 1; nine prefixes of 2,048 keys that leave little (int8) 46 with 4 tiles, 39 with 6.
+constexpr int kStreamTiles = 6, kStreamCost = 3;
 __host__ __device__ constexpr int stage_cost(int tile_rows) { return tile_rows <= 128 ? kStageCost : kBigStageCost; }
-// Sharing has to save this much per CU: a tile item takes longer than a light one, and its partial sums
-// go through memory.
-constexpr int kShareGain = 3;
+// Sharing has to save this much per CU, and this part of the light work: a tile item takes longer than a light
+// one, the more so beside others that stream, and its partial sums go through memory.  32 sequences of 9 rows
+// whose own keys are ten times the shared ones: 367 us shared, 326 not.
+constexpr int kShareGain = 3, kShareOf = 8;
 // Tiles of 256 rows take a tenth less per row; worth it with this much tile work per CU, as half tiles
 // spread it better.
 constexpr int kBigWork = 60;
@@ -254,17 +256,24 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
     atomicMin(&s_leader[g], e);
     atomicAdd(&s_members[g], 1);
   }
-  int t0[1], tokens[1];
-  plan_scan<1>({ql}, s_part, t0, tokens);
+  const int table_keys = (int)min((int64_t)p.bt_stride * p.block_size, (int64_t)0x7FFFFFFF);
+  const int rows_s = ql * p.group;
+  const bool light = rows_s <= kLightRows;
+  const int kend = min(min(ctx, p.max_ctx), table_keys);
+  // tokens, and the light work if no prefix were shared (of up to 2^27 / 1,024 keys a sequence)
+  int before[2], total[2];
+  plan_scan<2>({ql, ql > 0 && light ? min(cdiv(max(kend, 0), kTileKeys) * p.head_blocks / p.light_keys, 1 << 20) : 0}, s_part, before, total);
+  const int t0 = before[0], tokens = total[0];
+  auto stream_of = [&](float tiles) { return tiles >= (float)(kStreamTiles * kNumCu) ? kStreamCost : 1; };
+  const int stream_alone = stream_of((float)total[1]);
   if (e < n) {
-    s_token0[e] = t0[0];
+    s_token0[e] = t0;
     s_row[e] = qs;
   }
-  if (e == 0) s_token0[n] = tokens[0];
+  if (e == 0) s_token0[n] = tokens;
   __syncthreads();
   auto first_token = [&](int entry) { return s_token0[min(max(entry, 0), n)]; };
   // ---- group e ----
-  const int table_keys = (int)min((int64_t)p.bt_stride * p.block_size, (int64_t)0x7FFFFFFF);
   int rows = 0, stages = 0, prefix = 0;
   if (e < G && s_members[e] > 1) {
     prefix = min(min(stated, s_least[e]), min(max_prefix, p.max_ctx));
@@ -280,11 +289,8 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
   }
   __syncthreads();
   // ---- what the prefixes would cost read by every member ----
-  const int rows_s = ql * p.group;
-  const bool light = rows_s <= kLightRows;
-  const int kend = min(min(ctx, p.max_ctx), table_keys);
   if (ql > 0 && g >= 0 && s_prefix[g] > 0) {
-    const int64_t units = light ? (int64_t)(s_prefix[g] / kTileKeys) * p.head_blocks / p.light_keys
+    const int64_t units = light ? (int64_t)(s_prefix[g] / kTileKeys) * p.head_blocks * stream_alone / p.light_keys
                                 : (int64_t)cdiv(rows_s, 128) * cdiv(s_prefix[g], kQtKeys) * kStageCost * p.num_kv_heads;
     atomicAdd(&s_alone[g], (int)min(units, (int64_t)1 << 20));
   }
@@ -297,7 +303,7 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
                 light ? 0 : min(cdiv(rows_s, 128) * cdiv(max(kend, 0), kQtKeys), 1 << 20)},
                s_part, skip, sum);
   const bool big = ((int64_t)sum[1] + sum[2]) * p.num_kv_heads * kStageCost >= (int64_t)kBigWork * kNumCu;
-  if (!gains || sum[0] < kShareGain * kNumCu) prefix = rows = stages = 0;
+  if (!gains || sum[0] < max(kShareGain * kNumCu, total[1] / kShareOf * stream_alone)) prefix = rows = stages = 0;
   const int tile_rows = tile_rows_of(rows, big), tile_count = cdiv(rows, tile_rows);
   if (e < G) s_prefix[e] = prefix;
   __syncthreads();
@@ -317,13 +323,13 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
   int stream;
   {
     const int64_t mine = ((int64_t)tile_count * stages * stage_cost(tile_rows) + (int64_t)heavy_tiles * heavy_stages * stage_cost(tile_rows_s)) * p.num_kv_heads;
-    int before[5], total[5];  // tile work (1,024 of 48 bits), light work, and uncut items
+    int before[5], total[5];  // (of this block) tile work (1,024 of 48 bits), light work, and uncut items
     plan_scan<5>({(int)(mine & 0xFFFF), (int)((mine >> 16) & 0xFFFF), (int)(mine >> 32), tiles16,
                   min((tile_count + heavy_tiles) * p.num_kv_heads + (tiles16 > 0 ? p.head_blocks : 0), 1 << 20)},
                  s_part, before, total);
     const float tile_work = (float)total[0] + 65536.f * (float)total[1] + 4294967296.f * (float)total[2];
     const float light_work = (float)total[3] * (float)p.head_blocks / (float)p.light_keys;
-    stream = light_work + tile_work / (float)kStageCost >= (float)(kStreamTiles * kNumCu) ? kStreamCost : 1;
+    stream = stream_of(light_work + tile_work / (float)kStageCost);
     const float W = tile_work + light_work * (float)stream, B = (float)total[4];
     constexpr float F = kItemCost, C = kNumCu;
     const float b = C * F - W - F * B;
@@ -358,7 +364,7 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
     d[1] = qs;
     d[2] = from > 0 ? s_parts[g] : 0;  // parts of the shared prefix
     d[3] = parts_s;                    // parts of its own keys
-    d[4] = g >= 0 ? s_row0[g] + (t0[0] - group_token0) * p.group : 0;
+    d[4] = g >= 0 ? s_row0[g] + (t0 - group_token0) * p.group : 0;
     d[5] = g >= 0 ? (first_token(s_start[g + 1]) - group_token0) * p.group : 0;
     d[6] = srow0;
     d[7] = rows_s;
@@ -372,7 +378,7 @@ __global__ __launch_bounds__(kPlanMaxThreads) void shared_prefix_plan_kernel(SpP
   if (error) atomicOr(p.head, error);
   if (!fits) return;
   // ---- the groups' tokens, and the items ----
-  for (int i = e; i < tokens[0]; i += threads) {
+  for (int i = e; i < tokens; i += threads) {
     const int k = last_from(s_token0, n, i);  // (of entries with the same first token, the last holds it)
     p.tokens[i] = s_row[k] + i - s_token0[k];
   }
@@ -1066,14 +1072,17 @@ __global__ __launch_bounds__(kSpThreads) void shared_prefix_parts_kernel(SpParam
 
 // ---- merge ----
 constexpr int kMergeThreads = 256;
-constexpr int kMergeRows = kMergeThreads / 16;
 constexpr int kMergeAhead = 8;
+// Up to this many rows, which then have many parts each, 64 threads take a row's parts in turn: 320 rows of 63
+// parts 12.5 to 6 us; 1,280 rows of few parts would take 0.7 us longer.
+constexpr int kMergeFewRows = 1024;
 
+template <int LANES>
 __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpParams p, int blocks_per_seq) {
   const int seq = blockIdx.x / blocks_per_seq;
   const ConstI32* d = (const ConstI32*)(p.seqs + (int64_t)seq * kSpSeqInts);
   const int heads = p.num_kv_heads * p.group;
-  const int x = (blockIdx.x % blocks_per_seq) * kMergeRows + (threadIdx.x >> 4);  // query, then head
+  const int x = (blockIdx.x % blocks_per_seq) * (kMergeThreads / LANES) + (int)threadIdx.x / LANES;  // query, then head
   if (x >= d[0] * heads) return;
   const int i = x / heads, head = x % heads;
   const int kv = head / p.group, in = i * p.group + head % p.group;
@@ -1081,14 +1090,16 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
   const int64_t prefix0 = d[4] + kv * d[5] + in, own0 = d[6] + kv * d[7] + in;
   const int64_t prefix_step = p.num_kv_heads * d[5], own_step = p.num_kv_heads * d[7];
   const int cd = (threadIdx.x & 15) * 8;
+  constexpr int kTurns = LANES / 16;  // sets of 16 lanes that take parts in turn
+  const int turn = (int)threadIdx.x % LANES / 16;
   float M = kNegBig, L = 0.f;
   float acc[8] = {};
-  for (int s0 = 0; s0 < n; s0 += kMergeAhead) {
+  for (int s0 = turn; s0 < n; s0 += kMergeAhead * kTurns) {
     float2 ml[kMergeAhead];
     floatx4 a[kMergeAhead], b[kMergeAhead];
 #pragma unroll
     for (int j = 0; j < kMergeAhead; ++j) {
-      const int s = min(s0 + j, n - 1);
+      const int s = min(s0 + j * kTurns, n - 1);
       const int64_t row = s < np ? prefix0 + s * prefix_step : own0 + (s - np) * own_step;
       ml[j] = *(const float2*)(p.part_ml + row * 2);
       a[j] = *(const floatx4*)(p.part_o + row * kHeadDim + cd);
@@ -1096,7 +1107,7 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
     }
     float top = M;
 #pragma unroll
-    for (int j = 0; j < kMergeAhead; ++j) top = fmaxf(top, s0 + j < n ? ml[j].x : kNegBig);
+    for (int j = 0; j < kMergeAhead; ++j) top = fmaxf(top, s0 + j * kTurns < n ? ml[j].x : kNegBig);
     const float down = __builtin_amdgcn_exp2f(M - top);
     L *= down;
 #pragma unroll
@@ -1104,7 +1115,7 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
     M = top;
 #pragma unroll
     for (int j = 0; j < kMergeAhead; ++j) {
-      if (s0 + j >= n) continue;
+      if (s0 + j * kTurns >= n) continue;
       const float w = __builtin_amdgcn_exp2f(ml[j].x - M);
       L += w * ml[j].y;
 #pragma unroll
@@ -1112,6 +1123,18 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
         acc[c] += w * a[j][c];
         acc[c + 4] += w * b[j][c];
       }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o < LANES; o <<= 1) {  // the sets' sums, the same in each
+    const float top = fmaxf(M, __shfl_xor(M, o)), down = __builtin_amdgcn_exp2f(M - top);
+    M = top;
+    L *= down;
+    L += __shfl_xor(L, o);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      acc[c] *= down;
+      acc[c] += __shfl_xor(acc[c], o);
     }
   }
   if (d[9]) {  // values that are not finite, of keys that only some rows see: this row's
@@ -1126,6 +1149,7 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
       }
     }
   }
+  if (turn != 0) return;
   // a row that sees no key is zero
   const bool none = L == 0.f;
   const float inv = none ? 0.f : 1.f / L;
@@ -1246,8 +1270,11 @@ int sp_launch(const SpParams& p, hipStream_t s) {
   hipLaunchKernelGGL((shared_prefix_parts_kernel<INT8, SDT>), dim3(p.max_items), dim3(kSpThreads), kSpAllLds, s, p);
   const int rc = check_launch("shared_prefix_parts");
   if (rc != NE_OK) return rc;
-  const int per_seq = cdiv(p.max_q * p.num_kv_heads * p.group, kMergeRows);
-  hipLaunchKernelGGL(shared_prefix_merge_kernel, dim3(p.num_seqs * per_seq), dim3(kMergeThreads), 0, s, p, per_seq);
+  const int rows = p.max_q * p.num_kv_heads * p.group;
+  const bool few = p.num_seqs * rows <= kMergeFewRows;
+  const int per_seq = cdiv(rows, kMergeThreads / (few ? 64 : 16));
+  hipLaunchKernelGGL(few ? shared_prefix_merge_kernel<64> : shared_prefix_merge_kernel<16>, dim3(p.num_seqs * per_seq), dim3(kMergeThreads), 0, s, p,
+                     per_seq);
   return check_launch("shared_prefix_merge");
 }
 

@@ -546,12 +546,12 @@ class SharedPrefixPlan:
 
 
 SHARED_PREFIX_MAX_SEQS = 1024  # a plan's sequences
-# Bytes of keys and values per layer that sharing has to save for shared_prefix_attention to be faster
-# than paged_verify_attention.  16 query and 8 KV heads, us with / without: 64 sequences of 5 rows on 512
-# tokens (66 MB int8) 24.5 / 13.9, on 1,024 (132 MB int8) 26.9 / 26.3, (264 MB bf16) 25.2 / 27.8, on 2,048
-# (264 MB int8) 30.7 / 36.9, on 16,384 (2.1 GB int8) 98 / 197; 16 single rows on 2,048 (126 MB bf16)
-# 15.5 / 14.1; nine prefixes of 60 sequences (180 MB int8) 54 / 34, (360 MB bf16) 56 / 52.
-SHARED_PREFIX_MIN_BYTES = 192 << 20
+# Bytes of keys and values per layer that sharing has to save for a step to be faster with it.  28 layers of
+# 16 query and 8 KV heads, verify steps of 5 rows, us per layer without and with: 64 sequences on 512 tokens
+# (66 MB saved, int8) 66.7 / 67.6, on 1,024 (132 MB) 72.4 / 69.0, on 2,048 (264 MB) 86 / 72, on 8,192 161 / 84;
+# 16 on 2,048 (126 MB, bf16) 58.8 / 59.5, on 4,096 (126 MB, int8) 65.3 / 64.4; 60 on nine prefixes of 1,024
+# (107 MB, int8) 70.5 / 71.2, of 2,048 (428 MB, bf16) 88.5 / 80.5.
+SHARED_PREFIX_MIN_BYTES = 120 << 20
 
 
 def shared_prefix_pays(saved_tokens: int, num_kv_heads: int, kv_dtype: torch.dtype) -> bool:
