@@ -36,6 +36,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "ne_common.hpp"
 
 namespace ne {
@@ -51,20 +53,27 @@ constexpr int kBins = 1024;
 constexpr int kBinsPerLog2 = 16;
 constexpr int kScanThreads = 512;
 constexpr int kScanWaves = kScanThreads / kWave;
-constexpr int kScanSegs = 2;          // segments per wave and iteration
+constexpr int kScanLines = 2;         // lines (of a vector per lane) per wave and iteration
+constexpr int kSegVecs = 8;           // vectors of a segment
+constexpr int kLineSegs = kWave / kSegVecs;
+constexpr int kCountThreads = 1024;
+constexpr int kCountWaves = kCountThreads / kWave;
+constexpr int kCountLines = 4;
+constexpr int kCountMost = 127;       // lines of a chunk: 65,024 elements, whose counts fit 16 bits
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / kWave;
 constexpr int kList = 4096;           // tokens that pick sorts in LDS
 constexpr int kShortTopK = 1024;      // up to here the scan counts tokens and leaves their weights to pick
 constexpr int kSub = 2048;            // buckets of a narrowing pass
 constexpr int kSortBuckets = 2048;    // and of a sort
+constexpr int kSegsHeld = 4096;       // segments' largest keys that pick keeps in LDS
 constexpr int kRankMost = 64;         // tokens of a bucket that are ranked
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kRowBatch = 1024;       // rows per launch: bounds the workspace
 
 // One chunk's result; its histogram follows in arrays of their own.
 struct ChunkHead {
-  u64 best;     // first largest token (key, ~index); 0: no token
+  u64 best;     // largest key and its first vector (key, ~vector); 0: no token
   double base;  // Y
   uint32_t tokens;
   uint32_t pad[3];
@@ -125,50 +134,52 @@ __device__ __forceinline__ uint32_t word_key(u64 w) { return (uint32_t)(w >> 32)
 // element e of vector v is token v * kVec + e - skew.
 template <int DT>
 struct Row {
-  const char* base;  // of the row, any alignment of an element
+  const u32x4* base;  // vector 0: a scalar load of a vector needs its base on the grid too
   int skew, vocab, vecs;
   __device__ Row(const SampleParams& p, int row) {
     constexpr int kEsz = 16 / kVec<DT>;
-    base = (const char*)p.logits + (int64_t)row * p.ld * kEsz;
-    skew = (int)((uintptr_t)base & 15) / kEsz;
+    const char* at = (const char*)p.logits + (int64_t)row * p.ld * kEsz;
+    skew = (int)((uintptr_t)at & 15) / kEsz;
+    base = (const u32x4*)(at - skew * kEsz);
     vocab = p.vocab;
     vecs = (vocab + skew + kVec<DT> - 1) / kVec<DT>;
   }
-  // Keys of vector v; 0 for what lies outside the row.
-  __device__ __forceinline__ u32x4 raw(int v, bool& whole) const {
-    constexpr int kEsz = 16 / kVec<DT>;
+  // Vector v, NaN for what lies outside the row.
+  __device__ __forceinline__ u32x4 vec(int v) const {
     const int t0 = v * kVec<DT> - skew;
-    whole = t0 >= 0 && t0 + kVec<DT> <= vocab;
-    // an address that is read whatever the vector: its own, or the row's first whole vector's
-    u32x4 x = {0, 0, 0, 0};
-    if (whole) x = *(const u32x4*)(base + (int64_t)t0 * kEsz);
-    return x;
-  }
-  __device__ __forceinline__ float single(int t) const {
-    if (DT == NE_DTYPE_FP32) return ((const float*)base)[t];
-    if (DT == NE_DTYPE_FP16) return f16_to_f32(((const uint16_t*)base)[t]);
-    return bf16_to_f32(((const uint16_t*)base)[t]);
-  }
-  // The vector's values, NaN outside the row.
-  __device__ __forceinline__ void values(int v, u32x4 x, bool whole, float (&out)[kVec<DT>]) const {
-    if (whole) {
+    if (t0 >= 0 && t0 + kVec<DT> <= vocab) return base[v];
+    const uint32_t none = DT == NE_DTYPE_FP32 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+    u32x4 out = {none, none, none, none};
+    if (v >= vecs) return out;
 #pragma unroll
-      for (int e = 0; e < kVec<DT>; ++e) {
-        if constexpr (DT == NE_DTYPE_FP32) {
-          const uint32_t bits = x[e];  // (a bit cast of the vector's element itself reads element 0)
-          out[e] = __builtin_bit_cast(float, bits);
-        } else {
-          const uint16_t h = (uint16_t)(x[e / 2] >> (16 * (e & 1)));
-          out[e] = DT == NE_DTYPE_FP16 ? f16_to_f32(h) : bf16_to_f32(h);
-        }
+    for (int d = 0; d < 4; ++d) {
+      if constexpr (DT == NE_DTYPE_FP32) {
+        if (t0 + d >= 0 && t0 + d < vocab) out[d] = ((const uint32_t*)(base + v))[d];
+      } else {
+        const uint16_t* at = (const uint16_t*)(base + v) + 2 * d;
+        const int t = t0 + 2 * d;
+        const uint32_t lo = t >= 0 && t < vocab ? at[0] : 0x7FFF, hi = t + 1 >= 0 && t + 1 < vocab ? at[1] : 0x7FFF;
+        out[d] = lo | (hi << 16);
       }
-    } else {
-      const int t0 = v * kVec<DT> - skew;
-#pragma unroll
-      for (int e = 0; e < kVec<DT>; ++e) out[e] = t0 + e >= 0 && t0 + e < vocab ? single(t0 + e) : NAN;
     }
+    return out;
   }
 };
+// Element e of a dword's one or two.
+template <int DT>
+__device__ __forceinline__ float element(uint32_t d, int e) {
+  if (DT == NE_DTYPE_FP32) return __builtin_bit_cast(float, d);
+  const uint16_t h = (uint16_t)(d >> (16 * e));
+  return DT == NE_DTYPE_FP16 ? f16_to_f32(h) : bf16_to_f32(h);
+}
+template <int DT>
+__device__ __forceinline__ void values(u32x4 x, float (&out)[kVec<DT>]) {
+#pragma unroll
+  for (int e = 0; e < kVec<DT>; ++e) {
+    const uint32_t d = x[e * 4 / kVec<DT>];  // (a bit cast of the vector's element itself reads element 0)
+    out[e] = element<DT>(d, e % (kVec<DT> / 4));
+  }
+}
 
 // ---- row parameters ----
 struct RowParams {
@@ -239,23 +250,174 @@ __device__ __forceinline__ u64 weight_of_key(uint32_t key, const RowParams& r, d
   return b < kBins ? weight_int(weight_of(b, rem, s, roots)) : 0;
 }
 
-__device__ __forceinline__ u64 wave_max_u64(u64 v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const u64 x = __shfl_xor(v, o);
-    v = x > v ? x : v;
-  }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_u64(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+  return ((u64)hi << 32) | lo;
+}
+// Sums over the lanes up to each: within rows of 16 lanes, then over rows.
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+  v += dpp_u64<0x111, 0xF>(v);
+  v += dpp_u64<0x112, 0xF>(v);
+  v += dpp_u64<0x114, 0xF>(v);
+  v += dpp_u64<0x118, 0xF>(v);
+  v += dpp_u64<0x142, 0xA>(v);
+  v += dpp_u64<0x143, 0xC>(v);
   return v;
 }
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-  return v;
+__device__ __forceinline__ u64 last_lane(u64 v) {
+  return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), kWave - 1) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, kWave - 1);
+}
+__device__ __forceinline__ u64 max_u64(u64 a, u64 b) { return a > b ? a : b; }
+__device__ __forceinline__ u64 wave_max_u64(u64 v) {
+  v = max_u64(v, dpp_u64<0x111, 0xF>(v));
+  v = max_u64(v, dpp_u64<0x112, 0xF>(v));
+  v = max_u64(v, dpp_u64<0x114, 0xF>(v));
+  v = max_u64(v, dpp_u64<0x118, 0xF>(v));
+  v = max_u64(v, dpp_u64<0x142, 0xA>(v));
+  return last_lane(max_u64(v, dpp_u64<0x143, 0xC>(v)));
+}
+// The maximum over the 8 lanes of a segment, in each.
+__device__ __forceinline__ float seg_max_of(float v) {
+  auto from = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  v = fmaxf(v, from(v, std::integral_constant<int, 0xB1>{}));   // lanes 1 0 3 2
+  v = fmaxf(v, from(v, std::integral_constant<int, 0x4E>{}));   // 2 3 0 1
+  return fmaxf(v, from(v, std::integral_constant<int, 0x141>{}));  // 7 .. 0 of each 8
 }
 
-// ---- scan ----
+// Index of the first token of vector v that has this key.
 template <int DT>
+__device__ __forceinline__ uint32_t index_in(const Row<DT>& x, int v, uint32_t key) {
+  float val[kVec<DT>];
+  values<DT>(x.vec(v), val);
+  int at = kVec<DT> - 1;
+#pragma unroll
+  for (int e = kVec<DT> - 2; e >= 0; --e) at = key_of(val[e]) == key ? e : at;
+  return (uint32_t)(v * kVec<DT> + at - x.skew);
+}
+
+// ---- count: the scan of 16-bit logits ----
+// A work-group counts its chunk's values by their 16 bits (two counts a word: a value and its negative), and
+// weighs each value that occurs once, times its count: integers, so the sum is the tokens' own.
+struct CountShared {
+  uint32_t pair[32768];
+  u64 weight[kBins];
+  uint32_t count[kBins];
+  double roots[16];
+  u64 best[kCountWaves];
+  uint32_t tokens;
+};
+template <int DT>
+__global__ __launch_bounds__(kCountThreads) void sample_count_kernel(SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  CountShared& s = *(CountShared*)smem;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lane = tid % kWave;
+  const int row = blockIdx.x / p.chunks;
+  const int chunk = blockIdx.x % p.chunks;
+  const RowParams r = row_params(p, row);
+  const Row<DT> x(p, row);
+  const int lines = (x.vecs + kWave - 1) / kWave;
+  const int l0 = (int)((int64_t)lines * chunk / p.chunks), l1 = (int)((int64_t)lines * (chunk + 1) / p.chunks);
+  u32x4 raw[kCountLines];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int j = 0; j < kCountLines; ++j)
+      if (at + j * kCountWaves < l1) raw[j] = x.vec((at + j * kCountWaves) * kWave + lane);
+  };
+  load(l0 + wave);
+  for (int i = tid; i < 8192; i += kCountThreads) ((u32x4*)s.pair)[i] = u32x4{0, 0, 0, 0};
+  s.weight[tid] = 0;
+  s.count[tid] = 0;
+  if (tid < 16) s.roots[tid] = kRoots[tid];
+  if (tid == 0) s.tokens = 0;
+  __syncthreads();
+  float best = -INFINITY;
+  int best_vec = 0;
+  for (int at = l0 + wave; at < l1; at += kCountLines * kCountWaves) {
+    u32x4 now[kCountLines];
+#pragma unroll
+    for (int j = 0; j < kCountLines; ++j) now[j] = raw[j];
+    load(at + kCountLines * kCountWaves);
+#pragma unroll
+    for (int j = 0; j < kCountLines; ++j) {
+      const int line = at + j * kCountWaves;
+      if (line >= l1) continue;
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t u = now[j][e];
+        if (!r.greedy) {
+          atomicAdd(&s.pair[u & 0x7FFF], 1u << ((u >> 11) & 16));
+          atomicAdd(&s.pair[(u >> 16) & 0x7FFF], 1u << ((u >> 27) & 16));
+        }
+        top = fmaxf(fmaxf(top, element<DT>(u, 0)), element<DT>(u, 1));  // (not NaN)
+      }
+      if (top > best) {  // a lane's vectors come in order
+        best = top;
+        best_vec = line * kWave + lane;
+      }
+      top = seg_max_of(top);
+      if (lane % kSegVecs == 0) p.seg_max[(int64_t)row * p.segs + line * kLineSegs + lane / kSegVecs] = key_of(top);
+    }
+  }
+  const uint32_t key = key_of(best);
+  const u64 mine = wave_max_u64(key ? order_word(key, best_vec) : 0);
+  if (lane == 0) s.best[wave] = mine;
+  __syncthreads();
+  u64 all = 0;
+#pragma unroll
+  for (int w = 0; w < kCountWaves; ++w) all = s.best[w] > all ? s.best[w] : all;
+  const uint32_t all_key = word_key(all);
+  const double base = all && !r.greedy ? floor(finite(logit_of(all_key)) * r.scale / kBinsPerLog2) + 1.0 : 0.0;
+  uint32_t tokens = 0;
+  if (all && !r.greedy) {
+    const double base16 = kBinsPerLog2 * base;
+    // (a word per lane: the values that occur are few runs, which all waves share)
+#pragma unroll 4
+    for (int i = tid; i < 32768; i += kCountThreads) {
+      const uint32_t two = s.pair[i];
+      if (two == 0) continue;
+#pragma unroll
+      for (int sign = 0; sign < 2; ++sign) {  // (both at once: a chain of 64-bit operations each)
+        const float v = element<DT>((uint32_t)i | (uint32_t)sign << 15, 0);
+        const uint32_t n = v > -INFINITY ? sign ? two >> 16 : two & 0xFFFF : 0;
+        double rem;
+        const int b = bin_of(finite(v) * r.scale, base16, rem);
+        const u64 w = weight_int(weight_of(b, rem, p.weight_exp, s.roots));
+        tokens += n;
+        if (n != 0 && b < kBins - 1) {  // the last bin is what the others leave
+          atomicAdd(&s.count[b], n);
+          if (r.weigh) atomicAdd(&s.weight[b], n * w);
+        }
+      }
+    }
+    const uint32_t sum = (uint32_t)last_lane(wave_scan(tokens));
+    if (lane == 0 && sum) atomicAdd(&s.tokens, sum);
+  }
+  __syncthreads();
+  const int64_t to = (int64_t)row * p.chunks + chunk;
+  if (tid == 0) {
+    ChunkHead h;
+    h.best = all;
+    h.base = base;
+    h.tokens = s.tokens;
+    h.pad[0] = h.pad[1] = h.pad[2] = 0;
+    p.heads[to] = h;
+  }
+  if (r.greedy) return;
+  p.counts[to * kBins + tid] = s.count[tid];
+  if (r.weigh) p.weights[to * kBins + tid] = s.weight[tid];
+}
+
+// ---- scan of fp32 logits ----
 __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams p) {
+  constexpr int DT = NE_DTYPE_FP32;
   constexpr int E = kVec<DT>;
   __shared__ uint32_t s_count[kBins];
   __shared__ u64 s_weight[kBins];
@@ -270,9 +432,8 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
   const int chunk = blockIdx.x % p.chunks;
   const RowParams r = row_params(p, row);
   const Row<DT> x(p, row);
-  const int segs = (x.vecs + kWave - 1) / kWave;
-  const int seg0 = (int)((int64_t)segs * chunk / p.chunks);
-  const int seg1 = (int)((int64_t)segs * (chunk + 1) / p.chunks);
+  const int lines = (x.vecs + kWave - 1) / kWave;
+  const int l0 = (int)((int64_t)lines * chunk / p.chunks), l1 = (int)((int64_t)lines * (chunk + 1) / p.chunks);
   if (tid < 16) s_roots[tid] = kRoots[tid];
   if (tid == 0) s_tokens = 0;
 #pragma unroll
@@ -281,48 +442,46 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
     s_weight[tid + b * kScanThreads] = 0;
   }
   float best_logit = -INFINITY;
-  uint32_t best_index = 0, tokens = 0;
+  int best_vec = 0;
+  uint32_t tokens = 0;
   double base = 0;
   bool any = false;  // base is set
-  constexpr int kStep = kScanWaves * kScanSegs;
-  u32x4 raw[kScanSegs];
-  bool whole[kScanSegs];
+  constexpr int kStep = kScanWaves * kScanLines;
+  u32x4 raw[kScanLines];
   auto load = [&](int s0) {
 #pragma unroll
-    for (int j = 0; j < kScanSegs; ++j) {
-      const int seg = s0 + wave * kScanSegs + j;
-      whole[j] = false;
-      if (seg < seg1) raw[j] = x.raw(seg * kWave + lane, whole[j]);
+    for (int j = 0; j < kScanLines; ++j) {
+      const int line = s0 + wave * kScanLines + j;
+      if (line < l1) raw[j] = x.vec(line * kWave + lane);
     }
   };
-  load(seg0);
+  load(l0);
   int turn = 0;
-  for (int s0 = seg0; s0 < seg1; s0 += kStep, turn ^= 1) {
-    float val[kScanSegs][E];
+  for (int s0 = l0; s0 < l1; s0 += kStep, turn ^= 1) {
+    float val[kScanLines][E];
     float most = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kScanSegs; ++j) {
-      const int seg = s0 + wave * kScanSegs + j;
-      const int v = seg * kWave + lane;
+    for (int j = 0; j < kScanLines; ++j) {
+      const int line = s0 + wave * kScanLines + j;
+      const int v = line * kWave + lane;
 #pragma unroll
       for (int e = 0; e < E; ++e) val[j][e] = NAN;
-      if (seg < seg1) {
+      if (line < l1) {
         float here = -INFINITY;
-        if (v < x.vecs) x.values(v, raw[j], whole[j], val[j]);
+        values<DT>(raw[j], val[j]);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if (val[j][e] > best_logit) {  // a lane's tokens come in order of index
-            best_logit = val[j][e];
-            best_index = v * E + e - x.skew;
-          }
-          here = fmaxf(here, val[j][e]);  // (not NaN)
+        for (int e = 0; e < E; ++e) here = fmaxf(here, val[j][e]);  // (not NaN)
+        if (here > best_logit) {  // a lane's vectors come in order
+          best_logit = here;
+          best_vec = v;
         }
-        here = wave_max(here);
-        if (lane == 0) p.seg_max[(int64_t)row * p.segs + seg] = key_of(here);
+        here = seg_max_of(here);
+        if (lane % kSegVecs == 0) p.seg_max[(int64_t)row * p.segs + line * kLineSegs + lane / kSegVecs] = key_of(here);
         most = fmaxf(most, here);
       }
     }
-    if (s0 + kStep < seg1) load(s0 + kStep);
+    most = wave_max(most);
+    if (s0 + kStep < l1) load(s0 + kStep);
     if (lane == 0) s_max[turn][wave] = most;
     __syncthreads();
 #pragma unroll
@@ -353,7 +512,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
     }
     const double base16 = kBinsPerLog2 * base;
 #pragma unroll
-    for (int j = 0; j < kScanSegs; ++j) {
+    for (int j = 0; j < kScanLines; ++j) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const bool is = val[j][e] > -INFINITY;
@@ -368,7 +527,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
     }
   }
   const uint32_t best_key = key_of(best_logit);
-  const u64 best = wave_max_u64(best_key ? order_word(best_key, best_index) : 0);
+  const u64 best = wave_max_u64(best_key ? order_word(best_key, best_vec) : 0);
   if (lane == 0) s_best[wave] = best;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) tokens += __shfl_xor((int)tokens, o);
@@ -409,10 +568,11 @@ struct PickShared {
     int down[2 * kNumCu];  // each chunk's base below the row's
   };
   uint32_t bucket[kSortBuckets + 1];
+  uint32_t seg[kSegsHeld];  // the first segments' largest keys
   double roots[16];
   u64 part[2 * kPickWaves];
   u64 red[4];
-  uint32_t n;
+  uint32_t n, wanted;
 };
 
 // f * sum rounded down, or up; exact (equal weights make borders that a rounded product would
@@ -467,22 +627,6 @@ __device__ __forceinline__ int first_reaching(const T* sums, int n, u64 target) 
   return uni(lo);
 }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ u64 dpp_u64(u64 v) {
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
-  return ((u64)hi << 32) | lo;
-}
-// Sums over the lanes up to each: within rows of 16 lanes, then over rows.
-__device__ __forceinline__ u64 wave_scan(u64 v) {
-  v += dpp_u64<0x111, 0xF>(v);
-  v += dpp_u64<0x112, 0xF>(v);
-  v += dpp_u64<0x114, 0xF>(v);
-  v += dpp_u64<0x118, 0xF>(v);
-  v += dpp_u64<0x142, 0xA>(v);
-  v += dpp_u64<0x143, 0xC>(v);
-  return v;
-}
 // Sums of two values over the threads up to each, in thread order.
 __device__ __forceinline__ void block_scan(PickShared& s, u64& a, u64& b) {
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -591,7 +735,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
   const int lane = tid % kWave;
   const RowParams r = row_params(p, row);
   const Row<DT> x(p, row);
-  const int segs = (x.vecs + kWave - 1) / kWave;
+  const int segs = (x.vecs + kWave - 1) / kWave * kLineSegs;
   const uint32_t* seg_max = p.seg_max + (int64_t)row * p.segs;
   const ChunkHead* heads = p.heads + (int64_t)row * p.chunks;
   u64 best = 0, tokens = 0;
@@ -610,6 +754,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
   }
   base = uni(base);
   tokens = uni(tokens);
+  if (best != 0 && r.greedy) best = order_word(word_key(best), index_in(x, word_index(best), word_key(best)));
   RowResult out;
   out.last = best;
   out.base = base;
@@ -624,6 +769,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
   }
   const double base16 = kBinsPerLog2 * base;
   const uint32_t best_key = word_key(best);
+  for (int i = tid; i < min(segs, kSegsHeld); i += kPickThreads) s.seg[i] = seg_max[i];
   if (tid < 16) s.roots[tid] = kRoots[tid];
   // ---- the row's histogram, as sums from the first bin on ----
   for (int c = tid; c < p.chunks; c += kPickThreads)  // (at most 2 kNumCu of them)
@@ -634,15 +780,24 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
     u64 count = 0, weight = 0;
     const uint32_t* counts = p.counts + (int64_t)row * p.chunks * kBins;
     const u64* weights = p.weights + (int64_t)row * p.chunks * kBins;
-#pragma unroll 4
-    for (int c = 0; c < p.chunks; ++c) {
-      const int down = s.down[c];
-      const int from = max(tid - kBinsPerLog2 * down, 0);
-      const bool has = tid >= kBinsPerLog2 * down && down < 64;
-      const uint32_t n = counts[(int64_t)c * kBins + from];
-      const u64 w = r.weigh ? weights[(int64_t)c * kBins + from] : 0;
-      count += has ? n : 0;
-      weight += has ? w >> down : 0;
+    constexpr int kAhead = 8;
+    for (int c0 = 0; c0 < p.chunks; c0 += kAhead) {
+      uint32_t n[kAhead];
+      u64 w[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int c = min(c0 + j, p.chunks - 1);
+        const int64_t from = (int64_t)c * kBins + max(tid - kBinsPerLog2 * s.down[c], 0);
+        n[j] = counts[from];
+        w[j] = r.weigh ? weights[from] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int down = s.down[min(c0 + j, p.chunks - 1)];
+        const bool has = c0 + j < p.chunks && tid >= kBinsPerLog2 * down && down < 64;
+        count += has ? n[j] : 0;
+        weight += has ? w[j] >> down : 0;
+      }
     }
     block_scan(s, count, weight);
     s.count[tid] = tid == kBins - 1 ? (uint32_t)tokens : (uint32_t)count;
@@ -750,48 +905,57 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
       s.weight[tid] = 0;
     }
     __syncthreads();
-    // ---- the row's segments whose largest key reaches the pass's tokens, four at a time ----
+    // ---- the row's segments whose largest key reaches the pass's tokens, 32 at a time ----
     // (the bins as keys: an element costs two comparisons, and only those inside the rest)
     klo = max(klo, key_from(bhi, best_key, r, base16));
     khi = min(khi, blo > 0 ? key_from(blo - 1, best_key, r, base16) - 1 : best_key);
     const float xlo = logit_of(klo), xhi = logit_of(khi);
     u64 acc0 = act == kKeyRange ? 0xFFFFFFFFu : 0, acc1 = 0, acc2 = ~0ull;
-    for (int s0 = 0; s0 < segs && klo <= khi; s0 += kPickThreads) {
-      const int mine = s0 + lane * kPickWaves + wave;
-      u64 want = __ballot((mine < segs ? seg_max[mine] : 0) >= klo);
-      while (want) {
-        constexpr int kAhead = 4;
+    for (int s0 = 0; s0 < segs && klo <= khi; s0 += kSegsHeld) {
+      uint16_t* list = (uint16_t*)s.bucket;
+      __syncthreads();
+      if (tid == 0) s.wanted = 0;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kSegsHeld / kPickThreads; ++k) {
+        const int i = s0 + k * kPickThreads + tid;
+        if (i >= segs || (s0 == 0 ? s.seg[i] : seg_max[i]) < klo) continue;
+        list[atomicAdd(&s.wanted, 1u)] = (uint16_t)(i - s0);
+      }
+      __syncthreads();
+      const int wanted = uni((int)s.wanted);
+      constexpr int kAhead = 4;
+      for (int w0 = wave * kAhead * kLineSegs; w0 < wanted; w0 += kPickWaves * kAhead * kLineSegs) {
         u32x4 raw[kAhead];
-        bool whole[kAhead];
-        int seg[kAhead];
+        int vec[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-          seg[j] = -1;
-          whole[j] = false;
-          if (want) {
-            seg[j] = s0 + (int)__builtin_ctzll(want) * kPickWaves + wave;
-            want &= want - 1;
-            raw[j] = x.raw(seg[j] * kWave + lane, whole[j]);
-          }
+          const int at = w0 + j * kLineSegs + lane / kSegVecs;  // a segment for every 8 lanes
+          vec[j] = at < wanted ? (s0 + list[at]) * kSegVecs + lane % kSegVecs : x.vecs;  // past the row
+          raw[j] = x.vec(vec[j]);
         }
         uint32_t inside = 0;  // one bit per element
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-          if (seg[j] < 0) continue;
           float val[E];
-          x.values(seg[j] * kWave + lane, raw[j], whole[j], val);
+          values<DT>(raw[j], val);
 #pragma unroll
           for (int e = 0; e < E; ++e) inside |= (uint32_t)(val[e] >= xlo && val[e] <= xhi) << (j * E + e);
         }
         while (inside) {
           const int bit = __builtin_ctz(inside);
           inside &= inside - 1;
-          int of = seg[0];
+          int of = vec[0];
+          uint32_t dword = raw[0][0];
 #pragma unroll
-          for (int j = 1; j < kAhead; ++j) of = bit >= j * E ? seg[j] : of;
-          const int t = (of * kWave + lane) * E + bit % E - x.skew;
+          for (int j = 0; j < kAhead; ++j) {
+            of = bit >= j * E ? vec[j] : of;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) dword = bit >= j * E + d * E / 4 ? raw[j][d] : dword;
+          }
+          const int t = of * E + bit % E - x.skew;
           if ((uint32_t)t < ilo || (uint32_t)t > ihi) continue;
-          const float v = x.single(t);
+          const float v = element<DT>(dword, bit % (E / 4));
           const uint32_t k = key_of(v);
           if (act == kGather) {
             const uint32_t at = atomicAdd(&s.n, 1u);
@@ -1063,18 +1227,14 @@ __global__ __launch_bounds__(kProbsThreads) void sample_probs_kernel(SampleParam
   const double inv = 1.0 / r.sum, base16 = kBinsPerLog2 * r.base;
   float* to = p.probs + (int64_t)row * p.ld_probs;
   u32x4 raw[kProbsPer];
-  bool whole[kProbsPer];
 #pragma unroll
-  for (int j = 0; j < kProbsPer; ++j) {
-    whole[j] = false;
-    if (v0 + j * kProbsThreads < x.vecs) raw[j] = x.raw(v0 + j * kProbsThreads, whole[j]);
-  }
+  for (int j = 0; j < kProbsPer; ++j) raw[j] = x.vec(v0 + j * kProbsThreads);
 #pragma unroll
   for (int j = 0; j < kProbsPer; ++j) {
     const int v = v0 + j * kProbsThreads;
     if (v >= x.vecs) continue;
     float val[E], out[E];
-    x.values(v, raw[j], whole[j], val);
+    values<DT>(raw[j], val);
     const int t0 = v * E - x.skew;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -1089,7 +1249,7 @@ __global__ __launch_bounds__(kProbsThreads) void sample_probs_kernel(SampleParam
         out[e] = b < kFarBins ? (float)(weight_of(b, rem, 0, s_roots) * inv) : 0.f;
       }
     }
-    if (whole[j] && ((uintptr_t)(to + t0) & 15) == 0) {
+    if (t0 >= 0 && t0 + E <= x.vocab && ((uintptr_t)(to + t0) & 15) == 0) {
 #pragma unroll
       for (int e = 0; e < E; e += 4) *(floatx4*)(to + t0 + e) = floatx4{out[e], out[e + 1], out[e + 2], out[e + 3]};
     } else {
@@ -1103,11 +1263,14 @@ __global__ __launch_bounds__(kProbsThreads) void sample_probs_kernel(SampleParam
 // ---- host ----
 int elements_per_vec(int dtype) { return dtype == NE_DTYPE_FP32 ? 4 : 8; }
 
-// Chunks of a row: enough work-groups to fill the chip twice, at least one iteration of the scan each.
-int row_chunks(int rows, int segs) {
-  const int want = ceil_div(2 * kNumCu, rows < 1 ? 1 : rows);
-  const int most = ceil_div(segs, kScanWaves * kScanSegs);
-  return want < most ? want : most;
+// Chunks of a row.  fp32: enough work-groups to fill the chip twice, at least one iteration of the scan each;
+// 16 bits: a work-group per CU, whose table clears and reads take as long as 8,192 elements.
+int row_chunks(int rows, int lines, int dtype) {
+  rows = rows < 1 ? 1 : rows;
+  const int want = ceil_div(dtype == NE_DTYPE_FP32 ? 2 * kNumCu : kNumCu, rows);
+  const int most = ceil_div(lines, dtype == NE_DTYPE_FP32 ? kScanWaves * kScanLines : kCountWaves);
+  const int n = want < most ? want : most, least = ceil_div(lines, kCountMost);
+  return dtype == NE_DTYPE_FP32 || n > least ? n : least;
 }
 
 struct Layout {
@@ -1118,8 +1281,9 @@ Layout layout_of(int rows, int vocab, int dtype) {
   Layout l;
   const int e = elements_per_vec(dtype);
   rows = rows < kRowBatch ? rows : kRowBatch;
-  l.segs = ceil_div(vocab + e - 1, e * kWave);  // a row off the 16-byte grid may touch one vector more
-  l.chunks = row_chunks(rows, l.segs);
+  const int lines = ceil_div(vocab + e - 1, e * kWave);  // a row off the 16-byte grid may touch one vector more
+  l.segs = lines * kLineSegs;
+  l.chunks = row_chunks(rows, lines, dtype);
   const size_t n = (size_t)rows * l.chunks;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -1138,7 +1302,17 @@ Layout layout_of(int rows, int vocab, int dtype) {
 
 template <int DT>
 int launch(const SampleParams& p, hipStream_t s) {
-  hipLaunchKernelGGL(sample_scan_kernel<DT>, dim3(p.rows * p.chunks), dim3(kScanThreads), 0, s, p);
+  if constexpr (DT == NE_DTYPE_FP32) {
+    hipLaunchKernelGGL(sample_scan_kernel, dim3(p.rows * p.chunks), dim3(kScanThreads), 0, s, p);
+  } else {
+    static const hipError_t attr = hipFuncSetAttribute((const void*)sample_count_kernel<DT>,
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, sizeof(CountShared));
+    if (attr != hipSuccess) {
+      set_error("sample_count: cannot reserve %d bytes of LDS: %s", (int)sizeof(CountShared), hipGetErrorString(attr));
+      return NE_ELAUNCH;
+    }
+    hipLaunchKernelGGL(sample_count_kernel<DT>, dim3(p.rows * p.chunks), dim3(kCountThreads), sizeof(CountShared), s, p);
+  }
   int rc = check_launch("sample_scan");
   if (rc != NE_OK) return rc;
   static const hipError_t attr = hipFuncSetAttribute((const void*)sample_pick_kernel<DT>,
