@@ -134,8 +134,10 @@ __device__ __forceinline__ uint32_t word_key(u64 w) { return (uint32_t)(w >> 32)
 // element e of vector v is token v * kVec + e - skew.
 template <int DT>
 struct Row {
-  const u32x4* base;  // vector 0: a scalar load of a vector needs its base on the grid too
+  const u32x4* base;   // vector 0: a scalar load of a vector needs its base on the grid too
+  const u32x4* whole;  // the first vector that lies in the row, or some memory where none does
   int skew, vocab, vecs;
+  int whole0, wholes;  // vectors that lie in the row
   __device__ Row(const SampleParams& p, int row) {
     constexpr int kEsz = 16 / kVec<DT>;
     const char* at = (const char*)p.logits + (int64_t)row * p.ld * kEsz;
@@ -143,26 +145,37 @@ struct Row {
     base = (const u32x4*)(at - skew * kEsz);
     vocab = p.vocab;
     vecs = (vocab + skew + kVec<DT> - 1) / kVec<DT>;
+    whole0 = skew > 0;
+    wholes = max((vocab + skew) / kVec<DT> - whole0, 0);
+    whole = wholes > 0 ? base + whole0 : (const u32x4*)p.heads;
   }
+  __device__ __forceinline__ bool is_whole(int v) const { return (uint32_t)(v - whole0) < (uint32_t)wholes; }
+  // All of a line (a vector per lane) lies in the row.
+  __device__ __forceinline__ bool inner(int line) const { return line * kWave >= whole0 && (line + 1) * kWave <= whole0 + wholes; }
+  // Vector v where that lies in the row, else another: a load without a branch, so that those after it need
+  // not be waited for.
+  __device__ __forceinline__ u32x4 ahead(int v) const { return whole[min(max(v - whole0, 0), max(wholes - 1, 0))]; }
   // Vector v, NaN for what lies outside the row.
   __device__ __forceinline__ u32x4 vec(int v) const {
     const int t0 = v * kVec<DT> - skew;
-    if (t0 >= 0 && t0 + kVec<DT> <= vocab) return base[v];
+    if (is_whole(v)) return base[v];
     const uint32_t none = DT == NE_DTYPE_FP32 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
-    u32x4 out = {none, none, none, none};
-    if (v >= vecs) return out;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
+    uint32_t out[4] = {none, none, none, none};
+    if (v >= vecs) return u32x4{none, none, none, none};
+#pragma unroll 1
+    for (int e = 0; e < kVec<DT>; ++e) {
+      if (t0 + e < 0 || t0 + e >= vocab) continue;
+      uint32_t bits, keep = 0;
       if constexpr (DT == NE_DTYPE_FP32) {
-        if (t0 + d >= 0 && t0 + d < vocab) out[d] = ((const uint32_t*)(base + v))[d];
+        bits = ((const uint32_t*)(base + v))[e];
       } else {
-        const uint16_t* at = (const uint16_t*)(base + v) + 2 * d;
-        const int t = t0 + 2 * d;
-        const uint32_t lo = t >= 0 && t < vocab ? at[0] : 0x7FFF, hi = t + 1 >= 0 && t + 1 < vocab ? at[1] : 0x7FFF;
-        out[d] = lo | (hi << 16);
+        bits = (uint32_t)((const uint16_t*)(base + v))[e] << (16 * (e & 1));
+        keep = e & 1 ? 0xFFFFu : 0xFFFF0000u;
       }
+#pragma unroll
+      for (int d = 0; d < 4; ++d) out[d] = d == e * 4 / kVec<DT> ? (out[d] & keep) | bits : out[d];
     }
-    return out;
+    return u32x4{out[0], out[1], out[2], out[3]};
   }
 };
 // Element e of a dword's one or two.
@@ -184,8 +197,7 @@ __device__ __forceinline__ void values(u32x4 x, float (&out)[kVec<DT>]) {
 // ---- row parameters ----
 struct RowParams {
   double scale;  // 16 log2(e) / T
-  double log2_min_p;  // -inf: off
-  float top_p;
+  float top_p, min_p;
   int top_k;     // 0: off
   bool greedy;
   bool weigh;    // the scan sums weights
@@ -200,7 +212,7 @@ __device__ __forceinline__ RowParams row_params(const SampleParams& p, int row) 
   r.scale = r.greedy ? 0.0 : kBinsPerLog2 * 1.4426950408889634 / (double)t;
   r.top_k = k > 0 && k < p.vocab ? k : 0;
   r.weigh = !r.greedy && (r.top_k == 0 || r.top_k > kShortTopK);
-  r.log2_min_p = m > 0.f ? log2(fmin((double)m, 1.0)) : -INFINITY;
+  r.min_p = m;
   return r;
 }
 
@@ -279,6 +291,18 @@ __device__ __forceinline__ u64 wave_max_u64(u64 v) {
   v = max_u64(v, dpp_u64<0x142, 0xA>(v));
   return last_lane(max_u64(v, dpp_u64<0x143, 0xC>(v)));
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
+}
+// The maximum over 16 lanes, in the last.
+__device__ __forceinline__ uint32_t row_max_u32(uint32_t v) {
+  return dpp_max<0x118, 0xF>(dpp_max<0x114, 0xF>(dpp_max<0x112, 0xF>(dpp_max<0x111, 0xF>(v))));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  v = dpp_max<0x143, 0xC>(dpp_max<0x142, 0xA>(row_max_u32(v)));
+  return __builtin_amdgcn_readlane((int)v, kWave - 1);
+}
 // The maximum over the 8 lanes of a segment, in each.
 __device__ __forceinline__ float seg_max_of(float v) {
   auto from = [](float x, auto ctrl) {
@@ -301,99 +325,156 @@ __device__ __forceinline__ uint32_t index_in(const Row<DT>& x, int v, uint32_t k
 }
 
 // ---- count: the scan of 16-bit logits ----
-// A work-group counts its chunk's values by their 16 bits (two counts a word: a value and its negative), and
-// weighs each value that occurs once, times its count: integers, so the sum is the tokens' own.
+// A work-group counts its chunk's values by their bits (two counts a word: a value and its negative), and
+// weighs each value that occurs once, times its count: integers, so the sum is the tokens' own.  Counted are
+// magnitudes in a window, 2^-14 to 2^8 (bf16), 2^-7 to 2^7 (fp16); the few values outside are listed, and a
+// chunk of more than the list holds is read again for them.  The window leaves room for two work-groups per
+// CU: a table of all values took 53 us for 320 rows of 151,936.
+template <int DT>
+constexpr uint32_t kWindow = DT == NE_DTYPE_FP16 ? 14 * 1024 : 22 * 128;
+template <int DT>
+constexpr uint32_t kWindowFrom = DT == NE_DTYPE_FP16 ? (15 - 7) << 10 : (127 - 14) << 7;
+constexpr int kListed = 4096;
+template <int DT>
+constexpr int16_t kInfinity = DT == NE_DTYPE_FP16 ? 0x7C00 : 0x7F80;
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+// Two halves' order as signed integers, and back.  Positive NaN come out above everything.
+__device__ __forceinline__ i16x2 order_pair(uint32_t u) {
+  const i16x2 h = __builtin_bit_cast(i16x2, u);
+  return h ^ ((h >> 15) & (int16_t)0x7FFF);
+}
+template <int DT>
+__device__ __forceinline__ float logit_in_order(int v) { return element<DT>((uint16_t)(v ^ ((v >> 15) & 0x7FFF)), 0); }
+__device__ __forceinline__ int seg_max_of(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true));
+  return max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true));
+}
+template <int DT>
 struct CountShared {
-  uint32_t pair[32768];
+  uint32_t pair[kWindow<DT> + 4];  // (one more for what is outside)
   u64 weight[kBins];
   uint32_t count[kBins];
+  uint16_t listed[kListed];
   double roots[16];
-  u64 best[kCountWaves];
-  uint32_t tokens;
+  uint32_t best[kCountWaves];
+  uint32_t tokens, outside;
 };
 template <int DT>
-__global__ __launch_bounds__(kCountThreads) void sample_count_kernel(SampleParams p) {
+__global__ __launch_bounds__(kCountThreads, 8) void sample_count_kernel(SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  CountShared& s = *(CountShared*)smem;
+  CountShared<DT>& s = *(CountShared<DT>*)smem;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
-  const int row = blockIdx.x / p.chunks;
-  const int chunk = blockIdx.x % p.chunks;
+  const int row = blockIdx.y, chunk = blockIdx.x;
   const RowParams r = row_params(p, row);
   const Row<DT> x(p, row);
   const int lines = (x.vecs + kWave - 1) / kWave;
-  const int l0 = (int)((int64_t)lines * chunk / p.chunks), l1 = (int)((int64_t)lines * (chunk + 1) / p.chunks);
+  const int l0 = (uint32_t)(lines * chunk) / (uint32_t)p.chunks, l1 = (uint32_t)(lines * (chunk + 1)) / (uint32_t)p.chunks;
   u32x4 raw[kCountLines];
-  auto load = [&](int at) {
 #pragma unroll
-    for (int j = 0; j < kCountLines; ++j)
-      if (at + j * kCountWaves < l1) raw[j] = x.vec((at + j * kCountWaves) * kWave + lane);
-  };
-  load(l0 + wave);
-  for (int i = tid; i < 8192; i += kCountThreads) ((u32x4*)s.pair)[i] = u32x4{0, 0, 0, 0};
+  for (int j = 0; j < kCountLines; ++j) raw[j] = x.ahead((l0 + wave + j * kCountWaves) * kWave + lane);
+  // a token whose magnitude the window does not hold
+  auto is_outside = [](uint32_t bits) { return (bits & 0x7FFF) - kWindowFrom<DT> >= kWindow<DT> && element<DT>(bits, 0) > -INFINITY; };
+  for (int i = tid; i < (int)(kWindow<DT> / 4) + 1; i += kCountThreads) ((u32x4*)s.pair)[i] = u32x4{0, 0, 0, 0};
   s.weight[tid] = 0;
   s.count[tid] = 0;
   if (tid < 16) s.roots[tid] = kRoots[tid];
-  if (tid == 0) s.tokens = 0;
+  if (tid == 0) s.tokens = s.outside = 0;
   __syncthreads();
-  float best = -INFINITY;
-  int best_vec = 0;
+  int best_order = INT16_MIN, best_vec = l0 * kWave;
   for (int at = l0 + wave; at < l1; at += kCountLines * kCountWaves) {
-    u32x4 now[kCountLines];
-#pragma unroll
-    for (int j = 0; j < kCountLines; ++j) now[j] = raw[j];
-    load(at + kCountLines * kCountWaves);
+    int seg_top = INT16_MIN;  // of line lane % kSegVecs
 #pragma unroll
     for (int j = 0; j < kCountLines; ++j) {
       const int line = at + j * kCountWaves;
       if (line >= l1) continue;
-      float top = -INFINITY;
+      u32x4 now = raw[j];
+      raw[j] = x.ahead((line + kCountLines * kCountWaves) * kWave + lane);
+      if (!x.inner(line)) now = x.vec(line * kWave + lane);
+      i16x2 tops = {INT16_MIN, INT16_MIN};
+      uint32_t far = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t u = now[j][e];
-        if (!r.greedy) {
-          atomicAdd(&s.pair[u & 0x7FFF], 1u << ((u >> 11) & 16));
-          atomicAdd(&s.pair[(u >> 16) & 0x7FFF], 1u << ((u >> 27) & 16));
-        }
-        top = fmaxf(fmaxf(top, element<DT>(u, 0)), element<DT>(u, 1));  // (not NaN)
+        const uint32_t u = now[e];
+        // (as byte offsets)
+        const uint32_t lo = min(((u & 0x7FFF) << 2) - 4 * kWindowFrom<DT>, 4 * kWindow<DT>);
+        const uint32_t hi = min((((u >> 16) & 0x7FFF) << 2) - 4 * kWindowFrom<DT>, 4 * kWindow<DT>);
+        far = max(max(far, lo), hi);
+        atomicAdd((uint32_t*)((char*)s.pair + lo), (int16_t)u < 0 ? 0x10000u : 1u);
+        atomicAdd((uint32_t*)((char*)s.pair + hi), (int32_t)u < 0 ? 0x10000u : 1u);
+        tops = __builtin_elementwise_max(tops, order_pair(u));
       }
-      if (top > best) {  // a lane's vectors come in order
-        best = top;
+      int top = max(tops[0], tops[1]);
+      if (top > kInfinity<DT>) {  // a NaN among them
+        top = INT16_MIN;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const i16x2 h = order_pair(now[e]);
+          top = max(top, max(h[0] > kInfinity<DT> ? INT16_MIN : (int)h[0], h[1] > kInfinity<DT> ? INT16_MIN : (int)h[1]));
+        }
+      }
+      if (far == 4 * kWindow<DT>) {
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t d = e < 4 ? e < 2 ? now[0] : now[1] : e < 6 ? now[2] : now[3];
+          const uint32_t bits = d >> (16 * (e & 1)) & 0xFFFF;
+          if (!is_outside(bits)) continue;
+          const uint32_t to = atomicAdd(&s.outside, 1u);
+          if (to < (uint32_t)kListed) s.listed[to] = (uint16_t)bits;
+        }
+      }
+      if (top > best_order) {  // a lane's vectors come in order
+        best_order = top;
         best_vec = line * kWave + lane;
       }
       top = seg_max_of(top);
-      if (lane % kSegVecs == 0) p.seg_max[(int64_t)row * p.segs + line * kLineSegs + lane / kSegVecs] = key_of(top);
+      seg_top = lane % kSegVecs == j ? top : seg_top;
     }
+    const int line = at + lane % kSegVecs * kCountWaves;
+    if (lane % kSegVecs < kCountLines && line < l1)
+      p.seg_max[(int64_t)row * p.segs + line * kLineSegs + lane / kSegVecs] = key_of(logit_in_order<DT>(seg_top));
   }
-  const uint32_t key = key_of(best);
-  const u64 mine = wave_max_u64(key ? order_word(key, best_vec) : 0);
+  // the largest, and its first vector (of at most kCountMost lines)
+  const uint32_t mine = wave_max_u32((uint32_t)(best_order - INT16_MIN) << 16 | (0xFFFF - (best_vec - l0 * kWave)));
   if (lane == 0) s.best[wave] = mine;
   __syncthreads();
-  u64 all = 0;
-#pragma unroll
-  for (int w = 0; w < kCountWaves; ++w) all = s.best[w] > all ? s.best[w] : all;
-  const uint32_t all_key = word_key(all);
+  const uint32_t word = __builtin_amdgcn_readlane((int)row_max_u32(s.best[lane % kCountWaves]), 15);
+  const uint32_t all_key = key_of(logit_in_order<DT>((int)(word >> 16) + INT16_MIN));
+  const u64 all = all_key ? order_word(all_key, l0 * kWave + 0xFFFF - (word & 0xFFFF)) : 0;
   const double base = all && !r.greedy ? floor(finite(logit_of(all_key)) * r.scale / kBinsPerLog2) + 1.0 : 0.0;
   uint32_t tokens = 0;
   if (all && !r.greedy) {
     const double base16 = kBinsPerLog2 * base;
-    // (a word per lane: the values that occur are few runs, which all waves share)
-#pragma unroll 4
-    for (int i = tid; i < 32768; i += kCountThreads) {
+    auto add = [&](uint32_t bits, uint32_t n) {
+      const float v = element<DT>(bits, 0);
+      double rem;
+      const int b = bin_of(finite(v) * r.scale, base16, rem);
+      const u64 w = weight_int(weight_of(b, rem, p.weight_exp, s.roots));
+      tokens += n;
+      if (n != 0 && b < kBins - 1) {  // the last bin is what the others leave
+        atomicAdd(&s.count[b], n);
+        if (r.weigh) atomicAdd(&s.weight[b], n * w);
+      }
+    };
+    for (int i = tid; i < (int)kWindow<DT>; i += kCountThreads) {
       const uint32_t two = s.pair[i];
       if (two == 0) continue;
-#pragma unroll
-      for (int sign = 0; sign < 2; ++sign) {  // (both at once: a chain of 64-bit operations each)
-        const float v = element<DT>((uint32_t)i | (uint32_t)sign << 15, 0);
-        const uint32_t n = v > -INFINITY ? sign ? two >> 16 : two & 0xFFFF : 0;
-        double rem;
-        const int b = bin_of(finite(v) * r.scale, base16, rem);
-        const u64 w = weight_int(weight_of(b, rem, p.weight_exp, s.roots));
-        tokens += n;
-        if (n != 0 && b < kBins - 1) {  // the last bin is what the others leave
-          atomicAdd(&s.count[b], n);
-          if (r.weigh) atomicAdd(&s.weight[b], n * w);
+      add(kWindowFrom<DT> + i, two & 0xFFFF);  // (both at once: a chain of 64-bit operations each)
+      add((kWindowFrom<DT> + i) | 0x8000, two >> 16);
+    }
+    const uint32_t outside = s.outside;
+    if (outside <= (uint32_t)kListed) {
+      for (int i = tid; i < (int)outside; i += kCountThreads) add(s.listed[i], 1);
+    } else {
+      for (int line = l0 + wave; line < l1; line += kCountWaves) {
+        const u32x4 four = x.vec(line * kWave + lane);
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t d = e < 4 ? e < 2 ? four[0] : four[1] : e < 6 ? four[2] : four[3];
+          const uint32_t bits = d >> (16 * (e & 1)) & 0xFFFF;
+          if (is_outside(bits)) add(bits, 1);
         }
       }
     }
@@ -428,12 +509,11 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
-  const int row = blockIdx.x / p.chunks;
-  const int chunk = blockIdx.x % p.chunks;
+  const int row = blockIdx.y, chunk = blockIdx.x;
   const RowParams r = row_params(p, row);
   const Row<DT> x(p, row);
   const int lines = (x.vecs + kWave - 1) / kWave;
-  const int l0 = (int)((int64_t)lines * chunk / p.chunks), l1 = (int)((int64_t)lines * (chunk + 1) / p.chunks);
+  const int l0 = (uint32_t)(lines * chunk) / (uint32_t)p.chunks, l1 = (uint32_t)(lines * (chunk + 1)) / (uint32_t)p.chunks;
   if (tid < 16) s_roots[tid] = kRoots[tid];
   if (tid == 0) s_tokens = 0;
 #pragma unroll
@@ -452,7 +532,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
 #pragma unroll
     for (int j = 0; j < kScanLines; ++j) {
       const int line = s0 + wave * kScanLines + j;
-      if (line < l1) raw[j] = x.vec(line * kWave + lane);
+      raw[j] = x.ahead(line * kWave + lane);
     }
   };
   load(l0);
@@ -468,6 +548,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
       for (int e = 0; e < E; ++e) val[j][e] = NAN;
       if (line < l1) {
         float here = -INFINITY;
+        if (!x.inner(line)) raw[j] = x.vec(v);
         values<DT>(raw[j], val[j]);
 #pragma unroll
         for (int e = 0; e < E; ++e) here = fmaxf(here, val[j][e]);  // (not NaN)
@@ -806,9 +887,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
   __syncthreads();
   const u64 top_k = r.top_k && (u64)r.top_k < tokens ? r.top_k : tokens;
   const float u = p.uniforms[row];
-  const bool cut_p = r.top_p < 1.f, cut_m = r.log2_min_p != -INFINITY;
+  const bool cut_p = r.top_p < 1.f, cut_m = r.min_p > 0.f;
+  const double log2_min_p = cut_m ? log2(fmin((double)r.min_p, 1.0)) : -INFINITY;
   // min-p's border in sixteenths of log2, and its bin
-  const double y_min = uni(finite(logit_of(word_key(best))) * r.scale + kBinsPerLog2 * r.log2_min_p);
+  const double y_min = uni(finite(logit_of(word_key(best))) * r.scale + kBinsPerLog2 * log2_min_p);
   double rem;
   const int bin_m = uni(cut_m ? min(bin_of(y_min, base16, rem), kBins - 1) : kBins - 1);
   const int bin_k = first_reaching(s.count, kBins, top_k);
@@ -932,8 +1014,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
         for (int j = 0; j < kAhead; ++j) {
           const int at = w0 + j * kLineSegs + lane / kSegVecs;  // a segment for every 8 lanes
           vec[j] = at < wanted ? (s0 + list[at]) * kSegVecs + lane % kSegVecs : x.vecs;  // past the row
-          raw[j] = x.vec(vec[j]);
+          raw[j] = x.ahead(vec[j]);
         }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+          if (!x.is_whole(vec[j])) raw[j] = x.vec(vec[j]);
         uint32_t inside = 0;  // one bit per element
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
@@ -1228,11 +1313,12 @@ __global__ __launch_bounds__(kProbsThreads) void sample_probs_kernel(SampleParam
   float* to = p.probs + (int64_t)row * p.ld_probs;
   u32x4 raw[kProbsPer];
 #pragma unroll
-  for (int j = 0; j < kProbsPer; ++j) raw[j] = x.vec(v0 + j * kProbsThreads);
+  for (int j = 0; j < kProbsPer; ++j) raw[j] = x.ahead(v0 + j * kProbsThreads);
 #pragma unroll
   for (int j = 0; j < kProbsPer; ++j) {
     const int v = v0 + j * kProbsThreads;
     if (v >= x.vecs) continue;
+    if (!x.is_whole(v)) raw[j] = x.vec(v);
     float val[E], out[E];
     values<DT>(raw[j], val);
     const int t0 = v * E - x.skew;
@@ -1303,15 +1389,15 @@ Layout layout_of(int rows, int vocab, int dtype) {
 template <int DT>
 int launch(const SampleParams& p, hipStream_t s) {
   if constexpr (DT == NE_DTYPE_FP32) {
-    hipLaunchKernelGGL(sample_scan_kernel, dim3(p.rows * p.chunks), dim3(kScanThreads), 0, s, p);
+    hipLaunchKernelGGL(sample_scan_kernel, dim3(p.chunks, p.rows), dim3(kScanThreads), 0, s, p);
   } else {
     static const hipError_t attr = hipFuncSetAttribute((const void*)sample_count_kernel<DT>,
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, sizeof(CountShared));
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, sizeof(CountShared<DT>));
     if (attr != hipSuccess) {
-      set_error("sample_count: cannot reserve %d bytes of LDS: %s", (int)sizeof(CountShared), hipGetErrorString(attr));
+      set_error("sample_count: cannot reserve %d bytes of LDS: %s", (int)sizeof(CountShared<DT>), hipGetErrorString(attr));
       return NE_ELAUNCH;
     }
-    hipLaunchKernelGGL(sample_count_kernel<DT>, dim3(p.rows * p.chunks), dim3(kCountThreads), sizeof(CountShared), s, p);
+    hipLaunchKernelGGL(sample_count_kernel<DT>, dim3(p.chunks, p.rows), dim3(kCountThreads), sizeof(CountShared<DT>), s, p);
   }
   int rc = check_launch("sample_scan");
   if (rc != NE_OK) return rc;

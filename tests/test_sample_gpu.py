@@ -154,6 +154,18 @@ def test_masked_infinite_and_nan_logits(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("scale", [2.0**-14, 2.0**-7, 2.0**5, 2.0**9])
+def test_logits_of_any_magnitude(dtype, scale):
+    """Rows of tiny and huge logits, at the temperature that makes them ordinary ones, and rows with a few."""
+    x, u = make_logits(6, 40000, torch.float32, 5)
+    x = (x * scale).to(dtype)
+    x[3:, ::977] = torch.randn_like(x[3:, ::977].float()).to(dtype) * 2.0  # among them
+    for k, p, m in [(0, 1.0, 0.0), (50, 0.95, 0.02), (0, 0.8, 0.0), (3000, 0.99, 0.001)]:
+        check(x, u, max(scale, 2.0**-7), k, p, m)
+
+
+@pytest.mark.gpu
 def test_uniforms_off_their_range():
     x, _ = make_logits(5, 4000, torch.bfloat16, 8)
     check(x, torch.tensor([-1.0, 1.0, 7.5, math.inf, math.nan], device="cuda"), 0.9, 30, 0.9, 0.0)
