@@ -158,12 +158,12 @@ def copy_kv_blocks(buffers: list[torch.Tensor], block_size: int, src: list[int],
     if not buffers:
         raise ValueError("no buffers to copy in")
     first = buffers[0]
-    if any(t.get_device() != first.get_device() for t in buffers) or not first.is_cuda:
+    if not first.is_cuda or len(set(map(torch.Tensor.get_device, buffers))) > 1:
         _require_gpu(*buffers)  # names the tensor
     # (one call per tensor and check: a pool has four tensors per layer)
     shapes = [t.shape for t in buffers]
     num_slots = shapes[0][0] if shapes[0] else 0
-    _check(all(t.is_contiguous() for t in buffers) and all(s and s[0] == num_slots for s in shapes),
+    _check(all(map(torch.Tensor.is_contiguous, buffers)) and all([s and s[0] == num_slots for s in shapes]),
            "buffers must be contiguous and hold the same slots")
     _check(num_slots > 0, "buffers hold no slots")
     n = len(buffers)
