@@ -18,11 +18,12 @@
 // border of a flat row by 1e-7, a wrong token in a hundred rows of 100,000 tokens.
 //
 // Three kernels.
-//   scan   rows x chunks: reads the logits once.  Per 1 KB segment the largest key; per
-//          chunk the first largest token and a histogram over y in steps of 1/16 (1,024
+//   scan   rows x chunks: reads the logits once.  Per 128-byte segment the largest key; per
+//          chunk the largest and its vector, and a histogram over y in steps of 1/16 (1,024
 //          bins below the chunk's own base Y, counts and, unless top-k is short, weights).
 //          The base is an integer, so histograms of unlike bases merge by shifting 16 bins
-//          and one bit per step.
+//          and one bit per step.  16-bit logits are counted by value first, and each value
+//          is weighed once; fp32 ones are weighed one by one.
 //   pick   one work-group per row: merges the row's histograms, finds the last bin that can
 //          hold a kept token, and, where at most 4,096 tokens lie above its end, gathers
 //          them (only from segments whose largest key reaches it), sorts them in LDS and
@@ -31,8 +32,12 @@
 //          with more tokens than the list holds is narrowed by key first, and a run of
 //          equal logits by index.
 //   probs  rows x chunks: kept weight / sum per token, if asked for.
-// What bounds it: one read of the logits (scan), its ~25 64-bit operations per element
-// (full rate on this chip), and the chain of round trips in pick.
+// What bounds it, at 151,936 tokens a row.  320 rows (bf16, top-p, with probabilities) 152 us:
+// the scan 42, for its ~10 operations per element and the weights of ~3,000 values per chunk
+// (67% of the vector units' time); pick 46, the slowest row's chain of passes (40) on its one
+// work-group; probs 43, its bytes (292 MB, 6.9 TB/s).  64 rows 41 us: 11 and 24.  One row 31 us:
+// 6 and 20, a chain of round trips through memory and barriers.  200 rows of fp32 48 us: 22 (the
+// bytes, 5.6 TB/s) and 24.
 #include <math.h>
 #include <string.h>
 

@@ -140,14 +140,14 @@ __device__ __forceinline__ void plan_scan(const int (&v)[K], int (*s_part)[kPlan
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
   int incl[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) incl[k] = v[k];
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int y = __shfl_up(incl[k], o);
-      incl[k] += lane >= o ? y : 0;
-    }
+  for (int k = 0; k < K; ++k) {  // within rows of 16 lanes, then over rows
+    int x = v[k];
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    incl[k] = x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
   }
   __syncthreads();
   if (lane == kWave - 1) {

@@ -587,9 +587,11 @@ def shared_prefix_plan(
     (default: allocated here) is a uint8 tensor of :func:`shared_prefix_workspace_bytes` that no
     other plan uses until this one's calls are done."""
     device = _require_gpu(block_tables, ctx_len, q_start, q_len, groups.seqs, groups.start, groups.prefix_len)
-    for name, t in (("block_tables", block_tables), ("ctx_len", ctx_len), ("q_start", q_start), ("q_len", q_len),
-                    ("group seqs", groups.seqs), ("group start", groups.start), ("prefix_len", groups.prefix_len)):
-        _int32(t, name)
+    named = (("block_tables", block_tables), ("ctx_len", ctx_len), ("q_start", q_start), ("q_len", q_len),
+             ("group seqs", groups.seqs), ("group start", groups.start), ("prefix_len", groups.prefix_len))
+    for name, t in named:
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            _int32(t, name)
     num_seqs, num_groups = ctx_len.shape[0], groups.prefix_len.shape[0]
     _check(block_tables.dim() == 2 and block_tables.shape[0] >= num_seqs, "block_tables must be [b, max_blocks]")
     _check(q_start.shape[0] == num_seqs and q_len.shape[0] == num_seqs and groups.seqs.shape[0] == num_seqs
@@ -599,8 +601,8 @@ def shared_prefix_plan(
     _check(nbytes > 0 or num_seqs == 0, "bad attention shape")
     if workspace is None:
         workspace = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=device)
-    _check(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == device,
-           f"workspace must be contiguous uint8 on {device}")
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.device != device:
+        raise ValueError(f"workspace must be contiguous uint8 on {device}")
     if num_rows is None:
         num_rows = (1 << 31) - 1
     if num_blocks is None:
@@ -631,23 +633,26 @@ def shared_prefix_attention(
     device = _require_gpu(q, k_cache, v_cache, k_scale, v_scale, out, plan.workspace)
     _check(q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1,
            "q must be [rows, heads, 128] bf16")
-    _check(q.shape[1] == plan.num_q_heads, f"the plan is for {plan.num_q_heads} query heads")
-    _check(k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.dim() == 3
-           and k_cache.shape[1] == plan.num_kv_heads and k_cache.shape[2] == HEAD_DIM,
-           f"caches must be [slots, {plan.num_kv_heads}, 128]")
+    # (a step calls this once per layer: no message is built unless it is raised)
+    if q.shape[1] != plan.num_q_heads:
+        raise ValueError(f"the plan is for {plan.num_q_heads} query heads")
+    slots = k_cache.shape
+    if (slots != v_cache.shape or k_cache.dtype != v_cache.dtype or len(slots) != 3 or slots[1] != plan.num_kv_heads
+            or slots[2] != HEAD_DIM):
+        raise ValueError(f"caches must be [slots, {plan.num_kv_heads}, 128]")
     _check(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
     is_int8 = k_cache.dtype == torch.int8
     scale_code = DTYPE_BF16
     if is_int8:
         _check(k_scale is not None and v_scale is not None, "int8 cache needs scales")
         _check(k_scale.dtype == v_scale.dtype and k_scale.is_contiguous() and v_scale.is_contiguous()
-               and k_scale.numel() == v_scale.numel() == k_cache.shape[0] * k_cache.shape[1],
+               and k_scale.numel() == v_scale.numel() == slots[0] * slots[1],
                "scales must be contiguous, one per slot and KV head")
         scale_code = dtype_code(k_scale.dtype)
     else:
         _check(k_cache.dtype == torch.bfloat16, "cache must be int8 or bf16")
-    if plan.num_rows != (1 << 31) - 1:
-        _check(q.shape[0] >= plan.num_rows, f"q has {q.shape[0]} rows, the plan {plan.num_rows}")
+    if q.shape[0] < plan.num_rows != (1 << 31) - 1:
+        raise ValueError(f"q has {q.shape[0]} rows, the plan {plan.num_rows}")
     if out is None:
         out = torch.empty_like(q)
     _check(out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1, "out must match q")
@@ -657,7 +662,7 @@ def shared_prefix_attention(
     _call_on(device, "ne_shared_prefix_attention", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
              v_cache.data_ptr(), k_scale.data_ptr() if is_int8 else None, v_scale.data_ptr() if is_int8 else None,
              DTYPE_INT8 if is_int8 else DTYPE_BF16, scale_code, plan.block_tables.data_ptr(), plan.block_tables.stride(0),
-             plan.block_size, min(plan.num_blocks, k_cache.shape[0] // plan.block_size), groups.seqs.shape[0],
+             plan.block_size, min(plan.num_blocks, slots[0] // plan.block_size), groups.seqs.shape[0],
              groups.prefix_len.shape[0], plan.num_q_heads, plan.num_kv_heads, HEAD_DIM, plan.max_q_len, plan.max_ctx_len,
              groups.max_prefix_len, softmax_scale, out.data_ptr(), out.stride(0), out.stride(1), plan.workspace.data_ptr(),
              plan.workspace.numel(), _stream(device))
@@ -1065,20 +1070,20 @@ def sample(
            "logits must be [rows, vocab] with contiguous rows")
     _check(logits.dtype in (torch.bfloat16, torch.float16, torch.float32), "logits must be bf16, fp16 or fp32")
     rows, vocab = logits.shape
-    _check(uniforms.dtype == torch.float32 and uniforms.dim() == 1 and uniforms.shape[0] == rows
-           and uniforms.is_contiguous(), f"uniforms must be contiguous fp32 [{rows}]")
+    if uniforms.dtype != torch.float32 or uniforms.dim() != 1 or uniforms.shape[0] != rows or not uniforms.is_contiguous():
+        raise ValueError(f"uniforms must be contiguous fp32 [{rows}]")
     t_ptr, t = _row_parameter(temperature, rows, torch.float32, "temperature", device)
     k_ptr, k = _row_parameter(top_k, rows, torch.int32, "top_k", device)
     p_ptr, p = _row_parameter(top_p, rows, torch.float32, "top_p", device)
     m_ptr, m = _row_parameter(min_p, rows, torch.float32, "min_p", device)
-    if t_ptr is None:
-        _check(0.0 <= t < math.inf, f"temperature must be finite and >= 0, got {t}")
+    if t_ptr is None and not 0.0 <= t < math.inf:
+        raise ValueError(f"temperature must be finite and >= 0, got {t}")
     _check(p == p and m == m, "top_p and min_p must not be NaN")
     k = max(0, min(int(k), vocab))
     if out is None:
         out = torch.empty((rows,), dtype=torch.int32, device=device)
-    _check(out.dtype == torch.int32 and tuple(out.shape) == (rows,) and out.is_contiguous() and out.device == device,
-           f"out must be contiguous int32 [{rows}] on {device}")
+    elif out.dtype != torch.int32 or tuple(out.shape) != (rows,) or not out.is_contiguous() or out.device != device:
+        raise ValueError(f"out must be contiguous int32 [{rows}] on {device}")
     table = None
     if isinstance(probs, torch.Tensor):
         table = probs
@@ -1089,11 +1094,12 @@ def sample(
     if rows > 0:
         code = dtype_code(logits.dtype)
         nbytes = _native.load().ne_sample_workspace_size(rows, vocab, code)
-        _check(nbytes > 0, f"unsupported sampling shape: {rows} rows of {vocab}")
+        if nbytes == 0:
+            raise ValueError(f"unsupported sampling shape: {rows} rows of {vocab}")
         if workspace is None:
             workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
-        _check(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == device,
-               f"workspace must be contiguous uint8 on {device}")
+        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.device != device:
+            raise ValueError(f"workspace must be contiguous uint8 on {device}")
         _call_on(device, "ne_sample", logits.data_ptr(), code, logits.stride(0) if rows > 1 else vocab, rows, vocab,
                  uniforms.data_ptr(), t_ptr, t, k_ptr, k, p_ptr, p, m_ptr, m, out.data_ptr(),
                  None if table is None else table.data_ptr(), 0 if table is None or rows < 2 else table.stride(0),
