@@ -254,7 +254,7 @@ def find_shared_prefixes(tables: list) -> list[tuple[list[int], int]]:
     (``(members - 1) * common blocks``), so that a short prefix common to all gives way to
     longer ones common to some."""
     rows = [np.asarray(table, dtype=np.int64) for table in tables]
-    order = sorted(range(len(rows)), key=lambda i: rows[i].tolist())
+    order = sorted(range(len(rows)), key=lambda i: rows[i].astype(">i8").tobytes())  # (bytes in the order of the numbers)
 
     def common(a: np.ndarray, b: np.ndarray) -> int:
         n = min(len(a), len(b))
