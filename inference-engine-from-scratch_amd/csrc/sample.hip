@@ -947,7 +947,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
   };
   auto start_draw = [&]() { start_border(kDraw, false, draw_at(u, end_weight) + 1); };
   auto after_top_p = [&]() {
-    if (cut_m && uni(bin_m > 0 ? s.weight[bin_m - 1] : 0) < end_weight) {
+    // min-p can cut where a token kept so far lies in its border's bin or behind (weights do not say: one
+    // below 2^-S of the largest is 0)
+    const bool behind = end_word == 1 ? uni(bin_m > 0 ? (u64)s.count[bin_m - 1] : 0) < tokens
+                                      : bin_of(finite(logit_of(word_key(end_word))) * r.scale, base16, rem) >= bin_m;
+    if (cut_m && behind) {
       step = kMinP;
       act = kAbove;
       blo = bhi = bin_m;

@@ -166,6 +166,18 @@ def test_logits_of_any_magnitude(dtype, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("p", [1.0, 0.97])
+def test_min_p_among_tokens_of_no_weight(dtype, p):
+    """Steps of e^-20 among many tokens: min-p keeps the second and cuts the third, whose weight no sum holds."""
+    g = torch.Generator().manual_seed(3)
+    x = -torch.randint(0, 4, (3, 30000), generator=g).to(dtype).cuda()
+    for m in (1e-9, 1e-8, 1e-17, 1e-18, 1e-30):
+        for k in (0, 20000):
+            check(x, torch.rand(3, generator=g).cuda(), 0.05, k, p, m)
+
+
+@pytest.mark.gpu
 def test_uniforms_off_their_range():
     x, _ = make_logits(5, 4000, torch.bfloat16, 8)
     check(x, torch.tensor([-1.0, 1.0, 7.5, math.inf, math.nan], device="cuda"), 0.9, 30, 0.9, 0.0)
