@@ -420,6 +420,7 @@ __global__ __launch_bounds__(kCountThreads, 8) void sample_count_kernel(SamplePa
           top = max(top, max(h[0] > kInfinity<DT> ? INT16_MIN : (int)h[0], h[1] > kInfinity<DT> ? INT16_MIN : (int)h[1]));
         }
       }
+      top += top == -1;  // -0 is no smaller than +0
       if (far == 4 * kWindow<DT>) {
 #pragma unroll 1
         for (int e = 0; e < 8; ++e) {

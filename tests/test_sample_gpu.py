@@ -167,6 +167,18 @@ def test_logits_of_any_magnitude(dtype, scale):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_zeros_of_either_sign_are_equal(dtype):
+    g = torch.Generator().manual_seed(8)
+    x = torch.where(torch.rand(5, 3000, generator=g) < 0.5, 0.0, -0.0).to(dtype)
+    x[1:, : 40 * 5 : 1] = -math.inf
+    x[2:][torch.rand(3, 3000, generator=g) < 0.99] = -math.inf
+    u = torch.rand(5, generator=g).cuda()
+    for t, k, p, m in [(0.0, 0, 1.0, 0.0), (1.0, 1, 1.0, 0.0), (0.7, 5, 0.8, 0.1), (1.0, 0, 1.0, 1.0)]:
+        check(x.cuda(), u, t, k, p, m)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("p", [1.0, 0.97])
 def test_min_p_among_tokens_of_no_weight(dtype, p):
     """Steps of e^-20 among many tokens: min-p keeps the second and cuts the third, whose weight no sum holds."""
