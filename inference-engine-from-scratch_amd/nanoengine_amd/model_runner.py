@@ -162,18 +162,39 @@ class ModelRunner:
         logits, _ = self._model.compute_logits(hidden[:token_count])
         return logits
 
-    def _draw_filtered(self, logits: torch.Tensor, sequences: list, rows: list[int]) -> torch.Tensor:
-        params = [sequences[i].sampling_params for i in rows]
-        streams = [sequences[i].sampling_generator for i in rows]
+    def _draw_filtered(self, logits: torch.Tensor, sequences: list) -> torch.Tensor:
+        params = [s.sampling_params for s in sequences]
+        streams = [s.sampling_generator for s in sequences]
 
         def row(values, dtype=torch.float32):
             return torch.tensor(values, dtype=dtype, device=self._device)
 
         return kernels.sample(
-            logits[rows], row([sampling_uniform(s.seed, s.step) for s in streams]),
+            logits, row([sampling_uniform(s.seed, s.step) for s in streams]),
             temperature=row([p.temperature for p in params]),
             top_k=row([min(max(p.top_k, 0), self.vocab_size) for p in params], torch.int32),
             top_p=row([p.top_p for p in params]), min_p=row([p.min_p for p in params]))
+
+    def _accept_last(self, logits: torch.Tensor, sequences: list) -> torch.Tensor:
+        """Each row's token by the acceptance kernel, as a verify step without guesses."""
+        b = len(sequences)
+        params = [s.sampling_params for s in sequences]
+        drafts = torch.zeros((b, 1), dtype=torch.int32, device=self._device)
+        no_drafts = torch.zeros((b,), dtype=torch.int32, device=self._device)
+        row_start = torch.arange(b, dtype=torch.int32, device=self._device)
+        kwargs = {}
+        if any(p.temperature != GREEDY_TEMPERATURE for p in params):
+            kwargs = dict(
+                temperature=torch.tensor([p.temperature for p in params], dtype=torch.float32, device=self._device),
+                top_p=torch.tensor([p.top_p for p in params], dtype=torch.float32, device=self._device),
+                seeds=torch.tensor([s.sampling_generator.seed for s in sequences], dtype=torch.int64,
+                                   device=self._device),
+                steps=torch.tensor([s.sampling_generator.step for s in sequences], dtype=torch.int64,
+                                   device=self._device),
+                any_sampled=True,
+            )
+        out, _ = kernels.accept(drafts, no_drafts, row_start, self.vocab_size, logits=logits, **kwargs)
+        return out[:, 0]
 
     @torch.inference_mode()
     def run_step(self, sequences: list, token_counts: list[int] | None = None) -> list[int]:
@@ -187,30 +208,16 @@ class ModelRunner:
         hidden, starts, counts = self._forward(inputs, sequences)
         last = torch.tensor([s + n - 1 for s, n in zip(starts, counts, strict=True)], device=self._device)
         logits, _ = self._model.compute_logits(hidden[last].contiguous())
-        b = len(sequences)
-        params = [s.sampling_params for s in sequences]
-        sampled = [p.temperature != GREEDY_TEMPERATURE for p in params]
-        drafts = torch.zeros((b, 1), dtype=torch.int32, device=self._device)
-        no_drafts = torch.zeros((b,), dtype=torch.int32, device=self._device)
-        row_start = torch.arange(b, dtype=torch.int32, device=self._device)
-        kwargs = {}
-        if any(sampled):
-            kwargs = dict(
-                temperature=torch.tensor([p.temperature for p in params], dtype=torch.float32, device=self._device),
-                top_p=torch.tensor([p.top_p for p in params], dtype=torch.float32, device=self._device),
-                seeds=torch.tensor([s.sampling_generator.seed for s in sequences], dtype=torch.int64,
-                                   device=self._device),
-                steps=torch.tensor([s.sampling_generator.step for s in sequences], dtype=torch.int64,
-                                   device=self._device),
-                any_sampled=True,
-            )
-        out, _ = kernels.accept(drafts, no_drafts, row_start, self.vocab_size, logits=logits, **kwargs)
-        filtered = [i for i, p in enumerate(params) if p.is_filtered]
-        if filtered:
-            out[filtered, 0] = self._draw_filtered(logits, sequences, filtered)
-        tokens = out[:, 0].tolist()
-        for s, is_sampled in zip(sequences, sampled, strict=True):
-            if is_sampled:
+        filtered = [i for i, s in enumerate(sequences) if s.sampling_params.is_filtered]
+        if len(filtered) == len(sequences):
+            tokens = self._draw_filtered(logits, sequences).tolist()
+        else:
+            out = self._accept_last(logits, sequences)
+            if filtered:
+                out[filtered] = self._draw_filtered(logits[filtered], [sequences[i] for i in filtered])
+            tokens = out.tolist()
+        for s in sequences:
+            if s.sampling_params.temperature != GREEDY_TEMPERATURE:
                 s.sampling_generator.step += 1
         final_counts = token_counts or counts
         for s, n in zip(sequences, final_counts, strict=True):

@@ -5,6 +5,7 @@ the verify runner."""
 from __future__ import annotations
 
 import random
+from dataclasses import replace
 
 import numpy as np
 import pytest
@@ -15,13 +16,13 @@ from nanoengine_amd.config import EngineSettings
 from nanoengine_amd.interface import GenerationRequest, SamplingParams, sampling_uniform
 from nanoengine_amd.memory import KVCachePool, PagedSlotAllocator, PrefixCachingSlotAllocator, find_shared_prefixes
 from nanoengine_amd.model_runner import ModelRunner
-from nanoengine_amd.qwen3 import Qwen3Config, Qwen3VerifyModel, Qwen3Weights, random_state_dict
+from nanoengine_amd.qwen3 import QWEN3_0_6B, Qwen3VerifyModel, Qwen3Weights, random_state_dict
 from nanoengine_amd.runtime import create_verify_engine
 from nanoengine_amd.sequence_state import Sequence
 from oracle import accept as oracle_accept
 from test_sample_gpu import reference_row
 
-CFG = Qwen3Config(4096, 1024, 3072, 2, 16, 8, 128, 1e-6, 1e6, True)
+CFG = replace(QWEN3_0_6B, vocab_size=4096, num_hidden_layers=2)
 CPU = torch.device("cpu")
 
 
@@ -189,10 +190,24 @@ def test_answers_of_a_forked_prompt(int8, members, monkeypatch):
             assert s.num_cached_tokens == s.num_tokens == theirs[i].num_cached_tokens
             s.token_ids.append(tokens[i])
             theirs[i].token_ids.append(tokens[i])
+    only = [s for s in seqs if s.sampling_params.is_filtered]
+    for s in only:
+        ours.allocator.reserve(s, s.num_tokens)
+    logits.clear()
+    tokens = ours.run_step(only)
+    for i, s in enumerate(only):
+        p = s.sampling_params
+        want = reference_row(logits[0][i].double().cpu().numpy(), float(np.float32(sampling_uniform(s.sampling_generator.seed, 3))),
+                             float(np.float32(p.temperature)), min(p.top_k, 4096), float(np.float32(p.top_p)),
+                             float(np.float32(p.min_p)))[0]
+        assert tokens[i] == want and s.sampling_generator.step == 4
+        s.token_ids.append(tokens[i])
+    ours.allocator.reserve(seqs[0], seqs[0].num_tokens)
+    made = len(plans)
     for s in seqs[1:]:
         ours.allocator.free(s)
     few = ours.run_step([seqs[0]])  # one answer left: nothing is shared, nothing is planned
-    assert len(plans) == 3 and len(few) == 1
+    assert len(plans) == made and len(few) == 1
 
 
 def engine(state, members: int, shared: bool, graphs: bool):
