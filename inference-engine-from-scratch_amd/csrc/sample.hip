@@ -36,8 +36,8 @@
 // the scan 42, for its ~10 operations per element and the weights of ~3,000 values per chunk
 // (67% of the vector units' time); pick 46, the slowest row's chain of passes (40) on its one
 // work-group; probs 43, its bytes (292 MB, 6.9 TB/s).  64 rows 41 us: 11 and 24.  One row 31 us:
-// 6 and 20, a chain of round trips through memory and barriers.  200 rows of fp32 48 us: 22 (the
-// bytes, 5.6 TB/s) and 24.
+// 6 and 20, a chain of round trips through memory and barriers.  200 rows of 32,003 (fp32) 48 us: 22,
+// for 65 vector operations per element (half of it) and the sums in LDS, and 24.
 #include <math.h>
 #include <string.h>
 
