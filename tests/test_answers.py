@@ -267,6 +267,44 @@ def test_verify_steps_read_a_cached_prompt_once():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seed", [0, 1])
+def test_requests_come_and_go_on_shared_blocks(seed, monkeypatch):
+    """Random admissions, steps and releases of requests on nested prompts, every shared block read as one:
+    the captured engine gives the eager one's tokens, and each step plans for the groups of that moment."""
+    monkeypatch.setattr(kernels, "SHARED_PREFIX_MIN_BYTES", 1)
+    state = unit_norms()
+    g = torch.Generator().manual_seed(seed)
+    trunk = torch.randint(0, 512, (16,), generator=g).tolist() * 14
+    tails = [torch.randint(0, 512, (16,), generator=g).tolist() * n for n in (0, 3, 9)]
+    runners = [engine(state, 9, True, graphs).runner for graphs in (False, True)]
+    kept = [[], []]
+    r = random.Random(seed)
+    shared = 0
+    for turn in range(40):
+        op = r.choice(["add", "add", "step", "step", "step", "release"])
+        free, busy = runners[0].free_slots(), runners[0].active_slots
+        if op == "add" and free:
+            n = r.randrange(1, len(free) + 1)
+            made = [(f"{turn}.{i}", trunk + r.choice(tails) + [r.randrange(512) for _ in range(r.randrange(5))],
+                     dict(temperature=r.choice([0.0, 0.9]), seed=r.randrange(99), ignore_eos=True)) for i in range(n)]
+            for runner, all_of in zip(runners, kept):
+                seqs = [Sequence.from_request(request(rid, list(tokens), **params)) for rid, tokens, params in made]
+                all_of += seqs
+                runner.add(seqs)
+        elif op == "release" and busy:
+            slot = r.choice(busy)
+            for runner in runners:
+                runner.release(slot)
+        elif op == "step":
+            for runner in runners:
+                runner.step()
+            shared += runners[0].sharing
+        assert runners[0].active_slots == runners[1].active_slots and runners[0].sharing == runners[1].sharing
+        assert [s.token_ids for s in kept[0]] == [s.token_ids for s in kept[1]]
+    assert shared > 3 and all(runner.model.workspace.error_flag() == 0 for runner in runners)
+
+
+@pytest.mark.gpu
 def test_verification_refuses_filters_it_does_not_take():
     runner = engine(unit_norms(), 2, False, False).runner
     with pytest.raises(ValueError, match="top_k or min_p"):
