@@ -14,7 +14,8 @@
 // Weights are integers, rint(2^(y - Y) * 2^S) with 2^S * vocab <= 2^63, computed in 64-bit
 // floating point: a sum of them does not depend on its order (so neither on the work split
 // nor on atomics), and a border between two tokens is off by at most ~2^-S of the row's
-// largest weight per token (S = 45 for 151,936 tokens).  32-bit weights would move every
+// largest weight per token (S = 45 for 151,936 tokens): a draw in the tail, whose tokens weigh 1e-11 of
+// the largest, may fall on a neighbour, one in 1e6 of a peaked row's.  32-bit weights would move every
 // border of a flat row by 1e-7, a wrong token in a hundred rows of 100,000 tokens.
 //
 // Three kernels.

@@ -1063,7 +1063,8 @@ def sample(
     those the fewest that reach ``top_p`` of their weight, of those the ones at least ``min_p``
     times as likely as the first; the token is the first whose running weight exceeds the
     uniform's share of the kept weight.  ``temperature`` 0 takes the argmax.  Each parameter is
-    one value or a tensor ``[rows]`` (fp32; ``top_k`` int32).  NaN and -inf logits are never
+    one value or a tensor ``[rows]`` (fp32; ``top_k`` int32).  Weights are sums of integers in units of
+    2^-45 (151,936 tokens) of the row's largest, whatever their order.  NaN and -inf logits are never
     drawn; a row without any other gives -1."""
     device = _require_gpu(logits, uniforms)
     _check(logits.dim() == 2 and logits.stride(1) == 1 or logits.dim() == 2 and logits.shape[1] == 1,
