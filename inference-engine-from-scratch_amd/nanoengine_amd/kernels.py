@@ -8,7 +8,9 @@ fallback; a missing library or a CPU tensor raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -167,27 +169,25 @@ def copy_kv_blocks(buffers: list[torch.Tensor], block_size: int, src: list[int],
            "buffers must be contiguous and hold the same slots")
     _check(num_slots > 0, "buffers hold no slots")
     n = len(buffers)
-    block_bytes = (ctypes.c_int64 * n)(*[t.nbytes // num_slots * block_size for t in buffers])
-    _copy_blocks(first.device, _pointers(buffers), block_bytes, n, num_slots // block_size, src, dst)
+    block_bytes = array("q", [t.nbytes // num_slots * block_size for t in buffers])
+    pointers = array("Q", map(torch.Tensor.data_ptr, buffers))
+    _copy_blocks(first.device, pointers, block_bytes, n, num_slots // block_size, src, dst)
 
 
-def _pointers(buffers: list[torch.Tensor]):
-    return (ctypes.c_void_p * len(buffers))(*[t.data_ptr() for t in buffers])
-
-
-def _block_list(blocks: list[int]):
+def _block_list(blocks: list[int]) -> array:
     try:
-        return (ctypes.c_int32 * len(blocks))(*blocks)
+        return array("i", blocks)
     except TypeError as error:
         raise TypeError("blocks must be a list of ints") from error
 
 
-def _copy_blocks(device: torch.device, pointers, block_bytes, num_buffers: int, num_blocks: int, src: list[int],
-                 dst: list[int]) -> None:
+def _copy_blocks(device: torch.device, pointers: array, block_bytes: array, num_buffers: int, num_blocks: int,
+                 src: list[int], dst: list[int]) -> None:
     if len(src) and (max(max(src), max(dst)) >= num_blocks or min(min(src), min(dst)) < 0):
         raise ValueError(f"blocks outside [0, {num_blocks})")
-    _call_on(device, "ne_kv_copy_blocks", pointers, block_bytes, num_buffers, num_blocks, _block_list(src),
-             _block_list(dst), len(src), _stream(device))
+    sources, targets = _block_list(src), _block_list(dst)
+    _call_on(device, "ne_kv_copy_blocks", pointers.buffer_info()[0], block_bytes.buffer_info()[0], num_buffers,
+             num_blocks, sources.buffer_info()[0], targets.buffer_info()[0], len(src), _stream(device))
 
 
 # --------------------------------------------------------------------------- A6
@@ -535,6 +535,12 @@ class SharedPrefixPlan:
     num_blocks: int
     groups: PrefixGroups
 
+    @functools.cached_property
+    def _sizes(self) -> tuple:
+        """What every layer's call passes: sequences to the prefix bound, as the entry point takes them."""
+        return (self.groups.seqs.shape[0], self.groups.prefix_len.shape[0], self.num_q_heads, self.num_kv_heads, HEAD_DIM,
+                self.max_q_len, self.max_ctx_len, self.groups.max_prefix_len)
+
     def error_flag(self) -> int:
         """The error word of the plan and the calls on it (waits for them)."""
         return int(self.workspace[:4].view(torch.int32).item())
@@ -630,7 +636,9 @@ def shared_prefix_attention(
     function of the same pool, a prefix's keys read once for its whole group.  ``q`` / ``out``
     are ``[rows, q_heads, 128]`` bf16; the pool is bf16, or int8 with bf16 or fp16 scales.  The
     block tables and lengths the plan was made from must not have changed."""
-    device = _require_gpu(q, k_cache, v_cache, k_scale, v_scale, out, plan.workspace)
+    index = plan.workspace.get_device()
+    if q.get_device() != index or k_cache.get_device() != index or v_cache.get_device() != index:
+        _require_gpu(q, k_cache, v_cache, plan.workspace)  # names the devices
     _check(q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1,
            "q must be [rows, heads, 128] bf16")
     # (a step calls this once per layer: no message is built unless it is raised)
@@ -645,6 +653,7 @@ def shared_prefix_attention(
     scale_code = DTYPE_BF16
     if is_int8:
         _check(k_scale is not None and v_scale is not None, "int8 cache needs scales")
+        _require_gpu(plan.workspace, k_scale, v_scale)
         _check(k_scale.dtype == v_scale.dtype and k_scale.is_contiguous() and v_scale.is_contiguous()
                and k_scale.numel() == v_scale.numel() == slots[0] * slots[1],
                "scales must be contiguous, one per slot and KV head")
@@ -655,17 +664,17 @@ def shared_prefix_attention(
         raise ValueError(f"q has {q.shape[0]} rows, the plan {plan.num_rows}")
     if out is None:
         out = torch.empty_like(q)
-    _check(out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1, "out must match q")
+    _check(out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1 and out.get_device() == index,
+           "out must match q")
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(HEAD_DIM)
-    groups = plan.groups
+    device = plan.workspace.device
     _call_on(device, "ne_shared_prefix_attention", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
              v_cache.data_ptr(), k_scale.data_ptr() if is_int8 else None, v_scale.data_ptr() if is_int8 else None,
              DTYPE_INT8 if is_int8 else DTYPE_BF16, scale_code, plan.block_tables.data_ptr(), plan.block_tables.stride(0),
-             plan.block_size, min(plan.num_blocks, slots[0] // plan.block_size), groups.seqs.shape[0],
-             groups.prefix_len.shape[0], plan.num_q_heads, plan.num_kv_heads, HEAD_DIM, plan.max_q_len, plan.max_ctx_len,
-             groups.max_prefix_len, softmax_scale, out.data_ptr(), out.stride(0), out.stride(1), plan.workspace.data_ptr(),
-             plan.workspace.numel(), _stream(device))
+             plan.block_size, min(plan.num_blocks, slots[0] // plan.block_size), *plan._sizes, softmax_scale,
+             out.data_ptr(), out.stride(0), out.stride(1), plan.workspace.data_ptr(), plan.workspace.numel(),
+             _stream(device))
     return out
 
 
