@@ -1074,7 +1074,8 @@ def sample(
     uniform's share of the kept weight.  ``temperature`` 0 takes the argmax.  Each parameter is
     one value or a tensor ``[rows]`` (fp32; ``top_k`` int32).  Weights are sums of integers in units of
     2^-45 (151,936 tokens) of the row's largest, whatever their order.  NaN and -inf logits are never
-    drawn; a row without any other gives -1."""
+    drawn; a row without any other gives -1.  ``workspace`` (default: allocated here) is uint8 of
+    :func:`sample_workspace_bytes`, of one call at a time."""
     device = _require_gpu(logits, uniforms)
     _check(logits.dim() == 2 and logits.stride(1) == 1 or logits.dim() == 2 and logits.shape[1] == 1,
            "logits must be [rows, vocab] with contiguous rows")
