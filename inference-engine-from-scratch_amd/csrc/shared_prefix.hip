@@ -548,15 +548,15 @@ __device__ __forceinline__ int scale_exp(float x) { return (int)((__builtin_bit_
 // 2^e by its bits, e in [-126, 127].
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
-// A slot's block, or block 0 (and a flag) where the table names none of the pool's.
-__device__ __forceinline__ int sp_slot(const SpParams& p, const int32_t* bt, int key) {
-  int block = bt[key / p.block_size];
+// A key's slot in the block that the table names, or in block 0 (and a flag) where it names none of the pool's.
+__device__ __forceinline__ int sp_slot_in(const SpParams& p, int block, int key) {
   if (block < 0 || block >= p.num_blocks) {
     atomicOr(p.head, kErrBlock);
     block = 0;
   }
   return block * p.block_size + key % p.block_size;
 }
+__device__ __forceinline__ int sp_slot(const SpParams& p, const int32_t* bt, int key) { return sp_slot_in(p, bt[key / p.block_size], key); }
 
 // ---- tiles ----
 constexpr int kSpExpOff = kQtSlotOff + 2 * 8 * 4;  // int [2 buffers][2 waves]: the stage's largest value-scale exponents
@@ -870,7 +870,11 @@ __device__ __forceinline__ void sp_light(const SpParams& p, const SpItem& d, int
       copy_to_lds<4>((const char*)((lane & 16) ? p.v_scale : p.k_scale) + (at & ~1ll) * 2, dst + 2 * L::kTile);
     }
   };
+  // the first slots and the query rows, requested together
+  const int key0 = min(kstart0 + kTileKeys * lane, (kend0 - 1) & ~(kTileKeys - 1));
+  const int block0 = bt[key0 / p.block_size];
   SpState<INT8> st;
+  u32x4 raw[MT][4];
   int kend_row[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -881,7 +885,13 @@ __device__ __forceinline__ void sp_light(const SpParams& p, const SpItem& d, int
     const uint16_t* src = p.q + (int64_t)(d.token + t) * p.q_tok_stride +
                           (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride + 32 * g;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) st.q[mt].q[c] = sp_q_operand<INT8>(*(const u32x4*)(src + 8 * c));
+    for (int c = 0; c < 4; ++c) raw[mt][c] = *(const u32x4*)(src + 8 * c);
+  }
+  const int slot0 = sp_slot_in(p, block0, key0);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) st.q[mt].q[c] = sp_q_operand<INT8>(raw[mt][c]);
     st.m[mt] = kNegBig;
     st.l[mt] = 0.f;
 #pragma unroll
@@ -893,7 +903,7 @@ __device__ __forceinline__ void sp_light(const SpParams& p, const SpItem& d, int
     const int kend = min(kend0, kstart + kLightWindow * kTileKeys);
     const int n_tiles = (kend - kstart + kTileKeys - 1) / kTileKeys;
     const int n_steps = (n_tiles + 1) / 2;
-    for (int t = lane; t < n_tiles; t += kWave) s_slot[t] = sp_slot(p, bt, kstart + kTileKeys * t);
+    for (int t = lane; t < n_tiles; t += kWave) s_slot[t] = t < kWave && kstart == kstart0 ? slot0 : sp_slot(p, bt, kstart + kTileKeys * t);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int t = 0; t < L::kRing; ++t)
