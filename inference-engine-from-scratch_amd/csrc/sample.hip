@@ -36,8 +36,8 @@
 // What bounds it, at 151,936 tokens a row.  320 rows (bf16, top-p, with probabilities) 152 us:
 // the scan 42, for its ~10 operations per element and the weights of ~3,000 values per chunk
 // (67% of the vector units' time); pick 46, the slowest row's chain of passes (40) on its one
-// work-group; probs 43, its bytes (292 MB, 6.9 TB/s).  64 rows 41 us: 11 and 24.  One row 31 us:
-// 6 and 20, a chain of round trips through memory and barriers.  200 rows of 32,003 (fp32) 48 us: 22,
+// work-group; probs 43, its bytes (292 MB, 6.9 TB/s).  64 rows 41 us: 11 and 24.  One row 29 us:
+// 6 and 19, a chain of round trips through memory and barriers.  200 rows of 32,003 (fp32) 48 us: 22,
 // for 65 vector operations per element (half of it) and the sums in LDS, and 24.
 #include <math.h>
 #include <string.h>
@@ -65,6 +65,7 @@ constexpr int kLineSegs = kWave / kSegVecs;
 constexpr int kCountThreads = 1024;
 constexpr int kCountWaves = kCountThreads / kWave;
 constexpr int kCountLines = 4;
+constexpr int kCountLeast = 3 * kCountWaves;
 constexpr int kCountMost = 127;       // lines of a chunk: 65,024 elements, whose counts fit 16 bits
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / kWave;
@@ -1361,11 +1362,12 @@ __global__ __launch_bounds__(kProbsThreads) void sample_probs_kernel(SampleParam
 int elements_per_vec(int dtype) { return dtype == NE_DTYPE_FP32 ? 4 : 8; }
 
 // Chunks of a row.  fp32: enough work-groups to fill the chip twice, at least one iteration of the scan each;
-// 16 bits: a work-group per CU, whose table clears and reads take as long as 8,192 elements.
+// 16 bits: a work-group per CU, of three lines per wave at least, as each adds a histogram to merge (one to
+// eight rows 26 to 27 us, 27 to 28 with one line).
 int row_chunks(int rows, int lines, int dtype) {
   rows = rows < 1 ? 1 : rows;
   const int want = ceil_div(dtype == NE_DTYPE_FP32 ? 2 * kNumCu : kNumCu, rows);
-  const int most = ceil_div(lines, dtype == NE_DTYPE_FP32 ? kScanWaves * kScanLines : kCountWaves);
+  const int most = ceil_div(lines, dtype == NE_DTYPE_FP32 ? kScanWaves * kScanLines : kCountLeast);
   const int n = want < most ? want : most, least = ceil_div(lines, kCountMost);
   return dtype == NE_DTYPE_FP32 || n > least ? n : least;
 }
