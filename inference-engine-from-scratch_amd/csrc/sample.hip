@@ -127,6 +127,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return x > -INFINITY ? k : 0u;
 }
 constexpr uint32_t kLeastKey = 0x00800000u;  // of the largest negative number
+constexpr uint32_t kNegativeZero = 0x7FFFFFFFu;  // below +0's key, and no token's, as -0 has +0's
 __device__ __forceinline__ float logit_of(uint32_t key) {
   return __builtin_bit_cast(float, (key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
@@ -1003,6 +1004,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
     // (the bins as keys: an element costs two comparisons, and only those inside the rest)
     klo = max(klo, key_from(bhi, best_key, r, base16));
     khi = min(khi, blo > 0 ? key_from(blo - 1, best_key, r, base16) - 1 : best_key);
+    khi -= khi == kNegativeZero;  // (as a number this end of a range would take in +0, a key above it)
     const float xlo = logit_of(klo), xhi = logit_of(khi);
     u64 acc0 = act == kKeyRange ? 0xFFFFFFFFu : 0, acc1 = 0, acc2 = ~0ull;
     for (int s0 = 0; s0 < segs && klo <= khi; s0 += kSegsHeld) {

@@ -1,0 +1,50 @@
+"""Sampling where a border falls next to a special value: ``kernels.sample`` against the order
+of tokens itself, on rows whose kept tokens follow from a count."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from nanoengine_amd import kernels
+
+
+def first_tokens(x: np.ndarray, n: int) -> np.ndarray:
+    """The first ``n`` tokens by logit (descending), then index; zeros of either sign are equal."""
+    return np.argsort(-(x.astype(np.float64) + 0.0), kind="stable")[:n]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zero", [0.0, -0.0])
+@pytest.mark.parametrize("zeros,negatives,top_k", [(3000, 3900, 6000), (3000, 5000, 6000), (100, 4100, 3000), (5000, 5000, 5003)])
+def test_a_border_among_subnormal_numbers_below_zero(zero, zeros, negatives, top_k):
+    """More tokens next to zero than are sorted at once: the range of keys that holds the border
+    ends between the negative numbers and zero."""
+    rng = np.random.default_rng(zeros + negatives)
+    close = np.array([0x3C7FFFFF], np.uint32).view(np.float32)  # its key is whole buckets above zero's
+    row = np.concatenate([[100.0], close, np.full(zeros, zero), np.full(negatives, -1e-40)]).astype(np.float32)
+    x = np.stack([rng.permutation(row) for _ in range(3)])
+    u = torch.tensor([0.0, 0.5, 0.999], device="cuda")
+    logits = torch.from_numpy(x).cuda()
+    tokens, probs = kernels.sample(logits, u, top_k=top_k, probs=True)
+    # e^-100 for all but the first: below fp32's steps, so the first token is drawn ...
+    assert tokens.tolist() == [int(r.argmax()) for r in x]
+    for r in range(3):
+        kept = np.zeros(row.size, bool)
+        kept[first_tokens(x[r], top_k)] = True
+        # ... and e^-100, 3.7e-44, is what the others' probabilities hold
+        assert np.array_equal(probs[r].cpu().numpy() > 0, kept)
+    # the hundred left out, the rest is drawn evenly: token floor(u n) of the order
+    logits[logits == 100.0] = -torch.inf
+    tokens, probs = kernels.sample(logits, u, top_k=top_k, probs=True)
+    x[x == 100.0] = -np.inf
+    n = min(top_k, zeros + negatives + 1)
+    for r in range(3):
+        order = first_tokens(x[r], n)
+        kept = np.zeros(row.size, bool)
+        kept[order] = True
+        assert np.array_equal(probs[r].cpu().numpy() > 0, kept)
+        w = np.exp(x[r][order].astype(np.float64))
+        want = np.searchsorted(np.cumsum(w), float(u[r]) * w.sum(), side="right")
+        assert tokens[r].item() == order[want]
