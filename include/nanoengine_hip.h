@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define NE_ABI_VERSION 11
+#define NE_ABI_VERSION 12
 
 /* status codes */
 #define NE_OK 0
@@ -439,7 +439,9 @@ int ne_advance_and_propose(const int32_t* history, int64_t history_stride, const
  * ne_paged_verify_attention's; num_rows is the number of query tokens in q and out,
  * num_blocks the pool's blocks, and max_q_len, max_ctx_len, max_prefix_len bound the lengths.
  * A row that sees no key is 0.  Rows of no sequence are left as they are.  int8 pools need
- * |q| < 65504.
+ * |q| < 65504.  ne_shared_prefix_attention relies on the num_rows that the plan was given;
+ * ne_shared_prefix_attention_rows takes the rows of its own q and out, for a plan made
+ * before they are known: a sequence with rows past them is not computed (error 2).
  *
  * ne_shared_prefix_plan writes the work plan of a step into the workspace, from the step's
  * lengths and groups on the device; ne_shared_prefix_attention computes one layer with it, as
@@ -475,6 +477,17 @@ int ne_shared_prefix_attention(const void* q, int64_t q_token_stride, int64_t q_
                                int32_t max_prefix_len, float softmax_scale, void* out,
                                int64_t out_token_stride, int64_t out_head_stride, void* workspace,
                                size_t workspace_bytes, void* stream);
+int ne_shared_prefix_attention_rows(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                    int32_t num_rows, const void* k_cache, const void* v_cache,
+                                    const void* k_scale, const void* v_scale, int32_t kv_dtype,
+                                    int32_t scale_dtype, const int32_t* block_tables,
+                                    int32_t block_table_stride, int32_t block_size,
+                                    int32_t num_blocks, int32_t num_seqs, int32_t num_groups,
+                                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                    int32_t max_q_len, int32_t max_ctx_len, int32_t max_prefix_len,
+                                    float softmax_scale, void* out, int64_t out_token_stride,
+                                    int64_t out_head_stride, void* workspace,
+                                    size_t workspace_bytes, void* stream);
 
 /*
  * Copies of KV blocks within a pool (no counterpart in the reference, whose blocks are

@@ -593,8 +593,8 @@ __device__ __forceinline__ void sp_tile_item(const SpParams& p, const SpItem& d,
     const int row = wrow0 + kRows * mt + r;
     const bool valid = row < rows_total;
     const int t = valid ? row / p.group : 0;
-    // (a row past the last reads the first token; it is never stored)
-    const int token = of_group ? p.tokens[d.token + t] : d.token + t;
+    // (a row past the last reads the first token, a token past q the last one; neither is stored)
+    const int token = min(of_group ? p.tokens[d.token + t] : d.token + t, p.num_rows - 1);
     kend_row[mt] = valid ? (of_group ? kend : min(kend, first_seen + t)) : 0;
     const uint16_t* src = p.q + (int64_t)token * p.q_tok_stride +
                           (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride + 8 * g;
@@ -882,7 +882,7 @@ __device__ __forceinline__ void sp_light(const SpParams& p, const SpItem& d, int
     const bool valid = row < rows_total;
     const int t = valid ? row / p.group : 0;
     kend_row[mt] = valid ? min(kend0, first_seen + t) : 0;
-    const uint16_t* src = p.q + (int64_t)(d.token + t) * p.q_tok_stride +
+    const uint16_t* src = p.q + (int64_t)min(d.token + t, p.num_rows - 1) * p.q_tok_stride +
                           (int64_t)(head * p.group + (valid ? row - t * p.group : 0)) * p.q_head_stride + 32 * g;
 #pragma unroll
     for (int c = 0; c < 4; ++c) raw[mt][c] = *(const u32x4*)(src + 8 * c);
@@ -1094,6 +1094,10 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(SpPa
   const int heads = p.num_kv_heads * p.group;
   const int x = (blockIdx.x % blocks_per_seq) * (kMergeThreads / LANES) + (int)threadIdx.x / LANES;  // query, then head
   if (x >= d[0] * heads) return;
+  if (d[1] > p.num_rows - d[0]) {  // the plan was made for more rows than q has
+    if (threadIdx.x == 0) atomicOr(p.head, kErrRows);
+    return;
+  }
   const int i = x / heads, head = x % heads;
   const int kv = head / p.group, in = i * p.group + head % p.group;
   const int np = d[2], n = np + d[3];
@@ -1338,16 +1342,18 @@ extern "C" int ne_shared_prefix_plan(const int32_t* ctx_len, const int32_t* q_st
   return check_launch("shared_prefix_plan");
 }
 
-extern "C" int ne_shared_prefix_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
-                                          const void* v_cache, const void* k_scale, const void* v_scale, int32_t kv_dtype,
-                                          int32_t scale_dtype, const int32_t* block_tables, int32_t block_table_stride,
-                                          int32_t block_size, int32_t num_blocks, int32_t num_seqs, int32_t num_groups,
-                                          int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_q_len,
-                                          int32_t max_ctx_len, int32_t max_prefix_len, float softmax_scale, void* out,
-                                          int64_t out_token_stride, int64_t out_head_stride, void* workspace,
-                                          size_t workspace_bytes, void* stream) {
+extern "C" int ne_shared_prefix_attention_rows(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t num_rows,
+                                               const void* k_cache, const void* v_cache, const void* k_scale,
+                                               const void* v_scale, int32_t kv_dtype, int32_t scale_dtype,
+                                               const int32_t* block_tables, int32_t block_table_stride, int32_t block_size,
+                                               int32_t num_blocks, int32_t num_seqs, int32_t num_groups, int32_t num_q_heads,
+                                               int32_t num_kv_heads, int32_t head_dim, int32_t max_q_len, int32_t max_ctx_len,
+                                               int32_t max_prefix_len, float softmax_scale, void* out,
+                                               int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                                               size_t workspace_bytes, void* stream) {
   using namespace ne;
-  if (num_seqs == 0) return NE_OK;
+  NE_CHECK_ARG(num_rows >= 0, "shared_prefix_attention: bad row count %d", num_rows);
+  if (num_seqs == 0 || num_rows == 0) return NE_OK;
   NE_CHECK_SUPPORTED(head_dim == kHeadDim, "head_dim %d: only 128 is supported", head_dim);
   SpLayout l;
   const int rc = sp_check("shared_prefix_attention", num_seqs, num_groups, num_q_heads, num_kv_heads, max_q_len, max_ctx_len,
@@ -1381,6 +1387,7 @@ extern "C" int ne_shared_prefix_attention(const void* q, int64_t q_token_stride,
   p.num_blocks = num_blocks;
   p.num_seqs = num_seqs;
   p.num_groups = num_groups;
+  p.num_rows = num_rows;
   p.num_kv_heads = num_kv_heads;
   p.group = num_q_heads / num_kv_heads;
   p.max_q = max_q_len;
@@ -1392,4 +1399,19 @@ extern "C" int ne_shared_prefix_attention(const void* q, int64_t q_token_stride,
   if (!int8) return sp_launch<false, NE_DTYPE_BF16>(p, (hipStream_t)stream);
   return scale_dtype == NE_DTYPE_BF16 ? sp_launch<true, NE_DTYPE_BF16>(p, (hipStream_t)stream)
                                       : sp_launch<true, NE_DTYPE_FP16>(p, (hipStream_t)stream);
+}
+
+extern "C" int ne_shared_prefix_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                                          const void* v_cache, const void* k_scale, const void* v_scale, int32_t kv_dtype,
+                                          int32_t scale_dtype, const int32_t* block_tables, int32_t block_table_stride,
+                                          int32_t block_size, int32_t num_blocks, int32_t num_seqs, int32_t num_groups,
+                                          int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_q_len,
+                                          int32_t max_ctx_len, int32_t max_prefix_len, float softmax_scale, void* out,
+                                          int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  // as many rows as the plan was made for
+  return ne_shared_prefix_attention_rows(q, q_token_stride, q_head_stride, 0x7FFFFFFF, k_cache, v_cache, k_scale, v_scale, kv_dtype,
+                                         scale_dtype, block_tables, block_table_stride, block_size, num_blocks, num_seqs, num_groups,
+                                         num_q_heads, num_kv_heads, head_dim, max_q_len, max_ctx_len, max_prefix_len, softmax_scale,
+                                         out, out_token_stride, out_head_stride, workspace, workspace_bytes, stream);
 }

@@ -14,7 +14,7 @@ from pathlib import Path
 
 LIBRARY_NAME = "libnanoengine_hip.so"
 LIBRARY_PATH = Path(__file__).resolve().parent / LIBRARY_NAME
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 # status codes (nanoengine_hip.h)
 NE_OK = 0
@@ -171,6 +171,9 @@ SIGNATURES: dict[str, tuple] = {
         ],
     ),
 }
+# with q's rows after its strides
+_shared = SIGNATURES["ne_shared_prefix_attention"]
+SIGNATURES["ne_shared_prefix_attention_rows"] = (_shared[0], [*_shared[1][:3], _i32, *_shared[1][3:]])
 SIGNATURES["ne_paged_verify_attention_planned"] = SIGNATURES["ne_paged_verify_attention"]
 # the allocation-free variant: (workspace, bytes) replaced by the caller's error-flag word
 SIGNATURES["ne_paged_verify_attention_noalloc"] = (

@@ -588,8 +588,9 @@ def shared_prefix_plan(
     workspace: torch.Tensor | None = None,
 ) -> SharedPrefixPlan:
     """Plan a step's :func:`shared_prefix_attention` calls (one per layer) from its lengths and
-    groups on the device.  ``num_rows`` (default: the most the sequences can hold) bounds the
-    query rows, ``num_blocks`` (default: unknown) the block tables' entries.  ``workspace``
+    groups on the device.  ``num_rows`` (default: those of each call's ``q``) bounds the query
+    rows, ``num_blocks`` (default: those of each call's cache) the block tables' entries; a
+    sequence with rows past the bound is not computed, and flagged.  ``workspace``
     (default: allocated here) is a uint8 tensor of :func:`shared_prefix_workspace_bytes` that no
     other plan uses until this one's calls are done."""
     device = _require_gpu(block_tables, ctx_len, q_start, q_len, groups.seqs, groups.start, groups.prefix_len)
@@ -669,7 +670,7 @@ def shared_prefix_attention(
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(HEAD_DIM)
     device = plan.workspace.device
-    _call_on(device, "ne_shared_prefix_attention", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+    _call_on(device, "ne_shared_prefix_attention_rows", q.data_ptr(), q.stride(0), q.stride(1), q.shape[0], k_cache.data_ptr(),
              v_cache.data_ptr(), k_scale.data_ptr() if is_int8 else None, v_scale.data_ptr() if is_int8 else None,
              DTYPE_INT8 if is_int8 else DTYPE_BF16, scale_code, plan.block_tables.data_ptr(), plan.block_tables.stride(0),
              plan.block_size, min(plan.num_blocks, slots[0] // plan.block_size), *plan._sizes, softmax_scale,
