@@ -513,7 +513,7 @@ int ne_kv_copy_blocks(void* const* buffers, const int64_t* block_bytes, int32_t 
  *   n_k = top_k (all tokens when 0 or less),
  *   n_p = the fewest whose weight reaches top_p times the weight of the first n_k (all
  *         when top_p is 1 or more),
- *   n_m = the tokens with w_j >= min_p (all when min_p is 0 or less),
+ *   n_m = the tokens with w_j >= min_p (all when min_p is 0 or less or NaN, none above 1),
  * at least one; the token is the first whose running weight exceeds u times the kept
  * weight (u below 0 or NaN: the first; u of 1 or more: the last kept).  Temperature 0 (or
  * less, or NaN) takes the first token.  NaN and -inf logits are never drawn, tokens at

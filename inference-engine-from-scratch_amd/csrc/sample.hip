@@ -7,7 +7,7 @@
 //   n_k = top_k (all, where top_k is 0 or less),
 //   n_p = the fewest whose weight reaches top_p times the weight of the first n_k
 //         (all, where top_p is 1 or more),
-//   n_m = the tokens with weight at least min_p times the largest,
+//   n_m = the tokens with weight at least min_p times the largest (above 1: none),
 // and at least one.  The token drawn is the first whose running weight exceeds
 // u * (kept weight).  T = 0 keeps the first token alone.
 //
@@ -219,6 +219,7 @@ __device__ __forceinline__ RowParams row_params(const SampleParams& p, int row) 
   r.greedy = !(t > 0.f);
   r.scale = r.greedy ? 0.0 : kBinsPerLog2 * 1.4426950408889634 / (double)t;
   r.top_k = k > 0 && k < p.vocab ? k : 0;
+  if (m > 1.f && p.vocab > 1) r.top_k = 1;  // no token weighs more than the first: it alone is kept
   r.weigh = !r.greedy && (r.top_k == 0 || r.top_k > kShortTopK);
   r.min_p = m;
   return r;
@@ -897,7 +898,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
   const u64 top_k = r.top_k && (u64)r.top_k < tokens ? r.top_k : tokens;
   const float u = p.uniforms[row];
   const bool cut_p = r.top_p < 1.f, cut_m = r.min_p > 0.f;
-  const double log2_min_p = cut_m ? log2(fmin((double)r.min_p, 1.0)) : -INFINITY;
+  const double log2_min_p = cut_m ? log2(fmin((double)r.min_p, 1.0)) : -INFINITY;  // (above 1, top_k is 1)
   // min-p's border in sixteenths of log2, and its bin
   const double y_min = uni(finite(logit_of(word_key(best))) * r.scale + kBinsPerLog2 * log2_min_p);
   double rem;

@@ -1071,8 +1071,8 @@ def sample(
 
     Tokens are ordered by logit, equal ones by index.  Kept are the first ``top_k`` (0: all), of
     those the fewest that reach ``top_p`` of their weight, of those the ones at least ``min_p``
-    times as likely as the first; the token is the first whose running weight exceeds the
-    uniform's share of the kept weight.  ``temperature`` 0 takes the argmax.  Each parameter is
+    times as likely as the first (above 1: the first alone); the token is the first whose running
+    weight exceeds the uniform's share of the kept weight.  ``temperature`` 0 takes the argmax.  Each parameter is
     one value or a tensor ``[rows]`` (fp32; ``top_k`` int32).  Weights are sums of integers in units of
     2^-45 (151,936 tokens) of the row's largest, whatever their order.  NaN and -inf logits are never
     drawn; a row without any other gives -1.  ``workspace`` (default: allocated here) is uint8 of
