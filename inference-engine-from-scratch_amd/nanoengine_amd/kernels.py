@@ -197,8 +197,9 @@ class AttentionWorkspace:
 
     ``plan_key`` names the metadata the last :func:`paged_attention_plan` call used, so
     that a planned attention call on other metadata is refused.  ``frozen`` is set once a
-    captured HIP graph holds the buffer's address: from then on a call that would need a
-    larger buffer raises instead of reallocating under the graph."""
+    captured HIP graph holds the buffers' addresses: from then on a call that would need a
+    larger one raises instead of reallocating under the graph (a graph holds no buffer that
+    was not there yet)."""
 
     buffer: torch.Tensor | None = None
     layout: tuple | None = None
@@ -209,9 +210,8 @@ class AttentionWorkspace:
 
     def get(self, device: torch.device, nbytes: int, layout: tuple) -> torch.Tensor:
         if self.buffer is None or self.buffer.numel() < nbytes or self.buffer.device != device:
-            if self.frozen:
-                have = 0 if self.buffer is None else self.buffer.numel()
-                raise RuntimeError(f"attention workspace of {have} bytes is held by a captured HIP graph; "
+            if self.frozen and self.buffer is not None:
+                raise RuntimeError(f"attention workspace of {self.buffer.numel()} bytes is held by a captured HIP graph; "
                                    f"this call needs {nbytes} bytes on {device}: size it before capture")
             self.buffer = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
             self.layout = layout
