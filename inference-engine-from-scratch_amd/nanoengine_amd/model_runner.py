@@ -117,7 +117,11 @@ class ModelRunner:
         if shared < 0 or child.token_ids[:shared] != sequence.token_ids[:shared]:
             raise ValueError(f"{child.request_id} does not start with the cached tokens of {sequence.request_id}")
         src, dst = self.allocator.fork(sequence, child, shared)
-        self._pool.copy_blocks(src, dst)
+        try:
+            self._pool.copy_blocks(src, dst)
+        except BaseException:
+            self.allocator.free(child)
+            raise
         child.num_cached_tokens = shared
         return child
 
