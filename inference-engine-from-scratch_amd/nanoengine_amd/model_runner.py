@@ -23,6 +23,10 @@ from nanoengine_amd.qwen3 import AttentionBatch, Qwen3VerifyModel
 from nanoengine_amd.sequence_state import Sequence
 
 PADDING_TOKEN_ID = 0
+# A shared-prefix plan has room for the longest sequence's queries in every sequence: 64 sequences of which
+# one brings 1,024 queries would hold 1.1 GB of partial sums.  Past this many bytes a step of which more
+# than half is padding takes ordinary attention.
+SHARED_PREFIX_MAX_PADDED = 256 << 20
 
 
 @dataclass(frozen=True)
@@ -93,17 +97,23 @@ class ModelRunner:
     def vocab_size(self) -> int:
         return self._model.config.vocab_size
 
-    def _prefix_groups(self, sequences: list) -> kernels.PrefixGroups | None:
+    def _prefix_groups(self, sequences: list, counts: list[int], max_ctx_len: int) -> kernels.PrefixGroups | None:
+        """The sequences' groups, if this step's attention is to read their prefixes once."""
         if len(sequences) > kernels.SHARED_PREFIX_MAX_SEQS:
             return None
-        size = self._pool.block_size
+        c, size = self._model.config, self._pool.block_size
         found = find_shared_prefixes([self.allocator.block_table(s) for s in sequences])
         saved = sum((len(members) - 1) * blocks * size for members, blocks in found)
-        if not kernels.shared_prefix_pays(saved, self._model.config.num_key_value_heads,
-                                          self._pool.key_caches[0].dtype):
+        if not kernels.shared_prefix_pays(saved, c.num_key_value_heads, self._pool.key_caches[0].dtype):
             return None
         grouped = {i for members, _ in found for i in members}
         singles = [i for i in range(len(sequences)) if i not in grouped]
+        nbytes = kernels.shared_prefix_workspace_bytes(
+            len(sequences), len(found) + len(singles), c.num_attention_heads, c.num_key_value_heads, max(counts),
+            max_ctx_len, max(blocks for _, blocks in found) * size)
+        padded = len(counts) * max(counts) > 2 * sum(counts)
+        if nbytes == 0 or padded and nbytes > SHARED_PREFIX_MAX_PADDED:  # (0: a shape that no plan is made for)
+            return None
         return kernels.PrefixGroups.from_lists([members for members, _ in found] + [[i] for i in singles],
                                                [blocks * size for _, blocks in found] + [0] * len(singles),
                                                self._device)
@@ -145,7 +155,7 @@ class ModelRunner:
             block_tables=ctx.block_tables,
             max_q_len=max(counts),
             max_ctx_len=ctx.max_context_length,
-            prefix_groups=self._prefix_groups(sequences) if self.shared_prefix else None,
+            prefix_groups=self._prefix_groups(sequences, counts, ctx.max_context_length) if self.shared_prefix else None,
         )
         rows = sum(counts)
         if rows > self._model.max_rows:
