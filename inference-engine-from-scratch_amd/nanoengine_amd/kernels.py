@@ -552,7 +552,8 @@ class SharedPrefixPlan:
 
 
 SHARED_PREFIX_MAX_SEQS = 1024  # a plan's sequences
-# Bytes of keys and values per layer that sharing has to save for a step to be faster with it.  28 layers of
+# Sharing has to save more than this many bytes of keys and values per layer for a step to be faster with it
+# (at the border itself one measured case gains and one loses).  28 layers of
 # 16 query and 8 KV heads, verify steps of 5 rows, us per layer without and with: 64 sequences on 512 tokens
 # (66 MB saved, int8) 66.7 / 67.6, on 1,024 (132 MB) 72.4 / 69.0, on 2,048 (264 MB) 86 / 72, on 8,192 161 / 84;
 # 16 on 2,048 (126 MB, bf16) 58.8 / 59.5, on 4,096 (126 MB, int8) 65.3 / 64.4; 60 on nine prefixes of 1,024
@@ -563,7 +564,7 @@ SHARED_PREFIX_MIN_BYTES = 120 << 20
 def shared_prefix_pays(saved_tokens: int, num_kv_heads: int, kv_dtype: torch.dtype) -> bool:
     """Whether a batch that need not read ``saved_tokens`` cached tokens again (a prefix's tokens
     times its members but one, over the groups) is faster with :func:`shared_prefix_attention`."""
-    return saved_tokens * num_kv_heads * 2 * HEAD_DIM * kv_dtype.itemsize >= SHARED_PREFIX_MIN_BYTES
+    return saved_tokens * num_kv_heads * 2 * HEAD_DIM * kv_dtype.itemsize > SHARED_PREFIX_MIN_BYTES
 
 
 def shared_prefix_workspace_bytes(num_seqs: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_q_len: int,
