@@ -225,6 +225,9 @@ class VerifyRunner:
         # the active slot list and whether any samples, kept between slot changes
         self._active: list[int] | None = None
         self._sampled: bool | None = None
+        # a captured step per (sampled, shared) kind that a batch had so far, so that a load whose
+        # batches change between kinds captures each once, and the one of the last step
+        self._graphs: dict[tuple[bool, bool], torch.cuda.CUDAGraph] = {}
         self.graph: torch.cuda.CUDAGraph | None = None
         # whether the captured step computes full logits (some slot samples) or only the
         # LM head's argmax partials (every slot greedy)
@@ -241,7 +244,7 @@ class VerifyRunner:
                                           torch.zeros(max_seqs, **i32), self.capacity)
             self.shared_batch = replace(self.batch, prefix_groups=groups)
         self._sharing: bool | None = None  # None: to be found
-        self.graph_shared: bool | None = None
+        self.graph_shared: bool | None = None  # and whether it reads shared prefixes once
         # set to a list to record, per verify step, each slot's history, drafts,
         # emitted tokens and block table (used by the parity tests)
         self.trace: list | None = None
@@ -531,8 +534,8 @@ class VerifyRunner:
         reference captures its decode graphs when the engine is created
         (runtime.py:150-160, cuda_graph_runner.py:94-105), so that no request waits for a
         capture: the step runs once with every slot inactive (padding rows only, which
-        write the pool's scratch slot) and is then recorded.  A batch with sampled slots
-        captures its own graph at its first step."""
+        write the pool's scratch slot) and is then recorded.  A batch with sampled slots, or
+        with prefixes to share, captures its own graph at its first step."""
         if not self.use_graph or self.graph is not None or self.graph_failed or self.np_active.any():
             return
         self._run_device_step()
@@ -543,7 +546,8 @@ class VerifyRunner:
         if not self.graph_allowed():
             self._device_step(sampled, shared)
             return
-        if self.graph is None or self.graph_sampled != sampled or self.graph_shared != shared:
+        graph = self._graphs.get((sampled, shared))
+        if graph is None:
             # this step runs eagerly (which also allocates lazily created buffers and
             # workspaces); the capture below only records, so nothing runs twice
             self._device_step(sampled, shared)
@@ -557,13 +561,14 @@ class VerifyRunner:
                 # later step runs eagerly (this one already ran)
                 self.graph, self.graph_failed = None, True
                 del graph
+                self._graphs.clear()
                 torch.cuda.empty_cache()
                 return
-            self.graph = graph
+            self._graphs[sampled, shared] = graph
             self.model.bind_graph()
-            self.graph_sampled, self.graph_shared = sampled, shared
-            return
-        self.graph.replay()
+        else:
+            graph.replay()
+        self.graph, self.graph_sampled, self.graph_shared = graph, sampled, shared
 
     def step(self) -> dict[int, StepResult]:
         """One verify step over every active slot; returns what each slot emitted.
