@@ -528,8 +528,10 @@ int ne_kv_copy_blocks(void* const* buffers, const int64_t* block_bytes, int32_t 
  *             fp32 draft_rows)
  *   workspace ne_sample_workspace_size() bytes, 16-byte aligned; written and consumed
  *             within the call
- * Weights are 64-bit integers summed exactly, so results do not depend on the order of
- * any sum (sample.hip).
+ * Weights are 64-bit integers in units of 2^-S of the largest (2^S * vocab <= 2^63), so
+ * results do not depend on the order of any sum: the same call gives the same bits.  A row is
+ * split by the number of rows, so that a border between two tokens may lie a unit per
+ * token and per bin of a part's histogram elsewhere in a batch of another size (sample.hip).
  */
 size_t ne_sample_workspace_size(int32_t rows, int32_t vocab, int32_t dtype);
 int ne_sample(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t vocab,

@@ -12,9 +12,14 @@
 // u * (kept weight).  T = 0 keeps the first token alone.
 //
 // Weights are integers, rint(2^(y - Y) * 2^S) with 2^S * vocab <= 2^63, computed in 64-bit
-// floating point: a sum of them does not depend on its order (so neither on the work split
-// nor on atomics), and a border between two tokens is off by at most ~2^-S of the row's
-// largest weight per token (S = 45 for 151,936 tokens): a draw in the tail, whose tokens weigh 1e-11 of
+// floating point: a sum of them does not depend on its order (nor on that of atomics), so a call
+// repeated gives the same bits.  The split of a row into chunks does count.  A chunk weighs its
+// tokens relative to its own largest logit, and histograms brought to the row's drop up to a unit
+// of 2^-S per bin and chunk (fp32: and each time a chunk's largest logit rises).  Chunks follow
+// the number of rows, so a row may place a border that much apart in a batch of another size.
+// With the tokens' own rounding a border between two tokens is off by at most ~2^-S of the row's
+// largest weight per token, and per bin and chunk (S = 45 for 151,936 tokens, 3 to 7 chunks in 16
+// bits, up to 38 in fp32, 736 bins of any weight): a draw in the tail, whose tokens weigh 1e-11 of
 // the largest, may fall on a neighbour, one in 1e6 of a peaked row's.  32-bit weights would move every
 // border of a flat row by 1e-7, a wrong token in a hundred rows of 100,000 tokens.
 //

@@ -1074,8 +1074,9 @@ def sample(
     those the fewest that reach ``top_p`` of their weight, of those the ones at least ``min_p``
     times as likely as the first (above 1: the first alone); the token is the first whose running
     weight exceeds the uniform's share of the kept weight.  ``temperature`` 0 takes the argmax.  Each parameter is
-    one value or a tensor ``[rows]`` (fp32; ``top_k`` int32).  Weights are sums of integers in units of
-    2^-45 (151,936 tokens) of the row's largest, whatever their order.  NaN and -inf logits are never
+    one value or a tensor ``[rows]`` (fp32; ``top_k`` int32).  Weights are integers in units of
+    2^-45 (151,936 tokens) of the row's largest, so a call repeated gives the same bits; a batch of
+    another size splits its rows otherwise, and rounds a border's sum by other units.  NaN and -inf logits are never
     drawn; a row without any other gives -1.  ``workspace`` (default: allocated here) is uint8 of
     :func:`sample_workspace_bytes`, of one call at a time."""
     device = _require_gpu(logits, uniforms)
