@@ -567,6 +567,13 @@ def shared_prefix_pays(saved_tokens: int, num_kv_heads: int, kv_dtype: torch.dty
     return saved_tokens * num_kv_heads * 2 * HEAD_DIM * kv_dtype.itemsize > SHARED_PREFIX_MIN_BYTES
 
 
+def shared_prefix_supported(k_cache: torch.Tensor, k_scale: torch.Tensor | None) -> bool:
+    """Whether :func:`shared_prefix_attention` takes this cache (bf16, or int8 with bf16 or fp16 scales)."""
+    if k_cache.dtype == torch.bfloat16:
+        return True
+    return k_cache.dtype == torch.int8 and k_scale is not None and k_scale.dtype in (torch.bfloat16, torch.float16)
+
+
 def shared_prefix_workspace_bytes(num_seqs: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_q_len: int,
                                   max_ctx_len: int, max_prefix_len: int) -> int:
     return _native.load().ne_shared_prefix_workspace_size(num_seqs, num_groups, num_q_heads, num_kv_heads, max_q_len,

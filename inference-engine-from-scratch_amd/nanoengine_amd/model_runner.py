@@ -99,12 +99,14 @@ class ModelRunner:
 
     def _prefix_groups(self, sequences: list, counts: list[int], max_ctx_len: int) -> kernels.PrefixGroups | None:
         """The sequences' groups, if this step's attention is to read their prefixes once."""
-        if len(sequences) > kernels.SHARED_PREFIX_MAX_SEQS:
+        pool = self._pool
+        if len(sequences) > kernels.SHARED_PREFIX_MAX_SEQS or not kernels.shared_prefix_supported(
+                pool.key_caches[0], None if pool.key_scales is None else pool.key_scales[0]):
             return None
-        c, size = self._model.config, self._pool.block_size
+        c, size = self._model.config, pool.block_size
         found = find_shared_prefixes([self.allocator.block_table(s) for s in sequences])
         saved = sum((len(members) - 1) * blocks * size for members, blocks in found)
-        if not kernels.shared_prefix_pays(saved, c.num_key_value_heads, self._pool.key_caches[0].dtype):
+        if not kernels.shared_prefix_pays(saved, c.num_key_value_heads, pool.key_caches[0].dtype):
             return None
         grouped = {i for members, _ in found for i in members}
         singles = [i for i in range(len(sequences)) if i not in grouped]

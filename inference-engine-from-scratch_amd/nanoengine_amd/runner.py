@@ -235,9 +235,10 @@ class VerifyRunner:
         self.batch = AttentionBatch(self.positions, self.slot_mapping, self.q_start, self.q_len,
                                     self.ctx_len, self.block_tables, self.R, self.capacity)
         # the slots' common blocks, found anew after each slot change; the arrays keep their
-        # place (a captured step reads them), slots without a group follow one by one
+        # place (a captured step reads them), slots without a group follow one by one (None: never
+        # shared, as in a pool that only ordinary attention takes)
         self.shared_batch: AttentionBatch | None = None
-        if shared_prefix:
+        if shared_prefix and kernels.shared_prefix_supported(pool.key_caches[0], pool.key_scale_2d(0)):
             if max_seqs > kernels.SHARED_PREFIX_MAX_SEQS:
                 raise ValueError(f"shared_prefix takes at most {kernels.SHARED_PREFIX_MAX_SEQS} sequences")
             groups = kernels.PrefixGroups(torch.arange(max_seqs, **i32), torch.arange(max_seqs + 1, **i32),

@@ -40,7 +40,7 @@ def forward(counts: list[int], prefix: int = 2048):
     """The batch of a step in which sequence i brings ``counts[i]`` tokens after ``prefix`` shared ones."""
     model = Recorder()
     pool = SimpleNamespace(block_size=16, scratch_slot=0, key_caches=[torch.zeros(1, dtype=torch.int8)], value_caches=[],
-                           key_scales=None, value_scales=None)
+                           key_scales=[torch.zeros(1, dtype=torch.bfloat16)], value_scales=None)
     allocator = PrefixCachingSlotAllocator(prefix // 16 + sum(-(-n // 16) for n in counts) + 8, 16, CPU)
     runner = ModelRunner(model, pool, allocator, CPU, shared_prefix=True)
     parent = Sequence.from_request(GenerationRequest("p", list(range(prefix)), SamplingParams(max_new_tokens=8)))
