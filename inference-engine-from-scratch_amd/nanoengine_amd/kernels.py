@@ -543,12 +543,17 @@ class SharedPrefixPlan:
 
     def error_flag(self) -> int:
         """The error word of the plan and the calls on it (waits for them)."""
-        return int(self.workspace[:4].view(torch.int32).item())
+        return self._word(0)
+
+    def _word(self, i: int) -> int:
+        if self.groups.seqs.shape[0] == 0:  # nothing was planned, nor written
+            return 0
+        return int(self.workspace[4 * i : 4 * i + 4].view(torch.int32).item())
 
     def shared_items(self) -> int:
         """Work items that read a prefix for its whole group (waits for the plan): 0 where sharing
         would cost more than it saves, as for few sequences or short prefixes."""
-        return int(self.workspace[8:12].view(torch.int32).item())
+        return self._word(2)
 
 
 SHARED_PREFIX_MAX_SEQS = 1024  # a plan's sequences

@@ -64,3 +64,14 @@ def test_row_counts_are_checked_before_a_launch():
     assert attend(-1) == -1 and b"row count" in lib.ne_last_error()
     assert attend(0) == 0 and attend(0, q=None) == 0  # nothing to compute
     assert attend(20, q=None) == -1 and b"null" in lib.ne_last_error()
+
+
+@pytest.mark.gpu
+def test_an_empty_batch_has_no_errors_and_no_items():
+    """Its plan writes nothing, so what the workspace held before does not count."""
+    dev = torch.device("cuda:0")
+    empty = torch.zeros(0, dtype=torch.int32, device=dev)
+    workspace = torch.full((4096,), 255, dtype=torch.uint8, device=dev)
+    plan = kernels.shared_prefix_plan(torch.zeros(0, 1, dtype=torch.int32, device=dev), 16, empty, empty, empty,
+                                      kernels.PrefixGroups.from_lists([], [], dev), 16, 8, 1, 1, workspace=workspace)
+    assert plan.error_flag() == 0 and plan.shared_items() == 0
