@@ -626,7 +626,7 @@ def shared_prefix_plan(
     if num_rows is None:
         num_rows = (1 << 31) - 1
     if num_blocks is None:
-        num_blocks = ((1 << 31) - 1) // block_size
+        num_blocks = ((1 << 31) - 1) // max(block_size, 1)
     plan = SharedPrefixPlan(workspace, block_tables, block_size, num_rows, num_q_heads, num_kv_heads, max_q_len, max_ctx_len,
                             num_blocks, groups)
     _call_on(device, "ne_shared_prefix_plan", ctx_len.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), num_rows,

@@ -75,3 +75,11 @@ def test_an_empty_batch_has_no_errors_and_no_items():
     plan = kernels.shared_prefix_plan(torch.zeros(0, 1, dtype=torch.int32, device=dev), 16, empty, empty, empty,
                                       kernels.PrefixGroups.from_lists([], [], dev), 16, 8, 1, 1, workspace=workspace)
     assert plan.error_flag() == 0 and plan.shared_items() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block_size", [0, -16, 8, 24])
+def test_block_sizes_that_no_pool_has(block_size):
+    b = Batch([(32, [(4, 1), (5, 1)])]).to_gpu()
+    with pytest.raises(RuntimeError, match="block_size"):
+        kernels.shared_prefix_plan(b.d["tables"], block_size, b.d["ctx"], b.d["q_start"], b.d["q_len"], b.groups, 16, 8, 1, 100)
