@@ -451,9 +451,10 @@ int ne_advance_and_propose(const int32_t* history, int64_t history_stride, const
  * where that saves more than it costs; the workspace's third word is the number of work items
  * that do.  Its first word is the error word of the last plan and the calls on it: 1 a context
  * beyond max_ctx_len (keys past it are dropped), 2 a sequence of more than max_q_len queries or
- * with rows outside q (not computed), 4 a group list that is out of order or names a sequence
- * twice or outside the batch (such entries are not computed), 8 a block table entry outside the
- * pool (block 0 is read).
+ * with rows outside q (not computed), 4 a group list that is out of order (its entries share
+ * nothing; nothing at all is computed where it holds more than the batch) or names a sequence
+ * twice or outside the batch (such entries are not computed, nor is a sequence without an
+ * entry), 8 a block table entry outside the pool (block 0 is read).
  * head_dim 128, block_size a multiple of 16, at most 1,024 sequences, any number of query
  * heads per KV head; bf16 pools, or int8 pools with bf16 or fp16 scales.
  */

@@ -497,6 +497,8 @@ __device__ __forceinline__ void sp_softmax(const floatx4 (&s)[MT][2], const floa
     }
   };
   probs();
+  // (A row past the last has no reference, so its sum is infinite in a step without masks: a wave that holds one
+  // takes the way below each time.)
   bool grow = INT8 && down != 1.f;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) grow |= psum[mt] > kSpLazy;
