@@ -922,6 +922,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
   u64 end_word = 1, end_weight = 0;  // the last kept token (1: every token), and the kept weight
   u64 border_word = 0, border_weight = 0;
   u64 reach = ~0ull;  // top-p's share of the first top_k's weight
+  int all_end = kBins - 1;  // the last bin of the tokens that fit the list
 
   auto start_border = [&](Step what, bool count, u64 to) {
     step = what;
@@ -945,6 +946,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
     ilo = 0;
     bhi = min(bin_k, bin_m);
     if (cut_p) bhi = min(bhi, first_reaching(s.weight, kBins, reach != ~0ull ? reach : reach_at(r.top_p, uni(s.weight[bin_k]))));
+    // (the exact share may pass the histogram's by some units, and with them a bin's end)
+    all_end = bhi = min(bhi, all_end);
   };
   // the border of top_k is known (or there is none): top-p's, min-p's, or the draw
   auto after_top_k = [&]() {

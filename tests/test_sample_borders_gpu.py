@@ -48,3 +48,31 @@ def test_a_border_among_subnormal_numbers_below_zero(zero, zeros, negatives, top
         w = np.exp(x[r][order].astype(np.float64))
         want = np.searchsorted(np.cumsum(w), float(u[r]) * w.sum(), side="right")
         assert tokens[r].item() == order[want]
+
+
+# (tokens of 1.1, tokens of 1.0, top-p): the first kind's end is where top-p ends, to within a unit of
+# the integer weights per token, and the two ways of adding up the second kind lie on either side of it
+@pytest.mark.gpu
+@pytest.mark.parametrize("more,less,top_p", [(3993, 10145, 0.3178494870662689), (3942, 7020, 0.39943596720695496),
+                                             (3919, 12403, 0.2723730206489563), (3718, 11151, 0.28358253836631775),
+                                             (3652, 10841, 0.2858269512653351)])
+def test_a_top_p_share_next_to_a_bins_end(more, less, top_p):
+    """The share of the first top-k is found from a histogram, then from the exact weight: whichever
+    token that makes the last, it is next to the end of the tokens of 1.1."""
+    vocab, parts = 20480, 6
+    x = np.full(vocab, -np.inf, np.float32)
+    x[0] = 5.0  # alone in its part of the row, so that the others' weights are brought to its base
+    first = [80 * c // parts * 256 for c in range(parts)] + [vocab]
+    for c in range(parts - 1):
+        a, b = (n // 5 + (c < n % 5) for n in (more, less))
+        at = first[c + 1]
+        assert at + a + b < first[c + 2]
+        x[at : at + a], x[at + a : at + a + b] = 1.1, 1.0
+    x[vocab - 1] = -5.0  # one token past top-k
+    logits, u = torch.from_numpy(x[None]).cuda(), torch.tensor([0.999999], device="cuda")
+    kept = set()
+    for _ in range(8):
+        token, probs = kernels.sample(logits, u, 0.77, 1 + more + less, top_p, probs=True)
+        kept.add(int((probs > 0).sum()))
+        assert x[int(token)] == np.float32(1.1) or int((probs > 0).sum()) == 2 + more
+    assert len(kept) == 1 and kept <= {1 + more, 2 + more}
