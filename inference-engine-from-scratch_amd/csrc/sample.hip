@@ -689,11 +689,8 @@ __device__ __forceinline__ u64 share_of(float f, u64 sum, bool up) {
   }
   return whole + (up && rest != 0);
 }
-// floor(u * sum), below sum
-__device__ __forceinline__ u64 draw_at(float u, u64 sum) {
-  if (!(u > 0.f)) return 0;
-  return u < 1.f ? share_of(u, sum, false) : sum - 1;
-}
+// floor(u * sum), below sum (u < 1)
+__device__ __forceinline__ u64 draw_at(float u, u64 sum) { return u > 0.f ? share_of(u, sum, false) : 0; }
 // ceil(top_p * sum), 1 .. sum: the least integer weight that reaches it (top_p < 1)
 __device__ __forceinline__ u64 reach_at(float top_p, u64 sum) {
   if (!(top_p > 0.f)) return 1;
@@ -958,7 +955,13 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
       step = kTopP;
     }
   };
-  auto start_draw = [&]() { start_border(kDraw, false, draw_at(u, end_weight) + 1); };
+  // (a uniform of 1 takes the last kept token, which may have no weight: the row's last, unless one before it is the end)
+  auto start_draw = [&]() {
+    if (u >= 1.f)
+      start_border(kDraw, true, tokens);
+    else
+      start_border(kDraw, false, draw_at(u, end_weight) + 1);
+  };
   auto after_top_p = [&]() {
     // min-p can cut where a token kept so far lies in its border's bin or behind (weights do not say: one
     // below 2^-S of the largest is 0)
@@ -1276,7 +1279,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
       __syncthreads();
       const int kept = uni(max(1, min((int)min(s.red[0], s.red[1]), nk)));
       const u64 sum = uni(s.list.sum[kept - 1]);
-      const int at = first_reaching(s.list.sum, kept, draw_at(u, sum) + 1);
+      const int at = u >= 1.f ? kept - 1 : first_reaching(s.list.sum, kept, draw_at(u, sum) + 1);
       end_word = uni(s.list.word[kept - 1]);
       end_weight = sum;
       border_word = uni(s.list.word[at]);

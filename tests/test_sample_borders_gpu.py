@@ -76,3 +76,43 @@ def test_a_top_p_share_next_to_a_bins_end(more, less, top_p):
         kept.add(int((probs > 0).sum()))
         assert x[int(token)] == np.float32(1.1) or int((probs > 0).sum()) == 2 + more
     assert len(kept) == 1 and kept <= {1 + more, 2 + more}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("u", [1.0, 7.5, float("inf")])
+def test_uniforms_of_one_and_more_take_the_last_kept_token(dtype, u):
+    """Also where the tokens before it hold all the weight that any sum can hold."""
+    rng = np.random.default_rng(4)
+    rows = [np.array([0.0, -200.0]), np.array([-200.0, 3.0, -210.0, -210.0]),
+            rng.permutation(np.concatenate([[40.0], np.zeros(300), np.full(80, -60.0)])),
+            rng.permutation(np.concatenate([np.full(9000, 1.0), np.full(50, -90.0)])),
+            rng.permutation(np.concatenate([np.full(9000, 1.0), np.full(7000, -90.0)])),
+            rng.permutation(np.concatenate([[60.0], rng.normal(size=20000)])), rng.normal(size=30000)]
+    uniform = torch.tensor([u], device="cuda")
+    for row in rows:
+        logits = torch.from_numpy(row[None]).to(dtype).cuda()
+        x = logits.float().cpu().numpy()[0]
+        order = first_tokens(x, x.size)
+        n = x.size
+        for k in {0, 2, n - 1, n // 2 + 1}:
+            kept = n if k in (0, n) or k > n else max(k, 1)
+            assert kernels.sample(logits, uniform, top_k=k).item() == order[kept - 1], (n, k)
+        # min-p: those within 30 of the first, none of these rows has a logit near that border
+        near = int((x >= x.max() - 30.0).sum())
+        assert kernels.sample(logits, uniform, min_p=float(np.exp(-30.0))).item() == order[near - 1], n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("less", [4500, 9000, 16000])
+def test_a_uniform_of_one_where_the_histogram_holds_less_than_the_sum(less):
+    """The last kept token by its rank, whatever units the histogram dropped."""
+    vocab, parts = 20480, 6
+    x = np.full(vocab, -np.inf, np.float32)
+    x[0] = 5.0
+    first = [80 * c // parts * 256 for c in range(parts)]
+    for c in range(parts - 1):
+        x[first[c + 1] : first[c + 1] + less // 5] = 1.0
+    x[vocab - 1] = -16.0  # past top-k: of no weight
+    token = kernels.sample(torch.from_numpy(x[None]).cuda(), torch.ones(1, device="cuda"), 0.77, 1 + less)
+    assert token.item() == np.flatnonzero(x == 1.0)[-1]
