@@ -42,8 +42,9 @@
 // the scan 42, for its ~10 operations per element and the weights of ~3,000 values per chunk
 // (67% of the vector units' time); pick 46, rows' chains of passes (the longest 40) in two rounds of
 // work-groups, one per CU for its 103 KB of LDS and 1,024 threads of 128 registers; probs 43, its
-// bytes (292 MB, 6.9 TB/s).  64 rows 41 us: 11 and 24.  One row 29 us: 6 and 19, a chain of round trips through memory and barriers.  200 rows of 32,003 (fp32) 48 us: 22,
-// for 65 vector operations per element (half of it) and the sums in LDS, and 24.
+// bytes (292 MB, 6.9 TB/s).  64 rows 41 us: 11 and 24.  One row 29 us: 6 and 19, a chain of round
+// trips through memory and barriers.  200 rows of 32,003 (fp32) 48 us: 22, for 65 vector operations
+// per element (half of it) and the sums in LDS, and 24.
 #include <math.h>
 #include <string.h>
 
