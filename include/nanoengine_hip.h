@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define NE_ABI_VERSION 12
+#define NE_ABI_VERSION 13
 
 /* status codes */
 #define NE_OK 0
@@ -540,6 +540,86 @@ int ne_sample(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32
               const int32_t* top_ks, int32_t top_k, const float* top_ps, float top_p,
               const float* min_ps, float min_p, int32_t* tokens, float* probs, int64_t ld_probs,
               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rows of activations to 8-bit integers with one scale per row, what ne_w8a8_gemm multiplies
+ * (the formula of ne/models/int8_quantization.py:30-34, which the reference applies to weights
+ * and cache): s = max(max|x|, 1e-8) / 127 in fp32, q = rint(x / s) clamped to [-127, 127].
+ *   x       [rows, k] bf16 or fp16 (dtype), row stride ldx (a multiple of 8), 16-byte aligned
+ *   codes   [rows, k] int8 out, contiguous
+ *   scales  [rows] fp32 out
+ * k % 8 == 0.  A row that holds a NaN or an infinity gets the scale NaN and codes 0: its
+ * products are NaN.  The norm forms quantise the rows that ne_rmsnorm (ne_add_rmsnorm, which
+ * updates residual in place) would store, bit for bit, without storing them; hidden <= 4096.
+ */
+int ne_quantize_rows(const void* x, int32_t dtype, int64_t ldx, int32_t rows, int32_t k,
+                     int8_t* codes, float* scales, void* stream);
+int ne_rmsnorm_quantize(const void* x, const void* weight, int8_t* codes, float* scales,
+                        int32_t rows, int32_t hidden, float eps, void* stream);
+int ne_add_rmsnorm_quantize(void* residual, const void* delta, const void* weight, int8_t* codes,
+                            float* scales, int32_t rows, int32_t hidden, float eps, void* stream);
+
+/*
+ * W8A8 projection: y[m, n] = bf16((sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n]), 8-bit integers
+ * times 8-bit integers with an exact int32 sum (no counterpart in the reference, whose
+ * Int8Linear keeps 16-bit activations), on the weights and scales of ne_w8a16_gemm as they are.
+ *   x [m, k] int8 (row stride ldx, a multiple of 16), x_scale [m] fp32, w [n, k] int8,
+ *   w_scale [n] bf16/fp16/fp32, y [m, n_out] bf16 (row stride ldy); n_out = n, or n/2 for
+ *   NE_EPILOGUE_SWIGLU: weight rows in groups of 32 (16 gate rows then 16 up rows),
+ *   y[:, 16*i + j] = bf16(silu(gate) * up) of the pair in group i, row j, in fp32 before
+ *   the one rounding.
+ * k a multiple of 16, at most 131,056 (where the sum of any codes fits), n any number (SwiGLU:
+ * a multiple of 32), m from 0 on.  Wide stores need y 16-byte aligned and ldy % 8 == 0; others
+ * are stored element by element.  The sums are integers, so the same row and weights give the
+ * same bits in every batch.  ne_w8a8_kernel: which kernel serves a product of these sizes (host
+ * only; for tests and measurements).
+ */
+#define NE_W8A8_FEW_ROWS 0
+#define NE_W8A8_TILE_64X128 1
+#define NE_W8A8_TILE_128X128 2
+#define NE_W8A8_TILE_256X256 3
+int32_t ne_w8a8_kernel(int32_t m, int32_t n, int32_t k, int32_t epilogue);
+int ne_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
+                 const void* w_scale, int32_t scale_dtype, int32_t m, int32_t n, int32_t k, void* y,
+                 int64_t ldy, int32_t epilogue, void* stream);
+
+/*
+ * Logits under penalties for repeated tokens, biases of single tokens and masks of allowed ones
+ * (no counterpart in the reference, whose requests have a temperature and top-p), before
+ * ne_sample or ne_accept.  For row r of sequence b = row_seq[r] (null: r), with c the token's
+ * occurrences in history[b, prompt_len[b] .. history_len[b]) and among the guesses
+ * drafts[b, 0 .. row_drafts[r]), and "seen" its occurrence anywhere in history[b] or those guesses:
+ *   x1 = seen ? (x > 0 ? x / repetition : x * repetition) : x
+ *   x2 = x1 - (frequency * c + presence)   where c > 0
+ *   x3 = x2 + bias of the token,   x4 = x3 where the token is allowed, -inf elsewhere
+ * in fp32, rounded once.
+ *   logits     [rows, vocab] bf16, fp16 or fp32 (dtype), row stride ld; vocab <= 2^24
+ *   history    null (no penalties), or [num_seqs, capacity] int32 with its row stride and
+ *              history_len [num_seqs]; prompt_len [num_seqs], or null: all of it is output.
+ *              Tokens outside [0, vocab) count nowhere; a row whose row_seq is outside
+ *              [0, num_seqs) has no history
+ *   drafts     null, or [num_seqs, max_drafts] int32 with row_drafts [rows]: a verify step's row i
+ *              counts the i guesses before it
+ *   repetitions, presences, frequencies: [rows] device arrays, or null: the scalar beside each.
+ *              A repetition that is not positive and finite counts as 1, a NaN as 0
+ *   bias_start null (no biases), or [rows + 1] int32: row r's entries of bias_tokens and
+ *              bias_values [num_biases]; of a token listed twice in a row the last entry counts
+ *   allowed    null (all), or [num_allowed, allowed_stride] int32 words, bit j of word w for token
+ *              32 w + j; row r takes mask allowed_rows[r] (null: r).  A negative one allows
+ *              all, one past the masks none
+ *   out        [rows, vocab] of the logits' type or fp32, row stride ld_out; may be the logits
+ *              themselves, but must not overlap them otherwise
+ */
+int ne_adjust_logits(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t vocab,
+                     const int32_t* history, int64_t history_stride, int32_t capacity,
+                     const int32_t* history_len, const int32_t* prompt_len, int32_t num_seqs,
+                     const int32_t* drafts, int32_t max_drafts, const int32_t* row_seq,
+                     const int32_t* row_drafts, const float* repetitions, float repetition,
+                     const float* presences, float presence, const float* frequencies,
+                     float frequency, const int32_t* bias_start, const int32_t* bias_tokens,
+                     const float* bias_values, int32_t num_biases, const int32_t* allowed,
+                     int64_t allowed_stride, int32_t num_allowed, const int32_t* allowed_rows,
+                     void* out, int32_t out_dtype, int64_t ld_out, void* stream);
 
 /* Plain device copy of `bytes` bytes (16-byte aligned); used to calibrate the
  * hardware byte counters against a kernel of known traffic. */

@@ -1,0 +1,291 @@
+// Rows of activations to 8-bit integers with one scale per row, alone or in the RMSNorm that
+// comes before a projection: what ne_w8a8_gemm multiplies.
+//
+//   s_i = max(max_j |x_ij|, 1e-8) / 127 in fp32,  q_ij = rint(x_ij / s_i)  (the formula of the
+//   int8 cache and weights, ne/models/int8_quantization.py:30-34, per row of activations)
+//
+// The row maximum is taken over the bits of |x|, whose order is the values' with infinities and
+// NaN above all: a row that holds one gets the scale NaN and codes 0, so that what it is
+// multiplied into is NaN, as with the row itself.  Norm rows are the bits that ne_rmsnorm and
+// ne_add_rmsnorm store (same sums in the same order, both roundings), quantised without the
+// trip through memory.  What bounds it: memory, each row read once into registers.
+#include "ne_common.hpp"
+#include "qk_rope_kv.hpp"
+
+namespace ne {
+
+namespace {
+
+enum { kPlain = 0, kNorm = 1, kAddNorm = 2 };
+
+struct RowsParams {
+  const uint16_t* x;  // plain and norm: the rows; add norm: delta
+  int64_t ldx;
+  uint16_t* residual;      // add norm: updated in place
+  const uint16_t* weight;  // norm weight
+  float eps;
+  int8_t* codes;  // [rows][k]
+  float* scales;  // [rows]
+  int rows, k;
+};
+
+template <int VDT>
+__device__ __forceinline__ void unpack8(const u32x4 v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (VDT == NE_DTYPE_BF16) {
+      f[2 * i] = bf16_to_f32((uint16_t)(v[i] & 0xFFFFu));
+      f[2 * i + 1] = bf16_to_f32((uint16_t)(v[i] >> 16));
+    } else {
+      f[2 * i] = f16_to_f32((uint16_t)(v[i] & 0xFFFFu));
+      f[2 * i + 1] = f16_to_f32((uint16_t)(v[i] >> 16));
+    }
+  }
+}
+
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  return u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  return v;
+}
+
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// the row's scale from the bits of its largest magnitude
+__device__ __forceinline__ float row_scale(uint32_t top) {
+  if (top >= kInfBits) return __builtin_nanf("");
+  return fmaxf(__builtin_bit_cast(float, top), 1e-8f) / 127.f;
+}
+
+__device__ __forceinline__ uint32_t codes4(const float* t) {
+  uint32_t b[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = (uint32_t)(int)fminf(fmaxf(rintf(t[e]), -127.f), 127.f);
+  const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), lo, 0x05040100u);
+}
+
+// Codes of 8 values of a finite row.  x / s as x * v_rcp_f32(s): within 3e-5 of the fp32 quotient
+// at |x / s| <= 127, so both round to the same integer unless it lies within 4e-5 of a half;
+// a wave with such a lane divides (one chunk of 512 values in 25).
+__device__ __forceinline__ u32x2 quantize8(const float (&f)[8], float s, float rcp) {
+  float t[8], far = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    t[e] = f[e] * rcp;
+    far = fmaxf(far, fabsf(t[e] - rintf(t[e])));
+  }
+  if (__builtin_amdgcn_ballot_w64(far > 0.49996f) != 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = f[e] / s;
+  }
+  return u32x2{codes4(t), codes4(t + 4)};
+}
+
+// WAVES waves per row (1: four rows per work-group; 4: one), CPL 8-element chunks per lane held in
+// registers.  Every load of a row is issued before the first use.
+template <int MODE, int VDT, int CPL, int WAVES>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(RowsParams p) {
+  const int wave = threadIdx.x / kWave;
+  const int row = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  if (WAVES == 1 && row >= p.rows) return;  // wave-uniform, and no barrier follows
+  const int at = WAVES == 1 ? threadIdx.x % kWave : threadIdx.x;
+  constexpr int kThreads = WAVES * kWave;
+  const int chunks = p.k / 8;
+  const uint16_t* src = p.x + (int64_t)row * p.ldx;
+  u32x4 raw[CPL], wraw[CPL], draw[CPL];
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) {
+    const int ci = at + c * kThreads;
+    raw[c] = u32x4{0, 0, 0, 0};
+    if (ci < chunks) {
+      if constexpr (MODE == kAddNorm) {
+        raw[c] = *(const u32x4*)(p.residual + (int64_t)row * p.k + ci * 8);
+        draw[c] = *(const u32x4*)(src + ci * 8);
+      } else {
+        raw[c] = *(const u32x4*)(src + ci * 8);
+      }
+      if constexpr (MODE != kPlain) wraw[c] = *(const u32x4*)(p.weight + ci * 8);
+    }
+  }
+  float h[CPL][8];
+  uint32_t top = 0;
+  if constexpr (MODE == kPlain) {
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      unpack8<VDT>(raw[c], h[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, abs_bits(h[c][e]));
+    }
+  } else {
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      const int ci = at + c * kThreads;
+      if (ci < chunks) {
+        unpack8<VDT>(raw[c], h[c]);
+        if constexpr (MODE == kAddNorm) {
+          float d[8];
+          unpack8<VDT>(draw[c], d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[c][e] = bf16_round(h[c][e] + d[e]);
+          *(u32x4*)(p.residual + (int64_t)row * p.k + ci * 8) = pack8(h[c]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += h[c][e] * h[c][e];
+      }
+    }
+    ss = wave_sum(ss);
+    const float inv = rsqrtf(ss / (float)p.k + p.eps);
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      const int ci = at + c * kThreads;
+      if (ci < chunks) {
+        float w[8];
+        unpack8<VDT>(wraw[c], w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          h[c][e] = bf16_round(bf16_round(h[c][e] * inv) * w[e]);
+          top = max(top, abs_bits(h[c][e]));
+        }
+      }
+    }
+  }
+  top = wave_max_u32(top);
+  if constexpr (WAVES > 1) {
+    __shared__ uint32_t tops[WAVES];
+    if (threadIdx.x % kWave == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = max(top, tops[w]);
+  }
+  const float s = row_scale(top);
+  if (at == 0) p.scales[row] = s;
+  const bool finite = top < kInfBits;
+  const float rcp = __builtin_amdgcn_rcpf(s);
+  int8_t* dst = p.codes + (int64_t)row * p.k;
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) {
+    const int ci = at + c * kThreads;
+    if (ci < chunks) *(u32x2*)(dst + ci * 8) = finite ? quantize8(h[c], s, rcp) : u32x2{0, 0};
+  }
+}
+
+// Rows too long for the registers: one work-group per row reads it twice (the second time from a cache).
+template <int VDT>
+__global__ __launch_bounds__(1024) void quantize_long_rows_kernel(RowsParams p) {
+  __shared__ uint32_t tops[16];
+  const int row = blockIdx.x;
+  const int chunks = p.k / 8;
+  const uint16_t* src = p.x + (int64_t)row * p.ldx;
+  uint32_t top = 0;
+  float f[8];
+  for (int ci = threadIdx.x; ci < chunks; ci += 1024) {
+    unpack8<VDT>(*(const u32x4*)(src + (int64_t)ci * 8), f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, abs_bits(f[e]));
+  }
+  top = wave_max_u32(top);
+  if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 16; ++w) top = max(top, tops[w]);
+  const float s = row_scale(top);
+  if (threadIdx.x == 0) p.scales[row] = s;
+  const float rcp = __builtin_amdgcn_rcpf(s);
+  int8_t* dst = p.codes + (int64_t)row * p.k;
+  for (int ci = threadIdx.x; ci < chunks; ci += 1024) {
+    unpack8<VDT>(*(const u32x4*)(src + (int64_t)ci * 8), f);
+    *(u32x2*)(dst + (int64_t)ci * 8) = top < kInfBits ? quantize8(f, s, rcp) : u32x2{0, 0};
+  }
+}
+
+template <int MODE, int VDT>
+int launch_rows(const RowsParams& p, hipStream_t stream) {
+  const dim3 four(ceil_div(p.rows, 4)), one(p.rows), block(256);
+#define NE_ROWS(CPL, WAVES, GRID) \
+  hipLaunchKernelGGL((quantize_rows_kernel<MODE, VDT, CPL, WAVES>), GRID, block, 0, stream, p)
+  if (p.k <= 512) {
+    NE_ROWS(1, 1, four);
+  } else if (p.k <= 1024) {
+    NE_ROWS(2, 1, four);
+  } else if (p.k <= 2048) {
+    NE_ROWS(4, 1, four);
+  } else if (p.k <= 4096) {
+    NE_ROWS(8, 1, four);
+  } else if constexpr (MODE == kPlain) {
+    if (p.k <= 8192) {
+      NE_ROWS(4, 4, one);
+    } else if (p.k <= 16384) {
+      NE_ROWS(8, 4, one);
+    } else {
+      hipLaunchKernelGGL(quantize_long_rows_kernel<VDT>, one, dim3(1024), 0, stream, p);
+    }
+  }
+#undef NE_ROWS
+  return check_launch("quantize_rows");
+}
+
+constexpr int kMaxNormHidden = 4096;  // ne_rmsnorm's
+
+int check_rows(const void* codes, const float* scales, int32_t rows, int32_t k) {
+  NE_CHECK_ARG(rows >= 0 && k > 0, "bad shape: %d rows of %d", rows, k);
+  NE_CHECK_SUPPORTED(k % 8 == 0, "rows must be a multiple of 8 wide (got %d)", k);
+  if (rows == 0) return NE_OK;
+  NE_CHECK_ARG(codes && scales, "null pointer argument");
+  NE_CHECK_ARG((uintptr_t)codes % 8 == 0 && (uintptr_t)scales % 4 == 0, "codes must be 8-byte aligned, scales 4-byte aligned");
+  return NE_OK;
+}
+
+int check_norm(const void* a, const void* b, const void* weight, int32_t k) {
+  NE_CHECK_ARG(a && b && weight, "null pointer argument");
+  NE_CHECK_SUPPORTED(k <= kMaxNormHidden, "hidden must be at most %d (got %d)", kMaxNormHidden, k);
+  NE_CHECK_ARG((uintptr_t)a % 16 == 0 && (uintptr_t)b % 16 == 0 && (uintptr_t)weight % 16 == 0,
+               "rows and weight must be 16-byte aligned");
+  return NE_OK;
+}
+
+}  // namespace
+
+}  // namespace ne
+
+using namespace ne;
+
+extern "C" int ne_quantize_rows(const void* x, int32_t dtype, int64_t ldx, int32_t rows, int32_t k, int8_t* codes,
+                                float* scales, void* stream) {
+  int rc = check_rows(codes, scales, rows, k);
+  if (rc != NE_OK || rows == 0) return rc;
+  NE_CHECK_ARG(x != nullptr, "null x");
+  NE_CHECK_ARG(dtype == NE_DTYPE_BF16 || dtype == NE_DTYPE_FP16, "rows must be bf16 or fp16");
+  NE_CHECK_ARG(ldx >= k && ldx % 8 == 0 && (uintptr_t)x % 16 == 0, "rows must be 16-byte aligned, ldx >= k");
+  const RowsParams p{(const uint16_t*)x, ldx, nullptr, nullptr, 0.f, codes, scales, rows, k};
+  return dtype == NE_DTYPE_BF16 ? launch_rows<kPlain, NE_DTYPE_BF16>(p, (hipStream_t)stream)
+                                : launch_rows<kPlain, NE_DTYPE_FP16>(p, (hipStream_t)stream);
+}
+
+extern "C" int ne_rmsnorm_quantize(const void* x, const void* weight, int8_t* codes, float* scales, int32_t rows,
+                                   int32_t hidden, float eps, void* stream) {
+  int rc = check_rows(codes, scales, rows, hidden);
+  if (rc != NE_OK || rows == 0) return rc;
+  rc = check_norm(x, x, weight, hidden);
+  if (rc != NE_OK) return rc;
+  const RowsParams p{(const uint16_t*)x, hidden, nullptr, (const uint16_t*)weight, eps, codes, scales, rows, hidden};
+  return launch_rows<kNorm, NE_DTYPE_BF16>(p, (hipStream_t)stream);
+}
+
+extern "C" int ne_add_rmsnorm_quantize(void* residual, const void* delta, const void* weight, int8_t* codes, float* scales,
+                                       int32_t rows, int32_t hidden, float eps, void* stream) {
+  int rc = check_rows(codes, scales, rows, hidden);
+  if (rc != NE_OK || rows == 0) return rc;
+  rc = check_norm(residual, delta, weight, hidden);
+  if (rc != NE_OK) return rc;
+  const RowsParams p{(const uint16_t*)delta, hidden, (uint16_t*)residual, (const uint16_t*)weight, eps, codes, scales, rows,
+                     hidden};
+  return launch_rows<kAddNorm, NE_DTYPE_BF16>(p, (hipStream_t)stream);
+}

@@ -14,7 +14,7 @@ from pathlib import Path
 
 LIBRARY_NAME = "libnanoengine_hip.so"
 LIBRARY_PATH = Path(__file__).resolve().parent / LIBRARY_NAME
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 # status codes (nanoengine_hip.h)
 NE_OK = 0
@@ -158,6 +158,29 @@ SIGNATURES: dict[str, tuple] = {
             _f32,  # softmax scale
             _vp, _i64, _i64,  # out, strides
             _vp, _sz, _vp,  # workspace, bytes, stream
+        ],
+    ),
+    "ne_quantize_rows": (ctypes.c_int, [_vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "ne_rmsnorm_quantize": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp]),
+    "ne_add_rmsnorm_quantize": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp]),
+    "ne_w8a8_kernel": (_i32, [_i32, _i32, _i32, _i32]),
+    "ne_w8a8_gemm": (
+        ctypes.c_int,
+        [
+            _vp, _i64, _vp, _vp, _vp, _i32,  # codes, stride, scales, weight, its scales, their dtype
+            _i32, _i32, _i32, _vp, _i64, _i32, _vp,  # m, n, k, y, stride, epilogue, stream
+        ],
+    ),
+    "ne_adjust_logits": (
+        ctypes.c_int,
+        [
+            _vp, _i32, _i64, _i32, _i32,  # logits, dtype, ld, rows, vocab
+            _vp, _i64, _i32, _vp, _vp, _i32,  # history, stride, capacity, lengths, prompt lengths, seqs
+            _vp, _i32, _vp, _vp,  # drafts, max drafts, row seq, row drafts
+            _vp, _f32, _vp, _f32, _vp, _f32,  # repetition, presence, frequency: per row, or one for all
+            _vp, _vp, _vp, _i32,  # bias start, tokens, values, entries
+            _vp, _i64, _i32, _vp,  # allowed, its stride, masks, mask of each row
+            _vp, _i32, _i64, _vp,  # out, dtype, ld, stream
         ],
     ),
     "ne_sample_workspace_size": (_sz, [_i32, _i32, _i32]),

@@ -13,6 +13,7 @@ import math
 from array import array
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
 from nanoengine_amd import _native
@@ -731,6 +732,99 @@ def w8a16_gemm(
     return out
 
 
+# ------------------------------------------------------------------------- W8A8
+def _code_outputs(rows: int, k: int, codes, scales, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    if codes is None:
+        codes = torch.empty((rows, k), dtype=torch.int8, device=device)
+    elif codes.dtype != torch.int8 or tuple(codes.shape) != (rows, k) or not codes.is_contiguous() or codes.device != device:
+        raise ValueError(f"codes must be contiguous int8 [{rows}, {k}] on {device}")
+    if scales is None:
+        scales = torch.empty((rows,), dtype=torch.float32, device=device)
+    elif scales.dtype != torch.float32 or tuple(scales.shape) != (rows,) or not scales.is_contiguous() or scales.device != device:
+        raise ValueError(f"scales must be contiguous fp32 [{rows}] on {device}")
+    return codes, scales
+
+
+def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None,
+                  scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """int8 codes ``[m, k]`` of the rows of ``x [m, k]`` (bf16 or fp16) and fp32 scales ``[m]``: the
+    formula of :func:`~nanoengine_amd.int8_quantization.quantize_vectors` per row, for
+    :func:`w8a8_gemm`.  A row with a NaN or an infinity gets the scale NaN and codes 0."""
+    device = _require_gpu(x)
+    _check(x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1), "x must be [m, k] with contiguous rows")
+    _check(x.dtype in (torch.bfloat16, torch.float16), "x must be bf16 or fp16")
+    rows, k = x.shape
+    codes, scales = _code_outputs(rows, k, codes, scales, device)
+    _call_on(device, "ne_quantize_rows", x.data_ptr(), dtype_code(x.dtype), x.stride(0) if rows > 1 else k, rows, k,
+             codes.data_ptr(), scales.data_ptr(), _stream(device))
+    return codes, scales
+
+
+def _check_norm_rows(weight: torch.Tensor, *rows: torch.Tensor) -> None:
+    hidden = weight.shape[0] if weight.dim() == 1 else -1
+    for t in rows:
+        _check(t.dim() == 2 and t.shape[1] == hidden and t.dtype == torch.bfloat16 and t.is_contiguous()
+               and t.shape == rows[0].shape, "rows must be contiguous [rows, hidden] bf16, the weight [hidden]")
+    _check(weight.dtype == torch.bfloat16 and weight.is_contiguous(), "weight must be contiguous bf16")
+
+
+def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: torch.Tensor | None = None,
+                     scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`quantize_rows` of :func:`rmsnorm`'s rows (the same bits), in one pass; hidden at most 4,096."""
+    device = _require_gpu(x, weight)
+    _check_norm_rows(weight, x)
+    codes, scales = _code_outputs(*x.shape, codes, scales, device)
+    _call_on(device, "ne_rmsnorm_quantize", x.data_ptr(), weight.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+             *x.shape, eps, _stream(device))
+    return codes, scales
+
+
+def add_rmsnorm_quantize(residual: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, eps: float,
+                         codes: torch.Tensor | None = None,
+                         scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``residual += delta`` (bf16) in place, then :func:`quantize_rows` of its RMSNorm:
+    :func:`add_rmsnorm` with the same bits and its rows as codes."""
+    device = _require_gpu(residual, delta, weight)
+    _check_norm_rows(weight, residual, delta)
+    codes, scales = _code_outputs(*residual.shape, codes, scales, device)
+    _call_on(device, "ne_add_rmsnorm_quantize", residual.data_ptr(), delta.data_ptr(), weight.data_ptr(), codes.data_ptr(),
+             scales.data_ptr(), *residual.shape, eps, _stream(device))
+    return codes, scales
+
+
+def w8a8_gemm(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    weight_int8: torch.Tensor,
+    weight_scale: torch.Tensor,
+    epilogue: int = EPILOGUE_STORE,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``bf16((codes @ int8.T) * scales[:, None] * weight_scale)`` with an exact integer sum, on the
+    weights of :func:`w8a16_gemm`; SwiGLU epilogue pairs 16 gate rows with 16 up rows.  ``k`` is a
+    multiple of 16, at most 131,056; ``n`` is any number (SwiGLU: a multiple of 32)."""
+    device = _require_gpu(codes, scales, weight_int8, weight_scale)
+    _check(codes.dtype == torch.int8 and codes.dim() == 2 and codes.stride(1) == 1, "codes must be [m, k] int8")
+    _check(weight_int8.dtype == torch.int8 and weight_int8.dim() == 2 and weight_int8.is_contiguous(),
+           "weight must be contiguous [n, k] int8")
+    m, k = codes.shape
+    n = weight_int8.shape[0]
+    if weight_int8.shape[1] != k:
+        raise ValueError(f"k mismatch: codes have {k}, weight {weight_int8.shape[1]}")
+    _check(scales.dtype == torch.float32 and scales.numel() == m and scales.is_contiguous(), "one contiguous fp32 scale per row")
+    _check(weight_scale.numel() == n and weight_scale.is_contiguous(), "one contiguous scale per weight row")
+    n_out = n // 2 if epilogue == EPILOGUE_SWIGLU else n
+    if out is None:
+        out = torch.empty((m, n_out), dtype=torch.bfloat16, device=device)
+    else:
+        _check(out.shape == (m, n_out) and out.dtype == torch.bfloat16 and (out.stride(1) == 1 or n_out == 1)
+               and out.device == device, "bad out")
+    _call_on(device, "ne_w8a8_gemm", codes.data_ptr(), codes.stride(0) if m > 1 else k, scales.data_ptr(),
+             weight_int8.data_ptr(), weight_scale.data_ptr(), dtype_code(weight_scale.dtype), m, n, k, out.data_ptr(),
+             out.stride(0) if m > 1 else n_out, epilogue, _stream(device))
+    return out
+
+
 PROJ_TILE_ROWS = 80  # token rows per work-group of the W8A16 kernels
 SPLITK_TILE_ROWS = 48  # token rows per work-group of the split-K product
 PROJ_TILE_COLS = 64  # weight rows per work-group of the store / split-K kernels
@@ -1053,6 +1147,156 @@ def accept(
         _stream(device),
     )
     return out_tokens, num_out
+
+
+# ------------------------------------------------------------ adjusting logits
+@dataclass(frozen=True)
+class TokenPenalties:
+    """Penalties for the tokens of each sequence so far, for :func:`adjust_logits`: device tensors that a
+    step reads, so their contents may change between replays of a graph.
+
+    ``repetition`` divides positive logits (and multiplies others) of tokens anywhere in the history,
+    ``frequency`` times its count and ``presence`` are taken off a token of the output (what follows
+    ``prompt_len``; None: the whole history).  Each is one value, or an fp32 tensor with one per row.
+    Rows are the sequences' own (row i of sequence i) unless ``row_seq`` names them; ``row_drafts``
+    of the guesses in ``drafts`` count as output too (a verify step's row i: the i guesses before it)."""
+
+    history: torch.Tensor  # [seqs, capacity] int32
+    history_len: torch.Tensor  # [seqs] int32
+    prompt_len: torch.Tensor | None = None  # [seqs] int32
+    repetition: float | torch.Tensor = 1.0
+    presence: float | torch.Tensor = 0.0
+    frequency: float | torch.Tensor = 0.0
+    drafts: torch.Tensor | None = None  # [seqs, max_drafts] int32
+    row_seq: torch.Tensor | None = None  # [rows] int32
+    row_drafts: torch.Tensor | None = None  # [rows] int32
+
+
+@dataclass(frozen=True)
+class TokenBias:
+    """Biases of single tokens, for :func:`adjust_logits`: entries ``start[r] .. start[r + 1]`` are row r's."""
+
+    start: torch.Tensor  # [rows + 1] int32
+    tokens: torch.Tensor  # [entries] int32
+    values: torch.Tensor  # [entries] fp32
+
+    @classmethod
+    def from_dicts(cls, rows: list[dict[int, float] | None], device: torch.device) -> "TokenBias":
+        """From each row's token -> bias on the host (None: no biases)."""
+        start, tokens, values = [0], [], []
+        for biases in rows:
+            tokens += (biases or {}).keys()
+            values += (biases or {}).values()
+            start.append(len(tokens))
+        flat = torch.tensor(start + tokens, dtype=torch.int32).to(device)
+        return cls(flat[: len(start)], flat[len(start) :], torch.tensor(values, dtype=torch.float32).to(device))
+
+
+def allowed_words(vocab: int) -> int:
+    """32-bit words of a mask of ``vocab`` tokens."""
+    return (vocab + 31) // 32
+
+
+def allowed_mask(rows: list[list[int] | None], vocab: int, device: torch.device) -> torch.Tensor:
+    """Masks ``[rows, words]`` int32 for :func:`adjust_logits` from each row's allowed tokens on the host
+    (None: all): bit j of word w is token 32 w + j."""
+    bits = np.zeros((len(rows), allowed_words(vocab) * 32), dtype=np.uint8)
+    for row, tokens in zip(bits, rows):
+        if tokens is None:
+            row[:] = 1
+        elif len(tokens):
+            index = np.asarray(tokens, dtype=np.int64)
+            _check(index.min() >= 0 and index.max() < vocab, f"allowed tokens outside [0, {vocab})")
+            row[index] = 1
+    words = np.packbits(bits, axis=1, bitorder="little").view(np.int32)
+    return torch.from_numpy(words).to(device)
+
+
+def _int32_or_none(tensor: torch.Tensor | None, shape: tuple, name: str, device: torch.device):
+    """The device pointer (or None) of an optional contiguous int32 argument of a given shape."""
+    if tensor is None:
+        return None
+    if tensor.dtype != torch.int32 or tuple(tensor.shape) != shape or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {tensor.dtype} {list(tensor.shape)}")
+    if tensor.device != device:
+        raise RuntimeError(f"{name} is on {tensor.device}, the logits on {device}")
+    return tensor.data_ptr()
+
+
+def adjust_logits(
+    logits: torch.Tensor,
+    penalties: TokenPenalties | None = None,
+    bias: TokenBias | None = None,
+    allowed: torch.Tensor | None = None,
+    allowed_rows: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``logits [rows, vocab]`` (bf16, fp16 or fp32) under penalties, then biases, then a mask, before
+    :func:`sample` or :func:`accept`: in fp32, rounded once to ``out``'s type.
+
+    ``out`` (default: allocated) is of the logits' type, fp32, or ``logits`` itself.  ``allowed`` is
+    int32 ``[masks, allowed_words(vocab)]`` (:func:`allowed_mask`); a token whose bit is not set
+    becomes -inf, whatever its logit was.  ``allowed_rows [rows]`` int32 names each row's mask (default:
+    its own index; negative: no mask, one past the masks: no token).  Tokens outside the vocabulary
+    count nowhere."""
+    device = _require_gpu(logits)
+    _check(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits must be [rows, vocab] with contiguous rows")
+    code = dtype_code(logits.dtype)
+    _check(code != DTYPE_INT8, "logits must be bf16, fp16 or fp32")
+    rows, vocab = logits.shape
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+    elif out is not logits:
+        if (out.dtype != logits.dtype and out.dtype != torch.float32 or out.shape != logits.shape or out.device != device
+                or (out.stride(1) != 1 and vocab > 1)):
+            raise ValueError(f"out must be {logits.dtype} or fp32 [{rows}, {vocab}] on {device}")
+    history_args = (None, 0, 0, None, None, 0, None, 0, None, None, None, 1.0, None, 0.0, None, 0.0)
+    if penalties is not None:
+        h = penalties.history
+        _check(h.dtype == torch.int32 and h.dim() == 2 and (h.stride(1) == 1 or h.shape[1] <= 1),
+               "history must be [seqs, capacity] int32 with contiguous rows")
+        if h.device != device:
+            raise RuntimeError(f"history is on {h.device}, the logits on {device}")
+        seqs, capacity = h.shape
+        per_seq, per_row = (seqs,), (rows,)
+        _check(penalties.history_len is not None, "history needs history_len")
+        max_drafts = 0
+        if penalties.drafts is not None:
+            max_drafts = penalties.drafts.shape[-1]
+            _check(penalties.row_drafts is not None, "drafts need row_drafts")
+        r_ptr, r = _row_parameter(penalties.repetition, rows, torch.float32, "repetition", device)
+        p_ptr, p = _row_parameter(penalties.presence, rows, torch.float32, "presence", device)
+        f_ptr, f = _row_parameter(penalties.frequency, rows, torch.float32, "frequency", device)
+        history_args = (
+            h.data_ptr(), h.stride(0) if seqs > 1 else capacity, capacity,
+            _int32_or_none(penalties.history_len, per_seq, "history_len", device),
+            _int32_or_none(penalties.prompt_len, per_seq, "prompt_len", device), seqs,
+            _int32_or_none(penalties.drafts, (seqs, max_drafts), "drafts", device), max_drafts,
+            _int32_or_none(penalties.row_seq, per_row, "row_seq", device),
+            _int32_or_none(penalties.row_drafts, per_row, "row_drafts", device), r_ptr, r, p_ptr, p, f_ptr, f)
+        if capacity == 0 and seqs > 0:  # an empty tensor has no address, and guesses may still count
+            history_args = (penalties.history_len.data_ptr(),) + history_args[1:]
+    bias_args = (None, None, None, 0)
+    if bias is not None:
+        entries = bias.tokens.shape[0]
+        if bias.values.dtype != torch.float32 or tuple(bias.values.shape) != (entries,) or not bias.values.is_contiguous():
+            raise ValueError(f"bias values must be contiguous fp32 [{entries}]")
+        if bias.values.device != device:
+            raise RuntimeError(f"bias values are on {bias.values.device}, the logits on {device}")
+        bias_args = (_int32_or_none(bias.start, (rows + 1,), "bias start", device),
+                     _int32_or_none(bias.tokens, (entries,), "bias tokens", device), bias.values.data_ptr(), entries)
+        if entries == 0:
+            bias_args = (None, None, None, 0)
+    allowed_args = (None, 0, 0, None)
+    if allowed is not None:
+        masks, words = allowed.shape[0], allowed_words(vocab)
+        _check(masks > 0 or rows == 0, "no masks")
+        allowed_args = (_int32_or_none(allowed, (masks, words), "allowed", device), words, masks,
+                        _int32_or_none(allowed_rows, (rows,), "allowed_rows", device))
+    _call_on(device, "ne_adjust_logits", logits.data_ptr(), code, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+             *history_args, *bias_args, *allowed_args, out.data_ptr(), dtype_code(out.dtype),
+             out.stride(0) if rows > 1 else vocab, _stream(device))
+    return out
 
 
 # ---------------------------------------------------------------------- sampling

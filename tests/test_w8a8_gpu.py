@@ -1,0 +1,312 @@
+"""Rows quantised to int8 and W8A8 products against their definitions in 64 bits.
+
+Codes and scales have to be equal.  A product's sum is exact; its fp32 value (one rounding), the two
+scale factors (one each) and the rounding to bf16 give |y - y64| <= (2^-8 + 3 * 2^-24 * (1 + 2^-8)) |y64|,
+taken as 2^-8 + 2^-22.  SwiGLU: gate g and up u are off by 3 * 2^-24 relative; silu(g) changes by
+(1 + |g|) times g's relative error, exp's argument is rounded once (|g| 2^-24) and exp, the sum, the
+quotient and the product add at most 2^-21: for |g| <= 60 at most 61 * 3 * 2^-24 + 60 * 2^-24 + 2^-21 +
+3 * 2^-24 < 2^-15 relative, next to bf16's 2^-8.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from nanoengine_amd import _native, kernels
+from nanoengine_amd._native import EPILOGUE_STORE, EPILOGUE_SWIGLU
+
+STORE_REL = 2.0**-8 + 2.0**-22
+SWIGLU_REL = 2.0**-8 + 2.0**-15
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def rows_reference(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales): the fp32 quotients correctly rounded, through 64 bits."""
+    top = x.double().abs().amax(1).clamp(min=float(torch.tensor(1e-8)))
+    scales = (top / 127).float()
+    codes = (x.double() / scales.double()[:, None]).float().round().clamp(-127, 127)
+    bad = ~torch.isfinite(x.float()).all(1)
+    return codes.nan_to_num(0.0, 0.0, 0.0).masked_fill(bad[:, None], 0).to(torch.int8), scales.masked_fill(bad, float("nan"))
+
+
+def check_rows(got, x) -> None:
+    codes, scales = rows_reference(x)
+    assert torch.equal(got[0], codes)
+    assert torch.equal(got[1].nan_to_num(-1.0), scales.nan_to_num(-1.0))
+
+
+def make(m, n, k, seed=0, scale="bf16"):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(-127, 128, (m, k), device="cuda", generator=g, dtype=torch.int32).to(torch.int8)
+    w = torch.randint(-127, 128, (n, k), device="cuda", generator=g, dtype=torch.int32).to(torch.int8)
+    scales = 0.01 + 0.02 * torch.rand(m, device="cuda", generator=g)
+    w_scale = ((0.5 + torch.rand(n, device="cuda", generator=g)) / (73 * k**0.5)).to(DTYPES[scale])
+    return codes, scales, w, w_scale
+
+
+def product(codes, scales, w, w_scale) -> torch.Tensor:
+    y = codes.double() @ w.double().t().contiguous()
+    return y * scales.double()[:, None] * w_scale.double()
+
+
+def swiglu(y: torch.Tensor) -> torch.Tensor:
+    gate, up = y.view(y.shape[0], -1, 2, 16).unbind(2)
+    assert float(gate.abs().max()) <= 60
+    return (gate * torch.sigmoid(gate) * up).reshape(y.shape[0], -1)
+
+
+def check_product(got, codes, scales, w, w_scale, epilogue=EPILOGUE_STORE) -> None:
+    want = product(codes, scales, w, w_scale)
+    rel = STORE_REL
+    if epilogue == EPILOGUE_SWIGLU:
+        want, rel = swiglu(want), SWIGLU_REL
+    assert got.dtype == torch.bfloat16 and got.shape == want.shape
+    off = (got.double() - want).abs() - rel * want.abs()
+    assert float(off.max()) <= 1e-38
+
+
+# ------------------------------------------------------------------------- rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,k", [(1, 8), (3, 16), (5, 504), (4, 512), (7, 520), (9, 1024), (2, 2040), (6, 4096),
+                                    (3, 4104), (2, 8192), (3, 16376), (2, 16392), (1, 131056), (1025, 128)])
+def test_quantize_rows(rows, k, dtype):
+    g = torch.Generator(device="cuda").manual_seed(rows * k)
+    x = torch.randn(rows, k, device="cuda", generator=g) * (0.01 + 50 * torch.rand(rows, 1, device="cuda", generator=g))
+    x = x.to(DTYPES[dtype])
+    check_rows(kernels.quantize_rows(x), x)
+
+
+@pytest.mark.gpu
+def test_quantize_rows_ties_zeros_and_extremes():
+    k = 256
+    x = torch.zeros(7, k, device="cuda", dtype=torch.bfloat16)
+    x[1, :] = torch.arange(k, device="cuda") * 0.5 - 63.5  # scale 0.5: quotients on and next to halves
+    x[1, 0] = 63.5
+    x[2, 3] = 1e-38  # far below the least scale
+    x[3, 7] = torch.finfo(torch.bfloat16).max
+    x[4, :] = -2.0**-126
+    x[5, 11] = 127.0
+    x[5, 12], x[5, 13], x[5, 14] = 0.5, 1.5, -2.5  # scale 1: ties to even
+    x[6] = torch.randn(k, device="cuda")
+    got = kernels.quantize_rows(x)
+    check_rows(got, x)
+    assert got[0][5, 12:15].tolist() == [0, 2, -2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("k", [64, 5000, 20000])
+def test_rows_that_are_not_finite(k, value):
+    x = torch.randn(3, k, device="cuda").bfloat16()
+    x[1, k - 1] = value
+    codes, scales = kernels.quantize_rows(x)
+    check_rows((codes, scales), x)
+    part = codes[:, : k // 16 * 16].contiguous()  # (products take a k of whole 16s)
+    y = kernels.w8a8_gemm(part, scales, torch.ones_like(part[:1]).expand(16, -1).contiguous(), torch.ones(16, device="cuda"))
+    assert y[1].isnan().all() and not y[0].isnan().any() and not y[2].isnan().any()
+
+
+@pytest.mark.gpu
+def test_quantize_rows_of_a_strided_view_into_given_outputs():
+    big = torch.randn(9, 1024 + 64, device="cuda").bfloat16()
+    x = big[:, 64:]
+    codes = torch.full((11, 1024), 99, device="cuda", dtype=torch.int8)
+    scales = torch.full((11,), 99.0, device="cuda")
+    got = kernels.quantize_rows(x, codes=codes[1:10], scales=scales[1:10])
+    check_rows(got, x)
+    assert (codes[0] == 99).all() and (codes[10] == 99).all() and scales[0] == 99 and scales[10] == 99
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,hidden", [(1, 8), (5, 512), (3, 1024), (66, 1032), (7, 2048), (4, 4096)])
+def test_norm_rows_are_the_norms_bits(rows, hidden):
+    g = torch.Generator(device="cuda").manual_seed(hidden)
+    x = (3 * torch.randn(rows, hidden, device="cuda", generator=g)).bfloat16()
+    delta = torch.randn(rows, hidden, device="cuda", generator=g).bfloat16()
+    weight = (0.5 + torch.rand(hidden, device="cuda", generator=g)).bfloat16()
+    check_rows(kernels.rmsnorm_quantize(x, weight, 1e-6), kernels.rmsnorm(x, weight, 1e-6))
+    one, two = x.clone(), x.clone()
+    got = kernels.add_rmsnorm_quantize(one, delta, weight, 1e-6)
+    check_rows(got, kernels.add_rmsnorm(two, delta, weight, 1e-6))
+    assert torch.equal(one, two)
+    # and the norm's definition in 64 bits: two roundings to bf16 and half a step of the codes
+    h = one.double()
+    want = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-6) * weight.double()
+    s = got[1].double()[:, None]
+    assert ((got[0].double() * s - want).abs() <= s * 0.5001 + want.abs() * (2 * 2.0**-8 + 2.0**-15)).all()
+
+
+# ----------------------------------------------------------------------- products
+SHAPES = [
+    (1, 1, 16), (1, 15, 32), (1, 17, 48), (2, 4096, 1024), (15, 130, 112), (16, 541, 128), (17, 64, 1040), (33, 100, 2048),
+    (64, 1024, 2048), (48, 33, 4112), (65, 64, 16), (65, 127, 80), (100, 541, 608), (127, 129, 64), (128, 128, 192),
+    (200, 1000, 144), (129, 32003, 64), (64, 40000, 96), (3, 70000, 272), (300, 8192, 1024), (1000, 2048, 336), (2049, 4100, 80),
+    (1111, 9001, 1024), (4096, 2304, 208),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_product(m, n, k):
+    data = make(m, n, k, seed=m + n + k, scale=["bf16", "fp16", "fp32"][(m + n) % 3])
+    check_product(kernels.w8a8_gemm(*data), *data)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 32, 16), (1, 6144, 1024), (16, 96, 144), (31, 64, 1024), (64, 512, 272), (65, 32, 48),
+                                   (150, 320, 64), (333, 6144, 1024), (700, 4096, 176), (2100, 5152, 336)])
+def test_swiglu_product(m, n, k):
+    data = make(m, n, k, seed=m + n + k)
+    check_product(kernels.w8a8_gemm(*data, epilogue=EPILOGUE_SWIGLU), *data, epilogue=EPILOGUE_SWIGLU)
+
+
+def test_every_kernel_serves_some_shape():
+    if not _native.library_path().exists():
+        pytest.skip("libnanoengine_hip.so is not built")
+    lib = _native.load()
+    assert {lib.ne_w8a8_kernel(m, n, k, EPILOGUE_STORE) for m, n, k in SHAPES} == {0, 1, 2, 3}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(5, 100, 64), (70, 250, 160), (300, 4096, 128), (2200, 4096, 64)])
+@pytest.mark.parametrize("pad", [0, 1, 8])
+def test_product_strides_and_what_lies_beside_it(m, n, k, pad):
+    codes, scales, w, w_scale = make(m, n, k, seed=pad)
+    wide_codes = torch.full((m, k + 32), -128, device="cuda", dtype=torch.int8)
+    wide_codes[:, 16 : 16 + k] = codes
+    buffer = torch.full((m + 2, n + pad), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = buffer[1 : m + 1, :n]
+    got = kernels.w8a8_gemm(wide_codes[:, 16 : 16 + k], scales, w, w_scale, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    check_product(got, codes, scales, w, w_scale)
+    assert (buffer[0] == 7).all() and (buffer[m + 1] == 7).all() and (buffer[:, n:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 70])
+def test_longest_sum_of_the_largest_codes(m):
+    k, n = 131056, 32
+    codes = torch.full((m, k), -128, device="cuda", dtype=torch.int8)
+    w = torch.full((n, k), -128, device="cuda", dtype=torch.int8)
+    w[1] = 127
+    ones = torch.ones(m, device="cuda"), torch.ones(n, device="cuda")
+    check_product(kernels.w8a8_gemm(codes, ones[0], w, ones[1]), codes, ones[0], w, ones[1])
+
+
+@pytest.mark.gpu
+def test_a_row_has_the_same_bits_in_every_batch():
+    codes, scales, w, w_scale = make(2500, 4096, 1040)
+    want = kernels.w8a8_gemm(codes, scales, w, w_scale)
+    for m in (1, 16, 40, 64, 65, 300, 1000):
+        assert torch.equal(kernels.w8a8_gemm(codes[:m], scales[:m], w, w_scale), want[:m])
+    part = kernels.w8a8_gemm(codes[:300], scales[:300], w[:100], w_scale[:100])
+    assert torch.equal(part, want[:300, :100])
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    codes, scales, w, w_scale = make(4, 64, 64)
+    assert kernels.w8a8_gemm(codes[:0], scales[:0], w, w_scale).shape == (0, 64)
+    x = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16)
+    assert kernels.quantize_rows(x)[0].shape == (0, 64)
+    assert kernels.rmsnorm_quantize(x, torch.ones(64, device="cuda", dtype=torch.bfloat16), 1e-6)[1].shape == (0,)
+
+
+@pytest.mark.gpu
+def test_captured_chain_follows_its_inputs_on_another_stream():
+    """Norm, rows and product captured once and replayed on new rows, eager work in between."""
+    m, n, k = 130, 768, 512
+    _, _, w, w_scale = make(m, n, k)
+    weight = torch.rand(k, device="cuda").bfloat16()
+    x = torch.randn(m, k, device="cuda").bfloat16()
+    codes, scales = torch.empty(m, k, device="cuda", dtype=torch.int8), torch.empty(m, device="cuda")
+    out = torch.empty(m, n, device="cuda", dtype=torch.bfloat16)
+
+    def chain():
+        kernels.rmsnorm_quantize(x, weight, 1e-6, codes=codes, scales=scales)
+        kernels.w8a8_gemm(codes, scales, w, w_scale, out=out)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        chain()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain()
+    for seed in range(4):
+        x.copy_(torch.randn(m, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)))
+        graph.replay()
+        replayed = out.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            chain()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, out)
+        check_product(out, codes, scales, w, w_scale)
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_what_the_kernels_do_not_take():
+    codes, scales, w, w_scale = make(4, 64, 64)
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        kernels.w8a8_gemm(codes[:, :48], scales, w, w_scale)
+    with pytest.raises(ValueError):
+        kernels.w8a8_gemm(codes, scales[:3], w, w_scale)
+    with pytest.raises(ValueError):
+        kernels.w8a8_gemm(codes, scales.double(), w, w_scale)
+    with pytest.raises(ValueError):
+        kernels.w8a8_gemm(codes, scales, w, w_scale[:10])
+    with pytest.raises(ValueError):
+        kernels.w8a8_gemm(codes, scales, w, w_scale, out=torch.empty(4, 63, **bf))
+    with pytest.raises(RuntimeError):
+        kernels.w8a8_gemm(codes.cpu(), scales, w, w_scale)
+    with pytest.raises(_native.NativeError):  # k off 16
+        kernels.w8a8_gemm(codes[:, :40].contiguous(), scales, w[:, :40].contiguous(), w_scale)
+    with pytest.raises(_native.NativeError):  # codes off 16 bytes
+        kernels.w8a8_gemm(codes[:, 8:56], scales, w[:, :48].contiguous(), w_scale)
+    with pytest.raises(_native.NativeError):
+        kernels.w8a8_gemm(codes, scales, w[:48].contiguous(), w_scale[:48], epilogue=EPILOGUE_SWIGLU)
+    with pytest.raises(ValueError):
+        kernels.quantize_rows(torch.ones(4, 64, device="cuda"))
+    with pytest.raises(_native.NativeError):
+        kernels.quantize_rows(torch.ones(4, 60, **bf))
+    with pytest.raises(_native.NativeError):
+        kernels.quantize_rows(torch.ones(4, 72, **bf)[:, 4:68])
+    with pytest.raises(ValueError):
+        kernels.quantize_rows(torch.ones(4, 64, **bf), codes=torch.empty(4, 64, device="cuda"))
+    with pytest.raises(ValueError):
+        kernels.rmsnorm_quantize(torch.ones(4, 64, **bf), torch.ones(32, **bf), 1e-6)
+    with pytest.raises(_native.NativeError):
+        kernels.rmsnorm_quantize(torch.ones(4, 4104, **bf), torch.ones(4104, **bf), 1e-6)
+
+
+def test_entry_points_refuse_bad_arguments_without_launching():
+    if not _native.library_path().exists():
+        pytest.skip("libnanoengine_hip.so is not built")
+    lib = _native.load()
+    p, odd, null = ctypes.c_void_p(256), ctypes.c_void_p(264), ctypes.c_void_p(0)
+
+    def gemm(x=p, ldx=64, xs=p, w=p, ws=p, dt=0, m=4, n=64, k=64, y=p, ldy=64, epilogue=0):
+        return lib.ne_w8a8_gemm(x, ldx, xs, w, ws, dt, m, n, k, y, ldy, epilogue, null)
+
+    assert gemm(m=0, x=null) == 0
+    for bad in (dict(m=-1), dict(n=0), dict(k=0), dict(epilogue=7), dict(dt=3), dict(x=null), dict(xs=null), dict(ws=null),
+                dict(y=null), dict(x=odd), dict(w=odd), dict(ldx=48), dict(ldx=72), dict(ldx=1 << 23), dict(ldy=63)):
+        assert gemm(**bad) == -1, bad
+    for bad in (dict(k=72, ldx=80), dict(k=131072, ldx=131072), dict(epilogue=1, n=48)):
+        assert gemm(**bad) == -2, bad
+    assert lib.ne_quantize_rows(p, 0, 64, 0, 64, null, null, null) == 0
+    assert lib.ne_quantize_rows(p, 2, 64, 4, 64, p, p, null) == -1
+    assert lib.ne_quantize_rows(p, 0, 60, 4, 64, p, p, null) == -1
+    assert lib.ne_quantize_rows(odd, 0, 64, 4, 64, p, p, null) == -1
+    assert lib.ne_quantize_rows(p, 0, 64, 4, 60, p, p, null) == -2
+    assert lib.ne_quantize_rows(null, 0, 64, 4, 64, p, p, null) == -1
+    assert lib.ne_rmsnorm_quantize(p, null, p, p, 4, 64, 1e-6, null) == -1
+    assert lib.ne_rmsnorm_quantize(p, p, p, p, 4, 4104, 1e-6, null) == -2
+    assert lib.ne_add_rmsnorm_quantize(p, odd, p, p, p, 4, 64, 1e-6, null) == -1
