@@ -733,15 +733,26 @@ def w8a16_gemm(
 
 
 # ------------------------------------------------------------------------- W8A8
-def _code_outputs(rows: int, k: int, codes, scales, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+def _launch(index: int, name: str, *args) -> None:
+    """An entry point on device ``index``'s current torch stream (the last argument), that device current."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        _native.call(name, *args, stream)
+    else:
+        with torch.cuda.device(index):
+            _native.call(name, *args, stream)
+
+
+def _code_outputs(x: torch.Tensor, codes, scales) -> tuple[torch.Tensor, torch.Tensor]:
+    rows, k = x.shape
     if codes is None:
-        codes = torch.empty((rows, k), dtype=torch.int8, device=device)
-    elif codes.dtype != torch.int8 or tuple(codes.shape) != (rows, k) or not codes.is_contiguous() or codes.device != device:
-        raise ValueError(f"codes must be contiguous int8 [{rows}, {k}] on {device}")
+        codes = x.new_empty((rows, k), dtype=torch.int8)
+    elif codes.dtype != torch.int8 or codes.shape != x.shape or not codes.is_contiguous() or codes.device != x.device:
+        raise ValueError(f"codes must be contiguous int8 [{rows}, {k}] on {x.device}")
     if scales is None:
-        scales = torch.empty((rows,), dtype=torch.float32, device=device)
-    elif scales.dtype != torch.float32 or tuple(scales.shape) != (rows,) or not scales.is_contiguous() or scales.device != device:
-        raise ValueError(f"scales must be contiguous fp32 [{rows}] on {device}")
+        scales = x.new_empty((rows,), dtype=torch.float32)
+    elif scales.dtype != torch.float32 or scales.shape != (rows,) or not scales.is_contiguous() or scales.device != x.device:
+        raise ValueError(f"scales must be contiguous fp32 [{rows}] on {x.device}")
     return codes, scales
 
 
@@ -750,32 +761,34 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None,
     """int8 codes ``[m, k]`` of the rows of ``x [m, k]`` (bf16 or fp16) and fp32 scales ``[m]``: the
     formula of :func:`~nanoengine_amd.int8_quantization.quantize_vectors` per row, for
     :func:`w8a8_gemm`.  A row with a NaN or an infinity gets the scale NaN and codes 0."""
-    device = _require_gpu(x)
-    _check(x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1), "x must be [m, k] with contiguous rows")
-    _check(x.dtype in (torch.bfloat16, torch.float16), "x must be bf16 or fp16")
+    if not x.is_cuda:
+        _require_gpu(x)
+    if x.dim() != 2 or x.stride(1) != 1 and x.shape[1] != 1:
+        raise ValueError("x must be [m, k] with contiguous rows")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("x must be bf16 or fp16")
     rows, k = x.shape
-    codes, scales = _code_outputs(rows, k, codes, scales, device)
-    _call_on(device, "ne_quantize_rows", x.data_ptr(), dtype_code(x.dtype), x.stride(0) if rows > 1 else k, rows, k,
-             codes.data_ptr(), scales.data_ptr(), _stream(device))
+    codes, scales = _code_outputs(x, codes, scales)
+    _launch(x.get_device(), "ne_quantize_rows", x.data_ptr(), _DTYPE_CODES[x.dtype], x.stride(0) if rows > 1 else k, rows, k,
+            codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
-def _check_norm_rows(weight: torch.Tensor, *rows: torch.Tensor) -> None:
-    hidden = weight.shape[0] if weight.dim() == 1 else -1
-    for t in rows:
-        _check(t.dim() == 2 and t.shape[1] == hidden and t.dtype == torch.bfloat16 and t.is_contiguous()
-               and t.shape == rows[0].shape, "rows must be contiguous [rows, hidden] bf16, the weight [hidden]")
-    _check(weight.dtype == torch.bfloat16 and weight.is_contiguous(), "weight must be contiguous bf16")
+def _check_norm_rows(weight: torch.Tensor, rows: torch.Tensor) -> None:
+    if rows.get_device() != weight.get_device() or not rows.is_cuda:
+        _require_gpu(rows, weight)
+    if (rows.dim() != 2 or weight.shape != rows.shape[1:] or rows.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16
+            or not rows.is_contiguous() or not weight.is_contiguous()):
+        raise ValueError("rows must be contiguous [rows, hidden] bf16, the weight [hidden]")
 
 
 def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: torch.Tensor | None = None,
                      scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """:func:`quantize_rows` of :func:`rmsnorm`'s rows (the same bits), in one pass; hidden at most 4,096."""
-    device = _require_gpu(x, weight)
     _check_norm_rows(weight, x)
-    codes, scales = _code_outputs(*x.shape, codes, scales, device)
-    _call_on(device, "ne_rmsnorm_quantize", x.data_ptr(), weight.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-             *x.shape, eps, _stream(device))
+    codes, scales = _code_outputs(x, codes, scales)
+    _launch(x.get_device(), "ne_rmsnorm_quantize", x.data_ptr(), weight.data_ptr(), codes.data_ptr(), scales.data_ptr(), *x.shape,
+            eps)
     return codes, scales
 
 
@@ -784,11 +797,12 @@ def add_rmsnorm_quantize(residual: torch.Tensor, delta: torch.Tensor, weight: to
                          scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``residual += delta`` (bf16) in place, then :func:`quantize_rows` of its RMSNorm:
     :func:`add_rmsnorm` with the same bits and its rows as codes."""
-    device = _require_gpu(residual, delta, weight)
-    _check_norm_rows(weight, residual, delta)
-    codes, scales = _code_outputs(*residual.shape, codes, scales, device)
-    _call_on(device, "ne_add_rmsnorm_quantize", residual.data_ptr(), delta.data_ptr(), weight.data_ptr(), codes.data_ptr(),
-             scales.data_ptr(), *residual.shape, eps, _stream(device))
+    _check_norm_rows(weight, residual)
+    _check_norm_rows(weight, delta)
+    _check(residual.shape == delta.shape, "residual and delta must be of one shape")
+    codes, scales = _code_outputs(residual, codes, scales)
+    _launch(residual.get_device(), "ne_add_rmsnorm_quantize", residual.data_ptr(), delta.data_ptr(), weight.data_ptr(),
+            codes.data_ptr(), scales.data_ptr(), *residual.shape, eps)
     return codes, scales
 
 
@@ -803,25 +817,30 @@ def w8a8_gemm(
     """``bf16((codes @ int8.T) * scales[:, None] * weight_scale)`` with an exact integer sum, on the
     weights of :func:`w8a16_gemm`; SwiGLU epilogue pairs 16 gate rows with 16 up rows.  ``k`` is a
     multiple of 16, at most 131,056; ``n`` is any number (SwiGLU: a multiple of 32)."""
-    device = _require_gpu(codes, scales, weight_int8, weight_scale)
-    _check(codes.dtype == torch.int8 and codes.dim() == 2 and codes.stride(1) == 1, "codes must be [m, k] int8")
-    _check(weight_int8.dtype == torch.int8 and weight_int8.dim() == 2 and weight_int8.is_contiguous(),
-           "weight must be contiguous [n, k] int8")
+    index = codes.get_device()
+    if (not codes.is_cuda or scales.get_device() != index or weight_int8.get_device() != index
+            or weight_scale.get_device() != index):
+        _require_gpu(codes, scales, weight_int8, weight_scale)  # names the devices
+    if codes.dtype != torch.int8 or codes.dim() != 2 or codes.stride(1) != 1:
+        raise ValueError("codes must be [m, k] int8 with contiguous rows")
+    if weight_int8.dtype != torch.int8 or weight_int8.dim() != 2 or not weight_int8.is_contiguous():
+        raise ValueError("weight must be contiguous [n, k] int8")
     m, k = codes.shape
-    n = weight_int8.shape[0]
-    if weight_int8.shape[1] != k:
-        raise ValueError(f"k mismatch: codes have {k}, weight {weight_int8.shape[1]}")
-    _check(scales.dtype == torch.float32 and scales.numel() == m and scales.is_contiguous(), "one contiguous fp32 scale per row")
-    _check(weight_scale.numel() == n and weight_scale.is_contiguous(), "one contiguous scale per weight row")
+    n, k_weight = weight_int8.shape
+    if k != k_weight:
+        raise ValueError(f"k mismatch: codes have {k}, weight {k_weight}")
+    if scales.dtype != torch.float32 or scales.numel() != m or not scales.is_contiguous():
+        raise ValueError("scales must be contiguous fp32, one per row")
+    if weight_scale.numel() != n or not weight_scale.is_contiguous():
+        raise ValueError("weight_scale must be contiguous, one per weight row")
     n_out = n // 2 if epilogue == EPILOGUE_SWIGLU else n
     if out is None:
-        out = torch.empty((m, n_out), dtype=torch.bfloat16, device=device)
-    else:
-        _check(out.shape == (m, n_out) and out.dtype == torch.bfloat16 and (out.stride(1) == 1 or n_out == 1)
-               and out.device == device, "bad out")
-    _call_on(device, "ne_w8a8_gemm", codes.data_ptr(), codes.stride(0) if m > 1 else k, scales.data_ptr(),
-             weight_int8.data_ptr(), weight_scale.data_ptr(), dtype_code(weight_scale.dtype), m, n, k, out.data_ptr(),
-             out.stride(0) if m > 1 else n_out, epilogue, _stream(device))
+        out = codes.new_empty((m, n_out), dtype=torch.bfloat16)
+    elif out.shape != (m, n_out) or out.dtype != torch.bfloat16 or out.stride(1) != 1 and n_out > 1 or out.get_device() != index:
+        raise ValueError(f"out must be bf16 [{m}, {n_out}] with contiguous rows on cuda:{index}")
+    _launch(index, "ne_w8a8_gemm", codes.data_ptr(), codes.stride(0) if m > 1 else k, scales.data_ptr(), weight_int8.data_ptr(),
+            weight_scale.data_ptr(), dtype_code(weight_scale.dtype), m, n, k, out.data_ptr(), out.stride(0) if m > 1 else n_out,
+            epilogue)
     return out
 
 
@@ -1212,15 +1231,66 @@ def allowed_mask(rows: list[list[int] | None], vocab: int, device: torch.device)
     return torch.from_numpy(words).to(device)
 
 
-def _int32_or_none(tensor: torch.Tensor | None, shape: tuple, name: str, device: torch.device):
-    """The device pointer (or None) of an optional contiguous int32 argument of a given shape."""
+def _int32_pointer(tensor: torch.Tensor | None, shape: tuple, name: str, index: int) -> int | None:
+    """The address (None for None) of a contiguous int32 argument of a given shape on device ``index``."""
     if tensor is None:
         return None
-    if tensor.dtype != torch.int32 or tuple(tensor.shape) != shape or not tensor.is_contiguous():
+    if tensor.dtype != torch.int32 or tensor.shape != shape or not tensor.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {tensor.dtype} {list(tensor.shape)}")
-    if tensor.device != device:
-        raise RuntimeError(f"{name} is on {tensor.device}, the logits on {device}")
+    if tensor.get_device() != index:
+        raise RuntimeError(f"{name} is on {tensor.device}, the logits on cuda:{index}")
     return tensor.data_ptr()
+
+
+def _row_values(value, rows: int, name: str, index: int) -> tuple:
+    """(address or None, scalar) of a penalty: one value, or an fp32 one per row."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.dtype != torch.float32 or value.shape != (rows,) or not value.is_contiguous():
+        raise ValueError(f"{name} must be one value or contiguous fp32 [{rows}]")
+    if value.get_device() != index:
+        raise RuntimeError(f"{name} is on {value.device}, the logits on cuda:{index}")
+    return value.data_ptr(), 0.0
+
+
+_NO_PENALTIES = (None, 0, 0, None, None, 0, None, 0, None, None, None, 1.0, None, 0.0, None, 0.0)
+
+
+def _penalty_arguments(p: TokenPenalties, rows: int, index: int) -> tuple:
+    h, drafts = p.history, p.drafts
+    if h.dtype != torch.int32 or h.dim() != 2 or h.stride(1) != 1 and h.shape[1] > 1:
+        raise ValueError("history must be [seqs, capacity] int32 with contiguous rows")
+    if h.get_device() != index:
+        raise RuntimeError(f"history is on {h.device}, the logits on cuda:{index}")
+    seqs, capacity = h.shape
+    if seqs == 0:  # whose row_seq could name no sequence
+        _check(rows == 0 or p.row_seq is not None, "no sequences")
+        return _NO_PENALTIES
+    per_seq, per_row = (seqs,), (rows,)
+    length = _int32_pointer(p.history_len, per_seq, "history_len", index)
+    max_drafts = 0
+    if drafts is not None:
+        max_drafts = drafts.shape[-1] if drafts.dim() else 0
+        _check(p.row_drafts is not None, "drafts need row_drafts")
+    return (
+        # (an empty tensor has no address, and its rows' guesses may still count)
+        h.data_ptr() if capacity else length, h.stride(0) if seqs > 1 else capacity, capacity, length,
+        _int32_pointer(p.prompt_len, per_seq, "prompt_len", index), seqs,
+        _int32_pointer(drafts, (seqs, max_drafts), "drafts", index), max_drafts,
+        _int32_pointer(p.row_seq, per_row, "row_seq", index), _int32_pointer(p.row_drafts, per_row, "row_drafts", index),
+        *_row_values(p.repetition, rows, "repetition", index), *_row_values(p.presence, rows, "presence", index),
+        *_row_values(p.frequency, rows, "frequency", index))
+
+
+def _bias_arguments(bias: TokenBias, rows: int, index: int) -> tuple:
+    entries = bias.tokens.shape[0]
+    if bias.values.dtype != torch.float32 or bias.values.shape != (entries,) or not bias.values.is_contiguous():
+        raise ValueError(f"bias values must be contiguous fp32 [{entries}]")
+    if bias.values.get_device() != index:
+        raise RuntimeError(f"bias values are on {bias.values.device}, the logits on cuda:{index}")
+    start = _int32_pointer(bias.start, (rows + 1,), "bias start", index)
+    tokens = _int32_pointer(bias.tokens, (entries,), "bias tokens", index)
+    return (start, tokens, bias.values.data_ptr(), entries) if entries else (None, None, None, 0)
 
 
 def adjust_logits(
@@ -1239,63 +1309,32 @@ def adjust_logits(
     becomes -inf, whatever its logit was.  ``allowed_rows [rows]`` int32 names each row's mask (default:
     its own index; negative: no mask, one past the masks: no token).  Tokens outside the vocabulary
     count nowhere."""
-    device = _require_gpu(logits)
-    _check(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits must be [rows, vocab] with contiguous rows")
-    code = dtype_code(logits.dtype)
-    _check(code != DTYPE_INT8, "logits must be bf16, fp16 or fp32")
+    if not logits.is_cuda:
+        _require_gpu(logits)
+    index, dtype = logits.get_device(), logits.dtype
+    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] != 1:
+        raise ValueError("logits must be [rows, vocab] with contiguous rows")
+    code = dtype_code(dtype)
+    if code == DTYPE_INT8:
+        raise ValueError("logits must be bf16, fp16 or fp32")
     rows, vocab = logits.shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+        out = torch.empty((rows, vocab), dtype=dtype, device=logits.device)
     elif out is not logits:
-        if (out.dtype != logits.dtype and out.dtype != torch.float32 or out.shape != logits.shape or out.device != device
-                or (out.stride(1) != 1 and vocab > 1)):
-            raise ValueError(f"out must be {logits.dtype} or fp32 [{rows}, {vocab}] on {device}")
-    history_args = (None, 0, 0, None, None, 0, None, 0, None, None, None, 1.0, None, 0.0, None, 0.0)
-    if penalties is not None:
-        h = penalties.history
-        _check(h.dtype == torch.int32 and h.dim() == 2 and (h.stride(1) == 1 or h.shape[1] <= 1),
-               "history must be [seqs, capacity] int32 with contiguous rows")
-        if h.device != device:
-            raise RuntimeError(f"history is on {h.device}, the logits on {device}")
-        seqs, capacity = h.shape
-        per_seq, per_row = (seqs,), (rows,)
-        _check(penalties.history_len is not None, "history needs history_len")
-        max_drafts = 0
-        if penalties.drafts is not None:
-            max_drafts = penalties.drafts.shape[-1]
-            _check(penalties.row_drafts is not None, "drafts need row_drafts")
-        r_ptr, r = _row_parameter(penalties.repetition, rows, torch.float32, "repetition", device)
-        p_ptr, p = _row_parameter(penalties.presence, rows, torch.float32, "presence", device)
-        f_ptr, f = _row_parameter(penalties.frequency, rows, torch.float32, "frequency", device)
-        history_args = (
-            h.data_ptr(), h.stride(0) if seqs > 1 else capacity, capacity,
-            _int32_or_none(penalties.history_len, per_seq, "history_len", device),
-            _int32_or_none(penalties.prompt_len, per_seq, "prompt_len", device), seqs,
-            _int32_or_none(penalties.drafts, (seqs, max_drafts), "drafts", device), max_drafts,
-            _int32_or_none(penalties.row_seq, per_row, "row_seq", device),
-            _int32_or_none(penalties.row_drafts, per_row, "row_drafts", device), r_ptr, r, p_ptr, p, f_ptr, f)
-        if capacity == 0 and seqs > 0:  # an empty tensor has no address, and guesses may still count
-            history_args = (penalties.history_len.data_ptr(),) + history_args[1:]
-    bias_args = (None, None, None, 0)
-    if bias is not None:
-        entries = bias.tokens.shape[0]
-        if bias.values.dtype != torch.float32 or tuple(bias.values.shape) != (entries,) or not bias.values.is_contiguous():
-            raise ValueError(f"bias values must be contiguous fp32 [{entries}]")
-        if bias.values.device != device:
-            raise RuntimeError(f"bias values are on {bias.values.device}, the logits on {device}")
-        bias_args = (_int32_or_none(bias.start, (rows + 1,), "bias start", device),
-                     _int32_or_none(bias.tokens, (entries,), "bias tokens", device), bias.values.data_ptr(), entries)
-        if entries == 0:
-            bias_args = (None, None, None, 0)
-    allowed_args = (None, 0, 0, None)
+        if (out.dtype not in (dtype, torch.float32) or out.shape != logits.shape or out.get_device() != index
+                or out.stride(1) != 1 and vocab > 1):
+            raise ValueError(f"out must be {dtype} or fp32 [{rows}, {vocab}] with contiguous rows on cuda:{index}")
+    allowed_arguments = (None, 0, 0, None)
     if allowed is not None:
         masks, words = allowed.shape[0], allowed_words(vocab)
-        _check(masks > 0 or rows == 0, "no masks")
-        allowed_args = (_int32_or_none(allowed, (masks, words), "allowed", device), words, masks,
-                        _int32_or_none(allowed_rows, (rows,), "allowed_rows", device))
-    _call_on(device, "ne_adjust_logits", logits.data_ptr(), code, logits.stride(0) if rows > 1 else vocab, rows, vocab,
-             *history_args, *bias_args, *allowed_args, out.data_ptr(), dtype_code(out.dtype),
-             out.stride(0) if rows > 1 else vocab, _stream(device))
+        if masks == 0 and rows > 0:
+            raise ValueError("no masks")
+        allowed_arguments = (_int32_pointer(allowed, (masks, words), "allowed", index), words, masks,
+                             _int32_pointer(allowed_rows, (rows,), "allowed_rows", index))
+    _launch(index, "ne_adjust_logits", logits.data_ptr(), code, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+            *(_NO_PENALTIES if penalties is None else _penalty_arguments(penalties, rows, index)),
+            *((None, None, None, 0) if bias is None else _bias_arguments(bias, rows, index)), *allowed_arguments,
+            out.data_ptr(), _DTYPE_CODES[out.dtype], out.stride(0) if rows > 1 else vocab)
     return out
 
 
