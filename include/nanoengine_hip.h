@@ -578,6 +578,7 @@ int ne_add_rmsnorm_quantize(void* residual, const void* delta, const void* weigh
 #define NE_W8A8_TILE_64X128 1
 #define NE_W8A8_TILE_128X128 2
 #define NE_W8A8_TILE_256X256 3
+#define NE_W8A8_TILE_64X64 4
 int32_t ne_w8a8_kernel(int32_t m, int32_t n, int32_t k, int32_t epilogue);
 int ne_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
                  const void* w_scale, int32_t scale_dtype, int32_t m, int32_t n, int32_t k, void* y,

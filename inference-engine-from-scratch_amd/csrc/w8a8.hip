@@ -26,9 +26,6 @@ struct W8a8Params {
   int tiles_m, tiles_n;
 };
 
-// 16-byte source of the chunks past the end of k (a zero code adds nothing)
-__device__ const u32x4 zero_chunk = {0, 0, 0, 0};
-
 __device__ __forceinline__ void lds_dma16(const void* src, void* lds_wave_base) {
   __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
 }
@@ -52,6 +49,20 @@ __device__ __forceinline__ void wait_pending(int pend) {
       wait_vmcnt<D * P>();
     } else {
       wait_pending<D, P - 1>(pend);
+    }
+  }
+}
+
+// the same with S younger stores in flight
+template <int D, int P, int S>
+__device__ __forceinline__ void wait_pending_after(int pend) {
+  if constexpr (P <= 0) {
+    wait_vmcnt<S>();
+  } else {
+    if (pend >= P) {
+      wait_vmcnt<D * P + S>();
+    } else {
+      wait_pending_after<D, P - 1, S>(pend);
     }
   }
 }
@@ -112,206 +123,270 @@ __device__ __forceinline__ void store_columns(uint16_t* row, int col, int n_out,
 }
 
 // ---- many rows: tiles through LDS --------------------------------------------------
-//   stage = 64 KS k of BM rows and BN weight rows, copied by DMA (global_load_lds_dwordx4), the
-//           16-byte chunks of a row swizzled so that the fragment reads are free of bank conflicts
+//   stage = 128 k of BM rows and BN weight rows (whole 128-byte lines), copied by DMA
+//           (global_load_lds_dwordx4), the 16-byte chunks of a row swizzled so that the fragment
+//           reads are free of bank conflicts
 //   ring  = RING stages; a wave holds the next k-step's fragments while the MFMAs of the current
 //           one run, and the barrier that admits a stage sits between two batches of MFMAs
-template <int BM_, int BN_, int MW_, int NW_, int KS_, int RING_>
+//   tiles = a work-group walks several, its stages run on across them: the next tile's first
+//           stages are on their way while a tile is scaled, rounded and stored
+template <int BM_, int BN_, int MW_, int NW_, int RING_>
 struct TileLayout {
-  static constexpr int BM = BM_, BN = BN_, MW = MW_, NW = NW_, KS = KS_, RING = RING_;
+  static constexpr int BM = BM_, BN = BN_, MW = MW_, NW = NW_, RING = RING_;
   static constexpr int kWaves = MW * NW;
   static constexpr int PM = BM / MW / 16;   // token subtiles per wave
   static constexpr int NPW = BN / NW / 16;  // weight subtiles per wave
-  static constexpr int kRow = 64 * KS;      // bytes of a row in a stage
-  static constexpr int kStage = (BM + BN) * kRow;
+  static constexpr int kStage = (BM + BN) * 128;
   static constexpr int kCopies = kStage / 1024 / kWaves;  // per wave and stage
-  static constexpr int kXCopies = BM * kRow / 1024 / kWaves;
-  static constexpr int kLds = RING * kStage;
-  static_assert(KS == 1 || KS == 2, "k-steps per stage");
-  static_assert(BM * kRow % (1024 * kWaves) == 0 && BN * kRow % (1024 * kWaves) == 0, "copies split evenly over the waves");
-  static_assert(RING >= 2 && kCopies * (RING - 1) < 64 && kLds <= 160 * 1024, "ring");
+  static constexpr int kXCopies = BM / 8 / kWaves;
+  static constexpr int kScales = RING * kStage;  // LDS: the ring, then BM + BN scales
+  static constexpr int kEdge = kScales + (BM + BN) * 4;  // then 1 KiB per wave for tiles at an edge
+  static constexpr int kLds = kEdge + kWaves * 1024;
+  static constexpr int kPerCu = 160 * 1024 / kLds;  // work-groups
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "copies split evenly over the waves");
+  static_assert(BM + BN <= kWaves * kWave, "a scale per thread");
+  static_assert(RING >= 2 && kPerCu >= 1, "ring");
 };
 
 template <typename L, int EPI>
 __global__ __launch_bounds__(L::kWaves* kWave) void w8a8_tile_kernel(W8a8Params p) {
-  constexpr int PM = L::PM, NPW = L::NPW, KS = L::KS, RING = L::RING, D = L::kCopies;
-  constexpr int kChunks = L::kRow / 16;      // per row
-  constexpr int kCopyRows = 1024 / L::kRow;  // rows per copy
+  constexpr int PM = L::PM, NPW = L::NPW, RING = L::RING, D = L::kCopies;
+  constexpr int kOut = EPI == NE_EPILOGUE_SWIGLU ? NPW / 2 : NPW;
+  constexpr int kStores = PM * kOut / 2;  // of a wave's whole tile
+  static_assert(D * (RING - 1) + kStores < 64, "vmcnt range");
   __shared__ __attribute__((aligned(16))) char smem[L::kLds];
-  // Each XCD takes a contiguous eighth of the tiles, in an order that walks all weight
-  // tiles against groups of four row tiles: the group's rows stay in that XCD's L2.
-  const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
-  const int64_t per = (total + kNumXcd - 1) / kNumXcd;
-  const int64_t idx = (int64_t)(blockIdx.x % kNumXcd) * per + blockIdx.x / kNumXcd;
-  if (idx >= total) return;
-  constexpr int kGroup = 4;
-  const int grp = (int)(idx / ((int64_t)kGroup * p.tiles_n));
-  const int in_grp = (int)(idx - (int64_t)grp * kGroup * p.tiles_n);
-  const int rows_in = min(kGroup, p.tiles_m - grp * kGroup);
-  const int tn = in_grp / rows_in;
-  const int m0 = (grp * kGroup + in_grp - tn * rows_in) * L::BM;
-  const int n0 = tn * L::BN;
+  float* const scales = (float*)(smem + L::kScales);
+  // Each XCD takes a contiguous eighth of the tiles, in an order that walks all weight tiles
+  // against groups of four row tiles: the group's rows stay in that XCD's L2.  Its work-groups
+  // take them in turn.
+  const int total = p.tiles_m * p.tiles_n;
+  const int per = (total + kNumXcd - 1) / kNumXcd;
+  const int base = (int)(blockIdx.x % kNumXcd) * per;
+  const int here = max(min(per, total - base), 0);  // tiles of this XCD
+  const int first = blockIdx.x / kNumXcd, step = gridDim.x / kNumXcd;
+  if (first >= here) return;
+  const int my_tiles = (here - 1 - first) / step + 1;
+  auto place = [&](int i, int& m0, int& n0) {
+    const int idx = base + first + i * step;
+    constexpr int kGroup = 4;
+    const int grp = idx / (kGroup * p.tiles_n);
+    const int in_grp = idx - grp * kGroup * p.tiles_n;
+    const int rows_in = min(kGroup, p.tiles_m - grp * kGroup);
+    const int tn = in_grp / rows_in;
+    m0 = (grp * kGroup + in_grp - tn * rows_in) * L::BM;
+    n0 = tn * L::BN;
+  };
   const int lane = threadIdx.x % kWave;
   const int r = lane & 15;
   const int g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int mw = wave / L::NW, nw = wave % L::NW;
-  auto swizzle = [](int row) { return KS == 1 ? (row >> 1) & 3 : row & 7; };
+  const int n_stages = (p.k + 127) / 128;  // per tile
+  const int all = my_tiles * n_stages;
 
-  // Copy j of this wave is KiB j kWaves + wave of the stage: token rows, then weight rows.  Rows
-  // past m and n re-read the last one and are never stored.
-  const char* xbase = (const char*)p.x + (int64_t)m0 * p.ldx;
-  const char* wbase = (const char*)p.w + (int64_t)n0 * p.k;
-  uint32_t off[D];
-  auto chunk_of = [&](int j) {
-    const int row = (j * L::kWaves + wave) * kCopyRows + lane / kChunks - (j < L::kXCopies ? 0 : L::BM);
-    return (lane % kChunks) ^ swizzle(row);
-  };
-#pragma unroll
-  for (int j = 0; j < D; ++j) {
-    const int row = (j * L::kWaves + wave) * kCopyRows + lane / kChunks;
-    if (j < L::kXCopies) {
-      off[j] = (uint32_t)min(row, p.m - 1 - m0) * (uint32_t)p.ldx + (uint32_t)(chunk_of(j) * 16);
-    } else {
-      off[j] = (uint32_t)min(row - L::BM, p.n - 1 - n0) * (uint32_t)p.k + (uint32_t)(chunk_of(j) * 16);
+  // Copy j of this wave is KiB j kWaves + wave of the stage, eight rows: token rows, then weight
+  // rows.  LDS row `row` holds chunk c at position c ^ (row % 8), and row % 8 is lane / 8 in every
+  // copy.  Rows past m and n re-read the last one and are never stored; chunks past k re-read the
+  // last one, and the token rows' are then zeroed in LDS.
+  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;  // bytes
+  const uint32_t xrow = (uint32_t)(wave * 8 + (lane >> 3)) * (uint32_t)p.ldx;
+  const uint32_t wrow = (uint32_t)(wave * 8 + (lane >> 3)) * (uint32_t)p.k;
+  uint32_t xlast = 0, wlast = 0;  // of the last rows
+  const char *xbase = nullptr, *wbase = nullptr;
+  int next_tile = 0, next_stage = 0;  // of the copies
+  char* next_slot = smem;
+  int column = 0;
+  auto begin_copies = [&]() {
+    if (next_stage == 0) {
+      int m0, n0;
+      place(next_tile, m0, n0);
+      xbase = uniform_ptr((const char*)p.x + (int64_t)m0 * p.ldx);
+      wbase = uniform_ptr((const char*)p.w + (int64_t)n0 * p.k);
+      xlast = (uint32_t)(min(p.m - m0, L::BM) - 1) * (uint32_t)p.ldx;
+      wlast = (uint32_t)(min(p.n - n0, L::BN) - 1) * (uint32_t)p.k;
     }
-  }
-  const int n_stages = (p.k + L::kRow - 1) / L::kRow;
-  const int k_chunks = p.k / 16;
-  auto issue = [&](int t) {
-    char* slot = smem + (t % RING) * L::kStage;
-    const char* xs = uniform_ptr(xbase + (int64_t)t * L::kRow);
-    const char* ws = uniform_ptr(wbase + (int64_t)t * L::kRow);
-    if ((t + 1) * kChunks <= k_chunks) {
+    column = chunk - max(next_stage * 128 + chunk - (p.k - 16), 0);
+  };
+  auto copies = [&](int from, int to) {
 #pragma unroll
-      for (int j = 0; j < D; ++j) {
-        uint32_t o = off[j];
-        __asm__("" : "+v"(o));  // keep the lane offset 32-bit: scalar base + offset addressing
-        lds_dma16((j < L::kXCopies ? xs : ws) + o, slot + (j * L::kWaves + wave) * 1024);
-      }
-    } else {  // the last stage of a k off the stage's grid
-#pragma unroll
-      for (int j = 0; j < D; ++j) {
-        const char* src = (j < L::kXCopies ? xs : ws) + off[j];
-        if (t * kChunks + chunk_of(j) >= k_chunks) src = (const char*)&zero_chunk;
-        lds_dma16(src, slot + (j * L::kWaves + wave) * 1024);
-      }
+    for (int j = 0; j < D; ++j) {
+      if (j < from || j >= to) continue;
+      const uint32_t rows = (uint32_t)((j < L::kXCopies ? j : j - L::kXCopies) * L::kWaves * 8);
+      uint32_t o = (j < L::kXCopies ? min(xrow + rows * (uint32_t)p.ldx, xlast) : min(wrow + rows * (uint32_t)p.k, wlast)) + column;
+      __asm__("" : "+v"(o));  // keep the lane offset 32-bit: scalar base + offset addressing
+      lds_dma16((j < L::kXCopies ? xbase : wbase) + o, next_slot + (j * L::kWaves + wave) * 1024);
     }
   };
+  auto end_copies = [&]() {
+    xbase += 128;
+    wbase += 128;
+    next_slot = next_slot == smem + (RING - 1) * L::kStage ? smem : next_slot + L::kStage;
+    if (++next_stage == n_stages) {
+      next_stage = 0;
+      ++next_tile;
+    }
+  };
 
-  intx4 acc[PM][NPW];
-#pragma unroll
-  for (int mi = 0; mi < PM; ++mi)
-#pragma unroll
-    for (int ns = 0; ns < NPW; ++ns) acc[mi][ns] = intx4{0, 0, 0, 0};
+  auto issue = [&]() {
+    begin_copies();
+    copies(0, D);
+    end_copies();
+  };
+
   struct Frags {
     intx4 x[PM], w[NPW];
   };
-  // chunk 4 q + g of a row sits at position chunk ^ swizzle(row); rows 16 apart swizzle alike
-  auto read = [&](int t, int q, Frags& f) {
-    const char* slot = smem + (t % RING) * L::kStage + (((4 * q + g) ^ swizzle(r)) * 16 + r * L::kRow);
+  // chunk 4 q + g of a row sits at position chunk ^ (row % 8); rows 16 apart swizzle alike
+  auto read = [&](const char* slot, int q, Frags& f) {
+    const char* at = slot + (((4 * q + g) ^ (r & 7)) * 16 + r * 128);
 #pragma unroll
-    for (int ns = 0; ns < NPW; ++ns) f.w[ns] = *(const intx4*)(slot + (L::BM + (nw * NPW + ns) * 16) * L::kRow);
+    for (int ns = 0; ns < NPW; ++ns) f.w[ns] = *(const intx4*)(at + (L::BM + (nw * NPW + ns) * 16) * 128);
 #pragma unroll
-    for (int mi = 0; mi < PM; ++mi) f.x[mi] = *(const intx4*)(slot + (mw * PM + mi) * 16 * L::kRow);
+    for (int mi = 0; mi < PM; ++mi) f.x[mi] = *(const intx4*)(at + (mw * PM + mi) * 16 * 128);
   };
-  auto mma = [&](const Frags& f, int from, int to) {
+  // zeroes this wave's own copies of token chunks past k in a landed stage
+  auto clear_tail = [&](char* slot, int stage) {
+    if (stage * 128 + 128 > p.k && stage * 128 + chunk >= p.k) {
 #pragma unroll
-    for (int mi = 0; mi < PM; ++mi)
-      if (mi >= from && mi < to) {
-#pragma unroll
-        for (int ns = 0; ns < NPW; ++ns)
-          acc[mi][ns] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.w[ns], f.x[mi], acc[mi][ns], 0, 0, 0);
-      }
+      for (int j = 0; j < L::kXCopies; ++j) *(intx4*)(slot + (j * L::kWaves + wave) * 1024 + lane * 16) = intx4{0, 0, 0, 0};
+    }
   };
-  // stage t + 1 has landed and every wave has read all of stage t: its slot takes stage t + RING
-  auto advance = [&](int t) {
-    wait_pending<D, RING - 2>(min(n_stages - 1, t + RING - 1) - (t + 1));
-    wait_lgkmcnt0();
-    asm volatile("s_barrier" ::: "memory");
-    if (t + RING < n_stages) issue(t + RING);
+  intx4 acc[PM][NPW];
+  auto mma_row = [&](const Frags& f, int mi) {
+#pragma unroll
+    for (int ns = 0; ns < NPW; ++ns)
+      acc[mi][ns] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.w[ns], f.x[mi], acc[mi][ns], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto mma = [&](const Frags& f) {
+    __builtin_amdgcn_sched_barrier(0);  // the reads before it go out first
+#pragma unroll
+    for (int mi = 0; mi < PM; ++mi) mma_row(f, mi);
   };
 
-#pragma unroll
-  for (int s = 0; s < RING; ++s)
-    if (s < n_stages) issue(s);
-  wait_pending<D, RING - 1>(min(n_stages, RING) - 1);  // stage 0 has landed
+#pragma unroll 1
+  for (int s = 0; s < min(RING, all); ++s) issue();
+  wait_pending<D, RING - 1>(min(all, RING) - 1);  // stage 0 has landed
+  clear_tail(smem, 0);
+  wait_lgkmcnt0();
   asm volatile("s_barrier" ::: "memory");
 
   Frags a, b;
-  read(0, 0, a);
-  if constexpr (KS == 2) {
-    for (int t = 0; t + 1 < n_stages; ++t) {
-      read(t, 1, b);
-      __builtin_amdgcn_sched_barrier(0);  // the reads go out before the multiplies
-      mma(a, 0, PM);
-      __builtin_amdgcn_sched_barrier(0);
-      advance(t);
-      read(t + 1, 0, a);
-      __builtin_amdgcn_sched_barrier(0);
-      mma(b, 0, PM);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    read(n_stages - 1, 1, b);
-    mma(a, 0, PM);
-    mma(b, 0, PM);
-  } else {
-    auto step = [&](int t, Frags& cur, Frags& next) {
-      mma(cur, 0, PM / 2);
-      __builtin_amdgcn_sched_barrier(0);
-      advance(t);
-      read(t + 1, 0, next);
-      __builtin_amdgcn_sched_barrier(0);
-      mma(cur, PM / 2, PM);
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    int t = 0;
-    for (; t + 2 < n_stages; t += 2) {
-      step(t, a, b);
-      step(t + 1, b, a);
-    }
-    if (t + 1 < n_stages) {
-      step(t, a, b);
-      mma(b, 0, PM);
-    } else {
-      mma(a, 0, PM);
-    }
-  }
-
-  // lane (r, g): rows 16 mi + r, columns 16 ns + 4 g + i
-  float sc[NPW][4], sx[PM];
-#pragma unroll
-  for (int ns = 0; ns < NPW; ++ns)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sc[ns][i] = weight_scale(p, min(n0 + (nw * NPW + ns) * 16 + 4 * g + i, p.n - 1));
-#pragma unroll
-  for (int mi = 0; mi < PM; ++mi) sx[mi] = p.xs[min(m0 + (mw * PM + mi) * 16 + r, p.m - 1)];
-  constexpr int kOut = EPI == NE_EPILOGUE_SWIGLU ? NPW / 2 : NPW;
-  const int n_out = EPI == NE_EPILOGUE_SWIGLU ? p.n / 2 : p.n;
-  const int col0 = (EPI == NE_EPILOGUE_SWIGLU ? n0 / 2 : n0) + nw * kOut * 16;
+  char* slot = smem;
+  int s = 0;             // stage over all tiles
+  bool storing = false;  // the previous tile's kStores stores are younger than the copies up to stage s + RING - 1
   const bool wide = (uintptr_t)p.y % 16 == 0 && p.ldy % 8 == 0;
-#pragma unroll
-  for (int mi = 0; mi < PM; ++mi) {
-    const int m = m0 + (mw * PM + mi) * 16 + r;
-    uint16_t* row = p.y + (int64_t)m * p.ldy;
-    auto out4 = [&](int o) {
-      if constexpr (EPI == NE_EPILOGUE_SWIGLU)
-        return swiglu4(acc[mi][2 * o], acc[mi][2 * o + 1], sx[mi], sc[2 * o], sc[2 * o + 1]);
-      return store4(acc[mi][o], sx[mi], sc[o]);
+  const int n_out = EPI == NE_EPILOGUE_SWIGLU ? p.n / 2 : p.n;
+#pragma unroll 1
+  for (int i = 0; i < my_tiles; ++i) {
+    int m0, n0;
+    place(i, m0, n0);
+    // the bits of this thread's scale, one of BM + BN, so that nothing waits for them where they are loaded
+    auto my_scale = [&]() -> uint32_t {
+      const int t = threadIdx.x;
+      if (t < L::BM) return ((const uint32_t*)p.xs)[min(m0 + t, p.m - 1)];
+      const int n = min(n0 + min(t - L::BM, L::BN - 1), p.n - 1);
+      return p.ws_dtype == NE_DTYPE_FP32 ? ((const uint32_t*)p.ws)[n] : ((const uint16_t*)p.ws)[n];
     };
-    if constexpr (kOut % 2 == 0) {
+    auto put_scale = [&](uint32_t bits) {
+      const bool fp32 = threadIdx.x < L::BM || p.ws_dtype == NE_DTYPE_FP32;
+      const float half = p.ws_dtype == NE_DTYPE_BF16 ? bf16_to_f32((uint16_t)bits) : f16_to_f32((uint16_t)bits);
+      const float v = fp32 ? __uint_as_float(bits) : half;
+      if (L::BM + L::BN == L::kWaves * kWave || threadIdx.x < L::BM + L::BN) scales[threadIdx.x] = v;
+    };
+    uint32_t scale = 0;
+#pragma unroll
+    for (int mi = 0; mi < PM; ++mi)
+#pragma unroll
+      for (int ns = 0; ns < NPW; ++ns) acc[mi][ns] = intx4{0, 0, 0, 0};
+    read(slot, 0, a);
+#pragma unroll 1
+    for (int t = 0; t < n_stages; ++t, ++s) {
+      wait_lgkmcnt0();  // for a's reads, not for the next ones too
+      read(slot, 1, b);
+      if (t + 1 == n_stages) scale = my_scale();
+      mma(a);
+      if (s + 1 < all) {
+        // stage s + 1 has landed and every wave has read all of stage s: its slot takes stage s + RING
+        const int pend = min(all - 1, s + RING - 1) - (s + 1);
+        if (storing && t <= RING - 2) {
+          wait_pending_after<D, RING - 2, kStores>(pend);
+        } else {
+          wait_pending<D, RING - 2>(pend);
+        }
+        slot = slot == smem + (RING - 1) * L::kStage ? smem : slot + L::kStage;
+        clear_tail(slot, t + 1 == n_stages ? 0 : t + 1);
+        wait_lgkmcnt0();
+        asm volatile("s_barrier" ::: "memory");
+        if (t + 1 < n_stages) read(slot, 0, a);
+      } else {
+        wait_lgkmcnt0();
+      }
+      // the next copies go out between the MFMAs, which hide them
+      const bool more = s + RING < all && t + 1 < n_stages;
+      if (more) begin_copies();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int mi = 0; mi < PM; ++mi) {
+        mma_row(b, mi);
+        if (more) copies(D * mi / PM, D * (mi + 1) / PM);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (more) end_copies();
+    }
+    // The scales go through LDS.  Their load is waited for before the copies of the slot that the
+    // tile's last stage left, not after them.
+    if (n_stages == 1) lds_barrier();  // the previous tile's have been read
+    put_scale(scale);
+    if (s - 1 + RING < all) issue();
+    lds_barrier();
+
+    // lane (r, g): rows 16 mi + r, columns 16 ns + 4 g + i
+    int l = lane;
+    __asm__ volatile("" : "+v"(l));  // addresses made here, not kept in registers through the k loop
+    const int er = l & 15, eg = l >> 4;
+    float sc[NPW][4];
+#pragma unroll
+    for (int ns = 0; ns < NPW; ++ns) {
+      const floatx4 v = *(const floatx4*)(scales + L::BM + (nw * NPW + ns) * 16 + 4 * eg);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[ns][e] = v[e];
+    }
+    const int col0 = (EPI == NE_EPILOGUE_SWIGLU ? n0 / 2 : n0) + nw * kOut * 16;
+    const bool inside = wide && n0 + L::BN <= p.n;  // all of the tile's columns, in wide stores
+    auto out4 = [&](int mi, int o, float sx) {
+      if constexpr (EPI == NE_EPILOGUE_SWIGLU)
+        return swiglu4(acc[mi][2 * o], acc[mi][2 * o + 1], sx, sc[2 * o], sc[2 * o + 1]);
+      else
+        return store4(acc[mi][o], sx, sc[o]);
+    };
+    char* const edge = smem + L::kEdge + wave * 1024;
+#pragma unroll
+    for (int mi = 0; mi < PM; ++mi) {
+      const int lrow = (mw * PM + mi) * 16 + er;
+      const float sx = scales[lrow];
+      uint16_t* row = p.y + (int64_t)(m0 + lrow) * p.ldy + col0;
+      // a row's 16-column subtiles in pairs
+      static_assert(kOut % 2 == 0, "output subtiles in pairs");
 #pragma unroll
       for (int o = 0; o < kOut; o += 2) {
-        const u32x4 both = pair_columns(out4(o), out4(o + 1));
-        if (m < p.m) store_columns<4>(row, col0 + o * 16 + pair_column(g), n_out, wide, both);
-      }
-    } else {
-#pragma unroll
-      for (int o = 0; o < kOut; ++o) {
-        const u32x2 v = out4(o);
-        if (m < p.m) store_columns<2>(row, col0 + o * 16 + 4 * g, n_out, wide, v);
+        const u32x4 both = pair_columns(out4(mi, o, sx), out4(mi, o + 1, sx));
+        if (inside) {
+          if (m0 + lrow < p.m) *(u32x4*)(row + o * 16 + pair_column(eg)) = both;
+        } else {
+          // 16 rows of 32 columns through LDS, then two rows at a time, element by element
+          *(u32x4*)(edge + er * 64 + pair_column(eg) * 2) = both;
+#pragma unroll 1
+          for (int at = l; at < 16 * 32; at += kWave) {
+            const int m = m0 + (mw * PM + mi) * 16 + at / 32, col = col0 + o * 16 + at % 32;
+            if (m < p.m && col < n_out) p.y[(int64_t)m * p.ldy + col] = *(const uint16_t*)(edge + at * 2);
+          }
+        }
       }
     }
+    storing = inside && m0 + L::BM <= p.m;  // (every one of the stores was made)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);  // the stores stay before the next wait
   }
 }
 
@@ -320,8 +395,10 @@ int launch_tile(W8a8Params p, hipStream_t stream) {
   p.tiles_m = ceil_div(p.m, L::BM);
   p.tiles_n = ceil_div(p.n, L::BN);
   const int64_t per = ((int64_t)p.tiles_m * p.tiles_n + kNumXcd - 1) / kNumXcd;
-  NE_CHECK_SUPPORTED(per * kNumXcd < (int64_t(1) << 31) / 1024, "too many tiles: %d x %d", p.tiles_m, p.tiles_n);
-  hipLaunchKernelGGL((w8a8_tile_kernel<L, EPI>), dim3((unsigned)(per * kNumXcd)), dim3(L::kWaves * kWave), 0, stream, p);
+  const int64_t most = L::kPerCu * kNumCu / kNumXcd;
+  NE_CHECK_SUPPORTED(per < (int64_t(1) << 24), "too many tiles: %d x %d", p.tiles_m, p.tiles_n);
+  const unsigned grid = (unsigned)((per < most ? per : most) * kNumXcd);
+  hipLaunchKernelGGL((w8a8_tile_kernel<L, EPI>), dim3(grid), dim3(L::kWaves * kWave), 0, stream, p);
   return check_launch("w8a8_gemm");
 }
 
@@ -437,30 +514,80 @@ int launch_few(const W8a8Params& p, hipStream_t stream) {
   return check_launch("w8a8_gemm");
 }
 
-using Tile256x256 = TileLayout<256, 256, 2, 4, 1, 4>;
-using Tile128x128 = TileLayout<128, 128, 2, 2, 1, 4>;
-using Tile64x128 = TileLayout<64, 128, 1, 4, 1, 6>;
+// ---- which kernel --------------------------------------------------------------------
+// The least estimated time (us) over the kernels: a fixed part, and a cost per 128 k that grows
+// with the tiles (or work-groups) per CU.  Constants fitted to 192 shapes (m 1-4,096, n 256-16,384,
+// k 256-8,192, GPU time from graphs), over which the choice takes 1.5 % longer than the fastest
+// kernel of each shape on average, at most 30 % (200 rows, n = 16,384, k = 8,192: 71 against 54 us).
+// Examples (us; few rows / 64 x 64 / 64 x 128 / 128 x 128 / 256 x 256): 64 x 1,024 x 2,048 5.3 / 10.0 /
+// 12.1 / 15.0 / 27.8, 333 x 4,096 x 1,024 14.4 / 8.8 / 8.7 / 10.1 / 18.8, 2,048 x 4,096 x 1,024 - / 21.3 /
+// 19.4 / 16.0 / 21.9, 4,096 x 4,096 x 1,024 - / 37.6 / 32.1 / 25.2 / 23.2.
+struct Kernel {
+  int id;       // as ne_w8a8_kernel names it
+  int variant;  // of the few-rows kernel: token subtiles, and 10 for two weight subtiles, 20 for two column groups
+};
 
-int32_t choose_kernel(int32_t m, int32_t n, int32_t k, bool swiglu) {
-  if (m <= 64 && n <= 16384) return NE_W8A8_FEW_ROWS;
-  const int64_t big = (int64_t)ceil_div(m, 256) * ceil_div(n, 256);
-  if (big >= 128) return NE_W8A8_TILE_256X256;
-  const int64_t mid = (int64_t)ceil_div(m, 128) * ceil_div(n, 128);
-  return m > 64 && mid >= 128 ? NE_W8A8_TILE_128X128 : NE_W8A8_TILE_64X128;
+Kernel choose_kernel(int m, int n, int k, bool swiglu) {
+  const double stages = (k + 127) / 128;
+  Kernel best{};
+  double least = 1e30;
+  auto offer = [&](int id, int variant, double us) {
+    if (us < least) {
+      least = us;
+      best = Kernel{id, variant};
+    }
+  };
+  auto count = [&](int bm, int bn) { return (double)ceil_div(m, bm) * ceil_div(n, bn) / kNumCu; };
+  auto tile = [&](int id, int bm, int bn, double fixed, double stage, double a, double b) {
+    const double load = a + b * count(bm, bn);
+    offer(id, 0, fixed + stage * stages * (load > 1 ? load : 1));
+  };
+  const double big = count(256, 256);
+  offer(NE_W8A8_TILE_256X256, 0, 6.5 + 1.31 * stages * (big <= 0.125 ? 1 : 1.55 * ceil(big)));
+  tile(NE_W8A8_TILE_128X128, 128, 128, 4.2, 0.69, 0.5, 0.85);
+  tile(NE_W8A8_TILE_64X128, 64, 128, 4.0, 0.51, 0.25, 0.83);
+  tile(NE_W8A8_TILE_64X64, 64, 64, 3.7, 0.39, 0.35, 0.62);
+  auto few = [&](int variant, int rows, int columns, double line) {
+    offer(NE_W8A8_FEW_ROWS, variant, 3.5 + line * stages * ceil(count(rows, columns)));
+  };
+  if (!swiglu) {
+    few(1, 16, 16, 0.108);
+    few(2, 32, 16, 0.16);
+    few(4, 64, 16, 0.27);
+    if (m <= 16) {
+      const double load = count(16, 32);
+      offer(NE_W8A8_FEW_ROWS, 21, 4.0 + 0.16 * stages * (load > 1 ? load : 1));
+    }
+  } else {
+    few(11, 16, 32, 0.16);
+    few(12, 32, 32, 0.22);
+  }
+  few(14, 64, 32, 0.34);
+  return best;
 }
 
 template <int EPI>
-int launch_kernel(int32_t kernel, const W8a8Params& p, hipStream_t stream) {
-  constexpr int NS = EPI == NE_EPILOGUE_SWIGLU ? 2 : 1;
-  switch (kernel) {
-    case NE_W8A8_FEW_ROWS:
-      if (p.m <= 16) return launch_few<FewLayout<1, NS, 8, 1>, EPI>(p, stream);
-      if (p.m <= 32) return launch_few<FewLayout<2, NS, 8, 1>, EPI>(p, stream);
-      return launch_few<FewLayout<4, NS, 8, 1>, EPI>(p, stream);
-    case NE_W8A8_TILE_64X128: return launch_tile<Tile64x128, EPI>(p, stream);
-    case NE_W8A8_TILE_128X128: return launch_tile<Tile128x128, EPI>(p, stream);
-    default: return launch_tile<Tile256x256, EPI>(p, stream);
+int launch_kernel(const W8a8Params& p, hipStream_t stream) {
+  constexpr bool kSwiglu = EPI == NE_EPILOGUE_SWIGLU;
+  const Kernel kernel = choose_kernel(p.m, p.n, p.k, kSwiglu);
+  switch (kernel.id) {
+    case NE_W8A8_TILE_256X256: return launch_tile<TileLayout<256, 256, 4, 2, 2>, EPI>(p, stream);
+    case NE_W8A8_TILE_128X128: return launch_tile<TileLayout<128, 128, 2, 2, 2>, EPI>(p, stream);
+    case NE_W8A8_TILE_64X128: return launch_tile<TileLayout<64, 128, 2, 2, 3>, EPI>(p, stream);
+    case NE_W8A8_TILE_64X64:  // (gate and up subtiles in one wave)
+      return launch_tile<TileLayout<64, 64, kSwiglu ? 4 : 2, kSwiglu ? 1 : 2, 3>, EPI>(p, stream);
+    default: break;
   }
+  if constexpr (kSwiglu) {
+    if (kernel.variant == 11) return launch_few<FewLayout<1, 2, 8, 1>, EPI>(p, stream);
+    if (kernel.variant == 12) return launch_few<FewLayout<2, 2, 8, 1>, EPI>(p, stream);
+  } else {
+    if (kernel.variant == 1) return launch_few<FewLayout<1, 1, 8, 1>, EPI>(p, stream);
+    if (kernel.variant == 2) return launch_few<FewLayout<2, 1, 8, 1>, EPI>(p, stream);
+    if (kernel.variant == 4) return launch_few<FewLayout<4, 1, 8, 1>, EPI>(p, stream);
+    if (kernel.variant == 21) return launch_few<FewLayout<1, 1, 4, 2>, EPI>(p, stream);
+  }
+  return launch_few<FewLayout<4, 2, 8, 1>, EPI>(p, stream);
 }
 
 }  // namespace
@@ -471,7 +598,7 @@ using namespace ne;
 
 extern "C" int32_t ne_w8a8_kernel(int32_t m, int32_t n, int32_t k, int32_t epilogue) {
   if (m <= 0 || n <= 0 || k <= 0) return NE_W8A8_FEW_ROWS;
-  return choose_kernel(m, n, k, epilogue == NE_EPILOGUE_SWIGLU);
+  return choose_kernel(m, n, k, epilogue == NE_EPILOGUE_SWIGLU).id;
 }
 
 extern "C" int ne_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, const void* w_scale,
@@ -490,7 +617,6 @@ extern "C" int ne_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, 
   NE_CHECK_ARG(ldy >= (epilogue == NE_EPILOGUE_SWIGLU ? n / 2 : n), "ldy too small (%lld)", (long long)ldy);
   NE_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0, "x and w must be 16-byte aligned");
   const W8a8Params p{x, ldx, x_scale, w, w_scale, scale_dtype, m, n, k, (uint16_t*)y, ldy, 0, 0};
-  const int32_t kernel = choose_kernel(m, n, k, epilogue == NE_EPILOGUE_SWIGLU);
-  return epilogue == NE_EPILOGUE_SWIGLU ? launch_kernel<NE_EPILOGUE_SWIGLU>(kernel, p, (hipStream_t)stream)
-                                        : launch_kernel<NE_EPILOGUE_STORE>(kernel, p, (hipStream_t)stream);
+  return epilogue == NE_EPILOGUE_SWIGLU ? launch_kernel<NE_EPILOGUE_SWIGLU>(p, (hipStream_t)stream)
+                                        : launch_kernel<NE_EPILOGUE_STORE>(p, (hipStream_t)stream);
 }

@@ -145,7 +145,8 @@ SHAPES = [
     (1, 1, 16), (1, 15, 32), (1, 17, 48), (2, 4096, 1024), (15, 130, 112), (16, 541, 128), (17, 64, 1040), (33, 100, 2048),
     (64, 1024, 2048), (48, 33, 4112), (65, 64, 16), (65, 127, 80), (100, 541, 608), (127, 129, 64), (128, 128, 192),
     (200, 1000, 144), (129, 32003, 64), (64, 40000, 96), (3, 70000, 272), (300, 8192, 1024), (1000, 2048, 336), (2049, 4100, 80),
-    (1111, 9001, 1024), (4096, 2304, 208),
+    (1111, 9001, 1024), (4096, 2304, 208), (9000, 9100, 80), (4100, 5003, 1040), (8192, 4096, 256), (2048, 16384, 400), (350, 64, 2064),
+    (64, 151936, 64), (520, 4104, 144), (129, 4160, 2048),
 ]
 
 
@@ -158,7 +159,8 @@ def test_product(m, n, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(1, 32, 16), (1, 6144, 1024), (16, 96, 144), (31, 64, 1024), (64, 512, 272), (65, 32, 48),
-                                   (150, 320, 64), (333, 6144, 1024), (700, 4096, 176), (2100, 5152, 336)])
+                                   (150, 320, 64), (333, 6144, 1024), (700, 4096, 176), (2100, 5152, 336), (200, 192, 1040), (20, 6144, 528),
+                                   (9000, 9120, 144), (4100, 8192, 1040), (40, 40000, 64), (257, 4128, 2064)])
 def test_swiglu_product(m, n, k):
     data = make(m, n, k, seed=m + n + k)
     check_product(kernels.w8a8_gemm(*data, epilogue=EPILOGUE_SWIGLU), *data, epilogue=EPILOGUE_SWIGLU)
@@ -168,7 +170,7 @@ def test_every_kernel_serves_some_shape():
     if not _native.library_path().exists():
         pytest.skip("libnanoengine_hip.so is not built")
     lib = _native.load()
-    assert {lib.ne_w8a8_kernel(m, n, k, EPILOGUE_STORE) for m, n, k in SHAPES} == {0, 1, 2, 3}
+    assert {lib.ne_w8a8_kernel(m, n, k, EPILOGUE_STORE) for m, n, k in SHAPES} == {0, 1, 2, 3, 4}
 
 
 @pytest.mark.gpu
