@@ -10,7 +10,6 @@
 // ne_add_rmsnorm store (same sums in the same order, both roundings), quantised without the
 // trip through memory.  What bounds it: memory, each row read once into registers.
 #include "ne_common.hpp"
-#include "qk_rope_kv.hpp"
 
 namespace ne {
 
@@ -29,63 +28,84 @@ struct RowsParams {
   int rows, k;
 };
 
+typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
+
+// the two values of a 32-bit word
+template <int VDT>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (VDT == NE_DTYPE_BF16) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xFFFF0000u);
+  } else {
+    lo = f16_to_f32((uint16_t)(w & 0xFFFFu));
+    hi = f16_to_f32((uint16_t)(w >> 16));
+  }
+}
+
 template <int VDT>
 __device__ __forceinline__ void unpack8(const u32x4 v, float (&f)[8]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (VDT == NE_DTYPE_BF16) {
-      f[2 * i] = bf16_to_f32((uint16_t)(v[i] & 0xFFFFu));
-      f[2 * i + 1] = bf16_to_f32((uint16_t)(v[i] >> 16));
-    } else {
-      f[2 * i] = f16_to_f32((uint16_t)(v[i] & 0xFFFFu));
-      f[2 * i + 1] = f16_to_f32((uint16_t)(v[i] >> 16));
-    }
-  }
+  for (int i = 0; i < 4; ++i) unpack2<VDT>(v[i], f[2 * i], f[2 * i + 1]);
 }
 
 __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
   return u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
-
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+// largest magnitude of 16-bit values, by their bits, in each half of `top`
+__device__ __forceinline__ void max_magnitude(const u32x4 v, uint32_t& top) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-  return v;
+  for (int i = 0; i < 4; ++i)
+    top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, v[i] & 0x7FFF7FFFu),
+                                                                 __builtin_bit_cast(ushort2v, top)));
 }
 
-constexpr uint32_t kInfBits = 0x7F800000u;
+// the larger half over the wave, in every lane
+__device__ __forceinline__ uint32_t wave_max_half(uint32_t v) {
+  v = max(v & 0xFFFFu, v >> 16);
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));   // quad_perm [1, 0, 3, 2]
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));   // quad_perm [2, 3, 0, 1]
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));  // row_half_mirror
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));  // row_mirror
+  v = max(v, (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x401F));               // lanes 16 apart
+  return max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 32));
+}
 
-// the row's scale from the bits of its largest magnitude
+// the row's scale from the 16 bits of its largest magnitude; NaN where that is no number
+template <int VDT>
 __device__ __forceinline__ float row_scale(uint32_t top) {
-  if (top >= kInfBits) return __builtin_nanf("");
-  return fmaxf(__builtin_bit_cast(float, top), 1e-8f) / 127.f;
+  if (top >= (VDT == NE_DTYPE_BF16 ? 0x7F80u : 0x7C00u)) return __builtin_nanf("");
+  const float v = VDT == NE_DTYPE_BF16 ? bf16_to_f32((uint16_t)top) : f16_to_f32((uint16_t)top);
+  return fmaxf(v, 1e-8f) / 127.f;
 }
 
-__device__ __forceinline__ uint32_t codes4(const float* t) {
-  uint32_t b[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) b[e] = (uint32_t)(int)fminf(fmaxf(rintf(t[e]), -127.f), 127.f);
-  const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
-  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), lo, 0x05040100u);
-}
-
-// Codes of 8 values of a finite row.  x / s as x * v_rcp_f32(s): within 3e-5 of the fp32 quotient
-// at |x / s| <= 127, so both round to the same integer unless it lies within 4e-5 of a half;
-// a wave with such a lane divides (one chunk of 512 values in 25).
-__device__ __forceinline__ u32x2 quantize8(const float (&f)[8], float s, float rcp) {
-  float t[8], far = 0.f;
+// Codes of 8 values of a row with scale s, at most 127 in magnitude as no value exceeds the one the
+// scale comes from (a row without a scale: 0).  One fma rounds x * v_rcp_f32(s) to a whole number
+// in the low bits of 1.5 2^23; that product lies within 3e-5 of the fp32 quotient, so both round to the
+// same number unless it is within 4e-5 of a half.  A wave with such a lane divides (one chunk
+// of 512 values in 25).
+template <int VDT>
+__device__ __forceinline__ u32x2 quantize8(const u32x4 v, float s, float rcp) {
+  constexpr float kWhole = 12582912.f;
+  float f[8], t[8], far = 0.f;
+  unpack8<VDT>(v, f);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    t[e] = f[e] * rcp;
-    far = fmaxf(far, fabsf(t[e] - rintf(t[e])));
+    t[e] = __builtin_fmaf(f[e], rcp, kWhole);
+    far = fmaxf(far, fabsf(__builtin_fmaf(f[e], rcp, -(t[e] - kWhole))));
   }
   if (__builtin_amdgcn_ballot_w64(far > 0.49996f) != 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = f[e] / s;
+    for (int e = 0; e < 8; ++e) t[e] = f[e] / s + kWhole;
   }
-  return u32x2{codes4(t), codes4(t + 4)};
+  u32x2 codes;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(t[4 * i + 1]), __float_as_uint(t[4 * i]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(t[4 * i + 3]), __float_as_uint(t[4 * i + 2]), 0x0c0c0400u);
+    codes[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+  }
+  return s == s ? codes : u32x2{0, 0};
 }
 
 // WAVES waves per row (1: four rows per work-group; 4: one), CPL 8-element chunks per lane held in
@@ -114,31 +134,27 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(RowsParams p) {
       if constexpr (MODE != kPlain) wraw[c] = *(const u32x4*)(p.weight + ci * 8);
     }
   }
-  float h[CPL][8];
   uint32_t top = 0;
-  if constexpr (MODE == kPlain) {
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      unpack8<VDT>(raw[c], h[c]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, abs_bits(h[c][e]));
-    }
-  } else {
+  if constexpr (MODE != kPlain) {
+    // ne_rmsnorm's rows, by its operations in its order
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
       const int ci = at + c * kThreads;
       if (ci < chunks) {
-        unpack8<VDT>(raw[c], h[c]);
+        float h[8];
+        unpack8<VDT>(raw[c], h);
         if constexpr (MODE == kAddNorm) {
           float d[8];
           unpack8<VDT>(draw[c], d);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) h[c][e] = bf16_round(h[c][e] + d[e]);
-          *(u32x4*)(p.residual + (int64_t)row * p.k + ci * 8) = pack8(h[c]);
+          for (int e = 0; e < 8; ++e) h[e] += d[e];
+          raw[c] = pack8(h);
+          unpack8<VDT>(raw[c], h);
+          *(u32x4*)(p.residual + (int64_t)row * p.k + ci * 8) = raw[c];
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += h[c][e] * h[c][e];
+        for (int e = 0; e < 8; ++e) ss += h[e] * h[e];
       }
     }
     ss = wave_sum(ss);
@@ -147,17 +163,21 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(RowsParams p) {
     for (int c = 0; c < CPL; ++c) {
       const int ci = at + c * kThreads;
       if (ci < chunks) {
-        float w[8];
+        float h[8], w[8];
+        unpack8<VDT>(raw[c], h);
         unpack8<VDT>(wraw[c], w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          h[c][e] = bf16_round(bf16_round(h[c][e] * inv) * w[e]);
-          top = max(top, abs_bits(h[c][e]));
-        }
+        for (int e = 0; e < 8; ++e) h[e] *= inv;
+        unpack8<VDT>(pack8(h), h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] *= w[e];
+        raw[c] = pack8(h);
       }
     }
   }
-  top = wave_max_u32(top);
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) max_magnitude(raw[c], top);
+  top = wave_max_half(top);
   if constexpr (WAVES > 1) {
     __shared__ uint32_t tops[WAVES];
     if (threadIdx.x % kWave == 0) tops[wave] = top;
@@ -165,15 +185,14 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(RowsParams p) {
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) top = max(top, tops[w]);
   }
-  const float s = row_scale(top);
+  const float s = row_scale<VDT>(top);
   if (at == 0) p.scales[row] = s;
-  const bool finite = top < kInfBits;
   const float rcp = __builtin_amdgcn_rcpf(s);
   int8_t* dst = p.codes + (int64_t)row * p.k;
 #pragma unroll
   for (int c = 0; c < CPL; ++c) {
     const int ci = at + c * kThreads;
-    if (ci < chunks) *(u32x2*)(dst + ci * 8) = finite ? quantize8(h[c], s, rcp) : u32x2{0, 0};
+    if (ci < chunks) *(u32x2*)(dst + ci * 8) = quantize8<VDT>(raw[c], s, rcp);
   }
 }
 
@@ -185,25 +204,18 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(RowsParams p) 
   const int chunks = p.k / 8;
   const uint16_t* src = p.x + (int64_t)row * p.ldx;
   uint32_t top = 0;
-  float f[8];
-  for (int ci = threadIdx.x; ci < chunks; ci += 1024) {
-    unpack8<VDT>(*(const u32x4*)(src + (int64_t)ci * 8), f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, abs_bits(f[e]));
-  }
-  top = wave_max_u32(top);
+  for (int ci = threadIdx.x; ci < chunks; ci += 1024) max_magnitude(*(const u32x4*)(src + (int64_t)ci * 8), top);
+  top = wave_max_half(top);
   if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 16; ++w) top = max(top, tops[w]);
-  const float s = row_scale(top);
+  const float s = row_scale<VDT>(top);
   if (threadIdx.x == 0) p.scales[row] = s;
   const float rcp = __builtin_amdgcn_rcpf(s);
   int8_t* dst = p.codes + (int64_t)row * p.k;
-  for (int ci = threadIdx.x; ci < chunks; ci += 1024) {
-    unpack8<VDT>(*(const u32x4*)(src + (int64_t)ci * 8), f);
-    *(u32x2*)(dst + (int64_t)ci * 8) = top < kInfBits ? quantize8(f, s, rcp) : u32x2{0, 0};
-  }
+  for (int ci = threadIdx.x; ci < chunks; ci += 1024)
+    *(u32x2*)(dst + (int64_t)ci * 8) = quantize8<VDT>(*(const u32x4*)(src + (int64_t)ci * 8), s, rcp);
 }
 
 template <int MODE, int VDT>
