@@ -59,6 +59,7 @@ class EngineSettings:
     chunked_prefill: bool = False
     max_num_batched_tokens: int = 512
     quantization: str = "none"
+    int8_activations: bool = False  # prompts' projections with 8-bit activations too (W8A8)
     kv_cache_dtype: str = "auto"
     cuda_graphs: bool = False
     cuda_graph_max_context: int = 1024
@@ -104,6 +105,8 @@ class EngineSettings:
             raise ValueError("chunked_prefill needs scheduler=continuous")
         if self.kv_cache == "none" and (self.kv_cache_dtype == "int8" or self.cuda_graphs):
             raise ValueError("kv_cache_dtype=int8 and cuda_graphs need a KV cache")
+        if self.int8_activations and self.quantization != "int8":
+            raise ValueError("int8_activations needs quantization=int8 (its products take 8-bit weights)")
         if self.speculative != "none" and self.kv_cache == "none":
             raise ValueError("speculative decoding needs a KV cache")
         if self.speculative == "draft" and self.prefix_cache:

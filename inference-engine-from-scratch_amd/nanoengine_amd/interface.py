@@ -4,8 +4,8 @@ sampling helpers of ne/engine/sampling.py that stay on the host."""
 from __future__ import annotations
 
 import os
-from collections.abc import AsyncIterator
-from dataclasses import dataclass
+from collections.abc import AsyncIterator, Mapping
+from dataclasses import dataclass, field
 from typing import Protocol
 
 GREEDY_TEMPERATURE = 0.0
@@ -22,6 +22,22 @@ class SamplingParams:
     ignore_eos: bool = False
     top_k: int = 0  # 0: all tokens
     min_p: float = 0.0  # least probability, relative to the likeliest token's
+    # logits of tokens so far: of prompt and output divided (positive ones) or multiplied by
+    # repetition_penalty, of output lowered by frequency_penalty a time and presence_penalty once
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Mapping[int, float] | None = field(default=None, hash=False)  # added to single tokens' logits
+
+    @property
+    def is_penalized(self) -> bool:
+        """Whether the logits depend on the tokens so far."""
+        return self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+
+    @property
+    def is_adjusted(self) -> bool:
+        """Whether the request's logits are changed before a token is picked (greedily too)."""
+        return self.is_penalized or bool(self.logit_bias)
 
     @property
     def is_filtered(self) -> bool:

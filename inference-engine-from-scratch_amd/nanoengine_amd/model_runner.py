@@ -11,8 +11,10 @@ sequence's guesses with ``score_tokens``.
 from __future__ import annotations
 
 import math
+from array import array
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
 from nanoengine_amd import kernels
@@ -191,6 +193,34 @@ class ModelRunner:
             top_k=row([min(max(p.top_k, 0), self.vocab_size) for p in params], torch.int32),
             top_p=row([p.top_p for p in params]), min_p=row([p.min_p for p in params]))
 
+    def _adjust(self, logits: torch.Tensor, sequences: list, lengths: list[int], allowed: list) -> torch.Tensor:
+        """fp32 logits under the requests' penalties (for each sequence's first ``lengths`` tokens), biases
+        and masks."""
+        params = [s.sampling_params for s in sequences]
+        n, dev = len(sequences), self._device
+        penalties = bias = mask = mask_rows = None
+        if any(p.is_penalized for p in params):
+            lens = [length if p.is_penalized else 0 for p, length in zip(params, lengths)]
+            history = np.zeros((n, max(lens)), dtype=np.int32)
+            for row, s, length in zip(history, sequences, lens):
+                row[:length] = array("i", s.token_ids[:length])
+            column = lambda name: torch.tensor([getattr(p, name) for p in params], dtype=torch.float32, device=dev)
+            numbers = torch.tensor([lens, [s.num_prompt_tokens for s in sequences]], dtype=torch.int32).to(dev)
+            penalties = kernels.TokenPenalties(torch.from_numpy(history).to(dev), numbers[0], numbers[1],
+                                               column("repetition_penalty"), column("presence_penalty"),
+                                               column("frequency_penalty"))
+        if any(p.logit_bias for p in params):
+            bias = kernels.TokenBias.from_dicts([p.logit_bias for p in params], dev)
+        given = [i for i, a in enumerate(allowed) if a is not None]
+        if given:
+            mask = kernels.allowed_mask([allowed[i] for i in given], self.vocab_size, dev)
+            rows = [-1] * n
+            for at, i in enumerate(given):
+                rows[i] = at
+            mask_rows = torch.tensor(rows, dtype=torch.int32, device=dev)
+        return kernels.adjust_logits(logits, penalties, bias, mask, mask_rows,
+                                     out=torch.empty(logits.shape, dtype=torch.float32, device=dev))
+
     def _accept_last(self, logits: torch.Tensor, sequences: list) -> torch.Tensor:
         """Each row's token by the acceptance kernel, as a verify step without guesses."""
         b = len(sequences)
@@ -213,25 +243,47 @@ class ModelRunner:
         return out[:, 0]
 
     @torch.inference_mode()
-    def run_step(self, sequences: list, token_counts: list[int] | None = None) -> list[int]:
+    def run_step(self, sequences: list, token_counts: list[int] | None = None,
+                 allowed_tokens: list | None = None) -> list[int]:
         """Cache the next ``token_counts`` tokens of each sequence (default: all uncached)
         and pick a token after each one's last (model_runner.py:33-50): the argmax, or for a
         sampled request a draw under the explicit-uniform contract of the acceptance kernel
         at the request's temperature and top-p, advancing its sampling stream.  A request that
         also has a top-k or min-p gets the token that ``kernels.sample`` draws, from the
-        stream's uniform of its own at each step."""
+        stream's uniform of its own at each step, and so does one with penalties or biases, or
+        with an entry in ``allowed_tokens`` (one per sequence: the tokens that it may draw next, as a
+        grammar gives them, or None), from the logits that ``kernels.adjust_logits`` makes of its
+        own.  Where an entry leaves a sequence no token, the step raises and no sequence has moved."""
+        allowed = [None] * len(sequences) if allowed_tokens is None else allowed_tokens
+        if len(allowed) != len(sequences):
+            raise ValueError(f"allowed_tokens for {len(allowed)} of {len(sequences)} sequences")
+        for s in sequences:
+            if not 0.0 < s.sampling_params.repetition_penalty < math.inf:
+                raise ValueError(f"{s.request_id}: repetition_penalty must be positive and finite")
         inputs = build_step_inputs(sequences, self.allocator, self._pool, self._device, token_counts)
         hidden, starts, counts = self._forward(inputs, sequences)
         last = torch.tensor([s + n - 1 for s, n in zip(starts, counts, strict=True)], device=self._device)
         logits, _ = self._model.compute_logits(hidden[last].contiguous())
-        filtered = [i for i, s in enumerate(sequences) if s.sampling_params.is_filtered]
+        adjusted = [i for i, s in enumerate(sequences) if s.sampling_params.is_adjusted or allowed[i] is not None]
+        filtered = [i for i, s in enumerate(sequences) if s.sampling_params.is_filtered and i not in adjusted]
         if len(filtered) == len(sequences):
             tokens = self._draw_filtered(logits, sequences).tolist()
         else:
-            out = self._accept_last(logits, sequences)
+            if len(filtered) + len(adjusted) == len(sequences):
+                out = torch.empty(len(sequences), dtype=torch.int32, device=self._device)
+            else:
+                out = self._accept_last(logits, sequences)
             if filtered:
                 out[filtered] = self._draw_filtered(logits[filtered], [sequences[i] for i in filtered])
+            if adjusted:
+                chosen = [sequences[i] for i in adjusted]
+                ends = [sequences[i].num_cached_tokens + counts[i] for i in adjusted]
+                out[adjusted] = self._draw_filtered(
+                    self._adjust(logits[adjusted], chosen, ends, [allowed[i] for i in adjusted]), chosen)
             tokens = out.tolist()
+            for i in adjusted:
+                if tokens[i] < 0:
+                    raise ValueError(f"{sequences[i].request_id}: no token is allowed")
         for s in sequences:
             if s.sampling_params.temperature != GREEDY_TEMPERATURE:
                 s.sampling_generator.step += 1

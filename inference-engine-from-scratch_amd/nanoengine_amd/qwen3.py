@@ -21,6 +21,10 @@ from nanoengine_amd._native import EPILOGUE_SWIGLU
 from nanoengine_amd.int8_quantization import quantize_vectors
 
 
+# From this many rows on a forward with int8_activations takes the W8A8 products.
+W8A8_MIN_ROWS = 1536
+
+
 @dataclass(frozen=True)
 class Qwen3Config:
     """ne/models/qwen3.py:13-28."""
@@ -199,7 +203,11 @@ class AttentionBatch:
 class Qwen3VerifyModel:
     """The verify forward (qwen3.py:164-203) as a chain of HIP kernels over packed rows."""
 
-    def __init__(self, weights: Qwen3Weights, max_rows: int, device: torch.device) -> None:
+    def __init__(self, weights: Qwen3Weights, max_rows: int, device: torch.device,
+                 int8_activations: bool = False) -> None:
+        """``int8_activations``: forwards of many rows (``W8A8_MIN_ROWS``: prompts) quantise the
+        projections' activations to 8 bits with a scale per row and take the W8A8 products, on
+        the same weights; fewer rows keep bf16 activations."""
         c = weights.config
         if c.head_dim != kernels.HEAD_DIM:
             raise NotImplementedError("the HIP kernels support head_dim 128")
@@ -218,6 +226,11 @@ class Qwen3VerifyModel:
         self.q = torch.empty(max_rows, c.num_attention_heads, c.head_dim, **bf)
         self.attn = torch.empty(max_rows, c.num_attention_heads, c.head_dim, **bf)
         self.act = torch.empty(max_rows, c.intermediate_size, **bf)
+        self.int8_activations = int8_activations
+        self.codes = self.code_scales = None
+        if int8_activations and max_rows >= W8A8_MIN_ROWS:
+            self.codes = torch.empty(max_rows * max(h, q, c.intermediate_size), dtype=torch.int8, device=device)
+            self.code_scales = torch.empty(max_rows, dtype=torch.float32, device=device)
         # cos/sin per position (qwen3.py:47-57), computed once on the host as the
         # reference computes them per step; grown when a longer position appears
         self.rope_positions = 0
@@ -280,6 +293,7 @@ class Qwen3VerifyModel:
             kernels.paged_attention_plan(batch.block_tables, pool.block_size, batch.ctx_len, batch.q_start,
                                          batch.q_len, c.num_attention_heads, c.num_key_value_heads,
                                          batch.max_q_len, batch.max_ctx_len, ws)
+        int8 = self.codes is not None and rows >= W8A8_MIN_ROWS
         fuse = self.fuse_qkv and kernels.qkv_fusion_supported(pool.key_caches[0], pool.key_scale_2d(0))
         for i, layer in enumerate(w.layers):
             if fuse:  # QK-norm + RoPE + KV write in the QKV GEMM's epilogue (same bits)
@@ -307,14 +321,28 @@ class Qwen3VerifyModel:
                     batch.max_q_len, batch.max_ctx_len, self.softmax_scale, out=attn, workspace=ws,
                     planned=planned,
                 )
+            next_norm = w.layers[i + 1].input_layernorm if i + 1 < len(w.layers) else w.norm
+            if int8:
+                kernels.w8a8_gemm(*self._int8(attn.view(rows, -1)), layer.o_int8, layer.o_scale, out=delta)
+                codes, scales = kernels.add_rmsnorm_quantize(res, delta, layer.post_attention_layernorm, eps,
+                                                             *self._int8_buffers(res))
+                kernels.w8a8_gemm(codes, scales, layer.gate_up_int8, layer.gate_up_scale, epilogue=EPILOGUE_SWIGLU, out=act)
+                kernels.w8a8_gemm(*self._int8(act), layer.down_int8, layer.down_scale, out=delta)
+                kernels.add_rmsnorm(res, delta, next_norm, eps, out=normed)
+                continue
             self._project_add_norm(attn.view(rows, -1), layer.o_int8, layer.o_scale, self.o_splits[rows],
                                    layer.post_attention_layernorm, res, delta, normed)
             kernels.w8a16_gemm(normed, layer.gate_up_int8, layer.gate_up_scale, epilogue=EPILOGUE_SWIGLU,
                                out=act)
-            next_norm = w.layers[i + 1].input_layernorm if i + 1 < len(w.layers) else w.norm
             self._project_add_norm(act, layer.down_int8, layer.down_scale, self.down_splits[rows], next_norm,
                                    res, delta, normed)
         return normed
+
+    def _int8_buffers(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        return self.codes[: x.numel()].view(x.shape), self.code_scales[: x.shape[0]]
+
+    def _int8(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        return kernels.quantize_rows(x, *self._int8_buffers(x))
 
     def _prefix_plan(self, rows: int, batch: AttentionBatch, pool, ws) -> kernels.SharedPrefixPlan:
         """The step's plan, made once and read by every layer."""

@@ -46,7 +46,7 @@ import torch
 
 from nanoengine_amd import host_step, kernels
 from nanoengine_amd.draft import DeviceGuesses
-from nanoengine_amd.interface import find_finish_reason
+from nanoengine_amd.interface import SamplingParams, find_finish_reason
 from nanoengine_amd.memory import KVCachePool, PagedSlotAllocator, find_shared_prefixes
 from nanoengine_amd.qwen3 import AttentionBatch, Qwen3VerifyModel
 from nanoengine_amd.sequence_state import Sequence
@@ -79,6 +79,9 @@ def verify_graph_allowed(num_active: int, step_context: int, max_batch: int | No
     return max_context is None or step_context <= max_context
 
 
+NO_PENALTIES = SamplingParams(max_new_tokens=0)
+
+
 class StepResult(NamedTuple):
     """Tokens emitted for one sequence by one step, with its finish reason if it ended."""
 
@@ -102,6 +105,10 @@ class _Launched(NamedTuple):
 
 
 class VerifyRunner:
+    np_adjusted: np.ndarray | None = None  # slots with penalties
+    _adjusted: bool | None = None
+    graph_adjusted: bool | None = False  # whether the last captured step applies them
+
     def __init__(
         self,
         model: Qwen3VerifyModel,
@@ -219,15 +226,24 @@ class VerifyRunner:
         self.np_owned = np.zeros(max_seqs, dtype=np.int64)
         self.np_temp = np.zeros(max_seqs, dtype=np.float32)
         self.np_top_p = np.ones(max_seqs, dtype=np.float32)
+        # Penalties of the slots' rows for the tokens so far (1, 0, 0: none).  Row i of a slot's verify
+        # step counts the i guesses before it.
+        self.np_adjusted = np.zeros(max_seqs, dtype=bool)
+        self.prompt_len = torch.zeros(max_seqs, **i32)
+        f32 = dict(dtype=torch.float32, device=dev)
+        self.penalties = kernels.TokenPenalties(
+            self.history, self.history_len, self.prompt_len, torch.ones(rows, **f32), torch.zeros(rows, **f32),
+            torch.zeros(rows, **f32), drafts=self.drafts, row_seq=torch.arange(rows, **i32) // self.R,
+            row_drafts=torch.arange(rows, **i32) % self.R)
         # whether each slot's sequence ends at a stop token (ignore_eos unset)
         self.np_honours_stop = np.zeros(max_seqs, dtype=bool)
         self.slots: list[Sequence | None] = [None] * max_seqs
         # the active slot list and whether any samples, kept between slot changes
         self._active: list[int] | None = None
         self._sampled: bool | None = None
-        # a captured step per (sampled, shared) kind that a batch had so far, so that a load whose
+        # a captured step per (sampled, shared, adjusted) kind that a batch had so far, so that a load whose
         # batches change between kinds captures each once, and the one of the last step
-        self._graphs: dict[tuple[bool, bool], torch.cuda.CUDAGraph] = {}
+        self._graphs: dict[tuple[bool, bool, bool], torch.cuda.CUDAGraph] = {}
         self.graph: torch.cuda.CUDAGraph | None = None
         # whether the captured step computes full logits (some slot samples) or only the
         # LM head's argmax partials (every slot greedy)
@@ -278,6 +294,7 @@ class VerifyRunner:
     def _slots_changed(self) -> None:
         self._active = None
         self._sampled = None
+        self._adjusted = None
         self._sharing = None
 
     def free_slots(self) -> list[int]:
@@ -303,6 +320,20 @@ class VerifyRunner:
         if self._sampled is None:
             self._sampled = bool((self.np_temp[self.np_active] > 0).any())
         return self._sampled
+
+    @property
+    def any_adjusted(self) -> bool:
+        """Whether some active slot has penalties."""
+        if self._adjusted is None:
+            self._adjusted = self.np_adjusted is not None and bool(self.np_adjusted[self.np_active].any())
+        return self._adjusted
+
+    def _set_penalties(self, slot: int, params) -> None:
+        rows, p = slice(slot * self.R, (slot + 1) * self.R), self.penalties
+        for tensor, value in ((p.repetition, params.repetition_penalty), (p.presence, params.presence_penalty),
+                              (p.frequency, params.frequency_penalty)):
+            tensor[rows].fill_(value)
+        self.np_adjusted[slot] = params.is_penalized
 
     @property
     def sharing(self) -> bool:
@@ -346,6 +377,10 @@ class VerifyRunner:
             if seq.sampling_params.is_filtered:
                 raise ValueError(f"{seq.request_id}: speculative verification samples under temperature and top_p, "
                                  "not top_k or min_p")
+            if seq.sampling_params.logit_bias:
+                raise ValueError(f"{seq.request_id}: speculative verification takes penalties, not logit_bias")
+            if not 0.0 < seq.sampling_params.repetition_penalty < math.inf:
+                raise ValueError(f"{seq.request_id}: repetition_penalty must be positive and finite")
         slots = free[: len(sequences)]
         results = {}
         # prefill contiguous runs of slots together
@@ -396,6 +431,9 @@ class VerifyRunner:
             params = seq.sampling_params
             self.np_temp[slot] = max(float(params.temperature), 0.0)
             self.np_top_p[slot] = float(params.top_p)
+            if params.is_penalized:
+                self._set_penalties(slot, params)
+                self.prompt_len[slot : slot + 1].fill_(seq.num_prompt_tokens)
             pending.append([slot, seq, c, p])
         sl = slice(s0, s0 + n)
         self.history[sl, :width] = torch.from_numpy(hist)
@@ -467,9 +505,15 @@ class VerifyRunner:
             return
         last = hidden.index_select(0, (qs[:nf] + ql[:nf] - 1).long())
         sampled = bool((self.np_temp[s0 : s0 + nf] > 0).any())
-        logits, partials = self.model.compute_logits(last, logits=sampled, argmax=not sampled)
+        adjusted = bool(self.np_adjusted[s0 : s0 + nf].any())
+        logits, partials = self.model.compute_logits(last, logits=sampled or adjusted, argmax=not (sampled or adjusted))
         zeros = torch.zeros(nf, dtype=torch.int32, device=dev)
         sl = slice(s0, s0 + nf)
+        if adjusted:  # a prompt's last row: no guesses before it
+            p, first = self.penalties, slice(s0 * self.R, (s0 + nf) * self.R, self.R)
+            kernels.adjust_logits(logits, kernels.TokenPenalties(
+                self.history[sl], self.history_len[sl], self.prompt_len[sl], p.repetition[first].contiguous(),
+                p.presence[first].contiguous(), p.frequency[first].contiguous()), out=logits)
         kernels.accept(
             self.drafts[sl], zeros, torch.arange(nf, dtype=torch.int32, device=dev),
             self.model.config.vocab_size, logits=logits, argmax_partials=partials,
@@ -480,11 +524,12 @@ class VerifyRunner:
         )
 
     # ------------------------------------------------------------- verify step
-    def _device_step(self, sampled: bool, shared: bool) -> None:
+    def _device_step(self, sampled: bool, shared: bool, adjusted: bool = False) -> None:
         """Fixed-shape part of the verify step: pack, forward, LM head, accept.  ``sampled``:
         some slot samples, so the LM head writes every row's logits (greedy slots take
         their argmax from them); otherwise it writes only the argmax partials.  ``shared``:
-        attention reads the blocks that slots have in common once."""
+        attention reads the blocks that slots have in common once.  ``adjusted``: some slot has
+        penalties, which are applied to the logits where they lie."""
         kernels.prepare_verify_step(
             self.history, self.history_len, self.drafts, self.num_drafts, self.block_tables,
             self.block_size, self.pool.scratch_slot, self.tokens, self.positions, self.slot_mapping,
@@ -492,7 +537,7 @@ class VerifyRunner:
         )
         rows = self.max_seqs * self.R
         hidden = self.model.forward(rows, self.tokens, self.shared_batch if shared else self.batch, self.pool)
-        if not sampled:
+        if not sampled and not adjusted:
             self.model.compute_logits(hidden, logits=False, argmax=self.argmax_partials)
             logits = None
         else:
@@ -501,10 +546,12 @@ class VerifyRunner:
                                           device=self.device)
             self.model.compute_logits(hidden, logits=self.logits, argmax=False)
             logits = self.logits
+            if adjusted:
+                kernels.adjust_logits(logits, self.penalties, out=logits)
         draft_logits = None if not sampled or self.proposer is None else self.proposer.logits
         kernels.accept(
             self.drafts, self.num_drafts, self.row_start, self.model.config.vocab_size, logits=logits,
-            argmax_partials=None if sampled else self.argmax_partials,
+            argmax_partials=None if logits is not None else self.argmax_partials,
             temperature=self.temperatures, top_p=self.top_ps, any_sampled=sampled,
             seeds=self.seeds, steps=self.steps,
             out_tokens=self.out_tokens, num_out=self.num_out, history=self.history,
@@ -543,20 +590,20 @@ class VerifyRunner:
         torch.cuda.current_stream(self.device).synchronize()
 
     def _run_device_step(self) -> None:
-        sampled, shared = self.any_sampled, self.sharing
+        sampled, shared, adjusted = kind = self.any_sampled, self.sharing, self.any_adjusted
         if not self.graph_allowed():
-            self._device_step(sampled, shared)
+            self._device_step(*kind)
             return
-        graph = self._graphs.get((sampled, shared))
+        graph = self._graphs.get(kind)
         if graph is None:
             # this step runs eagerly (which also allocates lazily created buffers and
             # workspaces); the capture below only records, so nothing runs twice
-            self._device_step(sampled, shared)
+            self._device_step(*kind)
             torch.cuda.current_stream(self.device).synchronize()
             graph = torch.cuda.CUDAGraph()
             try:
                 with torch.cuda.graph(graph):
-                    self._device_step(sampled, shared)
+                    self._device_step(*kind)
             except torch.cuda.OutOfMemoryError:
                 # as cuda_graph_runner.py:193-207: without the memory to capture, every
                 # later step runs eagerly (this one already ran)
@@ -565,11 +612,11 @@ class VerifyRunner:
                 self._graphs.clear()
                 torch.cuda.empty_cache()
                 return
-            self._graphs[sampled, shared] = graph
+            self._graphs[kind] = graph
             self.model.bind_graph()
         else:
             graph.replay()
-        self.graph, self.graph_sampled, self.graph_shared = graph, sampled, shared
+        self.graph, self.graph_sampled, self.graph_shared, self.graph_adjusted = graph, sampled, shared, adjusted
 
     def step(self) -> dict[int, StepResult]:
         """One verify step over every active slot; returns what each slot emitted.
@@ -716,7 +763,8 @@ class VerifyRunner:
         free list holds the blocks the next step grows into (a pool that runs out raises
         at the next call, after this step's tokens are appended)."""
         if (not self.run_ahead or self.proposer is not None or self.trace is not None or not self._fifo_blocks
-                or self.graph is None or self.graph_sampled != self.any_sampled or len(self._stop_ids) > 64):
+                or self.graph is None or self.graph_sampled != self.any_sampled or self.graph_adjusted != self.any_adjusted
+                or len(self._stop_ids) > 64):
             return False
         out, num_out = self.np_out, self.np_num_out
         if not self.graph_allowed(self.np_len + num_out * act):  # the next step would run eagerly
@@ -741,7 +789,8 @@ class VerifyRunner:
         a stop token) is still run by the launched step, whose outputs for it are dropped
         when it completes.  The host mirrors are at the running step's start."""
         if (len(self._inflight) != 1 or not self.run_ahead or self.proposer is not None or self.trace is not None
-                or not self._fifo_blocks or self.graph is None or self.graph_sampled != self.any_sampled):
+                or not self._fifo_blocks or self.graph is None or self.graph_sampled != self.any_sampled
+                or self.graph_adjusted != self.any_adjusted):
             return
         running = self._inflight[0]
         act = self.np_active.copy()
@@ -894,3 +943,5 @@ class VerifyRunner:
             self.h_tables[slot].zero_()
         self.np_temp[slot] = 0.0
         self.np_top_p[slot] = 1.0
+        if self.np_adjusted is not None and self.np_adjusted[slot]:
+            self._set_penalties(slot, NO_PENALTIES)

@@ -64,7 +64,7 @@ def create_verify_engine(config: Qwen3Config, state_dict: dict[str, torch.Tensor
     weights = Qwen3Weights.from_state_dict(config, state_dict, device, dtype)
     max_seqs = settings.max_num_seqs if settings.is_batched else 1
     rows = max(max_seqs * (settings.num_speculative_tokens + 1), max_prefill_rows or settings.max_prefill_tokens)
-    model = Qwen3VerifyModel(weights, rows, device)
+    model = Qwen3VerifyModel(weights, rows, device, int8_activations=settings.int8_activations)
     proposer = None
     if settings.speculative == "draft":
         if draft_config is None or draft_state_dict is None:
