@@ -7,11 +7,23 @@
 // in fp32, rounded once to the output's type.
 //
 // The counts need no state from step to step: they come from the history itself, which the
-// caller holds anyway.  A work-group owns kRange tokens of one row, counts the history's tokens
-// of its range in LDS (integer atomics: no order matters) while its logits are on their way to
-// registers, and applies everything in one pass.  A word per token holds the output count in
-// its low 31 bits and "in the prompt" in its top bit.  A history is read once per range (19 of
-// 151,936 tokens), from the caches.
+// caller holds anyway.  A work-group owns a range of one row's tokens (4,096 or 8,192), counts the
+// history's tokens of its range in LDS (integer atomics: their order does not matter) while its
+// logits are on their way to registers, and applies everything in one pass over them.  So a history
+// is read once per range (19 or 38 times for 151,936 tokens), after the first from the L2s.
+//
+// A token has 16 bits of a table of counts: the output count below, "in the prompt" in the top bit;
+// and 16 bits of a second table for its bias, the entry's number in the row's list, so that of two
+// entries for one token the later one wins whatever the order of the lanes.  Histories of more than
+// 32,767 tokens and lists of more than 65,534 biases take words instead.  Half the LDS leaves room
+// for more work-groups per CU: 64 rows of 151,936 with 8 biases each and histories of up to 4,096 tokens,
+// bf16 to fp32, in 16.9 us against 18.3 with words for the biases and eight values per lane and load.
+//
+// Bound by memory where rows are many: those 64 rows move 58 MB (3.5 TB/s), 320 rows in bf16 behind
+// histories of up to 2,048 tokens 195 MB in 48 us (4.1 TB/s; a copy of 1 GiB reaches 5.1).  One row (4.5 us)
+// is the latency of its chain: arguments, history length, history, counts, stores.  A history of
+// 120,000 tokens is bound by its LDS atomics, 1,875 of a wave for each work-group: 16 rows of
+// 32,003 in 16.6 us, of which the logits themselves take 1.7.
 #include "ne_common.hpp"
 
 namespace ne {
@@ -46,15 +58,17 @@ struct AdjustParams {
 };
 
 using ConstF32 = __attribute__((address_space(4))) const float;  // as ConstI32
-constexpr int kMaxNarrow = 32767;
+constexpr int kMaxNarrowCount = 32767, kMaxNarrowBias = 65534;
 constexpr int kRowsPerSlice = 32767;  // of the grid
 
-// Eight values as they lie in memory, from any element's address (global accesses need not be
-// aligned).
-template <int DT>
+// VEC values as they lie in memory, from any element's address (global accesses need not be
+// aligned): 16 bytes of the wider of the two types, so that a wave's loads and stores are both
+// contiguous.
+template <int DT, int VEC>
 struct Raw {
-  static constexpr int kWords = DT == NE_DTYPE_FP32 ? 8 : 4;
-  uint32_t word[kWords];
+  static constexpr int kWords = DT == NE_DTYPE_FP32 ? VEC : VEC / 2;
+  typedef uint32_t vec __attribute__((ext_vector_type(kWords), aligned(2)));
+  vec word;
 };
 
 template <int DT>
@@ -62,55 +76,78 @@ __device__ __forceinline__ const void* element(const void* p, int64_t i) {
   return (const char*)p + i * (DT == NE_DTYPE_FP32 ? 4 : 2);
 }
 
-template <int DT>
-__device__ __forceinline__ Raw<DT> load8(const void* p, int64_t i) {
-  typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(2)));
-  Raw<DT> r;
-#pragma unroll
-  for (int w = 0; w < Raw<DT>::kWords; w += 4) {
-    const vec a = *(const vec*)((const char*)element<DT>(p, i) + w * 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r.word[w + e] = a[e];
+template <int DT, int VEC>
+__device__ __forceinline__ float value_of(const Raw<DT, VEC>& r, int e) {
+  if constexpr (DT == NE_DTYPE_FP32) {
+    return __uint_as_float(r.word[e]);
+  } else {
+    const uint32_t half = e % 2 ? r.word[e / 2] >> 16 : r.word[e / 2] & 0xFFFFu;
+    return DT == NE_DTYPE_BF16 ? bf16_to_f32((uint16_t)half) : f16_to_f32((uint16_t)half);
   }
-  return r;
 }
 
-template <int DT>
-__device__ __forceinline__ float value_of(const Raw<DT>& r, int e) {
-  if constexpr (DT == NE_DTYPE_FP32) return __uint_as_float(r.word[e]);
-  const uint32_t half = e % 2 ? r.word[e / 2] >> 16 : r.word[e / 2] & 0xFFFFu;
-  return DT == NE_DTYPE_BF16 ? bf16_to_f32((uint16_t)half) : f16_to_f32((uint16_t)half);
-}
-
-template <int DT>
-__device__ __forceinline__ void store8(void* p, int64_t i, const float (&f)[8]) {
-  typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(2)));
-  uint32_t word[Raw<DT>::kWords];
+template <int DT, int VEC>
+__device__ __forceinline__ void store_values(void* p, int64_t i, const float (&f)[VEC]) {
+  Raw<DT, VEC> r;
 #pragma unroll
-  for (int w = 0; w < Raw<DT>::kWords; ++w) {
+  for (int w = 0; w < Raw<DT, VEC>::kWords; ++w) {
     if constexpr (DT == NE_DTYPE_FP32) {
-      word[w] = __float_as_uint(f[w]);
+      r.word[w] = __float_as_uint(f[w]);
     } else if constexpr (DT == NE_DTYPE_BF16) {
-      word[w] = pack_bf16x2(f[2 * w], f[2 * w + 1]);
+      r.word[w] = pack_bf16x2(f[2 * w], f[2 * w + 1]);
     } else {
-      word[w] = (uint32_t)f32_to_f16(f[2 * w]) | (uint32_t)f32_to_f16(f[2 * w + 1]) << 16;
+      r.word[w] = (uint32_t)f32_to_f16(f[2 * w]) | (uint32_t)f32_to_f16(f[2 * w + 1]) << 16;
     }
   }
-#pragma unroll
-  for (int w = 0; w < Raw<DT>::kWords; w += 4)
-    *(vec*)((char*)element<DT>(p, i) + w * 4) = vec{word[w], word[w + 1], word[w + 2], word[w + 3]};
+  *(typename Raw<DT, VEC>::vec*)element<DT>(p, i) = r.word;
 }
 
-// WIDE: a 32-bit word per token; otherwise 16 bits (histories of at most kMaxNarrow tokens), two
-// to a word
+// A token's entry in an LDS table: a word, or (narrow) half of one.
+template <bool WIDE>
+__device__ __forceinline__ uint32_t entry_of(const uint32_t* table, int i) {
+  return WIDE ? table[i] : table[i / 2] >> i % 2 * 16 & 0xFFFFu;
+}
+
+// VEC entries from a multiple of VEC on
+template <bool WIDE, int VEC>
+struct Entries {
+  uint32_t word[WIDE ? VEC : VEC / 2];
+  __device__ __forceinline__ void read(const uint32_t* table, int i) {
+    constexpr int kWords = WIDE ? VEC : VEC / 2;
+    typedef uint32_t vec __attribute__((ext_vector_type(kWords > 4 ? 4 : kWords)));
+#pragma unroll
+    for (int w = 0; w < kWords; w += 4) {
+      const vec v = *(const vec*)(table + (WIDE ? i : i / 2) + w);
+#pragma unroll
+      for (int e = 0; e < 4 && w + e < kWords; ++e) word[w + e] = v[e];
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (uint32_t& w : word) w = 0;
+  }
+  __device__ __forceinline__ uint32_t any() const {
+    uint32_t a = 0;
+#pragma unroll
+    for (uint32_t w : word) a |= w;
+    return a;
+  }
+  __device__ __forceinline__ uint32_t at(int e) const {
+    return WIDE ? word[WIDE ? e : 0] : e % 2 ? word[e / 2] >> 16 : word[e / 2] & 0xFFFFu;
+  }
+};
+
+// WIDE: tables of 32-bit words; otherwise of 16 bits (histories of at most kMaxNarrowCount tokens and
+// at most kMaxNarrowBias biases).
 template <int IDT, int ODT, int THREADS, int VECTORS, bool WIDE, bool IN_PLACE>
 __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) {
-  constexpr int kVectors = VECTORS;
-  constexpr int kRange = THREADS * kVectors * 8;  // tokens of a work-group
-  constexpr int kCountWords = WIDE ? kRange : kRange / 2;
+  constexpr int VEC = ODT == NE_DTYPE_FP32 ? 4 : 8;
+  constexpr int kVectors = VECTORS * 8 / VEC;
+  constexpr int kRange = THREADS * VECTORS * 8;  // tokens of a work-group
+  constexpr int kTableWords = WIDE ? kRange : kRange / 2;
   constexpr uint32_t kInPrompt = WIDE ? 0x80000000u : 0x8000u;
-  extern __shared__ __attribute__((aligned(16))) uint32_t counts[];  // [kCountWords], then [kRange] bias entries + 1
-  uint32_t* const entries = counts + (p.history ? kCountWords : 0);
+  extern __shared__ __attribute__((aligned(16))) uint32_t counts[];  // [kTableWords], then the bias entries' numbers
+  uint32_t* const entries = counts + (p.history ? kTableWords : 0);
   // all arguments in one batch, before anything waits for one of them
   asm volatile("" ::"s"(p.logits), "s"(p.ld), "s"(p.out), "s"(p.ld_out), "s"(p.rows), "s"(p.vocab), "s"(p.history),
                "s"(p.row_seq), "s"(p.bias_start), "s"(p.allowed), "s"(p.allowed_rows));
@@ -122,28 +159,33 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
 
   // Logits are on their way while the history is counted: all of them, or those that the mask
   // does not ban; in place, only those that change are read at all, later.  The row's last
-  // vocab % 8 are taken one by one at the end.
-  Raw<IDT> raw[kVectors];
+  // vocab % VEC are taken one by one at the end.
+  Raw<IDT, VEC> raw[kVectors];
   uint32_t bits[kVectors];  // of this thread's tokens in the mask
-  auto token_of = [&](int v) { return base + (v * THREADS + tid) * 8; };
+  auto token_of = [&](int v) { return base + (v * THREADS + tid) * VEC; };
 #pragma unroll
-  for (int v = 0; v < kVectors; ++v) bits[v] = 0xFFu;
+  for (int v = 0; v < kVectors; ++v) bits[v] = (1u << VEC) - 1;
   if (p.allowed) {
     const int mask = p.allowed_rows ? ((ConstI32*)p.allowed_rows)[row] : row;
     if (mask >= 0) {
 #pragma unroll
-      for (int v = 0; v < kVectors; ++v)
+      for (int v = 0; v < kVectors; ++v) {
         bits[v] = mask < p.num_allowed && token_of(v) < p.vocab ? p.allowed[mask * p.allowed_stride + token_of(v) / 8] : 0u;
+        if (VEC == 4) bits[v] = bits[v] >> token_of(v) % 8 & 0xFu;
+      }
     }
   }
+  auto load = [&](int v) {
+    raw[v].word = *(const typename Raw<IDT, VEC>::vec*)element<IDT>(p.logits, (int64_t)row * p.ld + token_of(v));
+  };
   if constexpr (!IN_PLACE) {
 #pragma unroll
     for (int v = 0; v < kVectors; ++v)
-      if (bits[v] && token_of(v) + 8 <= p.vocab) raw[v] = load8<IDT>(p.logits, (int64_t)row * p.ld + token_of(v));
+      if (bits[v] && token_of(v) + VEC <= p.vocab) load(v);
   }
 
   if (counted || biased) {
-    const int words = (counted ? kCountWords : 0) + (biased ? kRange : 0);
+    const int words = (counted ? kTableWords : 0) + (biased ? kTableWords : 0);
     for (int i = tid * 4; i < words; i += THREADS * 4) *(u32x4*)(counts + i) = u32x4{0, 0, 0, 0};
     lds_barrier();
   }
@@ -207,11 +249,25 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
     if (tid < guesses) made(guess);
     for (int j = tid + THREADS; j < guesses; j += THREADS) made(drafts[j]);
   }
-  if (biased) {  // of a token listed twice the last entry counts
-    const int from = max(((ConstI32*)p.bias_start)[row], 0), to = min(((ConstI32*)p.bias_start)[row + 1], p.num_biases);
+  int from = 0;  // of the row's biases; of a token listed twice the last entry counts
+  if (biased) {
+    from = max(((ConstI32*)p.bias_start)[row], 0);
+    const int to = min(((ConstI32*)p.bias_start)[row + 1], p.num_biases);
     for (int i = from + tid; i < to; i += THREADS) {
       const uint32_t u = (uint32_t)(p.bias_tokens[i] - base);
-      if (u < limit) atomicMax(&entries[u], (uint32_t)i + 1);
+      if (u >= limit) continue;
+      if constexpr (WIDE) {
+        atomicMax(&entries[u], (uint32_t)(i - from) + 1);
+      } else {  // the larger number into half of a word
+        uint32_t* const word = &entries[u / 2];
+        const int shift = u % 2 * 16;
+        uint32_t old = *word;
+        while ((old >> shift & 0xFFFFu) < (uint32_t)(i - from) + 1) {
+          const uint32_t is = atomicCAS(word, old, (old & ~(0xFFFFu << shift)) | (uint32_t)(i - from + 1) << shift);
+          if (is == old) break;
+          old = is;
+        }
+      }
     }
   }
   if (counted || biased) lds_barrier();
@@ -225,51 +281,41 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
       const uint32_t n = word & ~kInPrompt;
       if (n != 0) x -= frequency * (float)n + presence;
     }
-    if (entry != 0) x += p.bias_values[entry - 1];
+    if (entry != 0) x += p.bias_values[from + (int)entry - 1];
     return bit ? x : -__builtin_inff();
   };
 #pragma unroll
   for (int v = 0; v < kVectors; ++v) {
-    const int local = (v * THREADS + tid) * 8;
+    const int local = (v * THREADS + tid) * VEC;
     const int token = base + local;
-    if (token + 8 <= p.vocab) {
-      u32x4 c[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}}, b[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-      if (counted) {
-        c[0] = *(const u32x4*)(counts + (WIDE ? local : local / 2));
-        if (WIDE) c[1] = *(const u32x4*)(counts + local + 4);
-      }
-      if (biased) {
-        b[0] = *(const u32x4*)(entries + local);
-        b[1] = *(const u32x4*)(entries + local + 4);
-      }
-      const u32x4 any = c[0] | c[1] | b[0] | b[1];
-      const bool touched = (any[0] | any[1] | any[2] | any[3]) != 0;
+    if (token + VEC <= p.vocab) {
+      Entries<WIDE, VEC> c, b;
+      c.clear();
+      b.clear();
+      if (counted) c.read(counts, local);
+      if (biased) b.read(entries, local);
+      const bool touched = (c.any() | b.any()) != 0;
       if constexpr (IN_PLACE) {
-        if (!touched && bits[v] == 0xFFu) continue;
-        if (bits[v]) raw[v] = load8<IDT>(p.logits, (int64_t)row * p.ld + token);
+        if (!touched && bits[v] == (1u << VEC) - 1) continue;
+        if (bits[v]) load(v);
       }
-      float x[8];
+      float x[VEC];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = value_of(raw[v], e);
+      for (int e = 0; e < VEC; ++e) x[e] = value_of(raw[v], e);
       if (touched) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t word = WIDE ? c[e / 4][e % 4] : e % 2 ? c[0][e / 2] >> 16 : c[0][e / 2] & 0xFFFFu;
-          x[e] = adjusted(x[e], word, b[e / 4][e % 4], 1);
-        }
+        for (int e = 0; e < VEC; ++e) x[e] = adjusted(x[e], c.at(e), b.at(e), 1);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < VEC; ++e)
         if (!(bits[v] >> e & 1)) x[e] = -__builtin_inff();
-      store8<ODT>(p.out, (int64_t)row * p.ld_out + token, x);
+      store_values<ODT, VEC>(p.out, (int64_t)row * p.ld_out + token, x);
     } else {
       for (int e = 0; token + e < p.vocab; ++e) {
         const float x = load_scale<IDT>(p.logits, (int64_t)row * p.ld + token + e);
-        const int at = local + e;
-        uint32_t word = 0;
-        if (counted) word = WIDE ? counts[at] : counts[at / 2] >> at % 2 * 16 & 0xFFFFu;
         store_scale<ODT>(p.out, (int64_t)row * p.ld_out + token + e,
-                         adjusted(x, word, biased ? entries[at] : 0, bits[v] >> e & 1));
+                         adjusted(x, counted ? entry_of<WIDE>(counts, local + e) : 0,
+                                  biased ? entry_of<WIDE>(entries, local + e) : 0, bits[v] >> e & 1));
       }
     }
   }
@@ -280,7 +326,7 @@ int launch_ranges(const AdjustParams& p, hipStream_t stream) {
   constexpr int kRange = THREADS * VECTORS * 8;
   NE_CHECK_SUPPORTED(p.rows <= kRowsPerSlice * 65535, "too many rows: %d", p.rows);
   const dim3 grid(ceil_div(p.vocab, kRange), p.rows < kRowsPerSlice ? p.rows : kRowsPerSlice, ceil_div(p.rows, kRowsPerSlice));
-  const size_t lds = (p.history ? kRange * (WIDE ? 4 : 2) : 0) + (p.bias_start ? kRange * 4 : 0);
+  const size_t lds = ((p.history ? 1 : 0) + (p.bias_start ? 1 : 0)) * kRange * (WIDE ? 4 : 2);
   if constexpr (IDT == ODT) {
     if (p.out == p.logits) {
       hipLaunchKernelGGL((adjust_logits_kernel<IDT, ODT, THREADS, VECTORS, WIDE, true>), grid, dim3(THREADS), lds, stream, p);
@@ -296,7 +342,8 @@ int launch_ranges(const AdjustParams& p, hipStream_t stream) {
 // are read by 16 waves, 16 rows of 32,003 with up to 120,000 tokens in 16.6 us (8 waves 21-23).
 template <int IDT, int ODT>
 int launch_adjust(const AdjustParams& p, hipStream_t stream) {
-  if (p.history && (int64_t)p.capacity + p.max_drafts > kMaxNarrow) return launch_ranges<IDT, ODT, 1024, 1, true>(p, stream);
+  const bool wide = p.history && (int64_t)p.capacity + p.max_drafts > kMaxNarrowCount;
+  if (wide || (p.bias_start && p.num_biases > kMaxNarrowBias)) return launch_ranges<IDT, ODT, 1024, 1, true>(p, stream);
   if ((int64_t)p.rows * ceil_div(p.vocab, 8192) <= 2 * kNumCu) return launch_ranges<IDT, ODT, 512, 1, false>(p, stream);
   return launch_ranges<IDT, ODT, 512, 2, false>(p, stream);
 }

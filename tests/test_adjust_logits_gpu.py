@@ -211,6 +211,27 @@ def test_a_token_listed_twice_takes_its_last_bias():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [9000, 30001])
+@pytest.mark.parametrize("penalty", [False, True])
+def test_lists_of_many_biases(vocab, penalty):
+    """More entries than 16 bits count, most of them for a token that is listed again."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    logits = make_logits(3, vocab, "bf16")
+    tokens = (torch.rand(66500, device="cuda", generator=g) * vocab).int()
+    start = torch.tensor([0, 700, 66400, 66500], device="cuda", dtype=torch.int32)
+    bias = kernels.TokenBias(start, tokens, 4 * torch.randn(66500, device="cuda", generator=g))
+    kw = dict(bias=bias, penalties=make_penalties(3, vocab) if penalty else None)
+    check(kernels.adjust_logits(logits, **kw), logits, **kw)
+    # the same lists, each in a call of its own
+    for row in range(3):
+        a, b = int(start[row]), int(start[row + 1])
+        one = kernels.TokenBias(torch.tensor([0, b - a], device="cuda", dtype=torch.int32), tokens[a:b], bias.values[a:b])
+        if not penalty:
+            whole = kernels.adjust_logits(logits, bias=bias)
+            assert torch.equal(kernels.adjust_logits(logits[row : row + 1], bias=one), whole[row : row + 1])
+
+
+@pytest.mark.gpu
 def test_infinities_and_nan_and_rows_that_allow_nothing():
     vocab = 700
     logits = make_logits(4, vocab, "fp32")
