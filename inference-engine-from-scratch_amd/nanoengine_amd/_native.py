@@ -224,6 +224,8 @@ def library_path() -> Path:
 def load() -> ctypes.CDLL:
     """Load the library once; raise if it is missing or has another ABI version."""
     global _library
+    if _library is not None:
+        return _library
     with _lock:
         if _library is not None:
             return _library

@@ -736,7 +736,7 @@ def w8a16_gemm(
 def _launch(index: int, name: str, *args) -> None:
     """An entry point on device ``index``'s current torch stream (the last argument), that device current."""
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         _native.call(name, *args, stream)
     else:
         with torch.cuda.device(index):
@@ -746,11 +746,11 @@ def _launch(index: int, name: str, *args) -> None:
 def _code_outputs(x: torch.Tensor, codes, scales) -> tuple[torch.Tensor, torch.Tensor]:
     rows, k = x.shape
     if codes is None:
-        codes = x.new_empty((rows, k), dtype=torch.int8)
+        codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     elif codes.dtype != torch.int8 or codes.shape != x.shape or not codes.is_contiguous() or codes.device != x.device:
         raise ValueError(f"codes must be contiguous int8 [{rows}, {k}] on {x.device}")
     if scales is None:
-        scales = x.new_empty((rows,), dtype=torch.float32)
+        scales = x.new_empty(rows, dtype=torch.float32)
     elif scales.dtype != torch.float32 or scales.shape != (rows,) or not scales.is_contiguous() or scales.device != x.device:
         raise ValueError(f"scales must be contiguous fp32 [{rows}] on {x.device}")
     return codes, scales
@@ -835,7 +835,7 @@ def w8a8_gemm(
         raise ValueError("weight_scale must be contiguous, one per weight row")
     n_out = n // 2 if epilogue == EPILOGUE_SWIGLU else n
     if out is None:
-        out = codes.new_empty((m, n_out), dtype=torch.bfloat16)
+        out = codes.new_empty(m, n_out, dtype=torch.bfloat16)
     elif out.shape != (m, n_out) or out.dtype != torch.bfloat16 or out.stride(1) != 1 and n_out > 1 or out.get_device() != index:
         raise ValueError(f"out must be bf16 [{m}, {n_out}] with contiguous rows on cuda:{index}")
     _launch(index, "ne_w8a8_gemm", codes.data_ptr(), codes.stride(0) if m > 1 else k, scales.data_ptr(), weight_int8.data_ptr(),
@@ -1169,7 +1169,7 @@ def accept(
 
 
 # ------------------------------------------------------------ adjusting logits
-@dataclass(frozen=True)
+@dataclass(slots=True)  # (one is made per step; frozen would take twice as long)
 class TokenPenalties:
     """Penalties for the tokens of each sequence so far, for :func:`adjust_logits`: device tensors that a
     step reads, so their contents may change between replays of a graph.
@@ -1191,7 +1191,7 @@ class TokenPenalties:
     row_drafts: torch.Tensor | None = None  # [rows] int32
 
 
-@dataclass(frozen=True)
+@dataclass(slots=True)  # (one is made per step; frozen would take twice as long)
 class TokenBias:
     """Biases of single tokens, for :func:`adjust_logits`: entries ``start[r] .. start[r + 1]`` are row r's."""
 
@@ -1319,7 +1319,7 @@ def adjust_logits(
         raise ValueError("logits must be bf16, fp16 or fp32")
     rows, vocab = logits.shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=dtype, device=logits.device)
+        out = logits.new_empty(rows, vocab)
     elif out is not logits:
         if (out.dtype not in (dtype, torch.float32) or out.shape != logits.shape or out.get_device() != index
                 or out.stride(1) != 1 and vocab > 1):
