@@ -221,6 +221,8 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(RowsParams p) 
 template <int MODE, int VDT>
 int launch_rows(const RowsParams& p, hipStream_t stream) {
   const dim3 four(ceil_div(p.rows, 4)), one(p.rows), block(256);
+  // a launch has fewer than 2^32 threads
+  NE_CHECK_SUPPORTED(p.rows < (p.k <= 4096 ? 1 << 26 : p.k <= 16384 ? 1 << 24 : 1 << 22), "too many rows of %d: %d", p.k, p.rows);
 #define NE_ROWS(CPL, WAVES, GRID) \
   hipLaunchKernelGGL((quantize_rows_kernel<MODE, VDT, CPL, WAVES>), GRID, block, 0, stream, p)
   if (p.k <= 512) {

@@ -610,12 +610,15 @@ extern "C" int ne_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, 
   NE_CHECK_SUPPORTED(epilogue == NE_EPILOGUE_STORE || n % 32 == 0, "paired gate and up rows come in groups of 32 (n=%d)", n);
   NE_CHECK_ARG(scale_dtype == NE_DTYPE_BF16 || scale_dtype == NE_DTYPE_FP16 || scale_dtype == NE_DTYPE_FP32,
                "scale_dtype must be bf16, fp16 or fp32");
+  NE_CHECK_SUPPORTED(m <= (1 << 30) && n <= (1 << 30), "m and n must be at most 2^30 (got %d, %d)", m, n);
   if (m == 0) return NE_OK;
   NE_CHECK_ARG(x && x_scale && w && w_scale && y, "null pointer argument");
   NE_CHECK_ARG(ldx >= k && ldx % 16 == 0 && ldx < (1 << 23), "ldx must be >= k, a multiple of 16 and below 2^23 (got %lld)",
                (long long)ldx);
   NE_CHECK_ARG(ldy >= (epilogue == NE_EPILOGUE_SWIGLU ? n / 2 : n), "ldy too small (%lld)", (long long)ldy);
   NE_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0, "x and w must be 16-byte aligned");
+  NE_CHECK_ARG((uintptr_t)x_scale % 4 == 0 && (uintptr_t)w_scale % (scale_dtype == NE_DTYPE_FP32 ? 4 : 2) == 0 && (uintptr_t)y % 2 == 0,
+               "scales or y off their type's alignment");
   const W8a8Params p{x, ldx, x_scale, w, w_scale, scale_dtype, m, n, k, (uint16_t*)y, ldy, 0, 0};
   return epilogue == NE_EPILOGUE_SWIGLU ? launch_kernel<NE_EPILOGUE_SWIGLU>(p, (hipStream_t)stream)
                                         : launch_kernel<NE_EPILOGUE_STORE>(p, (hipStream_t)stream);

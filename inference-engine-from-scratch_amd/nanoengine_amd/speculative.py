@@ -66,7 +66,8 @@ class NgramProposer:
 def verify_proposal(proposal: Proposal, target_logits: torch.Tensor, params: SamplingParams,
                     generator: SamplingStream) -> list[int]:
     """Kept guesses plus one target token (verifier.py:27-60) from device logits, with the
-    request's temperature and top-p (sampling.py:21-38).
+    request's temperature and top-p (sampling.py:21-38).  Penalties and biases are the caller's to
+    apply beforehand (``kernels.adjust_logits``: row i counts the i guesses before it).
 
     ``proposal.probabilities`` (a sampled draft) are the fp32 distributions the guesses
     were drawn from; the kernel uses them as given, as the reference does

@@ -280,6 +280,27 @@ def test_strides_and_what_lies_beside_the_rows(dtype):
 
 
 @pytest.mark.gpu
+def test_logits_past_32_bit_offsets():
+    """2.3 10^9 logits, in place and not: the rows around the limits against their definition."""
+    rows, vocab = 15_000, 151_936
+    base = make_logits(8, vocab, "bf16", seed=9)
+    logits = base.repeat(rows // 8, 1)
+    p = make_penalties(rows, vocab, capacity=300, seed=9)
+    before = logits.clone()
+    got = kernels.adjust_logits(logits, penalties=p)
+    assert torch.equal(logits, before)
+    del before
+    kernels.adjust_logits(logits, penalties=p, out=logits)
+    for row in (0, (1 << 31) // vocab, rows - 1):
+        one = slice(row, row + 1)
+        part = kernels.TokenPenalties(p.history[one], p.history_len[one], p.prompt_len[one], p.repetition[one], p.presence[one],
+                                      p.frequency[one])
+        check(got[one], base[row % 8 : row % 8 + 1], penalties=part)
+        assert torch.equal(got[one], logits[one])
+    assert torch.equal(got, logits)
+
+
+@pytest.mark.gpu
 def test_captured_call_follows_its_inputs():
     rows, vocab = 8, 30000
     logits = make_logits(rows, vocab, "bf16")

@@ -13,10 +13,12 @@ from nanoengine_amd.config import EngineSettings
 from nanoengine_amd.int8_quantization import Int8Linear, quantize_linear_layers
 from nanoengine_amd.interface import SamplingParams, sampling_uniform
 from nanoengine_amd.memory import KVCachePool
-from nanoengine_amd.qwen3 import AttentionBatch, Qwen3VerifyModel, Qwen3Weights
+from nanoengine_amd.qwen3 import AttentionBatch, Qwen3VerifyModel, Qwen3Weights, random_state_dict
 from nanoengine_amd.sequence_state import Sequence
 from test_adjust_logits_gpu import check, reference
 from test_answers import CFG, build, engine, request, unit_norms
+from test_draft_gpu import DCFG
+from test_draft_gpu import engine as draft_engine
 from test_sample_gpu import reference_row
 from test_w8a8_gpu import check_product, rows_reference
 
@@ -196,6 +198,31 @@ def test_penalties_come_and_go_in_eager_and_captured_steps():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("graphs", [False, True])
+def test_penalties_with_a_draft_models_guesses(graphs):
+    """The target's penalties hold whatever another model guesses, greedy and sampled: no token comes
+    twice under so large a penalty."""
+    draft = random_state_dict(DCFG, seed=7, std=0.02)
+    ways = [dict(presence_penalty=1000.0), dict(presence_penalty=1000.0, temperature=0.8), dict(),
+            dict(frequency_penalty=1000.0, temperature=1.2)]
+    runner = draft_engine(unit_norms(), DCFG, draft, len(ways), graphs=graphs).runner
+    runner.trace = None if graphs else []
+    seqs = [Sequence.from_request(request(f"{i}", [5, 6, 7, 8] * 5 + [i], **penalized(i, **w))) for i, w in enumerate(ways)]
+    runner.add(seqs)
+    while min(s.num_generated_tokens for s in seqs) < 24:
+        runner.step()
+    assert runner.proposer.forwards > 0 and runner.any_adjusted
+    assert not graphs or (runner.graph is not None and runner.graph_adjusted)
+    for s, way in zip(seqs, ways):
+        made = s.token_ids[s.num_prompt_tokens :]
+        assert len(set(made)) == len(made) or not way
+    for step in runner.trace or []:  # what was kept was guessed
+        for rec in step.values():
+            kept = len(rec["out"]) - 1
+            assert rec["out"][:kept] == rec["drafts"][:kept]
+
+
+@pytest.mark.gpu
 def test_verification_refuses_what_it_does_not_take():
     runner = engine(unit_norms(), 2, False, False).runner
     for kw in (dict(logit_bias={1: 1.0}), dict(repetition_penalty=0.0), dict(repetition_penalty=float("inf"))):
@@ -233,8 +260,7 @@ def test_prompts_through_the_8_bit_products(int8_cache, monkeypatch):
     pool, c, eps = pools[2], CFG, CFG.rms_norm_eps
     res, x = kernels.embed_rmsnorm(tokens, weights.embed, weights.layers[0].input_layernorm, eps)
     for i, layer in enumerate(weights.layers):
-        qkv = kernels.w8a8_gemm(*kernels.quantize_rows(x), layer.qkv_int8, layer.qkv_scale) if QKV_IN_8_BITS \
-            else kernels.w8a16_gemm(x, layer.qkv_int8, layer.qkv_scale)
+        qkv = kernels.w8a16_gemm(x, layer.qkv_int8, layer.qkv_scale)
         q = kernels.qk_norm_rope_kv_write(qkv, c.num_attention_heads, c.num_key_value_heads, layer.q_norm, layer.k_norm, eps,
                                           positions, model.rope, slots, pool.key_caches[i], pool.value_caches[i],
                                           pool.key_scale_2d(i), pool.value_scale_2d(i))
@@ -249,9 +275,6 @@ def test_prompts_through_the_8_bit_products(int8_cache, monkeypatch):
     # fewer rows keep 16-bit activations
     few = AttentionBatch(positions[:90], slots[:90], batch.q_start[:1], lengths[:1], lengths[:1], tables[:1], 90, 90)
     assert torch.equal(model.forward(90, tokens, few, pools[0]), other.forward(90, tokens, few, pools[1]))
-
-
-QKV_IN_8_BITS = False
 
 
 @pytest.mark.gpu

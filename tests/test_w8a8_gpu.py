@@ -210,6 +210,40 @@ def test_a_row_has_the_same_bits_in_every_batch():
 
 
 @pytest.mark.gpu
+def test_rows_and_outputs_past_32_bit_offsets():
+    """2.3 10^9 codes and 4.5 10^9 outputs: the last rows have the bits that they have by themselves."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    m, k, n = 1_100_003, 2048, 4096
+    x = torch.randn(40, k, device="cuda", generator=g).bfloat16()
+    rows = x.repeat(m // 40 + 1, 1)[:m]
+    codes, scales = kernels.quantize_rows(rows)
+    del rows
+    few = kernels.quantize_rows(x)
+    order = torch.arange(m - 300, m, device="cuda") % 40
+    assert torch.equal(codes[-300:], few[0][order]) and torch.equal(scales[-300:], few[1][order])
+    w = torch.randint(-127, 128, (n, k), device="cuda", dtype=torch.int8, generator=g)
+    ws = torch.rand(n, device="cuda", generator=g) * 0.01
+    y = kernels.w8a8_gemm(codes, scales, w, ws)
+    want = kernels.w8a8_gemm(*few, w, ws)
+    for at in (0, (1 << 31) // n - 20, (1 << 32) // n - 20, m - 40):
+        assert torch.equal(y[at : at + 40], want[torch.arange(at, at + 40, device="cuda") % 40])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 70, 700])
+def test_weights_past_32_bit_offsets(m):
+    g = torch.Generator(device="cuda").manual_seed(m)
+    n, k = 33_000, 131_056
+    w = torch.randint(-3, 4, (500, k), device="cuda", dtype=torch.int8, generator=g).repeat(n // 500, 1)
+    ws = torch.rand(500, device="cuda", generator=g).repeat(n // 500) * 0.01
+    codes = torch.randint(-127, 128, (m, k), device="cuda", dtype=torch.int8, generator=g)
+    scales = torch.rand(m, device="cuda", generator=g)
+    y = kernels.w8a8_gemm(codes, scales, w, ws).view(m, n // 500, 500)
+    assert torch.equal(y, y[:, :1].expand_as(y))
+    check_product(y[:, -1].contiguous(), codes, scales, w[:500], ws[:500])
+
+
+@pytest.mark.gpu
 def test_no_rows():
     codes, scales, w, w_scale = make(4, 64, 64)
     assert kernels.w8a8_gemm(codes[:0], scales[:0], w, w_scale).shape == (0, 64)
@@ -299,9 +333,12 @@ def test_entry_points_refuse_bad_arguments_without_launching():
 
     assert gemm(m=0, x=null) == 0
     for bad in (dict(m=-1), dict(n=0), dict(k=0), dict(epilogue=7), dict(dt=3), dict(x=null), dict(xs=null), dict(ws=null),
-                dict(y=null), dict(x=odd), dict(w=odd), dict(ldx=48), dict(ldx=72), dict(ldx=1 << 23), dict(ldy=63)):
+                dict(y=null), dict(x=odd), dict(w=odd), dict(ldx=48), dict(ldx=72), dict(ldx=1 << 23), dict(ldy=63),
+                dict(xs=ctypes.c_void_p(258)), dict(ws=ctypes.c_void_p(257)), dict(ws=ctypes.c_void_p(258), dt=2),
+                dict(y=ctypes.c_void_p(257))):
         assert gemm(**bad) == -1, bad
-    for bad in (dict(k=72, ldx=80), dict(k=131072, ldx=131072), dict(epilogue=1, n=48)):
+    for bad in (dict(k=72, ldx=80), dict(k=131072, ldx=131072), dict(epilogue=1, n=48), dict(m=(1 << 30) + 1),
+                dict(n=(1 << 30) + 1, ldy=1 << 31)):
         assert gemm(**bad) == -2, bad
     assert lib.ne_quantize_rows(p, 0, 64, 0, 64, null, null, null) == 0
     assert lib.ne_quantize_rows(p, 2, 64, 4, 64, p, p, null) == -1
@@ -309,6 +346,9 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     assert lib.ne_quantize_rows(odd, 0, 64, 4, 64, p, p, null) == -1
     assert lib.ne_quantize_rows(p, 0, 64, 4, 60, p, p, null) == -2
     assert lib.ne_quantize_rows(null, 0, 64, 4, 64, p, p, null) == -1
+    for rows, k in ((1 << 26, 8), (1 << 26, 4096), (1 << 24, 4104), (1 << 22, 16392)):  # 2^32 threads
+        assert lib.ne_quantize_rows(p, 0, k, rows, k, p, p, null) == -2
+    assert lib.ne_rmsnorm_quantize(p, p, p, p, 1 << 26, 64, 1e-6, null) == -2
     assert lib.ne_rmsnorm_quantize(p, null, p, p, 4, 64, 1e-6, null) == -1
     assert lib.ne_rmsnorm_quantize(p, p, p, p, 4, 4104, 1e-6, null) == -2
     assert lib.ne_add_rmsnorm_quantize(p, odd, p, p, p, 4, 64, 1e-6, null) == -1
