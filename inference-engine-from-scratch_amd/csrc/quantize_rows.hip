@@ -8,7 +8,9 @@
 // NaN above all: a row that holds one gets the scale NaN and codes 0, so that what it is
 // multiplied into is NaN, as with the row itself.  Norm rows are the bits that ne_rmsnorm and
 // ne_add_rmsnorm store (same sums in the same order, both roundings), quantised without the
-// trip through memory.  What bounds it: memory, each row read once into registers.
+// trip through memory.  Bound by memory where rows are many, each read once into registers (8,192 x
+// 8,192 fp16 39 us, 5.2 TB/s; 4,001 x 2,048 9.2, of which ~2 are the launch; norm 8,192 x 1,024 9-10.6);
+// few rows take a chain of one load, two reductions and a store (2.2-3.5 us).
 #include "ne_common.hpp"
 
 namespace ne {
@@ -218,29 +220,39 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(RowsParams p) 
     *(u32x2*)(dst + (int64_t)ci * 8) = quantize8<VDT>(*(const u32x4*)(src + (int64_t)ci * 8), s, rcp);
 }
 
+// Few waves per row leave a wave more to do, many take two rounds of the CUs.  us, one wave per row / four:
+// 64 x 2,048 5.3 / 4.6, 320 x 2,048 4.5 / 3.9, 4,001 x 2,048 9.2 / 9.6, 20,000 x 2,048 23.4 / 30.6;
+// 64 x 4,096 5.3 / 3.9, 4,001 x 4,096 15.3 / 12.8, 20,000 x 4,096 42.6 / 41.2.  The norm's sum keeps
+// ne_rmsnorm's order, one wave per row.
 template <int MODE, int VDT>
 int launch_rows(const RowsParams& p, hipStream_t stream) {
   const dim3 four(ceil_div(p.rows, 4)), one(p.rows), block(256);
   // a launch has fewer than 2^32 threads
-  NE_CHECK_SUPPORTED(p.rows < (p.k <= 4096 ? 1 << 26 : p.k <= 16384 ? 1 << 24 : 1 << 22), "too many rows of %d: %d", p.k, p.rows);
+  NE_CHECK_SUPPORTED(p.rows < (p.k <= (MODE == kPlain ? 2048 : 4096) ? 1 << 26 : p.k <= 16384 ? 1 << 24 : 1 << 22), "too many rows of %d: %d", p.k, p.rows);
 #define NE_ROWS(CPL, WAVES, GRID) \
   hipLaunchKernelGGL((quantize_rows_kernel<MODE, VDT, CPL, WAVES>), GRID, block, 0, stream, p)
   if (p.k <= 512) {
     NE_ROWS(1, 1, four);
   } else if (p.k <= 1024) {
     NE_ROWS(2, 1, four);
-  } else if (p.k <= 2048) {
-    NE_ROWS(4, 1, four);
-  } else if (p.k <= 4096) {
-    NE_ROWS(8, 1, four);
   } else if constexpr (MODE == kPlain) {
-    if (p.k <= 8192) {
+    if (p.k <= 2048 && p.rows <= 2 * kNumCu) {
+      NE_ROWS(1, 4, one);
+    } else if (p.k <= 2048) {
+      NE_ROWS(4, 1, four);
+    } else if (p.k <= 4096) {
+      NE_ROWS(2, 4, one);
+    } else if (p.k <= 8192) {
       NE_ROWS(4, 4, one);
     } else if (p.k <= 16384) {
       NE_ROWS(8, 4, one);
     } else {
       hipLaunchKernelGGL(quantize_long_rows_kernel<VDT>, one, dim3(1024), 0, stream, p);
     }
+  } else if (p.k <= 2048) {
+    NE_ROWS(4, 1, four);
+  } else {
+    NE_ROWS(8, 1, four);
   }
 #undef NE_ROWS
   return check_launch("quantize_rows");

@@ -72,7 +72,8 @@ def check_product(got, codes, scales, w, w_scale, epilogue=EPILOGUE_STORE) -> No
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("rows,k", [(1, 8), (3, 16), (5, 504), (4, 512), (7, 520), (9, 1024), (2, 2040), (6, 4096),
-                                    (3, 4104), (2, 8192), (3, 16376), (2, 16392), (1, 131056), (1025, 128)])
+                                    (3, 4104), (2, 8192), (3, 16376), (2, 16392), (1, 131056), (1025, 128),
+                                    (512, 2048), (513, 2048), (514, 1032), (30, 2056)])
 def test_quantize_rows(rows, k, dtype):
     g = torch.Generator(device="cuda").manual_seed(rows * k)
     x = torch.randn(rows, k, device="cuda", generator=g) * (0.01 + 50 * torch.rand(rows, 1, device="cuda", generator=g))
@@ -346,7 +347,7 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     assert lib.ne_quantize_rows(odd, 0, 64, 4, 64, p, p, null) == -1
     assert lib.ne_quantize_rows(p, 0, 64, 4, 60, p, p, null) == -2
     assert lib.ne_quantize_rows(null, 0, 64, 4, 64, p, p, null) == -1
-    for rows, k in ((1 << 26, 8), (1 << 26, 4096), (1 << 24, 4104), (1 << 22, 16392)):  # 2^32 threads
+    for rows, k in ((1 << 26, 8), (1 << 26, 2048), (1 << 24, 4096), (1 << 24, 4104), (1 << 22, 16392)):  # 2^32 threads
         assert lib.ne_quantize_rows(p, 0, k, rows, k, p, p, null) == -2
     assert lib.ne_rmsnorm_quantize(p, p, p, p, 1 << 26, 64, 1e-6, null) == -2
     assert lib.ne_rmsnorm_quantize(p, null, p, p, 4, 64, 1e-6, null) == -1
