@@ -17,13 +17,18 @@
 // entries for one token the later one wins whatever the order of the lanes.  Histories of more than
 // 32,767 tokens and lists of more than 65,534 biases take words instead.  Half the LDS leaves room
 // for more work-groups per CU: 64 rows of 151,936 with 8 biases each and histories of up to 4,096 tokens,
-// bf16 to fp32, in 16.9 us against 18.3 with words for the biases and eight values per lane and load.
+// bf16 to fp32, took 16.9 us with 16 bits for both against 18.3 with words for the biases.
 //
-// Bound by memory where rows are many: those 64 rows move 58 MB (3.5 TB/s), 320 rows in bf16 behind
-// histories of up to 2,048 tokens 195 MB in 48 us (4.1 TB/s; a copy of 1 GiB reaches 5.1).  One row (4.5 us)
-// is the latency of its chain: arguments, history length, history, counts, stores.  A history of
-// 120,000 tokens is bound by its LDS atomics, 1,875 of a wave for each work-group: 16 rows of
-// 32,003 in 16.6 us, of which the logits themselves take 1.7.
+// Tokens of other ranges count into a spare word of their lane, which takes three instructions where
+// leaving their lanes out takes five; a wave knows from its first token which side of the prompt's end it
+// is on, and has four loads in flight.  That is 16.0 us for those 64 rows, and 44.0 against 48 for 320
+// rows in bf16 behind histories of up to 2,048 tokens.
+//
+// Bound by memory where rows are many: the 64 rows move 58 MB (3.6 TB/s), the 320 rows 195 MB (4.4
+// TB/s; a copy of 1 GiB reaches 5.1).  One row (4.5 us) is the latency of its chain: arguments, history
+// length, history, counts, stores.  Long histories of repetitive text are bound by LDS atomics on
+// the same tokens: 16 rows of 32,003 with up to 120,000 tokens, the commonest of them 7.5 %, take 16.4 us
+// (12.9 where all tokens are alike and in the caches, 5.7 without a history; the logits alone 1.7).
 #include "ne_common.hpp"
 
 namespace ne {
@@ -145,9 +150,10 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
   constexpr int kVectors = VECTORS * 8 / VEC;
   constexpr int kRange = THREADS * VECTORS * 8;  // tokens of a work-group
   constexpr int kTableWords = WIDE ? kRange : kRange / 2;
+  constexpr int kCountWords = kTableWords + kWave;  // and a spare word per lane, for tokens of other ranges
   constexpr uint32_t kInPrompt = WIDE ? 0x80000000u : 0x8000u;
-  extern __shared__ __attribute__((aligned(16))) uint32_t counts[];  // [kTableWords], then the bias entries' numbers
-  uint32_t* const entries = counts + (p.history ? kTableWords : 0);
+  extern __shared__ __attribute__((aligned(16))) uint32_t counts[];  // [kCountWords], then the bias entries' numbers [kTableWords]
+  uint32_t* const entries = counts + (p.history ? kCountWords : 0);
   // all arguments in one batch, before anything waits for one of them
   asm volatile("" ::"s"(p.logits), "s"(p.ld), "s"(p.out), "s"(p.ld_out), "s"(p.rows), "s"(p.vocab), "s"(p.history),
                "s"(p.row_seq), "s"(p.bias_start), "s"(p.allowed), "s"(p.allowed_rows));
@@ -185,7 +191,7 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
   }
 
   if (counted || biased) {
-    const int words = (counted ? kTableWords : 0) + (biased ? kTableWords : 0);
+    const int words = (counted ? kCountWords : 0) + (biased ? kTableWords : 0);
     for (int i = tid * 4; i < words; i += THREADS * 4) *(u32x4*)(counts + i) = u32x4{0, 0, 0, 0};
     lds_barrier();
   }
@@ -203,49 +209,64 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
     if (ahead) first = *(const vec*)(tokens + tid * 4);
     const int len = min(max(((ConstI32*)p.history_len)[seq], 0), p.capacity);
     const int prompt = p.prompt_len ? min(max(((ConstI32*)p.prompt_len)[seq], 0), len) : 0;
+    const int lane = tid % kWave;
+    const uint32_t spare = kRange + (WIDE ? lane : 2 * lane);
     auto seen = [&](int token) {
-      const uint32_t u = (uint32_t)(token - base);
-      if (u < limit) atomicOr(&counts[WIDE ? u : u / 2], WIDE ? kInPrompt : kInPrompt << u % 2 * 16);
+      const uint32_t u = min((uint32_t)(token - base), spare);
+      atomicOr(&counts[WIDE ? u : u / 2], WIDE ? kInPrompt : kInPrompt << u % 2 * 16);
     };
     auto made = [&](int token) {
-      const uint32_t u = (uint32_t)(token - base);
-      if (u < limit) atomicAdd(&counts[WIDE ? u : u / 2], WIDE ? 1u : 1u << u % 2 * 16);
+      const uint32_t u = min((uint32_t)(token - base), spare);
+      atomicAdd(&counts[WIDE ? u : u / 2], WIDE ? 1u : 1u << u % 2 * 16);
     };
     const int guesses = p.drafts && p.row_drafts ? min(((ConstI32*)p.row_drafts)[row], p.max_drafts) : 0;
     const int32_t* drafts = p.drafts + (int64_t)seq * p.max_drafts;
     const int guess = tid < guesses ? drafts[tid] : -1;
-    // sixteen tokens per thread in flight
+    const int whole = len & ~3;  // in vectors; the last len % 4 by a thread each
+    const int last = tid < len - whole ? tokens[whole + tid] : -1;
+    // A wave takes 256 consecutive tokens at a time, kBatch such loads in flight; lanes past the
+    // end count the token -1, which no range has.
     constexpr int kStep = THREADS * 4, kBatch = 4;
-    auto count = [&](const vec& t, int at) {
-      if (at + 4 <= prompt) {
+    auto count = [&](const vec& t, int w) {
+      if (w + kWave * 4 <= prompt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) seen(t[e]);
-      } else if (at >= prompt) {
+      } else if (w >= prompt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) made(t[e]);
       } else {
-        for (int e = 0; e < 4; ++e) at + e < prompt ? seen(tokens[at + e]) : made(tokens[at + e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w + lane * 4 + e < prompt ? seen(t[e]) : made(t[e]);
       }
     };
-    int i = tid * 4;
-    if (ahead && i + 4 <= len) {
-      count(first, i);
-      i += kStep;
-    }
-    for (; i + (kBatch - 1) * kStep + 4 <= len; i += kBatch * kStep) {
-      vec t[kBatch];
+    auto cut = [&](vec& t, int w) {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) t[j] = *(const vec*)(tokens + i + j * kStep);
+      for (int e = 0; e < 4; ++e) t[e] = w + lane * 4 < whole ? t[e] : -1;
+    };
+    int w = __builtin_amdgcn_readfirstlane(tid / kWave) * (kWave * 4);
+    if (w < whole) {
+      cut(first, w);
+      count(first, w);
+      w += kStep;
+    }
+    vec t[kBatch];
+    for (; w + (kBatch - 1) * kStep + kWave * 4 <= whole; w += kBatch * kStep) {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) count(t[j], i + j * kStep);
+      for (int j = 0; j < kBatch; ++j) t[j] = *(const vec*)(tokens + w + j * kStep + lane * 4);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) count(t[j], w + j * kStep);
     }
-    for (; i < len; i += kStep) {
-      if (i + 4 <= len) {
-        count(*(const vec*)(tokens + i), i);
-      } else {
-        for (int e = i; e < len; ++e) e < prompt ? seen(tokens[e]) : made(tokens[e]);
-      }
+    if (w < whole) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) t[j] = *(const vec*)(tokens + min(w + j * kStep + lane * 4, whole - 4));
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (w + j * kStep < whole) {
+          cut(t[j], w + j * kStep);
+          count(t[j], w + j * kStep);
+        }
     }
+    if (tid < len - whole) whole + tid < prompt ? seen(last) : made(last);
     if (tid < guesses) made(guess);
     for (int j = tid + THREADS; j < guesses; j += THREADS) made(drafts[j]);
   }
@@ -321,25 +342,35 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
   }
 }
 
-template <int IDT, int ODT, int THREADS, int VECTORS, bool WIDE>
-int launch_ranges(const AdjustParams& p, hipStream_t stream) {
-  constexpr int kRange = THREADS * VECTORS * 8;
+template <int IDT, int ODT, int THREADS, int VECTORS, bool WIDE, bool IN_PLACE>
+int launch_kernel(const AdjustParams& p, hipStream_t stream) {
+  constexpr int kRange = THREADS * VECTORS * 8, kTable = kRange * (WIDE ? 4 : 2), kSpare = kWave * 4;
   NE_CHECK_SUPPORTED(p.rows <= kRowsPerSlice * 65535, "too many rows: %d", p.rows);
-  const dim3 grid(ceil_div(p.vocab, kRange), p.rows < kRowsPerSlice ? p.rows : kRowsPerSlice, ceil_div(p.rows, kRowsPerSlice));
-  const size_t lds = ((p.history ? 1 : 0) + (p.bias_start ? 1 : 0)) * kRange * (WIDE ? 4 : 2);
-  if constexpr (IDT == ODT) {
-    if (p.out == p.logits) {
-      hipLaunchKernelGGL((adjust_logits_kernel<IDT, ODT, THREADS, VECTORS, WIDE, true>), grid, dim3(THREADS), lds, stream, p);
-      return check_launch("adjust_logits");
+  const auto kernel = adjust_logits_kernel<IDT, ODT, THREADS, VECTORS, WIDE, IN_PLACE>;
+  if constexpr (WIDE) {  // more than the default dynamic LDS, once per instantiation
+    static const hipError_t attr = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kTable + kSpare);
+    if (attr != hipSuccess) {
+      set_error("adjust_logits: cannot reserve %d bytes of LDS: %s", 2 * kTable + kSpare, hipGetErrorString(attr));
+      return NE_ELAUNCH;
     }
   }
-  hipLaunchKernelGGL((adjust_logits_kernel<IDT, ODT, THREADS, VECTORS, WIDE, false>), grid, dim3(THREADS), lds, stream, p);
+  const dim3 grid(ceil_div(p.vocab, kRange), p.rows < kRowsPerSlice ? p.rows : kRowsPerSlice, ceil_div(p.rows, kRowsPerSlice));
+  const size_t lds = (p.history ? kTable + kSpare : 0) + (p.bias_start ? kTable : 0);
+  hipLaunchKernelGGL(kernel, grid, dim3(THREADS), lds, stream, p);
   return check_launch("adjust_logits");
 }
 
+template <int IDT, int ODT, int THREADS, int VECTORS, bool WIDE>
+int launch_ranges(const AdjustParams& p, hipStream_t stream) {
+  if constexpr (IDT == ODT) {
+    if (p.out == p.logits) return launch_kernel<IDT, ODT, THREADS, VECTORS, WIDE, true>(p, stream);
+  }
+  return launch_kernel<IDT, ODT, THREADS, VECTORS, WIDE, false>(p, stream);
+}
+
 // 8,192 tokens per work-group, 4,096 where that leaves CUs idle: one row of 151,936 (20 biases) 5.7 and
-// 4.5 us, 320 rows with histories of up to 2,048 tokens 48 and 61.  Histories that need wide counters
-// are read by 16 waves, 16 rows of 32,003 with up to 120,000 tokens in 16.6 us (8 waves 21-23).
+// 4.5 us, 320 rows with histories of up to 2,048 tokens 44 and 53.  Histories that need wide counters
+// are read by 16 waves, 16 rows of 32,003 with up to 120,000 tokens in 16.4 us (8 waves 17.6 and 19.6).
 template <int IDT, int ODT>
 int launch_adjust(const AdjustParams& p, hipStream_t stream) {
   const bool wide = p.history && (int64_t)p.capacity + p.max_drafts > kMaxNarrowCount;

@@ -157,11 +157,26 @@ def test_scalars_and_full_vocabulary():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("capacity", [0, 1, 3, 513, 2048, 5001, 70000])
+@pytest.mark.parametrize("capacity", [0, 1, 3, 255, 513, 2048, 2304, 5001, 8192, 10500, 32767, 32768, 70000])
 def test_history_lengths(capacity):
     rows, vocab = 3, 9000
     logits = make_logits(rows, vocab, "fp32")
     p = make_penalties(rows, vocab, capacity=capacity, seed=capacity)
+    check(kernels.adjust_logits(logits, penalties=p), logits, penalties=p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capacity", [6000, 40000])
+@pytest.mark.parametrize("length", [1, 2, 255, 256, 257, 2047, 2049, 4096, 4100, 5999])
+def test_prompts_that_end_anywhere(length, capacity):
+    """One token again and again at both ends of the vocabulary's ranges, and tokens far outside it."""
+    vocab = 16389
+    g = torch.Generator(device="cuda").manual_seed(length)
+    pool = torch.tensor([0, 4095, 4096, 8191, 8192, 16388, 16389, -1, -(2**31), 2**31 - 1, 2**30 + 5], dtype=torch.int32, device="cuda")
+    history = pool[torch.randint(0, 11, (8, capacity), device="cuda", generator=g)]
+    prompts = torch.tensor([0, 1, length // 2, length - 1, length, length + 1, 250, -3], dtype=torch.int32, device="cuda")
+    p = kernels.TokenPenalties(history, torch.full((8,), length, dtype=torch.int32, device="cuda"), prompts, 1.5, 0.25, 0.125)
+    logits = make_logits(8, vocab, "bf16", seed=length)
     check(kernels.adjust_logits(logits, penalties=p), logits, penalties=p)
 
 
