@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define NE_ABI_VERSION 13
+#define NE_ABI_VERSION 14
 
 /* status codes */
 #define NE_OK 0
@@ -583,6 +583,23 @@ int32_t ne_w8a8_kernel(int32_t m, int32_t n, int32_t k, int32_t epilogue);
 int ne_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
                  const void* w_scale, int32_t scale_dtype, int32_t m, int32_t n, int32_t k, void* y,
                  int64_t ldy, int32_t epilogue, void* stream);
+
+/*
+ * The QKV projection of a prompt with 8-bit activations: ne_w8a8_gemm (store epilogue) over the
+ * concatenated q | k | v weight ([(Hq+2*Hkv)*128, k] int8), each head of every row then taken as
+ * ne_qk_norm_rope_kv_write takes it (the same bits), without writing the product to memory:
+ * what ne_w8a16_qkv_norm_rope_kv is to ne_w8a16_gemm, with its arguments.  x, x_scale, w, w_scale
+ * and k as in ne_w8a8_gemm; kv_dtype NE_DTYPE_INT8 (scales bf16 or fp16) or NE_DTYPE_BF16; q_out
+ * and the caches 16-byte aligned, rope 8-byte, the norm weights 4-byte aligned.
+ */
+int ne_w8a8_qkv_norm_rope_kv(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
+                             const void* w_scale, int32_t scale_dtype, int32_t m,
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t k,
+                             const void* q_norm_weight, const void* k_norm_weight, float eps,
+                             const int32_t* positions, const void* rope_cos_sin,
+                             int32_t rope_positions, const int32_t* slot_mapping, int32_t kv_dtype,
+                             void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                             int32_t kv_scale_dtype, void* q_out, void* stream);
 
 /*
  * Logits under penalties for repeated tokens, biases of single tokens and masks of allowed ones

@@ -6,6 +6,7 @@
 // As in gemm.hip an MFMA computes D = W . X^T (v_mfma_i32_16x16x64_i8), so that a lane holds
 // four consecutive output columns of one token row.
 #include "ne_common.hpp"
+#include "qk_rope_kv.hpp"
 
 namespace ne {
 
@@ -26,8 +27,29 @@ struct W8a8Params {
   int tiles_m, tiles_n;
 };
 
+// the product's rows as head vectors, through QK-norm and RoPE into q_out and the KV cache
+constexpr int kEpilogueQkvBf16 = 2, kEpilogueQkvInt8 = 3;  // (by the cache's type)
+struct W8a8QkvParams : W8a8Params {
+  QkvRopeArgs qkv;
+  int kv_scale_dtype;
+};
+template <bool QKV>
+struct ParamsFor {
+  using type = W8a8Params;
+};
+template <>
+struct ParamsFor<true> {
+  using type = W8a8QkvParams;
+};
+template <int EPI>
+using ParamsOf = typename ParamsFor<(EPI >= 2)>::type;  // (a kernel's name spells this out: literals only)
+
 __device__ __forceinline__ void lds_dma16(const void* src, void* lds_wave_base) {
   __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+}
+
+__device__ __forceinline__ void lds_dma4(const void* src, void* lds_wave_base) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds_wave_base, 4, 0, 0);
 }
 
 // s_waitcnt vmcnt(n) leaving lgkmcnt/expcnt unconstrained (gfx9 encoding)
@@ -107,6 +129,100 @@ __device__ __forceinline__ u32x4 pair_columns(const u32x2& a, const u32x2& b) {
 }
 __device__ __forceinline__ int pair_column(int g) { return 16 * (g & 1) + 8 * (g >> 1); }
 
+// ---- the QKV epilogue's arithmetic: what qk_norm_rope_kv_vectors does, bit for bit ------
+// A lane holds columns 16 ns + 4 g + i (ns < 8, i < 4) of a row's 128, its RoPE pairs 64 apart
+// among them; a vector's sums are taken in the row kernel's order.
+__device__ __forceinline__ float plain_add(float a, float b) {
+#pragma clang fp contract(off)
+  return a + b;
+}
+__device__ __forceinline__ float add_xor16(float v) {
+  const auto o = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return plain_add(__uint_as_float(o[0]), __uint_as_float(o[1]));
+}
+__device__ __forceinline__ float add_xor32(float v) {
+  const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return plain_add(__uint_as_float(o[0]), __uint_as_float(o[1]));
+}
+__device__ __forceinline__ uint32_t max_over_groups(uint32_t v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(b[0], b[1]);
+}
+__device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_f32(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// 1 / rms of a row: the squares of each 16 columns and their partners, then the tree over 64 lanes
+__device__ __forceinline__ float inverse_rms(const u32x2 (&v)[8], float eps) {
+  float sums[4];
+#pragma unroll
+  for (int ns = 0; ns < 4; ++ns) {
+    float t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = i % 2 ? hi_f32(v[ns][i / 2]) : lo_f32(v[ns][i / 2]);
+      const float b = i % 2 ? hi_f32(v[ns + 4][i / 2]) : lo_f32(v[ns + 4][i / 2]);
+      t[i] = a * a + b * b;
+    }
+    sums[ns] = add_xor32(add_xor16(plain_add(plain_add(t[0], t[1]), plain_add(t[2], t[3]))));
+  }
+  return rsqrtf(plain_add(plain_add(sums[0], sums[1]), plain_add(sums[2], sums[3])) / 128.f + eps);
+}
+
+// two neighbouring columns of each half: norm, then rotation, in place
+__device__ __forceinline__ void norm_rope2(uint32_t& a, uint32_t& b, float inv, uint32_t wa, uint32_t wb, uint32_t c, uint32_t s) {
+  uint32_t x = pack_bf16x2(lo_f32(a) * inv, hi_f32(a) * inv), y = pack_bf16x2(lo_f32(b) * inv, hi_f32(b) * inv);
+  x = pack_bf16x2(lo_f32(x) * lo_f32(wa), hi_f32(x) * hi_f32(wa));
+  y = pack_bf16x2(lo_f32(y) * lo_f32(wb), hi_f32(y) * hi_f32(wb));
+  const uint32_t xc = pack_bf16x2(lo_f32(x) * lo_f32(c), hi_f32(x) * hi_f32(c));
+  const uint32_t ys = pack_bf16x2(-lo_f32(y) * lo_f32(s), -hi_f32(y) * hi_f32(s));
+  const uint32_t yc = pack_bf16x2(lo_f32(y) * lo_f32(c), hi_f32(y) * hi_f32(c));
+  const uint32_t xs = pack_bf16x2(lo_f32(x) * lo_f32(s), hi_f32(x) * hi_f32(s));
+  a = pack_bf16x2(lo_f32(xc) + lo_f32(ys), hi_f32(xc) + hi_f32(ys));
+  b = pack_bf16x2(lo_f32(yc) + lo_f32(xs), hi_f32(yc) + hi_f32(xs));
+}
+
+// a row's scale and the codes of this lane's columns, four in a word (as quantize_rows.hip's: the
+// quotients' own, by division only in waves with one next to a half)
+__device__ __forceinline__ float quantize_vector(const u32x2 (&v)[8], uint32_t (&codes)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int ns = 0; ns < 8; ++ns)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) top = max(top, max(v[ns][i] << 16 & 0x7FFF0000u, v[ns][i] & 0x7FFF0000u));
+  const float s = fmaxf(__uint_as_float(max_over_groups(top)), 1e-8f) / 127.f;
+  const float rcp = __builtin_amdgcn_rcpf(s);
+  constexpr float kWhole = 12582912.f;  // 1.5 2^23
+#pragma unroll
+  for (int ns = 0; ns < 8; ++ns) {
+    const float f[4] = {lo_f32(v[ns][0]), hi_f32(v[ns][0]), lo_f32(v[ns][1]), hi_f32(v[ns][1])};
+    float t[4], far = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      t[e] = __builtin_fmaf(f[e], rcp, kWhole);
+      far = fmaxf(far, fabsf(__builtin_fmaf(f[e], rcp, -(t[e] - kWhole))));
+    }
+    if (__builtin_amdgcn_ballot_w64(far > 0.49996f) != 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = f[e] / s + kWhole;
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(t[1]), __float_as_uint(t[0]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(t[3]), __float_as_uint(t[2]), 0x0c0c0400u);
+    codes[ns] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+  }
+  return s;
+}
+
+// words j of lane group g to word g of lane group j: lane group g then holds subtile g's 16 columns
+__device__ __forceinline__ u32x4 transpose_groups(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const auto ab = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  const auto cd = __builtin_amdgcn_permlane16_swap(c, d, false, false);
+  const auto even = __builtin_amdgcn_permlane32_swap(ab[0], cd[0], false, false);
+  const auto odd = __builtin_amdgcn_permlane32_swap(ab[1], cd[1], false, false);
+  return u32x4{even[0], odd[0], even[1], odd[1]};
+}
+
 // columns col .. + 2 N of a row of n_out, element by element where the row's end or the
 // alignment does not take a wide store
 template <int N, typename V>
@@ -157,12 +273,14 @@ struct TileLayout {
 };
 
 template <typename L, int EPI>
-__global__ __launch_bounds__(L::kWaves* kWave) void w8a8_tile_kernel(W8a8Params p) {
+__global__ __launch_bounds__(L::kWaves* kWave) void w8a8_tile_kernel(ParamsOf<EPI> p) {
   constexpr int PM = L::PM, NPW = L::NPW, RING = L::RING, D = L::kCopies;
   constexpr int kOut = EPI == NE_EPILOGUE_SWIGLU ? NPW / 2 : NPW;
-  constexpr int kStores = PM * kOut / 2;  // of a wave's whole tile
+  constexpr bool kQkv = EPI >= kEpilogueQkvBf16;
+  constexpr int kStores = EPI == kEpilogueQkvInt8 ? PM * 2 : PM * kOut / 2;  // of a wave's whole tile, at least
+  static_assert(!kQkv || L::BN == 128 * L::NW, "a wave's columns are a head");
   static_assert(D * (RING - 1) + kStores < 64, "vmcnt range");
-  __shared__ __attribute__((aligned(16))) char smem[L::kLds];
+  __shared__ __attribute__((aligned(16))) char smem[L::kLds + (kQkv ? L::BM * 16 : 0)];
   float* const scales = (float*)(smem + L::kScales);
   // Each XCD takes a contiguous eighth of the tiles, in an order that walks all weight tiles
   // against groups of four row tiles: the group's rows stay in that XCD's L2.  Its work-groups
@@ -291,18 +409,23 @@ __global__ __launch_bounds__(L::kWaves* kWave) void w8a8_tile_kernel(W8a8Params 
     place(i, m0, n0);
     // the bits of this thread's scale, one of BM + BN, so that nothing waits for them where they are loaded
     auto my_scale = [&]() -> uint32_t {
-      const int t = threadIdx.x;
+      int t = threadIdx.x;
+      if constexpr (kQkv) __asm__ volatile("" : "+v"(t));  // its registers are for the QKV epilogue
       if (t < L::BM) return ((const uint32_t*)p.xs)[min(m0 + t, p.m - 1)];
       const int n = min(n0 + min(t - L::BM, L::BN - 1), p.n - 1);
       return p.ws_dtype == NE_DTYPE_FP32 ? ((const uint32_t*)p.ws)[n] : ((const uint16_t*)p.ws)[n];
     };
     auto put_scale = [&](uint32_t bits) {
-      const bool fp32 = threadIdx.x < L::BM || p.ws_dtype == NE_DTYPE_FP32;
+      int t = threadIdx.x;
+      if constexpr (kQkv) __asm__ volatile("" : "+v"(t));
+      const bool fp32 = t < L::BM || p.ws_dtype == NE_DTYPE_FP32;
       const float half = p.ws_dtype == NE_DTYPE_BF16 ? bf16_to_f32((uint16_t)bits) : f16_to_f32((uint16_t)bits);
       const float v = fp32 ? __uint_as_float(bits) : half;
-      if (L::BM + L::BN == L::kWaves * kWave || threadIdx.x < L::BM + L::BN) scales[threadIdx.x] = v;
+      if (L::BM + L::BN == L::kWaves * kWave || t < L::BM + L::BN) scales[t] = v;
     };
     uint32_t scale = 0;
+    const int head = n0 / 128 + nw;  // QKV
+    int* const places = (int*)(smem + L::kLds) + (i & 1) * 2 * L::BM;  // QKV: the rows' positions, then their slots
 #pragma unroll
     for (int mi = 0; mi < PM; ++mi)
 #pragma unroll
@@ -312,7 +435,21 @@ __global__ __launch_bounds__(L::kWaves* kWave) void w8a8_tile_kernel(W8a8Params 
     for (int t = 0; t < n_stages; ++t, ++s) {
       wait_lgkmcnt0();  // for a's reads, not for the next ones too
       read(slot, 1, b);
-      if (t + 1 == n_stages) scale = my_scale();
+      if (t + 1 == n_stages) {
+        if constexpr (kQkv) {
+          // by DMA, as they are wanted next to no registers: a wave's 64 rows, and its head's norm weights
+          static_assert(RING == 2 && L::BM % kWave == 0 && L::BM / kWave <= L::kWaves, "rows by waves");
+          int l = lane;
+          __asm__ volatile("" : "+v"(l));
+          if (wave < L::BM / kWave) {
+            const int m = min(m0 + wave * kWave + l, p.m - 1);
+            lds_dma4(p.qkv.positions + m, places + wave * kWave);
+            lds_dma4(p.qkv.slot_mapping + m, places + L::BM + wave * kWave);
+          }
+          lds_dma4((const uint32_t*)(head < p.qkv.hq ? p.qkv.q_norm_w : p.qkv.k_norm_w) + l, smem + L::kEdge + wave * 1024);
+        }
+        scale = my_scale();
+      }
       mma(a);
       if (s + 1 < all) {
         // stage s + 1 has landed and every wave has read all of stage s: its slot takes stage s + RING
@@ -346,6 +483,7 @@ __global__ __launch_bounds__(L::kWaves* kWave) void w8a8_tile_kernel(W8a8Params 
     // tile's last stage left, not after them.
     if (n_stages == 1) lds_barrier();  // the previous tile's have been read
     put_scale(scale);
+    if constexpr (kQkv) wait_vmcnt<0>();  // (no copies are in flight here)
     if (s - 1 + RING < all) issue();
     lds_barrier();
 
@@ -353,53 +491,130 @@ __global__ __launch_bounds__(L::kWaves* kWave) void w8a8_tile_kernel(W8a8Params 
     int l = lane;
     __asm__ volatile("" : "+v"(l));  // addresses made here, not kept in registers through the k loop
     const int er = l & 15, eg = l >> 4;
-    float sc[NPW][4];
+    if constexpr (kQkv) {
+      const QkvRopeArgs& qa = p.qkv;
+      const bool is_q = head < qa.hq, is_v = head >= qa.hq + qa.hkv;
+      const bool is_head = head < qa.hq + 2 * qa.hkv;  // (the last tile's other half may be none)
+      const int kv_head = head - qa.hq - (is_v ? qa.hkv : 0);
+      const char* const norm = smem + L::kEdge + wave * 1024;
+      void* const cache = is_v ? qa.v_cache : qa.k_cache;
+      u32x2 rope[8];  // cosines and sines of this lane's columns
+      auto load_rope = [&](int mi) {
+        const uint16_t* at = qa.rope + (int64_t)min(max(places[(mw * PM + mi) * 16 + er], 0), qa.rope_positions - 1) * 128 + 4 * eg;
 #pragma unroll
-    for (int ns = 0; ns < NPW; ++ns) {
-      const floatx4 v = *(const floatx4*)(scales + L::BM + (nw * NPW + ns) * 16 + 4 * eg);
+        for (int ns = 0; ns < 4; ++ns) {
+          rope[ns] = *(const u32x2*)(at + 16 * ns);
+          rope[4 + ns] = *(const u32x2*)(at + 64 + 16 * ns);
+        }
+      };
+      if (is_head) {
+        load_rope(0);  // (also for v, which has no use for them: fewer registers than a choice)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[ns][e] = v[e];
-    }
-    const int col0 = (EPI == NE_EPILOGUE_SWIGLU ? n0 / 2 : n0) + nw * kOut * 16;
-    const bool inside = wide && n0 + L::BN <= p.n;  // all of the tile's columns, in wide stores
-    auto out4 = [&](int mi, int o, float sx) {
-      if constexpr (EPI == NE_EPILOGUE_SWIGLU)
-        return swiglu4(acc[mi][2 * o], acc[mi][2 * o + 1], sx, sc[2 * o], sc[2 * o + 1]);
-      else
-        return store4(acc[mi][o], sx, sc[o]);
-    };
-    char* const edge = smem + L::kEdge + wave * 1024;
+        for (int mi = 0; mi < PM; ++mi) {
+          const int lrow = (mw * PM + mi) * 16 + er;
+          const float sx = scales[lrow];
+          const bool real = m0 + lrow < p.m;
+          u32x2 v[8];
 #pragma unroll
-    for (int mi = 0; mi < PM; ++mi) {
-      const int lrow = (mw * PM + mi) * 16 + er;
-      const float sx = scales[lrow];
-      uint16_t* row = p.y + (int64_t)(m0 + lrow) * p.ldy + col0;
-      // a row's 16-column subtiles in pairs
-      static_assert(kOut % 2 == 0, "output subtiles in pairs");
+          for (int ns = 0; ns < 8; ++ns) {
+            const floatx4 sc = *(const floatx4*)(scales + L::BM + (nw * 8 + ns) * 16 + 4 * eg);
+            v[ns] = store4(acc[mi][ns], sx, {sc[0], sc[1], sc[2], sc[3]});
+          }
+          if (!is_v) {
+            const float inv = inverse_rms(v, qa.eps);
 #pragma unroll
-      for (int o = 0; o < kOut; o += 2) {
-        const u32x4 both = pair_columns(out4(mi, o, sx), out4(mi, o + 1, sx));
-        if (inside) {
-          if (m0 + lrow < p.m) *(u32x4*)(row + o * 16 + pair_column(eg)) = both;
-        } else {
-          // 16 rows of 32 columns through LDS, then two rows at a time, element by element
-          *(u32x4*)(edge + er * 64 + pair_column(eg) * 2) = both;
-#pragma unroll 1
-          for (int at = l; at < 16 * 32; at += kWave) {
-            const int m = m0 + (mw * PM + mi) * 16 + at / 32, col = col0 + o * 16 + at % 32;
-            if (m < p.m && col < n_out) p.y[(int64_t)m * p.ldy + col] = *(const uint16_t*)(edge + at * 2);
+            for (int ns = 0; ns < 4; ++ns) {
+              const u32x2 wa = *(const u32x2*)(norm + (16 * ns + 4 * eg) * 2), wb = *(const u32x2*)(norm + (64 + 16 * ns + 4 * eg) * 2);
+              const u32x2 c = rope[ns], sn = rope[4 + ns];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                uint32_t x = v[ns][i], y = v[ns + 4][i];
+                norm_rope2(x, y, inv, wa[i], wb[i], c[i], sn[i]);
+                v[ns][i] = x;
+                v[ns + 4][i] = y;
+              }
+            }
+          }
+          if (mi + 1 < PM) load_rope(mi + 1);
+          const int64_t vector = (int64_t)places[L::BM + lrow] * qa.hkv + kv_head;  // in the cache
+          if (EPI == kEpilogueQkvBf16 || is_q) {
+            uint16_t* to = is_q ? qa.q_out + ((int64_t)(m0 + lrow) * qa.hq + head) * 128 : (uint16_t*)cache + vector * 128;
+#pragma unroll
+            for (int o = 0; o < 8; o += 2) {
+              const u32x4 both = pair_columns(v[o], v[o + 1]);
+              if (real) *(u32x4*)(to + o * 16 + pair_column(eg)) = both;
+            }
+          } else {
+            uint32_t codes[8];
+            const float sv = quantize_vector(v, codes);
+            const u32x4 low = transpose_groups(codes[0], codes[1], codes[2], codes[3]);
+            const u32x4 high = transpose_groups(codes[4], codes[5], codes[6], codes[7]);
+            int8_t* to = (int8_t*)cache + vector * 128 + 16 * eg;
+            if (real) {
+              *(u32x4*)to = low;
+              *(u32x4*)(to + 64) = high;
+              if (eg == 0) {
+                void* const kv_scales = is_v ? qa.v_scale : qa.k_scale;
+                if (p.kv_scale_dtype == NE_DTYPE_BF16) {
+                  store_scale<NE_DTYPE_BF16>(kv_scales, vector, sv);
+                } else {
+                  store_scale<NE_DTYPE_FP16>(kv_scales, vector, sv);
+                }
+              }
+            }
           }
         }
       }
+      storing = is_head && m0 + L::BM <= p.m;
+    } else {
+      float sc[NPW][4];
+#pragma unroll
+      for (int ns = 0; ns < NPW; ++ns) {
+        const floatx4 v = *(const floatx4*)(scales + L::BM + (nw * NPW + ns) * 16 + 4 * eg);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[ns][e] = v[e];
+      }
+      const int col0 = (EPI == NE_EPILOGUE_SWIGLU ? n0 / 2 : n0) + nw * kOut * 16;
+      const bool inside = wide && n0 + L::BN <= p.n;  // all of the tile's columns, in wide stores
+      auto out4 = [&](int mi, int o, float sx) {
+        if constexpr (EPI == NE_EPILOGUE_SWIGLU)
+          return swiglu4(acc[mi][2 * o], acc[mi][2 * o + 1], sx, sc[2 * o], sc[2 * o + 1]);
+        else
+          return store4(acc[mi][o], sx, sc[o]);
+      };
+      char* const edge = smem + L::kEdge + wave * 1024;
+#pragma unroll
+      for (int mi = 0; mi < PM; ++mi) {
+        const int lrow = (mw * PM + mi) * 16 + er;
+        const float sx = scales[lrow];
+        uint16_t* row = p.y + (int64_t)(m0 + lrow) * p.ldy + col0;
+        // a row's 16-column subtiles in pairs
+        static_assert(kOut % 2 == 0, "output subtiles in pairs");
+#pragma unroll
+        for (int o = 0; o < kOut; o += 2) {
+          const u32x4 both = pair_columns(out4(mi, o, sx), out4(mi, o + 1, sx));
+          if (inside) {
+            if (m0 + lrow < p.m) *(u32x4*)(row + o * 16 + pair_column(eg)) = both;
+          } else {
+            // 16 rows of 32 columns through LDS, then two rows at a time, element by element
+            *(u32x4*)(edge + er * 64 + pair_column(eg) * 2) = both;
+#pragma unroll 1
+            for (int at = l; at < 16 * 32; at += kWave) {
+              const int m = m0 + (mw * PM + mi) * 16 + at / 32, col = col0 + o * 16 + at % 32;
+              if (m < p.m && col < n_out) p.y[(int64_t)m * p.ldy + col] = *(const uint16_t*)(edge + at * 2);
+            }
+          }
+        }
+      }
+      storing = inside && m0 + L::BM <= p.m;  // (every one of the stores was made)
     }
-    storing = inside && m0 + L::BM <= p.m;  // (every one of the stores was made)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);  // the stores stay before the next wait
   }
 }
 
 template <typename L, int EPI>
-int launch_tile(W8a8Params p, hipStream_t stream) {
+int launch_tile(ParamsOf<EPI> p, hipStream_t stream) {
   p.tiles_m = ceil_div(p.m, L::BM);
   p.tiles_n = ceil_div(p.n, L::BN);
   const int64_t per = ((int64_t)p.tiles_m * p.tiles_n + kNumXcd - 1) / kNumXcd;
@@ -599,11 +814,48 @@ int launch_kernel(const W8a8Params& p, hipStream_t stream) {
   return launch_few<FewLayout<4, 2, 8, 1>, EPI>(p, stream);
 }
 
+// A wave's tile has a head's 128 columns, so that a vector's sum and largest value are four lanes' work and
+// its RoPE pairs one lane's.  256 x 256 tiles where their last round over the CUs is nearly full,
+// else 128 x 128, two per CU (us, 16 + 8 heads, k = 1,024, int8 cache, 256 / 128; ne_w8a8_gemm into memory; the
+// W8A16 product with the same epilogue): 512 rows 30.6 / 15.2; 8.8; 17.7, 2,048 31.8 / 19.2; 14.8; 32.0,
+// 4,096 33.4 / 32.4; 21.8; 53.0 (bf16 cache 30.1 / 32.5), 6,000 55.9 / 48.1; 32.9; 80.4, 8,192 57.2 /
+// 58.3; 37.1; 91.1 (bf16 52.8 / 60.2), 16,384 107 / 111; 68; 171.  The row kernel alone takes 68-71 at 8,192.
+// What the epilogue adds is its arithmetic, ~500 vector operations per 16 rows of a head.
+template <int EPI>
+int launch_qkv(const W8a8QkvParams& p, hipStream_t stream) {
+  const int64_t tiles = (int64_t)ceil_div(p.m, 256) * ceil_div(p.n, 256);
+  if (tiles * 100 >= (tiles + kNumCu - 1) / kNumCu * kNumCu * 92)
+    return launch_tile<TileLayout<256, 256, 4, 2, 2>, EPI>(p, stream);
+  return launch_tile<TileLayout<128, 128, 4, 1, 2>, EPI>(p, stream);
+}
+
 }  // namespace
 
 }  // namespace ne
 
 using namespace ne;
+
+namespace {
+
+// what both products refuse
+int check_product(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, const void* w_scale,
+                  int32_t scale_dtype, int32_t m, int32_t n, int32_t k) {
+  NE_CHECK_ARG(m >= 0 && n > 0 && k > 0, "bad gemm shape m=%d n=%d k=%d", m, n, k);
+  NE_CHECK_SUPPORTED(k % 16 == 0 && k <= 131056, "k must be a multiple of 16 and at most 131,056 (got %d)", k);
+  NE_CHECK_ARG(scale_dtype == NE_DTYPE_BF16 || scale_dtype == NE_DTYPE_FP16 || scale_dtype == NE_DTYPE_FP32,
+               "scale_dtype must be bf16, fp16 or fp32");
+  NE_CHECK_SUPPORTED(m <= (1 << 30) && n <= (1 << 30), "m and n must be at most 2^30 (got %d, %d)", m, n);
+  if (m == 0) return NE_OK;
+  NE_CHECK_ARG(x && x_scale && w && w_scale, "null pointer argument");
+  NE_CHECK_ARG(ldx >= k && ldx % 16 == 0 && ldx < (1 << 23), "ldx must be >= k, a multiple of 16 and below 2^23 (got %lld)",
+               (long long)ldx);
+  NE_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0, "x and w must be 16-byte aligned");
+  NE_CHECK_ARG((uintptr_t)x_scale % 4 == 0 && (uintptr_t)w_scale % (scale_dtype == NE_DTYPE_FP32 ? 4 : 2) == 0,
+               "scales off their type's alignment");
+  return NE_OK;
+}
+
+}  // namespace
 
 extern "C" int32_t ne_w8a8_kernel(int32_t m, int32_t n, int32_t k, int32_t epilogue) {
   if (m <= 0 || n <= 0 || k <= 0) return NE_W8A8_FEW_ROWS;
@@ -613,22 +865,47 @@ extern "C" int32_t ne_w8a8_kernel(int32_t m, int32_t n, int32_t k, int32_t epilo
 extern "C" int ne_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, const void* w_scale,
                             int32_t scale_dtype, int32_t m, int32_t n, int32_t k, void* y, int64_t ldy, int32_t epilogue,
                             void* stream) {
-  NE_CHECK_ARG(m >= 0 && n > 0 && k > 0, "bad gemm shape m=%d n=%d k=%d", m, n, k);
   NE_CHECK_ARG(epilogue == NE_EPILOGUE_STORE || epilogue == NE_EPILOGUE_SWIGLU, "unknown epilogue %d", epilogue);
-  NE_CHECK_SUPPORTED(k % 16 == 0 && k <= 131056, "k must be a multiple of 16 and at most 131,056 (got %d)", k);
+  const int rc = check_product(x, ldx, x_scale, w, w_scale, scale_dtype, m, n, k);
+  if (rc != NE_OK) return rc;
   NE_CHECK_SUPPORTED(epilogue == NE_EPILOGUE_STORE || n % 32 == 0, "paired gate and up rows come in groups of 32 (n=%d)", n);
-  NE_CHECK_ARG(scale_dtype == NE_DTYPE_BF16 || scale_dtype == NE_DTYPE_FP16 || scale_dtype == NE_DTYPE_FP32,
-               "scale_dtype must be bf16, fp16 or fp32");
-  NE_CHECK_SUPPORTED(m <= (1 << 30) && n <= (1 << 30), "m and n must be at most 2^30 (got %d, %d)", m, n);
   if (m == 0) return NE_OK;
-  NE_CHECK_ARG(x && x_scale && w && w_scale && y, "null pointer argument");
-  NE_CHECK_ARG(ldx >= k && ldx % 16 == 0 && ldx < (1 << 23), "ldx must be >= k, a multiple of 16 and below 2^23 (got %lld)",
-               (long long)ldx);
+  NE_CHECK_ARG(y && (uintptr_t)y % 2 == 0, "null y, or off its type's alignment");
   NE_CHECK_ARG(ldy >= (epilogue == NE_EPILOGUE_SWIGLU ? n / 2 : n), "ldy too small (%lld)", (long long)ldy);
-  NE_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0, "x and w must be 16-byte aligned");
-  NE_CHECK_ARG((uintptr_t)x_scale % 4 == 0 && (uintptr_t)w_scale % (scale_dtype == NE_DTYPE_FP32 ? 4 : 2) == 0 && (uintptr_t)y % 2 == 0,
-               "scales or y off their type's alignment");
   const W8a8Params p{x, ldx, x_scale, w, w_scale, scale_dtype, m, n, k, (uint16_t*)y, ldy, 0, 0};
   return epilogue == NE_EPILOGUE_SWIGLU ? launch_kernel<NE_EPILOGUE_SWIGLU>(p, (hipStream_t)stream)
                                         : launch_kernel<NE_EPILOGUE_STORE>(p, (hipStream_t)stream);
+}
+
+extern "C" int ne_w8a8_qkv_norm_rope_kv(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
+                                        const void* w_scale, int32_t scale_dtype, int32_t m, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t k, const void* q_norm_w, const void* k_norm_w, float eps,
+                                        const int32_t* positions, const void* rope, int32_t rope_positions,
+                                        const int32_t* slot_mapping, int32_t kv_dtype, void* k_cache, void* v_cache,
+                                        void* k_scale, void* v_scale, int32_t kv_scale_dtype, void* q_out, void* stream) {
+  NE_CHECK_ARG(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads <= (1 << 20) && num_kv_heads <= (1 << 20),
+               "bad heads: %d and %d", num_q_heads, num_kv_heads);
+  const int32_t n = (num_q_heads + 2 * num_kv_heads) * 128;
+  const int rc = check_product(x, ldx, x_scale, w, w_scale, scale_dtype, m, n, k);
+  if (rc != NE_OK) return rc;
+  NE_CHECK_ARG(kv_dtype == NE_DTYPE_BF16 || kv_dtype == NE_DTYPE_INT8, "kv_dtype must be int8 or bf16");
+  const bool int8 = kv_dtype == NE_DTYPE_INT8;
+  NE_CHECK_SUPPORTED(!int8 || kv_scale_dtype == NE_DTYPE_BF16 || kv_scale_dtype == NE_DTYPE_FP16,
+                     "fused KV write supports bf16 or fp16 scales");
+  NE_CHECK_ARG(rope_positions > 0, "rope_positions must be > 0");
+  if (m == 0) return NE_OK;
+  NE_CHECK_ARG(q_norm_w && k_norm_w && positions && rope && slot_mapping && k_cache && v_cache && q_out,
+               "null pointer argument");
+  NE_CHECK_ARG(!int8 || (k_scale && v_scale), "an int8 cache needs k_scale and v_scale");
+  NE_CHECK_ARG((uintptr_t)q_out % 16 == 0 && (uintptr_t)k_cache % 16 == 0 && (uintptr_t)v_cache % 16 == 0,
+               "q_out and the caches must be 16-byte aligned");
+  NE_CHECK_ARG((uintptr_t)rope % 8 == 0 && (uintptr_t)q_norm_w % 4 == 0 && (uintptr_t)k_norm_w % 4 == 0,
+               "rope must be 8-byte aligned, the norm weights 4-byte aligned");
+  W8a8QkvParams p{};
+  static_cast<W8a8Params&>(p) = W8a8Params{x, ldx, x_scale, w, w_scale, scale_dtype, m, n, k, nullptr, 0, 0, 0};
+  p.qkv = QkvRopeArgs{num_q_heads, num_kv_heads, (const uint16_t*)q_norm_w, (const uint16_t*)k_norm_w, eps, positions,
+                      (const uint16_t*)rope, rope_positions, slot_mapping, k_cache, v_cache, k_scale, v_scale,
+                      (uint16_t*)q_out, 0};
+  p.kv_scale_dtype = kv_scale_dtype;
+  return int8 ? launch_qkv<kEpilogueQkvInt8>(p, (hipStream_t)stream) : launch_qkv<kEpilogueQkvBf16>(p, (hipStream_t)stream);
 }

@@ -1073,8 +1073,67 @@ def w8a16_qkv_norm_rope_kv(
     return q_out
 
 
+def w8a8_qkv_norm_rope_kv(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    w_int8: torch.Tensor,
+    w_scale: torch.Tensor,
+    num_q_heads: int,
+    num_kv_heads: int,
+    q_norm_weight: torch.Tensor,
+    k_norm_weight: torch.Tensor,
+    eps: float,
+    positions: torch.Tensor,
+    rope_cos_sin: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor | None,
+    v_scale: torch.Tensor | None,
+    q_out: torch.Tensor,
+) -> torch.Tensor:
+    """:func:`w8a16_qkv_norm_rope_kv` from rows in 8 bits (:func:`quantize_rows`): the same bits as
+    :func:`w8a8_gemm` followed by :func:`qk_norm_rope_kv_write`."""
+    device = _require_gpu(codes, scales, w_int8, w_scale, q_norm_weight, k_norm_weight, positions, rope_cos_sin,
+                          slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out)
+    _check(codes.dtype == torch.int8 and codes.dim() == 2 and codes.stride(1) == 1, "codes must be [m, k] int8 with contiguous rows")
+    rows, kdim = codes.shape
+    _check(scales.dtype == torch.float32 and scales.numel() == rows and scales.is_contiguous(),
+           "scales must be contiguous fp32, one per row")
+    channels = (num_q_heads + 2 * num_kv_heads) * HEAD_DIM
+    _check(w_int8.dtype == torch.int8 and w_int8.is_contiguous() and w_int8.shape == (channels, kdim),
+           f"w must be contiguous int8 [{channels}, {kdim}]")
+    _check(w_scale.numel() == channels and w_scale.is_contiguous(), "w_scale must be contiguous, one per weight row")
+    for norm in (q_norm_weight, k_norm_weight):
+        _check(norm.dtype == torch.bfloat16 and norm.numel() == HEAD_DIM and norm.is_contiguous(),
+               f"norm weights must be contiguous bf16 [{HEAD_DIM}]")
+    _int32(positions, "positions")
+    _int32(slot_mapping, "slot_mapping")
+    _check(positions.numel() >= rows and slot_mapping.numel() >= rows, "a position and a slot per row")
+    _check(rope_cos_sin.dtype == torch.bfloat16 and rope_cos_sin.dim() == 3 and rope_cos_sin.shape[1:] == (2, 64)
+           and rope_cos_sin.is_contiguous(), "rope_cos_sin must be contiguous [positions, 2, 64] bf16")
+    _check(q_out.shape == (rows, num_q_heads, HEAD_DIM) and q_out.dtype == torch.bfloat16 and q_out.is_contiguous(),
+           "q_out must be contiguous [rows, q_heads, 128] bf16")
+    for cache in (k_cache, v_cache):
+        _check(cache.dtype == k_cache.dtype and cache.dim() == 3 and cache.shape[1:] == (num_kv_heads, HEAD_DIM)
+               and cache.is_contiguous(), f"caches must be contiguous [slots, {num_kv_heads}, {HEAD_DIM}] of one type")
+    is_int8 = k_cache.dtype == torch.int8
+    if is_int8:
+        _check(k_scale is not None and v_scale is not None, "an int8 cache needs its scales")
+        for cache, scale in ((k_cache, k_scale), (v_cache, v_scale)):
+            _check(scale.dtype == k_scale.dtype and scale.shape == cache.shape[:2] and scale.is_contiguous(),
+                   "cache scales must be contiguous [slots, kv_heads] of one type")
+    _launch(device.index, "ne_w8a8_qkv_norm_rope_kv", codes.data_ptr(), codes.stride(0) if rows > 1 else kdim, scales.data_ptr(),
+            w_int8.data_ptr(), w_scale.data_ptr(), dtype_code(w_scale.dtype), rows, num_q_heads, num_kv_heads, kdim,
+            q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), float(eps), positions.data_ptr(), rope_cos_sin.data_ptr(),
+            rope_cos_sin.shape[0], slot_mapping.data_ptr(), dtype_code(k_cache.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr() if is_int8 else None, v_scale.data_ptr() if is_int8 else None,
+            dtype_code(k_scale.dtype) if is_int8 else DTYPE_BF16, q_out.data_ptr())
+    return q_out
+
+
 def qkv_fusion_supported(k_cache: torch.Tensor, k_scale: torch.Tensor | None) -> bool:
-    """Whether :func:`w8a16_qkv_norm_rope_kv` takes this cache (bf16, or int8 with bf16/fp16 scales)."""
+    """Whether the fused QKV projections take this cache (bf16, or int8 with bf16/fp16 scales)."""
     if k_cache.dtype == torch.bfloat16:
         return True
     return k_cache.dtype == torch.int8 and k_scale is not None and k_scale.dtype in (torch.bfloat16, torch.float16)

@@ -22,10 +22,9 @@ from nanoengine_amd.int8_quantization import quantize_vectors
 
 
 # From this many rows on a forward with int8_activations takes the W8A8 products.  Four layers of the 0.6B
-# shape, us with 16-bit / 8-bit activations: 320 rows 234 / 298, 512 338 / 336, 1,024 404 / 400, 1,536
-# 663 / 558, 2,048 723 / 623, 4,096 1,257 / 1,184, 8,192 2,539 / 2,365.  Up to 1,024 rows nothing is won
-# for the coarser rows.  The QKV product keeps 16 bits: its epilogue writes the cache, and norm, RoPE and
-# cache write as a kernel of their own (68-71 us at 8,192 rows) cost more than the 8-bit product saves.
+# shape, us with 16-bit / 8-bit activations: 320 rows 232 / 314, 512 339 / 332, 1,024 407 / 393, 1,536
+# 659 / 519, 2,048 723 / 577, 4,096 1,248 / 1,097, 8,192 2,520 / 2,214.  Up to 1,024 rows little is won
+# for the coarser rows.
 W8A8_MIN_ROWS = 1536
 
 
@@ -211,7 +210,8 @@ class Qwen3VerifyModel:
                  int8_activations: bool = False) -> None:
         """``int8_activations``: forwards of many rows (``W8A8_MIN_ROWS``: prompts) quantise the
         projections' activations to 8 bits with a scale per row and take the W8A8 products, on
-        the same weights; fewer rows keep bf16 activations."""
+        the same weights; fewer rows keep bf16 activations, and so do caches that the fused QKV
+        products do not take."""
         c = weights.config
         if c.head_dim != kernels.HEAD_DIM:
             raise NotImplementedError("the HIP kernels support head_dim 128")
@@ -297,10 +297,19 @@ class Qwen3VerifyModel:
             kernels.paged_attention_plan(batch.block_tables, pool.block_size, batch.ctx_len, batch.q_start,
                                          batch.q_len, c.num_attention_heads, c.num_key_value_heads,
                                          batch.max_q_len, batch.max_ctx_len, ws)
-        int8 = self.codes is not None and rows >= W8A8_MIN_ROWS
         fuse = self.fuse_qkv and kernels.qkv_fusion_supported(pool.key_caches[0], pool.key_scale_2d(0))
+        int8 = self.codes is not None and rows >= W8A8_MIN_ROWS and fuse
+        if int8:
+            codes, scales = self._int8(normed)
         for i, layer in enumerate(w.layers):
-            if fuse:  # QK-norm + RoPE + KV write in the QKV GEMM's epilogue (same bits)
+            if int8:
+                kernels.w8a8_qkv_norm_rope_kv(
+                    codes, scales, layer.qkv_int8, layer.qkv_scale, c.num_attention_heads, c.num_key_value_heads,
+                    layer.q_norm, layer.k_norm, eps, batch.positions, self.rope, batch.slot_mapping,
+                    pool.key_caches[i], pool.value_caches[i], pool.key_scale_2d(i), pool.value_scale_2d(i),
+                    q_out=q,
+                )
+            elif fuse:  # QK-norm + RoPE + KV write in the QKV GEMM's epilogue (same bits)
                 kernels.w8a16_qkv_norm_rope_kv(
                     normed, layer.qkv_int8, layer.qkv_scale, c.num_attention_heads, c.num_key_value_heads,
                     layer.q_norm, layer.k_norm, eps, batch.positions[:rows], self.rope,
@@ -332,7 +341,10 @@ class Qwen3VerifyModel:
                                                              *self._int8_buffers(res))
                 kernels.w8a8_gemm(codes, scales, layer.gate_up_int8, layer.gate_up_scale, epilogue=EPILOGUE_SWIGLU, out=act)
                 kernels.w8a8_gemm(*self._int8(act), layer.down_int8, layer.down_scale, out=delta)
-                kernels.add_rmsnorm(res, delta, next_norm, eps, out=normed)
+                if i + 1 < len(w.layers):
+                    codes, scales = kernels.add_rmsnorm_quantize(res, delta, next_norm, eps, *self._int8_buffers(res))
+                else:
+                    kernels.add_rmsnorm(res, delta, next_norm, eps, out=normed)
                 continue
             self._project_add_norm(attn.view(rows, -1), layer.o_int8, layer.o_scale, self.o_splits[rows],
                                    layer.post_attention_layernorm, res, delta, normed)

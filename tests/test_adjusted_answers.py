@@ -260,7 +260,7 @@ def test_prompts_through_the_8_bit_products(int8_cache, monkeypatch):
     pool, c, eps = pools[2], CFG, CFG.rms_norm_eps
     res, x = kernels.embed_rmsnorm(tokens, weights.embed, weights.layers[0].input_layernorm, eps)
     for i, layer in enumerate(weights.layers):
-        qkv = kernels.w8a16_gemm(x, layer.qkv_int8, layer.qkv_scale)
+        qkv = kernels.w8a8_gemm(*kernels.quantize_rows(x), layer.qkv_int8, layer.qkv_scale)
         q = kernels.qk_norm_rope_kv_write(qkv, c.num_attention_heads, c.num_key_value_heads, layer.q_norm, layer.k_norm, eps,
                                           positions, model.rope, slots, pool.key_caches[i], pool.value_caches[i],
                                           pool.key_scale_2d(i), pool.value_scale_2d(i))

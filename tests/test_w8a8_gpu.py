@@ -244,6 +244,97 @@ def test_weights_past_32_bit_offsets(m):
     check_product(y[:, -1].contiguous(), codes, scales, w[:500], ws[:500])
 
 
+def qkv_case(m, hq, hkv, k, cache, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n, slots, spots = (hq + 2 * hkv) * 128, m + 9, 50
+    codes, scales, w, w_scale = make(m, n, k, seed=seed)
+    one = lambda: torch.randn(128, device="cuda", generator=g).bfloat16()
+    i32 = lambda t: t.to(torch.int32)
+    positions = i32(torch.randint(-2, spots + 3, (m,), device="cuda", generator=g))  # (clamped to the table)
+    where = i32(torch.randperm(slots, device="cuda", generator=g)[:m])
+    rope = (torch.rand(spots, 2, 64, device="cuda", generator=g) * 2 - 1).bfloat16()
+    dtype, scale_dtype = cache
+    def pool():
+        caches = [torch.full((slots, hkv, 128), 7, device="cuda", dtype=dtype) for _ in range(2)]
+        return caches + [torch.full((slots, hkv), 7, device="cuda", dtype=scale_dtype) if scale_dtype else None for _ in range(2)]
+    return (codes, scales, w, w_scale), (one(), one(), 1e-6, positions, rope, where), pool
+
+
+CACHES = [(torch.bfloat16, None), (torch.int8, torch.bfloat16), (torch.int8, torch.float16)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("m,hq,hkv,k", [(1, 1, 1, 16), (5, 2, 1, 128), (130, 4, 2, 272), (300, 16, 8, 1024), (1000, 3, 1, 144),
+                                        (4100, 16, 8, 128), (4001, 16, 8, 208), (22017, 3, 1, 128), (22017, 2, 2, 640)])
+def test_qkv_product_is_the_two_calls_bits(m, hq, hkv, k, cache):
+    """Queries, cache and its scales of the product fused with norm, rotation and write, against the
+    product and the row kernel; slots that no row names stay as they were."""
+    product_args, (q_norm, k_norm, eps, positions, rope, where), pool = qkv_case(m, hq, hkv, k, cache, seed=m + k)
+    kc, vc, ks, vs = pool()
+    want = kernels.qk_norm_rope_kv_write(kernels.w8a8_gemm(*product_args), hq, hkv, q_norm, k_norm, eps, positions, rope, where,
+                                         kc, vc, ks, vs)
+    got_pool = pool()
+    q = torch.empty(m, hq, 128, device="cuda", dtype=torch.bfloat16)
+    got = kernels.w8a8_qkv_norm_rope_kv(*product_args, hq, hkv, q_norm, k_norm, eps, positions, rope, where, *got_pool, q)
+    assert got is q and torch.equal(q, want)
+    for a, b in zip(got_pool, (kc, vc, ks, vs)):
+        assert a is b is None or torch.equal(a, b)
+    unnamed = torch.ones(m + 9, dtype=torch.bool, device="cuda")
+    unnamed[where.long()] = False
+    assert (got_pool[0][unnamed] == 7).all() and (got_pool[1][unnamed] == 7).all()
+
+
+@pytest.mark.gpu
+def test_qkv_product_of_strided_codes_replayed_on_another_stream():
+    (codes, scales, w, w_scale), rest, pool = qkv_case(700, 4, 2, 256, CACHES[1])
+    q_norm, k_norm, eps, positions, rope, where = rest
+    wide = torch.zeros(700, 256 + 64, device="cuda", dtype=torch.int8)
+    caches = pool()
+    q = torch.empty(700, 4, 128, device="cuda", dtype=torch.bfloat16)
+    call = lambda out, to: kernels.w8a8_qkv_norm_rope_kv(wide[:, :256], scales, w, w_scale, 4, 2, q_norm, k_norm, eps, positions,
+                                                         rope, where, *to, out)
+    call(q, caches)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(q, caches)
+    stream = torch.cuda.Stream()
+    for step in range(3):
+        wide[:, :256] = codes.roll(step, 0)
+        positions.copy_(positions.roll(3))
+        graph.replay()
+        torch.cuda.synchronize()
+        others, out = pool(), torch.empty_like(q)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            call(out, others)
+        torch.cuda.synchronize()
+        assert torch.equal(q, out) and all(torch.equal(a, b) for a, b in zip(caches, others))
+
+
+@pytest.mark.gpu
+def test_qkv_product_refuses_what_it_does_not_take():
+    (codes, scales, w, w_scale), (q_norm, k_norm, eps, positions, rope, where), pool = qkv_case(6, 2, 1, 64, CACHES[1])
+    kc, vc, ks, vs = pool()
+    q = torch.empty(6, 2, 128, device="cuda", dtype=torch.bfloat16)
+    good = dict(codes=codes, scales=scales, w_int8=w, w_scale=w_scale, num_q_heads=2, num_kv_heads=1, q_norm_weight=q_norm,
+                k_norm_weight=k_norm, eps=eps, positions=positions, rope_cos_sin=rope, slot_mapping=where, k_cache=kc, v_cache=vc,
+                k_scale=ks, v_scale=vs, q_out=q)
+    for bad in (dict(codes=codes[:, :48]), dict(scales=scales[:5]), dict(w_int8=w[:128]), dict(num_q_heads=3),
+                dict(q_norm_weight=q_norm.float()), dict(positions=positions.long()), dict(positions=positions[:5]),
+                dict(slot_mapping=where[:5]), dict(rope_cos_sin=rope.float()), dict(q_out=q[:5]), dict(k_scale=None),
+                dict(k_scale=ks[:3]), dict(v_cache=vc.bfloat16()), dict(v_scale=vs.half()), dict(w_scale=w_scale[:3])):
+        with pytest.raises((ValueError, TypeError)):
+            kernels.w8a8_qkv_norm_rope_kv(**{**good, **bad})
+    with pytest.raises(_native.NativeError):
+        kernels.w8a8_qkv_norm_rope_kv(**{**good, "k_scale": ks.float(), "v_scale": vs.float()})
+    with pytest.raises(RuntimeError):
+        kernels.w8a8_qkv_norm_rope_kv(**{**good, "positions": positions.cpu()})
+    empty = {**good, "codes": codes[:0], "scales": scales[:0], "positions": positions[:0], "slot_mapping": where[:0], "q_out": q[:0]}
+    assert kernels.w8a8_qkv_norm_rope_kv(**empty).shape == (0, 2, 128)
+
+
 @pytest.mark.gpu
 def test_no_rows():
     codes, scales, w, w_scale = make(4, 64, 64)
@@ -341,6 +432,21 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     for bad in (dict(k=72, ldx=80), dict(k=131072, ldx=131072), dict(epilogue=1, n=48), dict(m=(1 << 30) + 1),
                 dict(n=(1 << 30) + 1, ldy=1 << 31)):
         assert gemm(**bad) == -2, bad
+
+    def qkv(x=p, ldx=64, xs=p, w=p, ws=p, dt=0, m=4, hq=2, hkv=1, k=64, qn=p, kn=p, pos=p, rope=p, spots=8, slots=p, kv=3, kc=p, vc=p,
+            ks=p, vs=p, sdt=0, q=p):
+        return lib.ne_w8a8_qkv_norm_rope_kv(x, ldx, xs, w, ws, dt, m, hq, hkv, k, qn, kn, 1e-6, pos, rope, spots, slots, kv, kc, vc, ks,
+                                            vs, sdt, q, null)
+
+    assert qkv(m=0, x=null) == 0
+    byte8, byte2 = ctypes.c_void_p(264), ctypes.c_void_p(258)
+    for bad in (dict(m=-1), dict(hq=0), dict(hkv=-1), dict(hq=1 << 21), dict(k=0), dict(dt=3), dict(x=null), dict(xs=null),
+                dict(ws=null), dict(x=odd), dict(w=odd), dict(ldx=72), dict(qn=null), dict(kn=byte2), dict(pos=null), dict(rope=null),
+                dict(rope=ctypes.c_void_p(260)), dict(spots=0), dict(slots=null), dict(kv=2), dict(kc=null), dict(vc=byte8),
+                dict(ks=null), dict(q=null), dict(q=byte8)):
+        assert qkv(**bad) == -1, bad
+    for bad in (dict(k=72, ldx=80), dict(sdt=2), dict(m=(1 << 30) + 1)):
+        assert qkv(**bad) == -2, bad
     assert lib.ne_quantize_rows(p, 0, 64, 0, 64, null, null, null) == 0
     assert lib.ne_quantize_rows(p, 2, 64, 4, 64, p, p, null) == -1
     assert lib.ne_quantize_rows(p, 0, 60, 4, 64, p, p, null) == -1
