@@ -208,7 +208,7 @@ class Qwen3VerifyModel:
 
     def __init__(self, weights: Qwen3Weights, max_rows: int, device: torch.device,
                  int8_activations: bool = False) -> None:
-        """``int8_activations``: forwards of many rows (``W8A8_MIN_ROWS``: prompts) quantise the
+        """``int8_activations``: forwards of ``W8A8_MIN_ROWS`` rows and more (prompts, mostly) quantise the
         projections' activations to 8 bits with a scale per row and take the W8A8 products, on
         the same weights; fewer rows keep bf16 activations, and so do caches that the fused QKV
         products do not take."""

@@ -14,6 +14,7 @@ from nanoengine_amd.int8_quantization import Int8Linear, quantize_linear_layers
 from nanoengine_amd.interface import SamplingParams, sampling_uniform
 from nanoengine_amd.memory import KVCachePool
 from nanoengine_amd.qwen3 import AttentionBatch, Qwen3VerifyModel, Qwen3Weights, random_state_dict
+from nanoengine_amd.runtime import create_verify_engine
 from nanoengine_amd.sequence_state import Sequence
 from test_adjust_logits_gpu import check, reference
 from test_answers import CFG, build, engine, request, unit_norms
@@ -275,6 +276,34 @@ def test_prompts_through_the_8_bit_products(int8_cache, monkeypatch):
     # fewer rows keep 16-bit activations
     few = AttentionBatch(positions[:90], slots[:90], batch.q_start[:1], lengths[:1], lengths[:1], tables[:1], 90, 90)
     assert torch.equal(model.forward(90, tokens, few, pools[0]), other.forward(90, tokens, few, pools[1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["int8", "auto"])
+def test_an_engines_prompts_in_8_bits_and_its_steps_in_16(cache, monkeypatch):
+    """Prompts of many rows take the 8-bit products, short ones and verify steps do not, captured or not."""
+    monkeypatch.setattr(qwen3, "W8A8_MIN_ROWS", 100)
+    rows = []
+    fused = kernels.w8a8_qkv_norm_rope_kv
+    monkeypatch.setattr(kernels, "w8a8_qkv_norm_rope_kv", lambda codes, *a, **kw: rows.append(codes.shape[0]) or fused(codes, *a, **kw))
+    tokens = []
+    for graphs in (False, True):
+        settings = EngineSettings(device="cuda", dtype="bfloat16", kv_cache="paged", scheduler="continuous", quantization="int8",
+                                  int8_activations=True, kv_cache_dtype=cache, speculative="ngram", num_speculative_tokens=4,
+                                  ngram_max_size=3, max_num_seqs=4, max_model_len=400, kv_cache_memory_mb=64, cuda_graphs=graphs,
+                                  cuda_graph_max_batch=4, cuda_graph_max_context=400)
+        runner = create_verify_engine(CFG, unit_norms(), settings, max_prefill_rows=160).runner
+        seqs = [Sequence.from_request(request(f"{i}", [5 + i, 6, 7, 8] * n, ignore_eos=True, seed=i, presence_penalty=0.1 * i))
+                for i, n in enumerate((14, 9, 16))]
+        runner.add(seqs)
+        late = Sequence.from_request(request("3", [1, 2, 3], ignore_eos=True))
+        runner.add([late])
+        while late.num_generated_tokens < 12:
+            runner.step()
+        while runner.pending:
+            runner.step()
+        tokens.append([s.token_ids[: s.num_prompt_tokens + 12] for s in (*seqs, late)])
+    assert rows == [156] * CFG.num_hidden_layers * 2 and tokens[0] == tokens[1]
 
 
 @pytest.mark.gpu
