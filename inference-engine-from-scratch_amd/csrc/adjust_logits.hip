@@ -142,6 +142,26 @@ struct Entries {
   }
 };
 
+struct Penalties {
+  float repetition = 1.f, presence = 0.f, frequency = 0.f;
+  __device__ __forceinline__ void read(const AdjustParams& p, int row) {
+    repetition = p.repetitions ? ((ConstF32*)p.repetitions)[row] : p.repetition;
+    presence = p.presences ? ((ConstF32*)p.presences)[row] : p.presence;
+    frequency = p.frequencies ? ((ConstF32*)p.frequencies)[row] : p.frequency;
+  }
+  __device__ __forceinline__ void check() {
+    if (!(repetition > 0.f && repetition < __builtin_inff())) repetition = 1.f;
+    if (presence != presence) presence = 0.f;
+    if (frequency != frequency) frequency = 0.f;
+  }
+  // of a token that was seen, n times in the output
+  __device__ __forceinline__ float apply(float x, uint32_t n) const {
+    x = x > 0.f ? x / repetition : x * repetition;
+    if (n != 0) x -= frequency * (float)n + presence;
+    return x;
+  }
+};
+
 // WIDE: tables of 32-bit words; otherwise of 16 bits (histories of at most kMaxNarrowCount tokens and
 // at most kMaxNarrowBias biases).
 template <int IDT, int ODT, int THREADS, int VECTORS, bool WIDE, bool IN_PLACE>
@@ -196,12 +216,10 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
     lds_barrier();
   }
   const uint32_t limit = (uint32_t)min(kRange, p.vocab - base);
-  float repetition = 1.f, presence = 0.f, frequency = 0.f;
+  Penalties penalties;
   const int seq = counted && p.row_seq ? ((ConstI32*)p.row_seq)[row] : row;
   if (counted && seq >= 0 && seq < p.num_seqs) {
-    repetition = p.repetitions ? ((ConstF32*)p.repetitions)[row] : p.repetition;
-    presence = p.presences ? ((ConstF32*)p.presences)[row] : p.presence;
-    frequency = p.frequencies ? ((ConstF32*)p.frequencies)[row] : p.frequency;
+    penalties.read(p, row);
     const int32_t* tokens = p.history + (int64_t)seq * p.history_stride;
     typedef int32_t vec __attribute__((ext_vector_type(4), aligned(4)));
     vec first;  // of this thread, loaded before the length is known
@@ -292,16 +310,10 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(AdjustParams p) 
     }
   }
   if (counted || biased) lds_barrier();
-  if (!(repetition > 0.f && repetition < __builtin_inff())) repetition = 1.f;
-  if (presence != presence) presence = 0.f;
-  if (frequency != frequency) frequency = 0.f;
+  penalties.check();
 
   auto adjusted = [&](float x, uint32_t word, uint32_t entry, uint32_t bit) {
-    if (word != 0) {
-      x = x > 0.f ? x / repetition : x * repetition;
-      const uint32_t n = word & ~kInPrompt;
-      if (n != 0) x -= frequency * (float)n + presence;
-    }
+    if (word != 0) x = penalties.apply(x, word & ~kInPrompt);
     if (entry != 0) x += p.bias_values[from + (int)entry - 1];
     return bit ? x : -__builtin_inff();
   };
@@ -347,7 +359,7 @@ int launch_kernel(const AdjustParams& p, hipStream_t stream) {
   constexpr int kRange = THREADS * VECTORS * 8, kTable = kRange * (WIDE ? 4 : 2), kSpare = kWave * 4;
   NE_CHECK_SUPPORTED(p.rows <= kRowsPerSlice * 65535, "too many rows: %d", p.rows);
   const auto kernel = adjust_logits_kernel<IDT, ODT, THREADS, VECTORS, WIDE, IN_PLACE>;
-  if constexpr (WIDE) {  // more than the default dynamic LDS, once per instantiation
+  if constexpr (2 * kTable + kSpare > 64 * 1024) {  // more than the default dynamic LDS, once per instantiation
     static const hipError_t attr = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kTable + kSpare);
     if (attr != hipSuccess) {
       set_error("adjust_logits: cannot reserve %d bytes of LDS: %s", 2 * kTable + kSpare, hipGetErrorString(attr));
@@ -368,11 +380,101 @@ int launch_ranges(const AdjustParams& p, hipStream_t stream) {
   return launch_kernel<IDT, ODT, THREADS, VECTORS, WIDE, false>(p, stream);
 }
 
+// Penalties alone, in place: only tokens of the history change, and a work-group takes a row's in one
+// pass.  An LDS table of 2^size slots, at least 1.5 times the tokens, takes each of them by linear probing
+// (so a free slot ends every search), its counts beside it; then each slot's logit is adjusted.
+constexpr int kSeenThreads = 512, kMaxSeen = 5461;  // tokens in a table of 8,192 slots, 64 KiB
+template <int DT>
+__global__ __launch_bounds__(kSeenThreads) void adjust_seen_kernel(AdjustParams p, int size) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t tokens_of[];  // [slots] token + 1, 0: free; then the counts
+  const int slots = 1 << size;
+  uint32_t* const counts = tokens_of + slots;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const int seq = p.row_seq ? ((ConstI32*)p.row_seq)[row] : row;
+  if (seq < 0 || seq >= p.num_seqs) return;
+  const int32_t* const tokens = p.history + (int64_t)seq * p.history_stride;
+  typedef int32_t vec __attribute__((ext_vector_type(4), aligned(4)));
+  vec first;  // of this thread, loaded before the length is known
+  if (tid * 4 + 4 <= p.capacity) first = *(const vec*)(tokens + tid * 4);
+  for (int i = tid * 4; i < 2 * slots; i += kSeenThreads * 4) *(u32x4*)(tokens_of + i) = u32x4{0, 0, 0, 0};
+  const int len = min(max(((ConstI32*)p.history_len)[seq], 0), p.capacity);
+  const int prompt = p.prompt_len ? min(max(((ConstI32*)p.prompt_len)[seq], 0), len) : 0;
+  const int guesses = p.drafts && p.row_drafts ? min(((ConstI32*)p.row_drafts)[row], p.max_drafts) : 0;
+  Penalties penalties;
+  penalties.read(p, row);
+  lds_barrier();
+  auto add = [&](int token, bool in_prompt) {
+    if ((uint32_t)token >= (uint32_t)p.vocab) return;
+    const uint32_t key = (uint32_t)token + 1;
+    uint32_t at = (uint32_t)token * 2654435761u >> (32 - size);
+    for (;;) {
+      uint32_t is = *(volatile uint32_t*)&tokens_of[at];  // repeated tokens read it side by side
+      if (is == 0) is = atomicCAS(&tokens_of[at], 0u, key);
+      if (is == 0 || is == key) break;
+      at = (at + 1) & (slots - 1);
+    }
+    if (in_prompt) {
+      atomicOr(&counts[at], 0x80000000u);
+    } else {
+      atomicAdd(&counts[at], 1u);
+    }
+  };
+  for (int i = tid * 4; i < len; i += kSeenThreads * 4) {
+    if (i + 4 <= len) {
+      const vec t = i == tid * 4 ? first : *(const vec*)(tokens + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add(t[e], i + e < prompt);
+    } else {
+      for (int e = i; e < len; ++e) add(tokens[e], e < prompt);
+    }
+  }
+  const int32_t* const drafts = p.drafts + (int64_t)seq * p.max_drafts;
+  for (int i = tid; i < guesses; i += kSeenThreads) add(drafts[i], false);
+  lds_barrier();
+  penalties.check();
+  constexpr int kBatch = 4;
+  for (int i = tid; i < slots; i += kSeenThreads * kBatch) {
+    uint32_t key[kBatch];
+    float x[kBatch];
+    int64_t at[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int slot = i + j * kSeenThreads;
+      key[j] = slot < slots ? tokens_of[slot] : 0;
+      at[j] = (int64_t)row * p.ld + key[j] - 1;
+      if (key[j]) x[j] = load_scale<DT>(p.logits, at[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (key[j]) store_scale<DT>(p.out, at[j], penalties.apply(x[j], counts[i + j * kSeenThreads] & 0x7FFFFFFFu));
+  }
+}
+
+template <int DT>
+int launch_seen(const AdjustParams& p, hipStream_t stream) {
+  int size = 9;
+  while ((2 << size) < 3 * (p.capacity + p.max_drafts)) ++size;
+  const size_t lds = (size_t)8 << size;
+  hipLaunchKernelGGL(adjust_seen_kernel<DT>, dim3(p.rows), dim3(kSeenThreads), lds, stream, p, size);
+  return check_launch("adjust_logits");
+}
+
+// In place under penalties alone a row's own tokens are cheaper than its vocabulary where rows are many and
+// histories short beside it (us, bf16, ranges / own tokens): 320 rows of 151,936 with 100 tokens 23.6 /
+// 6.5, with 2,000 36.6 / 21.5, 64 rows with 2,000 11.3 / 10.5; but 320 rows with 8,000 50 / 83, one row with 600
+// 4.9 / 6.3, 320 rows of 9,001 with 2,000 9.8 / 10.7.
+//
 // 8,192 tokens per work-group, 4,096 where that leaves CUs idle: one row of 151,936 (20 biases) 5.7 and
 // 4.5 us, 320 rows with histories of up to 2,048 tokens 44 and 53.  Histories that need wide counters
 // are read by 16 waves, 16 rows of 32,003 with up to 120,000 tokens in 16.4 us (8 waves 17.6 and 19.6).
 template <int IDT, int ODT>
 int launch_adjust(const AdjustParams& p, hipStream_t stream) {
+  if constexpr (IDT == ODT) {
+    const int64_t tokens = (int64_t)p.capacity + p.max_drafts;
+    if (p.out == p.logits && p.history && !p.bias_start && !p.allowed && tokens <= kMaxSeen && p.vocab > 16 * tokens &&
+        (int64_t)p.rows * ceil_div(p.vocab, 8192) > 2 * kNumCu && p.rows < (1 << 22))
+      return launch_seen<IDT>(p, stream);
+  }
   const bool wide = p.history && (int64_t)p.capacity + p.max_drafts > kMaxNarrowCount;
   if (wide || (p.bias_start && p.num_biases > kMaxNarrowBias)) return launch_ranges<IDT, ODT, 1024, 1, true>(p, stream);
   if ((int64_t)p.rows * ceil_div(p.vocab, 8192) <= 2 * kNumCu) return launch_ranges<IDT, ODT, 512, 1, false>(p, stream);

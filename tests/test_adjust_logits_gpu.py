@@ -295,6 +295,60 @@ def test_strides_and_what_lies_beside_the_rows(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("vocab,capacity,drafts", [(8193, 1, 0), (8193, 509, 3), (9001, 0, 4), (9001, 341, 0), (9001, 342, 0),
+                                                   (20000, 1249, 0), (20000, 1250, 0), (87377, 5457, 4), (87377, 5458, 4),
+                                                   (87377, 5461, 0), (151936, 2048, 4), (151936, 6000, 0)])
+@pytest.mark.parametrize("few", [False, True])
+def test_in_place_under_penalties_alone(vocab, capacity, drafts, few, dtype):
+    """A row's own tokens in one table (many rows): tokens again and again, all different, none and outside
+    the vocabulary; the same bits as into other memory."""
+    rows, ld = 9 if few else 520 // -(-vocab // 8192) + 1, vocab + 5
+    g = torch.Generator(device="cuda").manual_seed(capacity)
+    p = make_penalties(rows, vocab, seqs=5, capacity=capacity, seed=capacity, drafts=drafts) if drafts else \
+        make_penalties(rows, vocab, capacity=capacity, seed=capacity)
+    p.history_len[0] = capacity
+    p.history_len[2:4] = capacity
+    if capacity:
+        p.history[2] = torch.randperm(vocab + 7, device="cuda", generator=g)[:capacity].int() - 3
+        p.history[3] = vocab - 1
+    if drafts:
+        p.row_seq[1], p.row_drafts[2], p.row_seq[:1] = 9, -1, 3
+    base = make_logits(rows, ld, dtype, seed=vocab)
+    base[:, 7], base[:, vocab - 1] = float("inf"), float("nan")
+    logits = base[:, 2 : vocab + 2]
+    want = kernels.adjust_logits(logits, penalties=p)
+    if capacity < 400 and few:
+        check(want, logits, penalties=p)
+    inside = base.clone()
+    view = inside[:, 2 : vocab + 2]
+    assert kernels.adjust_logits(view, penalties=p, out=view) is view
+    assert torch.equal(view.nan_to_num(123.0), want.nan_to_num(123.0))
+    inside[:, 2 : vocab + 2] = logits
+    assert torch.equal(inside.nan_to_num(123.0), base.nan_to_num(123.0))  # nothing beside the rows
+
+
+@pytest.mark.gpu
+def test_in_place_call_replayed():
+    rows, vocab = 200, 30000
+    p = make_penalties(rows, vocab, seqs=4, capacity=500, drafts=4)
+    logits = make_logits(rows, vocab, "bf16")
+    graph = torch.cuda.CUDAGraph()
+    kernels.adjust_logits(logits, penalties=p, out=logits)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        kernels.adjust_logits(logits, penalties=p, out=logits)
+    for seed in range(4):
+        fresh = make_logits(rows, vocab, "bf16", seed=seed)
+        logits.copy_(fresh)
+        p.history_len.random_(0, 501)
+        p.row_drafts.random_(0, 5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(logits, kernels.adjust_logits(fresh, penalties=p))
+
+
+@pytest.mark.gpu
 def test_logits_past_32_bit_offsets():
     """2.3 10^9 logits, in place and not: the rows around the limits against their definition."""
     rows, vocab = 15_000, 151_936
