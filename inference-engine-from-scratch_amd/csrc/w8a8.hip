@@ -129,7 +129,7 @@ __device__ __forceinline__ u32x4 pair_columns(const u32x2& a, const u32x2& b) {
 }
 __device__ __forceinline__ int pair_column(int g) { return 16 * (g & 1) + 8 * (g >> 1); }
 
-// ---- the QKV epilogue's arithmetic: what qk_norm_rope_kv_vectors does, bit for bit ------
+// ---- the QKV epilogue's arithmetic: what qk_norm_rope_kv_vectors does, bit for bit for finite rows ----
 // A lane holds columns 16 ns + 4 g + i (ns < 8, i < 4) of a row's 128, its RoPE pairs 64 apart
 // among them; a vector's sums are taken in the row kernel's order.
 __device__ __forceinline__ float plain_add(float a, float b) {

@@ -1093,7 +1093,7 @@ def w8a8_qkv_norm_rope_kv(
     q_out: torch.Tensor,
 ) -> torch.Tensor:
     """:func:`w8a16_qkv_norm_rope_kv` from rows in 8 bits (:func:`quantize_rows`): the same bits as
-    :func:`w8a8_gemm` followed by :func:`qk_norm_rope_kv_write`."""
+    :func:`w8a8_gemm` followed by :func:`qk_norm_rope_kv_write` (of finite rows)."""
     device = _require_gpu(codes, scales, w_int8, w_scale, q_norm_weight, k_norm_weight, positions, rope_cos_sin,
                           slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out)
     _check(codes.dtype == torch.int8 and codes.dim() == 2 and codes.stride(1) == 1, "codes must be [m, k] int8 with contiguous rows")
