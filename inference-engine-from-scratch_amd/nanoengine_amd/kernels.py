@@ -743,8 +743,7 @@ def _launch(index: int, name: str, *args) -> None:
             _native.call(name, *args, stream)
 
 
-def _code_outputs(x: torch.Tensor, codes, scales) -> tuple[torch.Tensor, torch.Tensor]:
-    rows, k = x.shape
+def _code_outputs(x: torch.Tensor, rows: int, k: int, codes, scales) -> tuple[torch.Tensor, torch.Tensor]:
     if codes is None:
         codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     elif codes.dtype != torch.int8 or codes.shape != x.shape or not codes.is_contiguous() or codes.device != x.device:
@@ -763,13 +762,14 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None,
     :func:`w8a8_gemm`.  A row with a NaN or an infinity gets the scale NaN and codes 0."""
     if not x.is_cuda:
         _require_gpu(x)
-    if x.dim() != 2 or x.stride(1) != 1 and x.shape[1] != 1:
+    whole = x.is_contiguous()
+    if x.dim() != 2 or not whole and x.stride(1) != 1 and x.shape[1] != 1:
         raise ValueError("x must be [m, k] with contiguous rows")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("x must be bf16 or fp16")
     rows, k = x.shape
-    codes, scales = _code_outputs(x, codes, scales)
-    _launch(x.get_device(), "ne_quantize_rows", x.data_ptr(), _DTYPE_CODES[x.dtype], x.stride(0) if rows > 1 else k, rows, k,
+    codes, scales = _code_outputs(x, rows, k, codes, scales)
+    _launch(x.get_device(), "ne_quantize_rows", x.data_ptr(), _DTYPE_CODES[x.dtype], k if whole else x.stride(0), rows, k,
             codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
@@ -777,7 +777,7 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None,
 def _check_norm_rows(weight: torch.Tensor, rows: torch.Tensor) -> None:
     if rows.get_device() != weight.get_device() or not rows.is_cuda:
         _require_gpu(rows, weight)
-    if (rows.dim() != 2 or weight.shape != rows.shape[1:] or rows.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16
+    if (rows.dim() != 2 or weight.dim() != 1 or weight.numel() != rows.shape[1] or rows.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16
             or not rows.is_contiguous() or not weight.is_contiguous()):
         raise ValueError("rows must be contiguous [rows, hidden] bf16, the weight [hidden]")
 
@@ -786,8 +786,9 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: t
                      scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """:func:`quantize_rows` of :func:`rmsnorm`'s rows (the same bits), in one pass; hidden at most 4,096."""
     _check_norm_rows(weight, x)
-    codes, scales = _code_outputs(x, codes, scales)
-    _launch(x.get_device(), "ne_rmsnorm_quantize", x.data_ptr(), weight.data_ptr(), codes.data_ptr(), scales.data_ptr(), *x.shape,
+    rows, hidden = x.shape
+    codes, scales = _code_outputs(x, rows, hidden, codes, scales)
+    _launch(x.get_device(), "ne_rmsnorm_quantize", x.data_ptr(), weight.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, hidden,
             eps)
     return codes, scales
 
@@ -800,7 +801,7 @@ def add_rmsnorm_quantize(residual: torch.Tensor, delta: torch.Tensor, weight: to
     _check_norm_rows(weight, residual)
     _check_norm_rows(weight, delta)
     _check(residual.shape == delta.shape, "residual and delta must be of one shape")
-    codes, scales = _code_outputs(residual, codes, scales)
+    codes, scales = _code_outputs(residual, *residual.shape, codes, scales)
     _launch(residual.get_device(), "ne_add_rmsnorm_quantize", residual.data_ptr(), delta.data_ptr(), weight.data_ptr(),
             codes.data_ptr(), scales.data_ptr(), *residual.shape, eps)
     return codes, scales
@@ -818,10 +819,10 @@ def w8a8_gemm(
     weights of :func:`w8a16_gemm`; SwiGLU epilogue pairs 16 gate rows with 16 up rows.  ``k`` is a
     multiple of 16, at most 131,056; ``n`` is any number (SwiGLU: a multiple of 32)."""
     index = codes.get_device()
-    if (not codes.is_cuda or scales.get_device() != index or weight_int8.get_device() != index
-            or weight_scale.get_device() != index):
+    if index < 0 or scales.get_device() != index or weight_int8.get_device() != index or weight_scale.get_device() != index:
         _require_gpu(codes, scales, weight_int8, weight_scale)  # names the devices
-    if codes.dtype != torch.int8 or codes.dim() != 2 or codes.stride(1) != 1:
+    whole = codes.is_contiguous()
+    if codes.dtype != torch.int8 or codes.dim() != 2 or not whole and codes.stride(1) != 1:
         raise ValueError("codes must be [m, k] int8 with contiguous rows")
     if weight_int8.dtype != torch.int8 or weight_int8.dim() != 2 or not weight_int8.is_contiguous():
         raise ValueError("weight must be contiguous [n, k] int8")
@@ -835,12 +836,13 @@ def w8a8_gemm(
         raise ValueError("weight_scale must be contiguous, one per weight row")
     n_out = n // 2 if epilogue == EPILOGUE_SWIGLU else n
     if out is None:
-        out = codes.new_empty(m, n_out, dtype=torch.bfloat16)
+        out, ldy = codes.new_empty(m, n_out, dtype=torch.bfloat16), n_out
     elif out.shape != (m, n_out) or out.dtype != torch.bfloat16 or out.stride(1) != 1 and n_out > 1 or out.get_device() != index:
         raise ValueError(f"out must be bf16 [{m}, {n_out}] with contiguous rows on cuda:{index}")
-    _launch(index, "ne_w8a8_gemm", codes.data_ptr(), codes.stride(0) if m > 1 else k, scales.data_ptr(), weight_int8.data_ptr(),
-            weight_scale.data_ptr(), dtype_code(weight_scale.dtype), m, n, k, out.data_ptr(), out.stride(0) if m > 1 else n_out,
-            epilogue)
+    else:
+        ldy = out.stride(0) if m > 1 else n_out
+    _launch(index, "ne_w8a8_gemm", codes.data_ptr(), k if whole else codes.stride(0), scales.data_ptr(), weight_int8.data_ptr(),
+            weight_scale.data_ptr(), dtype_code(weight_scale.dtype), m, n, k, out.data_ptr(), ldy, epilogue)
     return out
 
 
@@ -1301,11 +1303,22 @@ def _int32_pointer(tensor: torch.Tensor | None, shape: tuple, name: str, index: 
     return tensor.data_ptr()
 
 
+def _int32_vector(tensor: torch.Tensor | None, n: int, name: str, index: int) -> int | None:
+    """:func:`_int32_pointer` of ``n`` values in a row."""
+    if tensor is None:
+        return None
+    if tensor.dtype != torch.int32 or tensor.dim() != 1 or tensor.numel() != n or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{n}], got {tensor.dtype} {list(tensor.shape)}")
+    if tensor.get_device() != index:
+        raise RuntimeError(f"{name} is on {tensor.device}, the logits on cuda:{index}")
+    return tensor.data_ptr()
+
+
 def _row_values(value, rows: int, name: str, index: int) -> tuple:
     """(address or None, scalar) of a penalty: one value, or an fp32 one per row."""
     if not isinstance(value, torch.Tensor):
         return None, value
-    if value.dtype != torch.float32 or value.shape != (rows,) or not value.is_contiguous():
+    if value.dtype != torch.float32 or value.dim() != 1 or value.numel() != rows or not value.is_contiguous():
         raise ValueError(f"{name} must be one value or contiguous fp32 [{rows}]")
     if value.get_device() != index:
         raise RuntimeError(f"{name} is on {value.device}, the logits on cuda:{index}")
@@ -1317,7 +1330,8 @@ _NO_PENALTIES = (None, 0, 0, None, None, 0, None, 0, None, None, None, 1.0, None
 
 def _penalty_arguments(p: TokenPenalties, rows: int, index: int) -> tuple:
     h, drafts = p.history, p.drafts
-    if h.dtype != torch.int32 or h.dim() != 2 or h.stride(1) != 1 and h.shape[1] > 1:
+    whole = h.is_contiguous()
+    if h.dtype != torch.int32 or h.dim() != 2 or not whole and h.stride(1) != 1 and h.shape[1] > 1:
         raise ValueError("history must be [seqs, capacity] int32 with contiguous rows")
     if h.get_device() != index:
         raise RuntimeError(f"history is on {h.device}, the logits on cuda:{index}")
@@ -1325,30 +1339,30 @@ def _penalty_arguments(p: TokenPenalties, rows: int, index: int) -> tuple:
     if seqs == 0:  # whose row_seq could name no sequence
         _check(rows == 0 or p.row_seq is not None, "no sequences")
         return _NO_PENALTIES
-    per_seq, per_row = (seqs,), (rows,)
-    length = _int32_pointer(p.history_len, per_seq, "history_len", index)
+    length = _int32_vector(p.history_len, seqs, "history_len", index)
     max_drafts = 0
     if drafts is not None:
         max_drafts = drafts.shape[-1] if drafts.dim() else 0
         _check(p.row_drafts is not None, "drafts need row_drafts")
     return (
         # (an empty tensor has no address, and its rows' guesses may still count)
-        h.data_ptr() if capacity else length, h.stride(0) if seqs > 1 else capacity, capacity, length,
-        _int32_pointer(p.prompt_len, per_seq, "prompt_len", index), seqs,
+        h.data_ptr() if capacity else length, capacity if whole else h.stride(0), capacity, length,
+        _int32_vector(p.prompt_len, seqs, "prompt_len", index), seqs,
         _int32_pointer(drafts, (seqs, max_drafts), "drafts", index), max_drafts,
-        _int32_pointer(p.row_seq, per_row, "row_seq", index), _int32_pointer(p.row_drafts, per_row, "row_drafts", index),
+        _int32_vector(p.row_seq, rows, "row_seq", index), _int32_vector(p.row_drafts, rows, "row_drafts", index),
         *_row_values(p.repetition, rows, "repetition", index), *_row_values(p.presence, rows, "presence", index),
         *_row_values(p.frequency, rows, "frequency", index))
 
 
 def _bias_arguments(bias: TokenBias, rows: int, index: int) -> tuple:
-    entries = bias.tokens.shape[0]
-    if bias.values.dtype != torch.float32 or bias.values.shape != (entries,) or not bias.values.is_contiguous():
+    entries = bias.tokens.numel()
+    if (bias.values.dtype != torch.float32 or bias.values.dim() != 1 or bias.values.numel() != entries
+            or not bias.values.is_contiguous()):
         raise ValueError(f"bias values must be contiguous fp32 [{entries}]")
     if bias.values.get_device() != index:
         raise RuntimeError(f"bias values are on {bias.values.device}, the logits on cuda:{index}")
-    start = _int32_pointer(bias.start, (rows + 1,), "bias start", index)
-    tokens = _int32_pointer(bias.tokens, (entries,), "bias tokens", index)
+    start = _int32_vector(bias.start, rows + 1, "bias start", index)
+    tokens = _int32_vector(bias.tokens, entries, "bias tokens", index)
     return (start, tokens, bias.values.data_ptr(), entries) if entries else (None, None, None, 0)
 
 
@@ -1371,7 +1385,8 @@ def adjust_logits(
     if not logits.is_cuda:
         _require_gpu(logits)
     index, dtype = logits.get_device(), logits.dtype
-    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] != 1:
+    whole = logits.is_contiguous()
+    if logits.dim() != 2 or not whole and logits.stride(1) != 1 and logits.shape[1] != 1:
         raise ValueError("logits must be [rows, vocab] with contiguous rows")
     code = dtype_code(dtype)
     if code == DTYPE_INT8:
@@ -1389,11 +1404,11 @@ def adjust_logits(
         if masks == 0 and rows > 0:
             raise ValueError("no masks")
         allowed_arguments = (_int32_pointer(allowed, (masks, words), "allowed", index), words, masks,
-                             _int32_pointer(allowed_rows, (rows,), "allowed_rows", index))
-    _launch(index, "ne_adjust_logits", logits.data_ptr(), code, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                             _int32_vector(allowed_rows, rows, "allowed_rows", index))
+    _launch(index, "ne_adjust_logits", logits.data_ptr(), code, vocab if whole else logits.stride(0), rows, vocab,
             *(_NO_PENALTIES if penalties is None else _penalty_arguments(penalties, rows, index)),
             *((None, None, None, 0) if bias is None else _bias_arguments(bias, rows, index)), *allowed_arguments,
-            out.data_ptr(), _DTYPE_CODES[out.dtype], out.stride(0) if rows > 1 else vocab)
+            out.data_ptr(), _DTYPE_CODES[out.dtype], vocab if out.is_contiguous() else out.stride(0))
     return out
 
 
