@@ -15,7 +15,6 @@ A case is a dict of plain values; ``kind`` says which operator it runs:
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -30,7 +29,6 @@ EPS = 1e-6
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
-@functools.cache  # a user's program imports once
 def _kernels():
     package = str(Path(__file__).resolve().parents[1] / "inference-engine-from-scratch_amd")
     if package not in sys.path:
