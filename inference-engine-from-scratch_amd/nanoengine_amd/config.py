@@ -59,7 +59,7 @@ class EngineSettings:
     chunked_prefill: bool = False
     max_num_batched_tokens: int = 512
     quantization: str = "none"
-    int8_activations: bool = False  # prompts' projections with 8-bit activations too (W8A8)
+    int8_activations: bool = False  # prompts' projections with 8-bit activations too (W8A8), 1,536 rows and more
     kv_cache_dtype: str = "auto"
     cuda_graphs: bool = False
     cuda_graph_max_context: int = 1024

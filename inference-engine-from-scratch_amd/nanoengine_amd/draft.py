@@ -228,7 +228,7 @@ class DraftModelProposer:
         c = self._cu
         n, r = self.max_seqs, self.k + 1
         batch = AttentionBatch(c["positions"], c["slots"], c["q_start"], c["q_len"], c["ctx"], c["tables"], r,
-                               self.max_tokens)
+                               self.max_tokens, prompt=False)
         hidden = self.model.forward(n * r, c["tokens"], batch, self.pool, workspace=self._cu_ws)
         torch.index_select(hidden, 0, c["last_rows"], out=c["last"])
         self.model.compute_logits(c["last"], logits=False, argmax=c["partials"])
@@ -314,7 +314,7 @@ class DraftModelProposer:
         d = self._dec
         n = self.max_seqs
         batch = AttentionBatch(d["positions"], d["slots"], d["q_start"], d["q_len"], d["ctx"], d["tables"], 1,
-                               self.max_tokens)
+                               self.max_tokens, prompt=False)
         hidden = self.model.forward(n, d["tokens"], batch, self.pool)
         self.model.compute_logits(hidden, logits=False, argmax=d["partials"])
         kernels.accept(self.no_drafts, self.zero_counts, self.last_rows, self.model.config.vocab_size,
@@ -445,7 +445,8 @@ class DraftModelProposer:
         ql = torch.tensor(q_len, dtype=torch.int32, device=dev)
         cl = torch.tensor(ctx_len, dtype=torch.int32, device=dev)
         bt = torch.from_numpy(np.stack(tables)).to(dev)
-        batch = AttentionBatch(posn, slots, qs, ql, cl, bt, max(q_len), max(ctx_len))
+        # (a catch-up or decode row's piece has at most k + 1)
+        batch = AttentionBatch(posn, slots, qs, ql, cl, bt, max(q_len), max(ctx_len), prompt=min(q_len) > self.k + 1)
         self.model.ensure_rope(max(ctx_len))
         hidden = self.model.forward(rows, tok, batch, self.pool, workspace=self.model.eager_workspace)
         self.forwards += 1

@@ -160,6 +160,7 @@ class ModelRunner:
             max_q_len=max(counts),
             max_ctx_len=ctx.max_context_length,
             prefix_groups=self._prefix_groups(sequences, counts, ctx.max_context_length) if self.shared_prefix else None,
+            prompt=all(s.num_cached_tokens + n <= s.num_prompt_tokens for s, n in zip(sequences, counts)),
         )
         rows = sum(counts)
         if rows > self._model.max_rows:

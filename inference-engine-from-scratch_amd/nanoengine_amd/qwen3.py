@@ -21,7 +21,7 @@ from nanoengine_amd._native import EPILOGUE_SWIGLU
 from nanoengine_amd.int8_quantization import quantize_vectors
 
 
-# From this many rows on a forward with int8_activations takes the W8A8 products.  Four layers of the 0.6B
+# From this many rows on a prompt's forward with int8_activations takes the W8A8 products.  Four layers of the 0.6B
 # shape, us with 16-bit / 8-bit activations: 320 rows 232 / 314, 512 339 / 332, 1,024 407 / 393, 1,536
 # 659 / 519, 2,048 723 / 577, 4,096 1,248 / 1,097, 8,192 2,520 / 2,214.  Up to 1,024 rows little is won
 # for the coarser rows.
@@ -201,6 +201,8 @@ class AttentionBatch:
     max_ctx_len: int
     # sequences that start with the same blocks: attention reads those once for each group
     prefix_groups: kernels.PrefixGroups | None = None
+    # whether the rows are prompts': only those take 8-bit activations, however many rows there are
+    prompt: bool = True
 
 
 class Qwen3VerifyModel:
@@ -208,9 +210,10 @@ class Qwen3VerifyModel:
 
     def __init__(self, weights: Qwen3Weights, max_rows: int, device: torch.device,
                  int8_activations: bool = False) -> None:
-        """``int8_activations``: forwards of ``W8A8_MIN_ROWS`` rows and more (prompts, mostly) quantise the
-        projections' activations to 8 bits with a scale per row and take the W8A8 products, on
-        the same weights; fewer rows keep bf16 activations, and so do caches that the fused QKV
+        """``int8_activations``: forwards of prompts (``AttentionBatch.prompt``) with ``W8A8_MIN_ROWS`` rows
+        and more, all their prompts' together, quantise the projections' activations to 8 bits with a
+        scale per row and take the W8A8 products, on the same weights; fewer rows keep bf16
+        activations, and so do verify and decode steps of any size and caches that the fused QKV
         products do not take."""
         c = weights.config
         if c.head_dim != kernels.HEAD_DIM:
@@ -298,7 +301,7 @@ class Qwen3VerifyModel:
                                          batch.q_len, c.num_attention_heads, c.num_key_value_heads,
                                          batch.max_q_len, batch.max_ctx_len, ws)
         fuse = self.fuse_qkv and kernels.qkv_fusion_supported(pool.key_caches[0], pool.key_scale_2d(0))
-        int8 = self.codes is not None and rows >= W8A8_MIN_ROWS and fuse
+        int8 = self.codes is not None and batch.prompt and rows >= W8A8_MIN_ROWS and fuse
         if int8:
             codes, scales = self._int8(normed)
         for i, layer in enumerate(w.layers):

@@ -249,7 +249,7 @@ class VerifyRunner:
         # LM head's argmax partials (every slot greedy)
         self.graph_sampled: bool | None = None
         self.batch = AttentionBatch(self.positions, self.slot_mapping, self.q_start, self.q_len,
-                                    self.ctx_len, self.block_tables, self.R, self.capacity)
+                                    self.ctx_len, self.block_tables, self.R, self.capacity, prompt=False)
         # the slots' common blocks, found anew after each slot change; the arrays keep their
         # place (a captured step reads them), slots without a group follow one by one (None: never
         # shared, as in a pool that only ordinary attention takes)
