@@ -11,6 +11,7 @@ in groups of 16 rows so that one GEMM with a SwiGLU epilogue replaces
 from __future__ import annotations
 
 import math
+import warnings
 from dataclasses import dataclass, fields
 from typing import Any
 
@@ -214,7 +215,7 @@ class Qwen3VerifyModel:
         and more, all their prompts' together, quantise the projections' activations to 8 bits with a
         scale per row and take the W8A8 products, on the same weights; fewer rows keep bf16
         activations, and so do verify and decode steps of any size and caches that the fused QKV
-        products do not take."""
+        products do not take.  Where that leaves the setting without effect, a warning says so."""
         c = weights.config
         if c.head_dim != kernels.HEAD_DIM:
             raise NotImplementedError("the HIP kernels support head_dim 128")
@@ -238,6 +239,9 @@ class Qwen3VerifyModel:
         if int8_activations and max_rows >= W8A8_MIN_ROWS:
             self.codes = torch.empty(max_rows * max(h, q, c.intermediate_size), dtype=torch.int8, device=device)
             self.code_scales = torch.empty(max_rows, dtype=torch.float32, device=device)
+        elif int8_activations:
+            warnings.warn(f"int8_activations has no effect: forwards have at most {max_rows} rows, and only prompts of "
+                          f"{W8A8_MIN_ROWS} and more take 8 bits", stacklevel=2)
         # cos/sin per position (qwen3.py:47-57), computed once on the host as the
         # reference computes them per step; grown when a longer position appears
         self.rope_positions = 0
@@ -301,7 +305,10 @@ class Qwen3VerifyModel:
                                          batch.q_len, c.num_attention_heads, c.num_key_value_heads,
                                          batch.max_q_len, batch.max_ctx_len, ws)
         fuse = self.fuse_qkv and kernels.qkv_fusion_supported(pool.key_caches[0], pool.key_scale_2d(0))
-        int8 = self.codes is not None and batch.prompt and rows >= W8A8_MIN_ROWS and fuse
+        int8 = self.codes is not None and batch.prompt and rows >= W8A8_MIN_ROWS
+        if int8 and not fuse:
+            warnings.warn("int8_activations has no effect: this cache's QKV projection is not fused", stacklevel=2)
+            int8 = False
         if int8:
             codes, scales = self._int8(normed)
         for i, layer in enumerate(w.layers):

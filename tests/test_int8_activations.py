@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import warnings
+from dataclasses import replace
 from types import SimpleNamespace
 
 import pytest
@@ -9,9 +11,9 @@ import torch
 
 from nanoengine_amd import kernels, model_runner, qwen3
 from nanoengine_amd.config import EngineSettings
-from nanoengine_amd.memory import PagedSlotAllocator
+from nanoengine_amd.memory import KVCachePool, PagedSlotAllocator
 from nanoengine_amd.model_runner import ModelRunner
-from nanoengine_amd.qwen3 import random_state_dict
+from nanoengine_amd.qwen3 import AttentionBatch, Qwen3VerifyModel, Qwen3Weights, random_state_dict
 from nanoengine_amd.runtime import create_verify_engine
 from nanoengine_amd.sequence_state import Sequence
 from test_answers import CFG, request, unit_norms
@@ -19,6 +21,8 @@ from test_draft_gpu import DCFG
 from test_draft_gpu import engine as draft_engine
 
 CPU = torch.device("cpu")
+SMALL = replace(CFG, vocab_size=512, hidden_size=256, intermediate_size=512, num_hidden_layers=1, num_attention_heads=4,
+                num_key_value_heads=2)
 
 
 class Recorder:
@@ -69,6 +73,38 @@ def test_a_steps_batch_says_whether_its_rows_are_prompts():
     other.token_ids += [4, 5, 6]
     runner.score_tokens(other, 3)
     assert [b.prompt for b in model.batches[3:]] == [True, False]
+
+
+def test_a_model_too_small_for_8_bit_activations_says_so():
+    state = random_state_dict(SMALL, seed=0, std=0.02)
+    weights = Qwen3Weights.from_state_dict(SMALL, state, CPU, torch.bfloat16)
+    with pytest.warns(UserWarning, match="int8_activations has no effect: forwards have at most 1535 rows"):
+        Qwen3VerifyModel(weights, 1535, CPU, int8_activations=True)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert Qwen3VerifyModel(weights, 1535, CPU).codes is None
+        assert Qwen3VerifyModel(weights, 1536, CPU, int8_activations=True).codes is not None
+
+
+@pytest.mark.gpu
+def test_a_prompt_into_a_cache_without_8_bit_products_says_so(monkeypatch):
+    """An int8 cache with fp32 scales, which the fused products do not take, and a model that does not fuse."""
+    monkeypatch.setattr(qwen3, "W8A8_MIN_ROWS", 100)
+    dev = torch.device("cuda")
+    weights = Qwen3Weights.from_state_dict(SMALL, random_state_dict(SMALL, seed=0, std=0.02), dev, torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device=dev)
+    at, n = torch.arange(112, **i32), torch.tensor([112], **i32)
+    batch = AttentionBatch(at, at, torch.tensor([0], **i32), n, n, torch.arange(7, **i32)[None], 112, 112)
+    for dtype, fuse in ((torch.float32, True), (torch.bfloat16, False)):
+        pool = KVCachePool(1, 2, 128, 128, dev, dtype, True, 16)
+        models = [Qwen3VerifyModel(weights, 128, dev, int8_activations=int8) for int8 in (True, False)]
+        for model in models:
+            model.fuse_qkv = fuse
+        with pytest.warns(UserWarning, match="int8_activations has no effect"):
+            got = models[0].forward(112, at, batch, pool).clone()
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            assert torch.equal(got, models[1].forward(112, at, batch, pool))
 
 
 @pytest.mark.gpu
