@@ -3,6 +3,7 @@ sampling helpers of ne/engine/sampling.py that stay on the host."""
 
 from __future__ import annotations
 
+import math
 import os
 from collections.abc import AsyncIterator, Mapping
 from dataclasses import dataclass, field
@@ -33,6 +34,18 @@ class SamplingParams:
     def is_penalized(self) -> bool:
         """Whether the logits depend on the tokens so far."""
         return self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+
+    def penalty_error(self) -> str | None:
+        """Why no logits can be made under these penalties, or None.  (An infinite one bans, or forces, the
+        tokens that it is for; of opposite signs two make no sum.)"""
+        if not 0.0 < self.repetition_penalty < math.inf:
+            return "repetition_penalty must be positive and finite"
+        for name in ("presence_penalty", "frequency_penalty"):
+            if math.isnan(getattr(self, name)):
+                return f"{name} must not be NaN"
+        if math.isnan(self.presence_penalty + self.frequency_penalty):
+            return "presence_penalty and frequency_penalty must not be infinite in opposite directions"
+        return None
 
     @property
     def is_adjusted(self) -> bool:

@@ -259,8 +259,9 @@ class ModelRunner:
         if len(allowed) != len(sequences):
             raise ValueError(f"allowed_tokens for {len(allowed)} of {len(sequences)} sequences")
         for s in sequences:
-            if not 0.0 < s.sampling_params.repetition_penalty < math.inf:
-                raise ValueError(f"{s.request_id}: repetition_penalty must be positive and finite")
+            problem = s.sampling_params.penalty_error()
+            if problem is not None:
+                raise ValueError(f"{s.request_id}: {problem}")
         inputs = build_step_inputs(sequences, self.allocator, self._pool, self._device, token_counts)
         hidden, starts, counts = self._forward(inputs, sequences)
         last = torch.tensor([s + n - 1 for s, n in zip(starts, counts, strict=True)], device=self._device)

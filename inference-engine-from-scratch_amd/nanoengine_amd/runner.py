@@ -379,8 +379,9 @@ class VerifyRunner:
                                  "not top_k or min_p")
             if seq.sampling_params.logit_bias:
                 raise ValueError(f"{seq.request_id}: speculative verification takes penalties, not logit_bias")
-            if not 0.0 < seq.sampling_params.repetition_penalty < math.inf:
-                raise ValueError(f"{seq.request_id}: repetition_penalty must be positive and finite")
+            problem = seq.sampling_params.penalty_error()
+            if problem is not None:
+                raise ValueError(f"{seq.request_id}: {problem}")
         slots = free[: len(sequences)]
         results = {}
         # prefill contiguous runs of slots together
