@@ -588,7 +588,8 @@ int ne_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, const int8_
  * The QKV projection of a prompt with 8-bit activations: ne_w8a8_gemm (store epilogue) over the
  * concatenated q | k | v weight ([(Hq+2*Hkv)*128, k] int8), each head of every row then taken as
  * ne_qk_norm_rope_kv_write takes it (the same bits; of a row that is not finite the codes in
- * an int8 cache may differ), without writing the product to memory: what
+ * an int8 cache may differ, and a row whose scale is NaN leaves vectors of at most 1e-8 there, NaN in
+ * q_out and in a bf16 cache), without writing the product to memory: what
  * ne_w8a16_qkv_norm_rope_kv is to ne_w8a16_gemm, with its arguments.  x, x_scale, w, w_scale and k
  * as in ne_w8a8_gemm; kv_dtype NE_DTYPE_INT8 (scales bf16 or fp16) or NE_DTYPE_BF16; q_out and the
  * caches 16-byte aligned, rope 8-byte, the norm weights 4-byte aligned.
