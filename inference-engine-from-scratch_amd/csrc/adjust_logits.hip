@@ -381,7 +381,8 @@ int launch_ranges(const AdjustParams& p, hipStream_t stream) {
 }
 
 // Penalties alone, in place: only tokens of the history change, and a work-group takes a row's in one
-// pass.  An LDS table of 2^size slots, at least 1.5 times the tokens, takes each of them by linear probing
+// pass: 320 rows with 2,000 tokens each read 19.6 and write 14.8 MB (6.8 us at a copy's rate) in 19.7-21.5; the rest
+// is its chain, length, history, table and scattered logits.  An LDS table of 2^size slots, at least 1.5 times the tokens, takes each of them by linear probing
 // (so a free slot ends every search), its counts beside it; then each slot's logit is adjusted.
 constexpr int kSeenThreads = 512, kMaxSeen = 5461;  // tokens in a table of 8,192 slots, 64 KiB
 template <int DT>
@@ -460,9 +461,13 @@ int launch_seen(const AdjustParams& p, hipStream_t stream) {
 }
 
 // In place under penalties alone a row's own tokens are cheaper than its vocabulary where rows are many and
-// histories short beside it (us, bf16, ranges / own tokens): 320 rows of 151,936 with 100 tokens 23.6 /
-// 6.5, with 2,000 36.6 / 21.5, 64 rows with 2,000 11.3 / 10.5; but 320 rows with 8,000 50 / 83, one row with 600
-// 4.9 / 6.3, 320 rows of 9,001 with 2,000 9.8 / 10.7.
+// histories short beside it (us, bf16, ranges / own tokens): 320 rows of 151,936, histories of their own in buffers of
+// 2,048 tokens, with 100 tokens 23.6 / 6.5, with 2,000 36.6 / 21.5, 64 rows with 2,000 of 4,096 11.3 / 10.5; but 320 rows
+// with 8,000 of 8,192 50 / 83, one row with 600 4.9 / 6.3, 320 rows of 9,001 with 2,000 9.8 / 10.7.
+//
+// The host knows a buffer's width, not the lengths in it, so every rule here goes by the width, and what a
+// short history costs depends on it: 64 sequences' 320 verify rows with 100 tokens take 5.6 us in a buffer of 108, 8.3
+// in one of 4,101 and 38.7 in one of 40,965 (32-bit tables), with 2,000 tokens 19.7 (of 2,008), 20.3 and 49.3.
 //
 // 8,192 tokens per work-group, 4,096 where that leaves CUs idle: one row of 151,936 (20 biases) 5.7 and
 // 4.5 us, 320 rows with histories of up to 2,048 tokens 44 and 53.  Histories that need wide counters

@@ -9,8 +9,10 @@
 // multiplied into is NaN, as with the row itself.  Norm rows are the bits that ne_rmsnorm and
 // ne_add_rmsnorm store (same sums in the same order, both roundings), quantised without the
 // trip through memory.  Bound by memory where rows are many, each read once into registers (8,192 x
-// 8,192 fp16 39 us, 5.2 TB/s; 4,001 x 2,048 9.2, of which ~2 are the launch; norm 8,192 x 1,024 9-10.6);
-// few rows take a chain of one load, two reductions and a store (2.2-3.5 us).
+// 8,192 fp16 35-39 us, 5.2-5.8 TB/s; 4,001 x 2,048 8.6-8.9, of which ~2 are the launch; 8,192 x 1,024 through the
+// norm 9.4, through add and norm 13.1, floors 4.9 and 11.5); few rows take a chain of one load, two
+// reductions and a store (64 x 2,048 2.3-2.7 us replayed one after another, 64 x 1,024 through the norm 3.3, and
+// up to 5.1 behind work that left the caches without them).
 #include "ne_common.hpp"
 
 namespace ne {
@@ -220,10 +222,10 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(RowsParams p) 
     *(u32x2*)(dst + (int64_t)ci * 8) = quantize8<VDT>(*(const u32x4*)(src + (int64_t)ci * 8), s, rcp);
 }
 
-// Few waves per row leave a wave more to do, many take two rounds of the CUs.  us, one wave per row / four:
-// 64 x 2,048 5.3 / 4.6, 320 x 2,048 4.5 / 3.9, 4,001 x 2,048 9.2 / 9.6, 20,000 x 2,048 23.4 / 30.6;
-// 64 x 4,096 5.3 / 3.9, 4,001 x 4,096 15.3 / 12.8, 20,000 x 4,096 42.6 / 41.2.  The norm's sum keeps
-// ne_rmsnorm's order, one wave per row.
+// Few waves per row leave a wave more to do, many take two rounds of the CUs.  us (bf16, replayed one after
+// another on other rows each), one wave per row / four: 64 x 2,048 3.0 / 2.3, 320 x 2,048 3.5 / 3.0, 1,024 x
+// 2,048 4.1 / 4.0, 4,001 x 2,048 8.9 / 8.8, 20,000 x 2,048 25.8 / 30.6; 64 x 4,096 4.3 / 2.6, 4,001 x 4,096 15.6 /
+// 12.6, 20,000 x 4,096 50.8 / 45.6.  The norm's sum keeps ne_rmsnorm's order, one wave per row.
 template <int MODE, int VDT>
 int launch_rows(const RowsParams& p, hipStream_t stream) {
   const dim3 four(ceil_div(p.rows, 4)), one(p.rows), block(256);

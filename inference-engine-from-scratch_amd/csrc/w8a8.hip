@@ -742,7 +742,7 @@ int launch_few(const W8a8Params& p, hipStream_t stream) {
 // The least estimated time (us) over the kernels: a fixed part, and a cost per 128 k that grows
 // with the tiles (or work-groups) per CU.  Constants fitted to 192 shapes (m 1-4,096, n 256-16,384,
 // k 256-8,192, GPU time from graphs), over which the choice takes 1.5 % longer than the fastest
-// kernel of each shape on average, at most 30 % (200 rows, n = 16,384, k = 8,192: 71 against 54 us).
+// kernel of each shape on average, at most 32 % (200 rows, n = 16,384, k = 8,192: 71 against 54 us).
 // Examples (us; few rows / 64 x 64 / 64 x 128 / 128 x 128 / 256 x 256): 64 x 1,024 x 2,048 5.3 / 10.0 /
 // 12.1 / 15.0 / 27.8, 333 x 4,096 x 1,024 14.4 / 8.8 / 8.7 / 10.1 / 18.8, 2,048 x 4,096 x 1,024 - / 21.3 /
 // 19.4 / 16.0 / 21.9, 4,096 x 4,096 x 1,024 - / 37.6 / 32.1 / 25.2 / 23.2.
@@ -815,8 +815,9 @@ int launch_kernel(const W8a8Params& p, hipStream_t stream) {
 }
 
 // A wave's tile has a head's 128 columns, so that a vector's sum and largest value are four lanes' work and
-// its RoPE pairs one lane's.  256 x 256 tiles where their last round over the CUs is nearly full,
-// else 128 x 128, two per CU (us, 16 + 8 heads, k = 1,024, int8 cache, 256 / 128; ne_w8a8_gemm into memory; the
+// its RoPE pairs one lane's.  256 x 256 tiles where their last round over the CUs is nearly full (92 %: a rule
+// fitted to the shape below alone, and off by about 1 us there at 3,000 rows with a bf16 cache, 30.2 / 29.0, and
+// at 4,096 with an int8 one), else 128 x 128, two per CU (us, 16 + 8 heads, k = 1,024, int8 cache, 256 / 128; ne_w8a8_gemm into memory; the
 // W8A16 product with the same epilogue): 512 rows 30.6 / 15.2; 8.8; 17.7, 2,048 31.8 / 19.2; 14.8; 32.0,
 // 4,096 33.4 / 32.4; 21.8; 53.0 (bf16 cache 30.1 / 32.5), 6,000 55.9 / 48.1; 32.9; 80.4, 8,192 57.2 /
 // 58.3; 37.1; 91.1 (bf16 52.8 / 60.2), 16,384 107 / 111; 68; 171.  The row kernel alone takes 68-71 at 8,192.

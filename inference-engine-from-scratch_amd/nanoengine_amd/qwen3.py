@@ -25,7 +25,7 @@ from nanoengine_amd.int8_quantization import quantize_vectors
 # From this many rows on a prompt's forward with int8_activations takes the W8A8 products.  Four layers of the 0.6B
 # shape, us with 16-bit / 8-bit activations: 320 rows 232 / 314, 512 339 / 332, 1,024 407 / 393, 1,536
 # 659 / 519, 2,048 723 / 577, 4,096 1,248 / 1,097, 8,192 2,520 / 2,214.  Up to 1,024 rows little is won
-# for the coarser rows.
+# for the coarser rows.  The one shape that was measured: wider layers gain from fewer rows on.
 W8A8_MIN_ROWS = 1536
 
 
